@@ -251,7 +251,7 @@ def prepare(c, seed):
         s.k = _normal((T, c["hkv"], c["d"]), c["dtype"], g)
         s.v = _normal((T, c["hkv"], c["d"]), c["dtype"], g)
     else:  # the buffer that the program keeps for split sums, zeroed once
-        s.ws = torch.zeros(32 << 20, dtype=torch.uint8, device="cuda")
+        s.ws = torch.zeros(64 << 20, dtype=torch.uint8, device="cuda")
     return s
 
 
