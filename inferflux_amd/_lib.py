@@ -1,4 +1,4 @@
-"""Loads libifx_qgemm.so (the HIP kernels behind include/ifx_qgemm.h) with
+"""Loads libifx_qgemm.so (the HIP kernels behind include/ifx_*.h) with
 ctypes and declares every exported C entry point.
 
 There is no fallback: if the library is missing this raises, so nothing can
@@ -95,6 +95,19 @@ SIGNATURES.update({
     "ifx_gguf_type_name": ([_i32], _cp),
     "ifx_gguf_parse_name": ([_cp, ctypes.POINTER(_i32), _cp, _u64, _cp, _u64], _i32),
     "ifx_gguf_status_string": ([_i32], _cp),
+})
+
+# Every symbol include/ifx_attention.h declares.
+SIGNATURES.update({
+    "ifx_plan_batch": ([_vp, _vp, _vp, _i32, _vp, _i32, _vp, _i32, _i32, _i32] + [_vp] * 7, _i32),
+    "ifx_rope_append": ([_vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _i32,
+                         _i32, _i32, _i32, _vp, _i64, _vp, _vp, _i32, _i64, _i32, _vp], _i32),
+    "ifx_attn_paged_workspace_bytes": ([_i32] * 7, _i64),
+    "ifx_attn_paged": ([_vp, _i64, _i32, _vp, _vp, _i64, _i32, _vp, _i32, _vp, _vp, _i32, _i32,
+                        _i32, _i32, _i32, _i32, _i32, ctypes.c_float, _i32, _vp, _i64, _i32, _vp,
+                        _i64, _vp], _i32),
+    "ifx_attn_prompt": ([_vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _i32, _i32, _i32, _i32, _i32,
+                         _i32, _i32, _i32, ctypes.c_float, _vp, _i64, _i32, _vp], _i32),
 })
 
 _lib = None

@@ -1,0 +1,296 @@
+"""The attention of a serving step for torch device tensors, over the C ABI of
+include/ifx_attention.h: what lies between a layer's Q/K/V projections and its
+O projection (`ops`).
+
+    k_cache, v_cache = attention.kv_cache(pages, kv_heads, head_dim)   # per layer
+    ws = attention.workspace()                                         # per stream
+
+    # per step: B requests, new_len[b] new tokens behind ctx_len[b] cached ones
+    p = attention.plan_batch(ctx_len, new_len, table, free, free_count, 64, T)
+    # per layer: the projections' rows q [T, Hq, D], k and v [T, Hkv, D]
+    q = attention.rope_append(q, k, v, p.positions, p.slots, k_cache, v_cache, inv_freq)
+    o = attention.paged_attention(q, k_cache, v_cache, table, p.cu_q, p.kv_len,
+                                  max_q, max_kv, workspace=ws, out_dtype=torch.float16)
+
+Whole prompts that no cache is kept for (scoring, embedding) go through
+prompt_attention instead.  Integers are int32, caches and rows of Q fp16 or
+bf16.  Nothing here synchronises the host, and with outputs given nothing
+allocates, so every call can be captured into a graph.  Calls run on the
+current stream of the tensors' device, or on `stream`, one of that device.
+Errors are those of `ops`: NotHandled, HipError, ValueError, TypeError.
+"""
+from collections import namedtuple
+
+import torch
+
+from . import _lib
+from .ops import _check
+
+MAX_BATCH = 4096
+WORKSPACE_BYTES = 64 << 20  # IFX_ATTN_WORKSPACE_BYTES: enough for every call
+PAGE_SIZES = (16, 32, 64, 128, 256)
+HEAD_DIMS = (64, 96, 128, 256)
+# bits of BatchPlan.status
+NO_PAGES, NARROW, NO_ROOM, BAD_LENGTH = 1, 2, 4, 8
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_ELEMS = (torch.float16, torch.bfloat16)
+
+BatchPlan = namedtuple("BatchPlan", "cu_q kv_len positions slots free_left status")
+
+
+class _on:
+    """Makes `device` the current one for a launch, if it is not."""
+
+    def __init__(self, device):
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _stream(device, stream):
+    if stream is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    if stream.device != device:
+        raise ValueError(f"the stream is of {stream.device}, the tensors of {device}")
+    return stream.cuda_stream
+
+
+def _new(shape, dtype, device, stream):
+    """An output of a call: the allocator is told of a stream that is not the
+    current one, so that it does not hand the memory out while in use there."""
+    t = torch.empty(shape, dtype=dtype, device=device)
+    if stream is not None:
+        t.record_stream(stream)
+    return t
+
+
+def _same_device(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} must be on {device}")
+
+
+def _i32(t, name, n):
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} must be int32")
+    if not t.is_contiguous() or t.numel() < n:
+        raise ValueError(f"{name} must be contiguous with at least {n} values")
+    return t.data_ptr()
+
+
+def _rows(t, name, T, H, D):
+    """Pointer and row stride of rows [T, H, D]: heads of D values one after
+    the other, rows any distance apart."""
+    if t.dim() != 3 or t.shape[0] != T or t.shape[1] != H or t.shape[2] != D:
+        raise ValueError(f"{name} must be [{T}, {H}, {D}], got {list(t.shape)}")
+    st = t.stride()
+    if T == 0:
+        return t.data_ptr(), H * D
+    if (D > 1 and st[2] != 1) or (H > 1 and st[1] != D):
+        raise ValueError(f"{name}: a row's heads must lie one after the other")
+    return t.data_ptr(), (st[0] if T > 1 else H * D)
+
+
+def _caches(k_cache, v_cache):
+    """(pages, kv heads, page size, head size) of a layer's caches."""
+    if k_cache.dtype not in _ELEMS or v_cache.dtype != k_cache.dtype:
+        raise TypeError("the caches must be float16 or bfloat16, both the same")
+    if k_cache.dim() != 5 or v_cache.dim() != 5:
+        raise ValueError("the caches must be as kv_cache makes them")
+    n, h, d8, p, e = k_cache.shape
+    if e != 8 or tuple(v_cache.shape) != (n, h, p // 8, d8 * 8, 8):
+        raise ValueError("the caches must be as kv_cache makes them: [pages, heads, D / 8, page, 8] "
+                         "and [pages, heads, page / 8, D, 8]")
+    if not k_cache.is_contiguous() or not v_cache.is_contiguous():
+        raise ValueError("the caches must be contiguous")
+    return n, h, p, d8 * 8
+
+
+def kv_cache(num_pages, kv_heads, head_dim, page_size=64, dtype=torch.float16, device="cuda"):
+    """One layer's paged cache (K, V), zeroed: num_pages pages of page_size
+    tokens, in the layout of include/ifx_attention.h."""
+    if page_size not in PAGE_SIZES:
+        raise ValueError(f"page_size must be one of {PAGE_SIZES}")
+    if head_dim % 8 or dtype not in _ELEMS:
+        raise ValueError("head_dim must be a multiple of 8, dtype float16 or bfloat16")
+    k = torch.zeros(num_pages, kv_heads, head_dim // 8, page_size, 8, dtype=dtype, device=device)
+    v = torch.zeros(num_pages, kv_heads, page_size // 8, head_dim, 8, dtype=dtype, device=device)
+    return k, v
+
+
+def workspace(device="cuda"):
+    """A workspace for paged_attention's split sums that is large enough for
+    any call.  One per stream: calls that share one must not overlap."""
+    return torch.zeros(WORKSPACE_BYTES, dtype=torch.uint8, device=device)
+
+
+def plan_batch(ctx_len, new_len, block_table, free_pages, free_count, page_size, max_tokens,
+               out=None, stream=None):
+    """Pages, slots, positions and row offsets of one step, on the device
+    (ifx_plan_batch).  ctx_len, new_len [B]; block_table [B, W], updated in
+    place; free_pages: a stack of free page numbers of which the first
+    free_count[0] are valid, taken from the end.  Returns a BatchPlan of int32
+    tensors (`out`: one of an earlier call to write into):
+
+      cu_q [B + 1], kv_len [B], positions and slots [max_tokens] (behind the
+      last token: 0 and -1), free_left [1], status [1] (0, or a sum of
+      NO_PAGES, NARROW, NO_ROOM, BAD_LENGTH: then nothing is taken, cu_q is 0
+      and every slot -1)."""
+    dev, B = ctx_len.device, ctx_len.numel()
+    if not ctx_len.is_cuda:
+        raise ValueError("ctx_len must be a device tensor")
+    if block_table.dim() != 2 or block_table.shape[0] != B:
+        raise ValueError("block_table must be [B, pages]")
+    if out is None:
+        out = BatchPlan(*(_new(n, torch.int32, dev, stream)
+                          for n in (B + 1, B, max_tokens, max_tokens, 1, 1)))
+    _same_device(dev, new_len=new_len, block_table=block_table, free_pages=free_pages,
+                 free_count=free_count, **out._asdict())
+    W = block_table.shape[1]
+    with _on(dev):
+        rc = _lib.load().ifx_plan_batch(
+            _i32(ctx_len, "ctx_len", B), _i32(new_len, "new_len", B),
+            _i32(block_table, "block_table", B * W), W, _i32(free_pages, "free_pages", 0),
+            free_pages.numel(), _i32(free_count, "free_count", 1), page_size, B, max_tokens,
+            _i32(out.cu_q, "cu_q", B + 1), _i32(out.kv_len, "kv_len", B),
+            _i32(out.positions, "positions", max_tokens), _i32(out.slots, "slots", max_tokens),
+            _i32(out.free_left, "free_left", 1), _i32(out.status, "status", 1),
+            _stream(dev, stream))
+    _check(rc, "ifx_plan_batch")
+    return out
+
+
+def rope_append(q, k, v, positions, slots, k_cache, v_cache, inv_freq=None, interleaved=False,
+                q_out=None, stream=None):
+    """Rotates q [T, Hq, D] and k [T, Hkv, D] by positions * inv_freq and writes
+    k and v into the caches at `slots` (ifx_rope_append); returns the rotated
+    q in the caches' type.  q, k and v: fp32, fp16 or bf16 as the projections
+    wrote them, slices of one buffer's rows among them.  inv_freq: fp64
+    [rot_dim / 2] on the device, None for no rotation.  Tokens whose slot is
+    outside the cache (-1) are left out, their rows of q_out as well."""
+    n, Hkv, P, D = _caches(k_cache, v_cache)
+    dev = k_cache.device
+    if not k_cache.is_cuda:
+        raise ValueError("k_cache must be a device tensor")
+    if q.dim() != 3:
+        raise ValueError("q must be [T, Hq, D]")
+    T, Hq = q.shape[0], q.shape[1]
+    src = _DTYPES.get(q.dtype)
+    if src is None or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("q, k and v must be float32, float16 or bfloat16, all the same")
+    rot = 0
+    if inv_freq is not None:
+        if inv_freq.dtype != torch.float64 or not inv_freq.is_contiguous():
+            raise TypeError("inv_freq must be contiguous float64")
+        rot = 2 * inv_freq.numel()
+    if q_out is None:
+        q_out = _new((T, Hq, D), k_cache.dtype, dev, stream)
+    elif q_out.dtype != k_cache.dtype:
+        raise TypeError("q_out must have the caches' type")
+    _same_device(dev, q=q, k=k, v=v, positions=positions, slots=slots, v_cache=v_cache,
+                 inv_freq=inv_freq, q_out=q_out)
+    qp, qs = _rows(q, "q", T, Hq, D)
+    kp, ks = _rows(k, "k", T, Hkv, D)
+    vp, vs = _rows(v, "v", T, Hkv, D)
+    op, os = _rows(q_out, "q_out", T, Hq, D)
+    with _on(dev):
+        rc = _lib.load().ifx_rope_append(
+            qp, qs, kp, ks, vp, vs, src, _i32(positions, "positions", T), _i32(slots, "slots", T),
+            inv_freq.data_ptr() if rot else None, rot, int(bool(interleaved)), T, Hq, Hkv, D, op,
+            os, k_cache.data_ptr(), v_cache.data_ptr(), _DTYPES[k_cache.dtype], n, P,
+            _stream(dev, stream))
+    _check(rc, "ifx_rope_append")
+    return q_out
+
+
+def _out(q, out, out_dtype, stream):
+    if out is None:
+        return _new(q.shape, out_dtype or q.dtype, q.device, stream)
+    if out.dtype not in _DTYPES or (out_dtype is not None and out.dtype != out_dtype):
+        raise TypeError("out must be float32, float16 or bfloat16, and of out_dtype if that is given")
+    return out
+
+
+def paged_workspace_bytes(B, T, Hq, Hkv, head_dim, max_q, max_kv):
+    """Bytes of workspace that paged_attention needs for this shape (0: none;
+    WORKSPACE_BYTES is enough for all)."""
+    return int(_lib.load().ifx_attn_paged_workspace_bytes(B, T, Hq, Hkv, head_dim, max_q, max_kv))
+
+
+def paged_attention(q, k_cache, v_cache, block_table, cu_q, kv_len, max_q, max_kv, scale=None,
+                    window=0, out=None, out_dtype=None, workspace=None, stream=None):
+    """Attention of the new tokens q [T, Hq, D] over the paged cache, which
+    holds them already (ifx_attn_paged).  cu_q [B + 1]: the requests' first
+    rows; kv_len [B]: their tokens, the new ones included; max_q, max_kv: bounds
+    of both.  A query sees its own position and what is before it, the last
+    `window` keys of it where window > 0.  scale: head_dim ** -0.5 if None.
+    Returns out [T, Hq, D] (out_dtype: fp32, fp16 or bf16, q's type if None);
+    its rows from cu_q[B] on are left as they were.  workspace: see
+    `workspace` and paged_workspace_bytes."""
+    n, Hkv, P, D = _caches(k_cache, v_cache)
+    dev = q.device
+    if not q.is_cuda or q.dim() != 3:
+        raise ValueError("q must be a device tensor [T, Hq, D]")
+    if q.dtype != k_cache.dtype:
+        raise TypeError("q must have the caches' type")
+    T, Hq = q.shape[0], q.shape[1]
+    B = kv_len.numel()
+    if block_table.dim() != 2 or block_table.shape[0] != B:
+        raise ValueError("block_table must be [B, pages]")
+    W = block_table.shape[1]
+    out = _out(q, out, out_dtype, stream)
+    _same_device(dev, k_cache=k_cache, v_cache=v_cache, block_table=block_table, cu_q=cu_q,
+                 kv_len=kv_len, out=out, workspace=workspace)
+    qp, qs = _rows(q, "q", T, Hq, D)
+    op, os = _rows(out, "out", T, Hq, D)
+    wp, wn = None, 0
+    if workspace is not None:
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
+        wp, wn = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    with _on(dev):
+        rc = _lib.load().ifx_attn_paged(
+            qp, qs, _DTYPES[q.dtype], k_cache.data_ptr(), v_cache.data_ptr(), n, P,
+            _i32(block_table, "block_table", B * W), W, _i32(cu_q, "cu_q", B + 1),
+            _i32(kv_len, "kv_len", B), B, T, Hq, Hkv, D, max_q, max_kv,
+            D ** -0.5 if scale is None else scale, window, op, os, _DTYPES[out.dtype], wp, wn,
+            _stream(dev, stream))
+    _check(rc, "ifx_attn_paged")
+    return out
+
+
+def prompt_attention(q, k, v, cu_len, max_len, causal=True, window=0, scale=None, out=None,
+                     out_dtype=None, stream=None):
+    """Attention over whole prompts packed one after the other, without a cache
+    (ifx_attn_prompt): q [T, Hq, D], k and v [T, Hkv, D] (fp16 or bf16), rows
+    cu_len[b] .. cu_len[b + 1] - 1 are prompt b, max_len bounds the lengths.
+    A row sees its prompt's rows; where causal those up to its own, the last
+    `window` of them where window > 0.  Returns out [T, Hq, D] (out_dtype:
+    fp32, fp16 or bf16, q's type if None)."""
+    dev = q.device
+    if not q.is_cuda or q.dim() != 3 or k.dim() != 3:
+        raise ValueError("q, k and v must be device tensors [T, heads, D]")
+    if q.dtype not in _ELEMS or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("q, k and v must be float16 or bfloat16, all the same")
+    T, Hq, D = q.shape
+    Hkv, B = k.shape[1], cu_len.numel() - 1
+    out = _out(q, out, out_dtype, stream)
+    _same_device(dev, k=k, v=v, cu_len=cu_len, out=out)
+    qp, qs = _rows(q, "q", T, Hq, D)
+    kp, ks = _rows(k, "k", T, Hkv, D)
+    vp, vs = _rows(v, "v", T, Hkv, D)
+    op, os = _rows(out, "out", T, Hq, D)
+    with _on(dev):
+        rc = _lib.load().ifx_attn_prompt(
+            qp, qs, kp, ks, vp, vs, _DTYPES[q.dtype], _i32(cu_len, "cu_len", B + 1), B, T, Hq, Hkv,
+            D, max_len, int(bool(causal)), window, D ** -0.5 if scale is None else scale, op, os,
+            _DTYPES[out.dtype], _stream(dev, stream))
+    _check(rc, "ifx_attn_prompt")
+    return out

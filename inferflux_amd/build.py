@@ -32,6 +32,7 @@ if os.environ.get("IFX_TUNING") == "1":
 EXACT = {"quantize.hip", "dequant.hip"}
 SOURCES = ["api.hip", "quantize.hip", "dequant.hip", "gemv.hip", "mmq_skinny.hip", "mmvq.hip", "gemm_mfma.hip", "gemv_lds.hip", "gemv_slot.hip", "gemm_f16.hip", "gemm_f16_q4.hip", "gemm_f16_q6.hip", "gemm_f16_q8.hip",
            "gemv_dq.hip", "packed.hip",
+           "attention_api.hip", "kv_plan.hip", "rope_append.hip", "attn_rows.hip", "attn_tile.hip",
            "../host/fused_quant_gemm.cpp", "../host/native_dispatch.cpp", "../host/gguf.cpp", "../host/gguf_model.cpp"]
 
 

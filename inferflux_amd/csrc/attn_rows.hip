@@ -1,0 +1,340 @@
+// attn_rows.hip -- paged attention of requests with few query rows (at most
+// 32 = new tokens x query heads of a group: decode steps).
+//
+//   s_j = c q . k_j (c = scale log2 e), p_j = 2^(s_j - m), l = sum p_j,
+//   o = sum p_j v_j / l
+//
+// Bound by HBM: every key and value of the request is read once for 2 x 32
+// (padded) x D multiply-adds an element, well under the MFMA rate.  So what
+// counts is bytes in flight.  The cache's layout is the MFMA operand order:
+// each wave reads its 32 keys' K and V straight into operand registers with
+// contiguous 16-byte loads, 16 KB a wave at D = 128, and nothing passes
+// through LDS.  Waves take tiles of 32 keys in turn, each with its own running
+// maximum and sums; they meet once, in LDS, at the end.  The keys of a request
+// are split over workgroups in chunks of a length that is the same for all
+// requests (long ones get more workgroups, not longer ones); the last
+// workgroup of a request and head to finish adds the chunks in their order.
+#include "ifx_attn.h"
+
+namespace ifx {
+
+namespace {
+
+constexpr int kWaves = 4;
+
+// The four dwords of an 8-key piece with the keys outside [lo, hi] cleared.
+struct PieceMask {
+  uint32_t m[4];
+};
+__device__ __forceinline__ PieceMask piece_mask(int key, int lo, int hi) {
+  PieceMask r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int k0 = key + 2 * j, k1 = k0 + 1;
+    r.m[j] = (k0 >= lo && k0 <= hi ? 0xFFFFu : 0u) | (k1 >= lo && k1 <= hi ? 0xFFFF0000u : 0u);
+  }
+  return r;
+}
+
+}  // namespace
+
+template <int DT, int D>
+__global__ __launch_bounds__(256, 2) void k_attn_rows(const AttnArgs a, int lds_rows) {
+  using T = Elem<DT>;
+  constexpr int ND = D / 32, NS = D / 16;
+  extern __shared__ float red[];  // [wave][D / 4][row][4]
+  __shared__ float red_m[kWaves][32], red_l[kWaves][32];
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kvh = blockIdx.x, b = blockIdx.y, z = blockIdx.z;
+  const int sh = a.page_shift, P = 1 << sh;
+
+  const int q0 = min(max(a.cu[b], 0), a.T), q1 = min(max(a.cu[b + 1], 0), a.T);
+  const int kv = min(max(a.kv_len[b], 0), a.table_width << sh);
+  const int nq = q1 - q0, R = min(nq * a.G, lds_rows);
+  if (nq <= 0) return;
+  const int ctx = kv - nq;  // position of the first row; below 0 it sees nothing
+  const int lo0 = a.window > 0 ? max(0, ctx - a.window + 1) : 0;
+  const int kbeg = lo0 & ~(kRowKeys - 1), kend = kv;  // the last row sees kv - 1
+  const int chunk = split_chunk(a, kend - kbeg, kRowKeys);
+  const int ns = kend > kbeg ? (kend - kbeg + chunk - 1) / chunk : 1;
+  if (z >= ns) return;
+  const int zbeg = kbeg + z * chunk, zend = min(zbeg + chunk, kend);
+
+  // this lane's row: what it sees is [lo, hi]; rows behind the last repeat it
+  const int row = min(n, R - 1), tok = row / a.G, head = kvh * a.G + row % a.G;
+  const int hi = ctx + tok, lo = a.window > 0 ? max(0, hi - a.window + 1) : 0;
+  u32x4 qf[NS];
+  {
+    const uint16_t *q = static_cast<const uint16_t *>(a.q) + (q0 + tok) * a.q_stride +
+                        static_cast<int64_t>(head) * D + 8 * h;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) qf[s] = ldg<u32x4>(q + 16 * s);
+  }
+
+  f32x16 acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
+  float m = -__builtin_inff(), l = 0.0f;
+
+  const int kn = key_of_row(n);  // the key of a tile whose K this lane loads
+  const int32_t *table = a.table + static_cast<int64_t>(b) * a.table_width;
+  const int last_page = static_cast<int>(a.num_pages) - 1;
+  const int64_t page_elems = (static_cast<int64_t>(a.Hkv) * D) << sh;
+  const uint16_t *K = static_cast<const uint16_t *>(a.k) + ((static_cast<int64_t>(kvh) * D) << sh);
+  const uint16_t *V = static_cast<const uint16_t *>(a.v) + ((static_cast<int64_t>(kvh) * D) << sh);
+  const int wmax = a.table_width - 1;
+
+  for (int k0 = zbeg + 32 * wave; k0 < zend; k0 += 32 * kWaves) {
+    // the pages of the tile's two 16-key halves
+    const int pg0 = min(max(table[min(k0 >> sh, wmax)], 0), last_page);
+    const int pg1 = min(max(table[min((k0 + 16) >> sh, wmax)], 0), last_page);
+    const int64_t e0 = pg0 * page_elems, e1 = pg1 * page_elems;
+    u32x4 kf[NS], vf[2][ND];
+    {
+      const uint16_t *kp = K + (kn & 16 ? e1 : e0) + ((k0 + kn) & (P - 1)) * 8 + ((h * 8) << sh);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) kf[s] = ldg<u32x4>(kp + ((s * 16) << sh));
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const uint16_t *vp = V + (ks ? e1 : e0) +
+                             (((k0 + 16 * ks) & (P - 1)) + 8 * h) * D + n * 8;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) vf[ks][d] = ldg<u32x4>(vp + d * 256);
+      }
+    }
+    f32x16 s;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) s = T::mfma32(kf[i], qf[i], s);
+
+    const bool edge = k0 + 31 > ctx || (a.window > 0 && k0 < ctx + nq - a.window);
+    if (edge) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int key = k0 + 16 * (r >> 3) + 8 * h + (r & 7);
+        s[r] = key >= lo && key <= hi ? s[r] : -__builtin_inff();
+      }
+      // values that no row sees: the pages' unwritten slots among them
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const PieceMask pm = piece_mask(k0 + 16 * ks + 8 * h, lo0, kv - 1);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) vf[ks][d][j] &= pm.m[j];
+      }
+    }
+    float mt = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mt = fmaxf(mt, s[r]);
+    mt = halves_max(mt);
+    if (__any((mt - m) * a.c > kLag)) {
+      const float mn = fmaxf(m, mt);
+      const float w = mn == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * a.c);
+      l *= w;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] *= w;
+      m = mn;
+    }
+    const float mc = m == -__builtin_inff() ? 0.0f : m * a.c - T::kShift;
+    u32x4 pf[2];
+    float sum = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -mc));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], a.c, -mc));
+      sum += p0 + p1;
+      pf[r >> 3][(r & 7) >> 1] = T::pack(p0, p1);
+    }
+    l += sum;
+
+    bool apart = false;  // an infinity or NaN in V that some rows see and others do not
+    if (edge && nq > 1) {
+      f32x16 probe;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) probe[r] = 0.0f;
+      const u32x4 zero = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) probe = T::mfma32(vf[ks][d], zero, probe);
+      float any = probe[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) any += probe[r];
+      apart = __any(any != 0.0f);
+    }
+    if (!apart) {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[d] = T::mfma32(vf[ks][d], pf[ks], acc[d]);
+    } else {
+      // key by key, so that a row takes only the values that it sees
+#pragma unroll 1
+      for (int i = 0; i < 32; ++i) {
+        const int key = k0 + i, w = (i & 7) >> 1;
+        const u32x4 pk = i < 16 ? pf[0] : pf[1];
+        const uint32_t pd = w == 0 ? pk[0] : w == 1 ? pk[1] : w == 2 ? pk[2] : pk[3];
+        const uint32_t mine = (pd >> (16 * (i & 1))) & 0xFFFFu;
+        const float p = T::value(static_cast<uint32_t>(
+            __shfl(static_cast<int>(mine), n + 32 * ((i >> 3) & 1))));
+        if (key < lo0 || key >= kv) continue;
+        const bool seen = key >= lo && key <= hi;
+        const uint16_t *vp = V + (i < 16 ? e0 : e1) + ((key & (P - 1)) & ~7) * D + (key & 7);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float v = T::value(vp[(32 * d + 8 * (r >> 2) + 4 * h + (r & 3)) * 8]);
+            acc[d][r] = seen ? __builtin_fmaf(p, v, acc[d][r]) : acc[d][r];
+          }
+      }
+    }
+  }
+
+  // the four waves' sums, in the waves' order
+  l = halves_sum(l);
+  if (h == 0) {
+    red_m[wave][n] = m;
+    red_l[wave][n] = l;
+  }
+  __syncthreads();
+  float top = red_m[0][n];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) top = fmaxf(top, red_m[w][n]);
+  const float scale = weight(m, top, a.c);
+  if (n < R) {
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        f32x4 v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = acc[d][4 * g + r] * scale;
+        __builtin_memcpy(red + ((wave * (D / 4) + 8 * d + 2 * g + h) * R + n) * 4, &v, 16);
+      }
+  }
+  float lt = 0.0f;  // of row n
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const float mw = red_m[w][n];
+    lt += red_l[w][n] * weight(mw, top, a.c);
+  }
+  __syncthreads();  // all waves have read red_m / red_l
+  if (wave == 0 && h == 0) {
+    red_m[0][n] = top;
+    red_l[0][n] = lt;
+  }
+  __syncthreads();
+
+  const int elems = R * (D / 4);  // groups of four dims of a row
+  const int head0 = kvh * a.G;
+  if (ns == 1) {
+    for (int i = tid; i < elems; i += 256) {
+      const int r = i % R, d4 = i / R;
+      f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) v += ldg<f32x4>(red + ((w * (D / 4) + d4) * R + r) * 4);
+      const int t = r / a.G;
+      // a row that sees no key is 0; one whose keys all weigh nothing is not a number
+      const float inv = ctx + t < 0 ? 0.0f : 1.0f / red_l[0][r];
+      v = ctx + t < 0 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : v * inv;
+      char *o = static_cast<char *>(a.out) +
+                ((q0 + t) * a.out_stride + static_cast<int64_t>(head0 + r % a.G) * D) *
+                    dtype_bytes(a.out_dtype);
+      store4(o, a.out_dtype, d4 * 4, v);
+    }
+    return;
+  }
+
+  // split: this chunk's sums to its slot, (m, l) of its rows behind them
+  const rsrc_t part = make_rsrc(a.part, a.part_bytes);
+  const uint32_t slot_bytes = lds_rows * (D + 4) * 4;
+  const uint32_t slot0 = static_cast<uint32_t>((b * a.Hkv + kvh) * a.splits) * slot_bytes;
+  const uint32_t slot = slot0 + z * slot_bytes;
+  for (int i = tid; i < elems; i += 256) {
+    const int r = i % R, d4 = i / R;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) v += ldg<f32x4>(red + ((w * (D / 4) + d4) * R + r) * 4);
+    st_dev4(part, slot + i * 16, v);
+  }
+  if (tid < R) st_dev4(part, slot + (elems + tid) * 16, f32x4{red_m[0][tid], red_l[0][tid], 0.0f, 0.0f});
+  wait_own_memory();
+  uint32_t *cnt = a.cnt + b * a.Hkv + kvh;
+  if (!split_arrive_last(cnt, ns)) return;
+  // every chunk's (m, l) to LDS, then each row's total and the chunks' weights
+  float *ml = red;  // [row + R * chunk][2]: the waves' sums are no longer needed
+  for (int i = tid; i < R * ns; i += 256) {
+    const int y = i / R;
+    const f32x4 v = ld_dev4(part, slot0 + y * slot_bytes + (elems + i - y * R) * 16);
+    ml[2 * i] = v.x;
+    ml[2 * i + 1] = v.y;
+  }
+  __syncthreads();
+  if (tid < R) {
+    float mx = -__builtin_inff(), sum = 0.0f;
+    for (int y = 0; y < ns; ++y) mx = fmaxf(mx, ml[2 * (y * R + tid)]);
+    for (int y = 0; y < ns; ++y) sum += ml[2 * (y * R + tid) + 1] * weight(ml[2 * (y * R + tid)], mx, a.c);
+    red_m[0][tid] = mx;
+    red_l[0][tid] = 1.0f / sum;
+  }
+  __syncthreads();
+  for (int i = tid; i < R * ns; i += 256) {
+    const int r = i % R;
+    ml[2 * i] = weight(ml[2 * i], red_m[0][r], a.c) * red_l[0][r];
+  }
+  __syncthreads();
+  for (int i = tid; i < elems; i += 256) {
+    const int r = i % R, d4 = i / R, t = r / a.G;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int y = 0; y < ns; ++y) v += ld_dev4(part, slot0 + y * slot_bytes + i * 16) * ml[2 * (y * R + r)];
+    if (ctx + t < 0) v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    char *o = static_cast<char *>(a.out) +
+              ((q0 + t) * a.out_stride + static_cast<int64_t>(head0 + r % a.G) * D) *
+                  dtype_bytes(a.out_dtype);
+    store4(o, a.out_dtype, d4 * 4, v);
+  }
+  split_reset(cnt);
+}
+
+namespace {
+template <int DT, int D>
+hipError_t launch_rows(const AttnArgs &a, int max_rows, hipStream_t s) {
+  constexpr int row_bytes = kWaves * D * 4;  // LDS of a row: the waves' sums
+  if constexpr (row_bytes * kRowsMax > 65536) {
+    static std::atomic<uint64_t> done{0};
+    if (!dry_run()) {
+      const hipError_t e = allow_lds(reinterpret_cast<const void *>(&k_attn_rows<DT, D>),
+                                     row_bytes * kRowsMax, done);
+      if (e != hipSuccess) return e;
+    }
+  }
+  IFX_LAUNCH(k_attn_rows, (DT, D), dim3(a.Hkv, a.B, a.splits), dim3(64 * kWaves),
+             static_cast<size_t>(row_bytes) * max_rows, s, a, max_rows);
+  return last_error();
+}
+template <int DT>
+hipError_t launch_rows(const AttnArgs &a, int D, int max_rows, hipStream_t s) {
+  switch (D) {
+    case 64: return launch_rows<DT, 64>(a, max_rows, s);
+    case 96: return launch_rows<DT, 96>(a, max_rows, s);
+    case 128: return launch_rows<DT, 128>(a, max_rows, s);
+    default: return launch_rows<DT, 256>(a, max_rows, s);
+  }
+}
+}  // namespace
+
+hipError_t launch_attn_rows(const AttnArgs &a, int dtype, int D, int max_rows, hipStream_t s) {
+  return dtype == IFX_ATTN_F16 ? launch_rows<IFX_ATTN_F16>(a, D, max_rows, s)
+                               : launch_rows<IFX_ATTN_BF16>(a, D, max_rows, s);
+}
+
+}  // namespace ifx
