@@ -124,7 +124,7 @@ int ifx_attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cac
  * q [T][Hq][D], k and v [T][Hkv][D], rows cu_len[b] .. cu_len[b + 1] - 1 are
  * prompt b.  Row i of a prompt of n sees its rows j < n, and j <= i where
  * causal, and j > i - window where causal and window > 0.  Otherwise as
- * ifx_attn_paged.  max_len bounds the prompts' lengths (0 < max_len): the
+ * ifx_attn_paged; k_stride, v_stride < 2^23.  max_len bounds the prompts' lengths (0 < max_len): the
  * launch is planned for it. */
 int ifx_attn_prompt(const void *q, int64_t q_stride, const void *k, int64_t k_stride,
                     const void *v, int64_t v_stride, int dtype, const int32_t *cu_len, int B,

@@ -210,7 +210,10 @@ int ifx_attn_prompt(const void *q, int64_t q_stride, const void *k, int64_t k_st
       !(scale > 0.0f) || !std::isfinite(scale))
     return IFX_BAD_GEOMETRY;
   const int64_t qn = static_cast<int64_t>(Hq) * D, kn = static_cast<int64_t>(Hkv) * D;
-  if (q_stride < qn || k_stride < kn || v_stride < kn || out_stride < qn) return IFX_BAD_GEOMETRY;
+  // 64 rows of K or V are addressed by 32-bit offsets
+  if (q_stride < qn || k_stride < kn || v_stride < kn || out_stride < qn ||
+      k_stride >= (1 << 23) || v_stride >= (1 << 23))
+    return IFX_BAD_GEOMETRY;
   if (T == 0) return IFX_OK;
   if (!q || !k || !v || !cu_len || !out) return IFX_NULL_POINTER;
   AttnArgs a{};

@@ -33,6 +33,17 @@ constexpr int TK = kTileKeys;
 // lanes that a read serves at a time reach 16 different piece columns (256
 // bytes: all banks).  K's lanes differ in the row, V's transposing reads take
 // four rows of four neighbouring pieces.
+// 16 bytes a lane from memory to 64 consecutive places in LDS.
+__device__ __forceinline__ void to_lds(const void *from, u32x4 *to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                   (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+}
+
+__device__ __forceinline__ void to_lds(rsrc_t from, int voff, int soff, u32x4 *to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)to, 16,
+                                           voff, soff, 0, 0);
+}
+
 template <int D>
 __device__ __forceinline__ int swap_k(int m) {  // m: the A-operand row of the key
   return D == 64 ? (m >> 1) & 7 : D == 96 ? (m >> 2) & 3 : m & 15;
@@ -113,8 +124,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
     for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
   float m = -__builtin_inff(), l = 0.0f;
 
-  // ---- stages: loads to registers, then to LDS
-  u32x4 kreg[NL], vreg[NL];
+  // ---- stages: memory to LDS, 1 KB (64 pieces) an instruction
   const int sh = a.page_shift, P = 1 << sh;
   const int32_t *table = PAGED ? a.table + static_cast<int64_t>(b) * a.table_width : nullptr;
   const int wmax = a.table_width - 1, last_page = static_cast<int>(a.num_pages) - 1;
@@ -125,92 +135,115 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
   const uint16_t *V = static_cast<const uint16_t *>(a.v) +
                       (PAGED ? (static_cast<int64_t>(kvh) * D) << sh
                              : q0 * a.v_stride + static_cast<int64_t>(kvh) * D);
-  auto page_of = [&](int k0) {  // of key k0 + lane
-    return min(max(table[min((k0 + lane) >> sh, wmax)], 0), last_page);
-  };
-  auto load = [&](int k0, int page) {
+  // packed rows: where the piece that this lane loads first lies in a stage.
+  // Its next ones lie whole groups of rows further, 16 or 32, with the same
+  // exchange of pieces (kSame)
+  constexpr bool kSame = D == 64 || D == 128;
+  const int k_row = static_cast<int>(a.k_stride) * 2, v_row = static_cast<int>(a.v_stride) * 2;
+  int k_off = 0, v_off = 0;
+  if constexpr (!PAGED && kSame) {
+    const int p = wave * 64 + lane, key = p / NP, c = p - key * NP;
+    k_off = key * k_row + (c ^ swap_k<D>(key_of_row(key))) * 16;
+    v_off = key * v_row + (c ^ swap_v<D>(key)) * 16;
+  }
+  // of key k0 + lane, as the table has it: it is read a stage ahead and looked
+  // at only when that stage's loads are issued
+  auto entry_of = [&](int k0) { return table[min((k0 + lane) >> sh, wmax)]; };
+  auto load = [&](int k0, int entry, int buf) {
+    const int page = min(max(entry, 0), last_page);
+    u32x4 *sk = lds + buf * 2 * kPieces, *sv = sk + kPieces;
     if constexpr (PAGED) {
       const uint16_t *kp = K + page * page_elems + ((k0 + lane) & (P - 1)) * 8;
 #pragma unroll
-      for (int i = 0; i < NL; ++i)  // piece (NP / NL ... ): 64 keys of one dim group
-        kreg[i] = ldg<u32x4>(kp + (static_cast<int64_t>((i * kNW + wave) * 8) << sh));
+      for (int i = 0; i < NL; ++i) {  // the 64 keys' pieces of one dim group
+        const int c = i * kNW + wave;
+        to_lds(kp + (static_cast<int64_t>(c * 8) << sh), sk + c * TK);
+      }
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const int p = i * 64 * kNW + tid, g = p / D, dim = p - g * D;
-        const int64_t e = __shfl(page, 8 * g) * page_elems;
-        vreg[i] = ldg<u32x4>(V + e + ((k0 + 8 * g) & (P - 1)) * D + dim * 8);
-      }
-      if (k0 + TK > kv) {  // slots behind the last token: no value may come from them
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-          const int key = k0 + 8 * ((i * 64 * kNW + tid) / D);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            vreg[i][j] &= (key + 2 * j < kv ? 0xFFFFu : 0u) | (key + 2 * j + 1 < kv ? 0xFFFF0000u : 0u);
+        const int p0 = (i * kNW + wave) * 64;
+        if constexpr (D % 64 == 0) {  // 64 dims of one key group
+          const int g = p0 / D;
+          const int64_t e = __builtin_amdgcn_readlane(page, 8 * g) * page_elems;
+          const uint16_t *vp = V + e + ((k0 + 8 * g) & (P - 1)) * D + (p0 - g * D) * 8;
+          to_lds(vp + lane * 8, sv + p0);
+        } else {
+          const int p = p0 + lane, g = p / D, dim = p - g * D;
+          const int64_t e = __shfl(page, 8 * g) * page_elems;
+          to_lds(V + e + ((k0 + 8 * g) & (P - 1)) * D + dim * 8, sv + p0);
         }
       }
     } else {
+      // Ranges of the stage's rows: rows behind the request's last read as 0.
+      // 64 places in order, each with the piece that belongs there.
+      const int rows = min(kv - k0, TK);
+      const rsrc_t rk = make_rsrc(K + k0 * a.k_stride, rows * k_row);
+      const rsrc_t rv = make_rsrc(V + k0 * a.v_stride, rows * v_row);
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const int p = i * 64 * kNW + tid, key = p / NP, c = p - key * NP;
-        const int64_t r = min(k0 + key, kv - 1);
-        kreg[i] = ldg<u32x4>(K + r * a.k_stride + c * 8);
-        vreg[i] = ldg<u32x4>(V + r * a.v_stride + c * 8);
-      }
-    }
-  };
-  auto store = [&](int buf) {
-    u32x4 *sk = lds + buf * 2 * kPieces, *sv = sk + kPieces;
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int p = i * 64 * kNW + tid;
-      if constexpr (PAGED) {
-        sk[p] = kreg[i];
-        sv[p] = vreg[i];
-      } else {
-        const int key = p / NP, c = p - key * NP;
-        sk[key * NP + (c ^ swap_k<D>(key_of_row(key & 31)))] = kreg[i];
-        sv[key * NP + (c ^ swap_v<D>(key))] = vreg[i];
+        const int p0 = (i * kNW + wave) * 64;
+        if constexpr (kSame) {
+          to_lds(rk, k_off, i * (kNW * 64 / NP) * k_row, sk + p0);
+          to_lds(rv, v_off, i * (kNW * 64 / NP) * v_row, sv + p0);
+        } else {
+          const int p = p0 + lane, key = p / NP, c = p - key * NP;
+          to_lds(rk, key * k_row + (c ^ swap_k<D>(key_of_row(key & 31))) * 16, 0, sk + p0);
+          to_lds(rv, key * v_row + (c ^ swap_v<D>(key)) * 16, 0, sv + p0);
+        }
       }
     }
   };
 
   // ---- operands from LDS
-  const int kn = key_of_row(n);
-  auto k_at = [&](const u32x4 *sk, int sub, int s) {
-    const int key = 32 * sub + kn, c = 2 * s + h;
-    return PAGED ? sk[c * TK + key] : sk[key * NP + (c ^ swap_k<D>(n))];
+  // Byte offsets of this lane's pieces; what changes with the step, dim tile or
+  // key group is an immediate, or exclusive-ored in where pieces are exchanged.
+  const int kn = key_of_row(n), ti = lane & 15;
+  int k_lane, k_swap, v_lane, v_swap;
+  if constexpr (PAGED) {
+    k_lane = (h * TK + kn) * 16, k_swap = 0;
+    v_lane = (h * D + n) * 16, v_swap = 0;
+  } else {
+    k_lane = kn * NP * 16, k_swap = (h ^ swap_k<D>(n)) * 16;
+    // V is read transposing: each group of 16 lanes reads four rows of 16 dims
+    // and gets four keys of one dim a lane
+    v_lane = (8 * h + (ti >> 2)) * NP * 16 + ((lane & 16) >> 3) * 16 + (ti & 3) * 8;
+    v_swap = swap_v<D>(ti >> 2) * 16;
+  }
+  auto k_at = [&](const char *sk, int sub, int s) {
+    const char *p = PAGED ? sk + (k_lane + (2 * s * TK + 32 * sub) * 16)
+                          : sk + ((k_swap ^ (32 * s)) + k_lane) + 32 * sub * NP * 16;
+    return *reinterpret_cast<const u32x4 *>(p);
   };
-  auto v_at = [&](const u32x4 *sv, int ks, int d) -> u32x4 {
+  auto v_at = [&](const char *sv, int ks, int d) -> u32x4 {
     if constexpr (PAGED) {
-      return sv[(2 * ks + h) * D + 32 * d + n];
+      return *reinterpret_cast<const u32x4 *>(sv + (v_lane + (2 * ks * D + 32 * d) * 16));
     } else {
-      // each group of 16 lanes reads four rows of 16 dims and gets, transposed,
-      // four keys of one dim a lane
       typedef short s16x4 __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) s16x4 *lds4;
-      const int i = lane & 15, dim = 32 * d + (lane & 16) + 4 * (i & 3);
-      u32x4 r;
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const int key = 16 * ks + 8 * h + 4 * w + (i >> 2);
-        const u32x4 *piece = sv + key * NP + ((dim >> 3) ^ swap_v<D>(key));
-        const u32x2 t = __builtin_bit_cast(
-            u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                       (lds4)(reinterpret_cast<const char *>(piece) + 8 * (i & 1))));
-        r[2 * w] = t.x;
-        r[2 * w + 1] = t.y;
-      }
-      return r;
+      const char *p = sv + ((v_swap ^ (64 * d)) + v_lane) + 16 * ks * NP * 16;
+      const u32x2 t = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p));
+      const u32x2 u = __builtin_bit_cast(
+          u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 4 * NP * 16)));
+      return u32x4{t.x, t.y, u.x, u.y};
     }
   };
-  auto v_one = [&](const u32x4 *sv, int key, int dim) {  // one value, for the rare path
-    const uint16_t *e = reinterpret_cast<const uint16_t *>(
-        PAGED ? sv + (key >> 3) * D + dim : sv + key * NP + ((dim >> 3) ^ swap_v<D>(key)));
-    return T::value(e[PAGED ? key & 7 : dim & 7]);
+  // the same without what lies behind the last token: a page's unwritten slots
+  auto v_in = [&](int k0, const char *sv, int ks, int d) -> u32x4 {
+    u32x4 r = v_at(sv, ks, d);
+    if constexpr (PAGED) {
+      const int key = k0 + 16 * ks + 8 * h;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        r[j] &= (key + 2 * j < kv ? 0xFFFFu : 0u) | (key + 2 * j + 1 < kv ? 0xFFFF0000u : 0u);
+    }
+    return r;
+  };
+  auto v_one = [&](const char *sv, int key, int dim) {  // one value, for the rare path
+    const int piece = PAGED ? (key >> 3) * D + dim : key * NP + ((dim >> 3) ^ swap_v<D>(key));
+    return T::value(reinterpret_cast<const uint16_t *>(sv + piece * 16)[PAGED ? key & 7 : dim & 7]);
   };
 
-  auto step = [&](int k0, const u32x4 *sk, const u32x4 *sv, auto edge_c) {
+  auto step = [&](int k0, const char *sk, const char *sv, auto edge_c) {
     constexpr bool EDGE = decltype(edge_c)::value;
     f32x16 s[2];
 #pragma unroll
@@ -266,7 +299,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-        for (int d = 0; d < ND; ++d) probe = T::mfma32(v_at(sv, ks, d), zero, probe);
+        for (int d = 0; d < ND; ++d) probe = T::mfma32(v_in(k0, sv, ks, d), zero, probe);
       float any = probe[0];
 #pragma unroll
       for (int r = 1; r < 16; ++r) any += probe[r];
@@ -294,31 +327,31 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-      for (int d = 0; d < ND; ++d) acc[d] = T::mfma32(v_at(sv, ks, d), pf[ks], acc[d]);
+      for (int d = 0; d < ND; ++d)
+        acc[d] = T::mfma32(EDGE ? v_in(k0, sv, ks, d) : v_at(sv, ks, d), pf[ks], acc[d]);
   };
 
   if (zbeg < zend) {
-    int page = 0;
-    if constexpr (PAGED) page = page_of(zbeg);
-    load(zbeg, page);
-    if constexpr (PAGED) page = page_of(zbeg + TK);
-    store(0);
+    int entry = 0;
+    if constexpr (PAGED) entry = entry_of(zbeg);
+    load(zbeg, entry, 0);
+    if constexpr (PAGED) entry = entry_of(zbeg + TK);
     int buf = 0;
     for (int k0 = zbeg; k0 < zend; k0 += TK, buf ^= 1) {
+      wait_own_memory();
       __syncthreads();  // this stage is in LDS, and no wave reads the other one
-      const bool more = k0 + TK < zend;
-      if (more) {
-        load(k0 + TK, page);
-        if constexpr (PAGED) page = page_of(k0 + 2 * TK);
+      if (k0 + TK < zend) {
+        load(k0 + TK, entry, buf ^ 1);
+        if constexpr (PAGED) entry = entry_of(k0 + 2 * TK);
       }
-      const u32x4 *sk = lds + buf * 2 * kPieces, *sv = sk + kPieces;
+      const char *sk = reinterpret_cast<const char *>(lds + buf * 2 * kPieces);
+      const char *sv = sk + kPieces * 16;
       if (k0 <= hi_z && k0 + TK > lo_a) {
         if (k0 >= lo_z && k0 + TK - 1 <= hi_a)
           step(k0, sk, sv, std::false_type{});
         else
           step(k0, sk, sv, std::true_type{});
       }
-      if (more) store(buf ^ 1);
     }
   }
 
