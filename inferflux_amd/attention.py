@@ -39,48 +39,52 @@ _ELEMS = (torch.float16, torch.bfloat16)
 BatchPlan = namedtuple("BatchPlan", "cu_q kv_len positions slots free_left status")
 
 
-class _on:
-    """Makes `device` the current one for a launch, if it is not."""
-
-    def __init__(self, device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-
-
-def _stream(device, stream):
+def _launch(fn, what, device, stream, *args):
+    """Calls a C entry point on `stream` or the current one of device number
+    `device`, which is made the current device for the call if it is not."""
     if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream
-    if stream.device != device:
-        raise ValueError(f"the stream is of {stream.device}, the tensors of {device}")
-    return stream.cuda_stream
+        raw = torch._C._cuda_getCurrentRawStream(device)
+    elif stream.device_index != device:
+        raise ValueError(f"the stream is of cuda:{stream.device_index}, the tensors of cuda:{device}")
+    else:
+        raw = stream.cuda_stream
+    if device == torch._C._cuda_getDevice():
+        rc = fn(*args, raw)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, raw)
+    if rc:
+        _check(rc, what)
 
 
-def _new(shape, dtype, device, stream):
+def _device(t, name):
+    """Number of the GPU that t is on; the other tensors of a call are held to it."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a device tensor")
+    return t.get_device()
+
+
+def _new(shape, dtype, like, stream):
     """An output of a call: the allocator is told of a stream that is not the
     current one, so that it does not hand the memory out while in use there."""
-    t = torch.empty(shape, dtype=dtype, device=device)
+    t = torch.empty(shape, dtype=dtype, device=like.device)
     if stream is not None:
         t.record_stream(stream)
     return t
 
 
-def _same_device(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} must be on {device}")
+def _on(t, name, device):
+    if t.get_device() != device:
+        raise ValueError(f"{name} must be on cuda:{device}")
+    return t
 
 
-def _i32(t, name, n):
-    if t.dtype != torch.int32:
+def _i32(t, name, n, device):
+    if t.dtype is not torch.int32:
         raise TypeError(f"{name} must be int32")
-    if not t.is_contiguous() or t.numel() < n:
+    if t.get_device() != device:
+        raise ValueError(f"{name} must be on cuda:{device}")
+    if t.numel() < n or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous with at least {n} values")
     return t.data_ptr()
 
@@ -88,29 +92,28 @@ def _i32(t, name, n):
 def _rows(t, name, T, H, D):
     """Pointer and row stride of rows [T, H, D]: heads of D values one after
     the other, rows any distance apart."""
-    if t.dim() != 3 or t.shape[0] != T or t.shape[1] != H or t.shape[2] != D:
+    if tuple(t.shape) != (T, H, D):
         raise ValueError(f"{name} must be [{T}, {H}, {D}], got {list(t.shape)}")
-    st = t.stride()
-    if T == 0:
-        return t.data_ptr(), H * D
-    if (D > 1 and st[2] != 1) or (H > 1 and st[1] != D):
+    row, head, one = t.stride()
+    if T <= 1:
+        row = H * D
+    if T and ((one != 1 and D > 1) or (head != D and H > 1)):
         raise ValueError(f"{name}: a row's heads must lie one after the other")
-    return t.data_ptr(), (st[0] if T > 1 else H * D)
+    return t.data_ptr(), row
 
 
 def _caches(k_cache, v_cache):
     """(pages, kv heads, page size, head size) of a layer's caches."""
-    if k_cache.dtype not in _ELEMS or v_cache.dtype != k_cache.dtype:
+    if k_cache.dtype not in _ELEMS or v_cache.dtype is not k_cache.dtype:
         raise TypeError("the caches must be float16 or bfloat16, both the same")
-    if k_cache.dim() != 5 or v_cache.dim() != 5:
-        raise ValueError("the caches must be as kv_cache makes them")
-    n, h, d8, p, e = k_cache.shape
-    if e != 8 or tuple(v_cache.shape) != (n, h, p // 8, d8 * 8, 8):
-        raise ValueError("the caches must be as kv_cache makes them: [pages, heads, D / 8, page, 8] "
-                         "and [pages, heads, page / 8, D, 8]")
-    if not k_cache.is_contiguous() or not v_cache.is_contiguous():
-        raise ValueError("the caches must be contiguous")
-    return n, h, p, d8 * 8
+    if k_cache.dim() == 5 and v_cache.dim() == 5:
+        n, h, d8, p, e = k_cache.shape
+        if e == 8 and tuple(v_cache.shape) == (n, h, p // 8, d8 * 8, 8):
+            if not k_cache.is_contiguous() or not v_cache.is_contiguous():
+                raise ValueError("the caches must be contiguous")
+            return n, h, p, d8 * 8
+    raise ValueError("the caches must be as kv_cache makes them: [pages, heads, D / 8, page, 8] "
+                     "and [pages, heads, page / 8, D, 8]")
 
 
 def kv_cache(num_pages, kv_heads, head_dim, page_size=64, dtype=torch.float16, device="cuda"):
@@ -143,27 +146,22 @@ def plan_batch(ctx_len, new_len, block_table, free_pages, free_count, page_size,
       last token: 0 and -1), free_left [1], status [1] (0, or a sum of
       NO_PAGES, NARROW, NO_ROOM, BAD_LENGTH: then nothing is taken, cu_q is 0
       and every slot -1)."""
-    dev, B = ctx_len.device, ctx_len.numel()
-    if not ctx_len.is_cuda:
-        raise ValueError("ctx_len must be a device tensor")
+    dev, B = _device(ctx_len, "ctx_len"), ctx_len.numel()
     if block_table.dim() != 2 or block_table.shape[0] != B:
         raise ValueError("block_table must be [B, pages]")
     if out is None:
-        out = BatchPlan(*(_new(n, torch.int32, dev, stream)
-                          for n in (B + 1, B, max_tokens, max_tokens, 1, 1)))
-    _same_device(dev, new_len=new_len, block_table=block_table, free_pages=free_pages,
-                 free_count=free_count, **out._asdict())
+        n = (B + 1, B, max_tokens, max_tokens, 1, 1)
+        out = BatchPlan(*_new(sum(n), torch.int32, ctx_len, stream).split(n))
     W = block_table.shape[1]
-    with _on(dev):
-        rc = _lib.load().ifx_plan_batch(
-            _i32(ctx_len, "ctx_len", B), _i32(new_len, "new_len", B),
-            _i32(block_table, "block_table", B * W), W, _i32(free_pages, "free_pages", 0),
-            free_pages.numel(), _i32(free_count, "free_count", 1), page_size, B, max_tokens,
-            _i32(out.cu_q, "cu_q", B + 1), _i32(out.kv_len, "kv_len", B),
-            _i32(out.positions, "positions", max_tokens), _i32(out.slots, "slots", max_tokens),
-            _i32(out.free_left, "free_left", 1), _i32(out.status, "status", 1),
-            _stream(dev, stream))
-    _check(rc, "ifx_plan_batch")
+    _launch(_lib.load().ifx_plan_batch, "ifx_plan_batch", dev, stream,
+            _i32(ctx_len, "ctx_len", B, dev), _i32(new_len, "new_len", B, dev),
+            _i32(block_table, "block_table", B * W, dev), W,
+            _i32(free_pages, "free_pages", 0, dev), free_pages.numel(),
+            _i32(free_count, "free_count", 1, dev), page_size, B, max_tokens,
+            _i32(out.cu_q, "cu_q", B + 1, dev), _i32(out.kv_len, "kv_len", B, dev),
+            _i32(out.positions, "positions", max_tokens, dev),
+            _i32(out.slots, "slots", max_tokens, dev),
+            _i32(out.free_left, "free_left", 1, dev), _i32(out.status, "status", 1, dev))
     return out
 
 
@@ -176,43 +174,38 @@ def rope_append(q, k, v, positions, slots, k_cache, v_cache, inv_freq=None, inte
     [rot_dim / 2] on the device, None for no rotation.  Tokens whose slot is
     outside the cache (-1) are left out, their rows of q_out as well."""
     n, Hkv, P, D = _caches(k_cache, v_cache)
-    dev = k_cache.device
-    if not k_cache.is_cuda:
-        raise ValueError("k_cache must be a device tensor")
+    dev = _device(k_cache, "k_cache")
     if q.dim() != 3:
         raise ValueError("q must be [T, Hq, D]")
     T, Hq = q.shape[0], q.shape[1]
     src = _DTYPES.get(q.dtype)
-    if src is None or k.dtype != q.dtype or v.dtype != q.dtype:
+    if src is None or k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise TypeError("q, k and v must be float32, float16 or bfloat16, all the same")
-    rot = 0
+    rot, freq = 0, None
     if inv_freq is not None:
-        if inv_freq.dtype != torch.float64 or not inv_freq.is_contiguous():
+        if inv_freq.dtype is not torch.float64 or not inv_freq.is_contiguous():
             raise TypeError("inv_freq must be contiguous float64")
-        rot = 2 * inv_freq.numel()
+        rot, freq = 2 * inv_freq.numel(), _on(inv_freq, "inv_freq", dev).data_ptr()
     if q_out is None:
-        q_out = _new((T, Hq, D), k_cache.dtype, dev, stream)
-    elif q_out.dtype != k_cache.dtype:
+        q_out = _new((T, Hq, D), k_cache.dtype, k_cache, stream)
+    elif q_out.dtype is not k_cache.dtype:
         raise TypeError("q_out must have the caches' type")
-    _same_device(dev, q=q, k=k, v=v, positions=positions, slots=slots, v_cache=v_cache,
-                 inv_freq=inv_freq, q_out=q_out)
+    for t, name in ((q, "q"), (k, "k"), (v, "v"), (v_cache, "v_cache"), (q_out, "q_out")):
+        _on(t, name, dev)
     qp, qs = _rows(q, "q", T, Hq, D)
     kp, ks = _rows(k, "k", T, Hkv, D)
     vp, vs = _rows(v, "v", T, Hkv, D)
     op, os = _rows(q_out, "q_out", T, Hq, D)
-    with _on(dev):
-        rc = _lib.load().ifx_rope_append(
-            qp, qs, kp, ks, vp, vs, src, _i32(positions, "positions", T), _i32(slots, "slots", T),
-            inv_freq.data_ptr() if rot else None, rot, int(bool(interleaved)), T, Hq, Hkv, D, op,
-            os, k_cache.data_ptr(), v_cache.data_ptr(), _DTYPES[k_cache.dtype], n, P,
-            _stream(dev, stream))
-    _check(rc, "ifx_rope_append")
+    _launch(_lib.load().ifx_rope_append, "ifx_rope_append", dev, stream, qp, qs, kp, ks, vp, vs, src,
+            _i32(positions, "positions", T, dev), _i32(slots, "slots", T, dev), freq, rot,
+            1 if interleaved else 0, T, Hq, Hkv, D, op, os, k_cache.data_ptr(), v_cache.data_ptr(),
+            _DTYPES[k_cache.dtype], n, P)
     return q_out
 
 
 def _out(q, out, out_dtype, stream):
     if out is None:
-        return _new(q.shape, out_dtype or q.dtype, q.device, stream)
+        return _new(q.shape, out_dtype or q.dtype, q, stream)
     if out.dtype not in _DTYPES or (out_dtype is not None and out.dtype != out_dtype):
         raise TypeError("out must be float32, float16 or bfloat16, and of out_dtype if that is given")
     return out
@@ -235,10 +228,10 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_q, kv_len, max_q, max_k
     its rows from cu_q[B] on are left as they were.  workspace: see
     `workspace` and paged_workspace_bytes."""
     n, Hkv, P, D = _caches(k_cache, v_cache)
-    dev = q.device
-    if not q.is_cuda or q.dim() != 3:
-        raise ValueError("q must be a device tensor [T, Hq, D]")
-    if q.dtype != k_cache.dtype:
+    dev = _device(q, "q")
+    if q.dim() != 3:
+        raise ValueError("q must be [T, Hq, D]")
+    if q.dtype is not k_cache.dtype:
         raise TypeError("q must have the caches' type")
     T, Hq = q.shape[0], q.shape[1]
     B = kv_len.numel()
@@ -246,23 +239,20 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_q, kv_len, max_q, max_k
         raise ValueError("block_table must be [B, pages]")
     W = block_table.shape[1]
     out = _out(q, out, out_dtype, stream)
-    _same_device(dev, k_cache=k_cache, v_cache=v_cache, block_table=block_table, cu_q=cu_q,
-                 kv_len=kv_len, out=out, workspace=workspace)
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache"), (out, "out")):
+        _on(t, name, dev)
     qp, qs = _rows(q, "q", T, Hq, D)
     op, os = _rows(out, "out", T, Hq, D)
     wp, wn = None, 0
     if workspace is not None:
         if not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous")
-        wp, wn = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    with _on(dev):
-        rc = _lib.load().ifx_attn_paged(
-            qp, qs, _DTYPES[q.dtype], k_cache.data_ptr(), v_cache.data_ptr(), n, P,
-            _i32(block_table, "block_table", B * W), W, _i32(cu_q, "cu_q", B + 1),
-            _i32(kv_len, "kv_len", B), B, T, Hq, Hkv, D, max_q, max_kv,
-            D ** -0.5 if scale is None else scale, window, op, os, _DTYPES[out.dtype], wp, wn,
-            _stream(dev, stream))
-    _check(rc, "ifx_attn_paged")
+        wp, wn = _on(workspace, "workspace", dev).data_ptr(), workspace.nbytes
+    _launch(_lib.load().ifx_attn_paged, "ifx_attn_paged", dev, stream, qp, qs, _DTYPES[q.dtype],
+            k_cache.data_ptr(), v_cache.data_ptr(), n, P,
+            _i32(block_table, "block_table", B * W, dev), W, _i32(cu_q, "cu_q", B + 1, dev),
+            _i32(kv_len, "kv_len", B, dev), B, T, Hq, Hkv, D, max_q, max_kv,
+            D ** -0.5 if scale is None else scale, window, op, os, _DTYPES[out.dtype], wp, wn)
     return out
 
 
@@ -274,23 +264,22 @@ def prompt_attention(q, k, v, cu_len, max_len, causal=True, window=0, scale=None
     A row sees its prompt's rows; where causal those up to its own, the last
     `window` of them where window > 0.  Returns out [T, Hq, D] (out_dtype:
     fp32, fp16 or bf16, q's type if None)."""
-    dev = q.device
-    if not q.is_cuda or q.dim() != 3 or k.dim() != 3:
-        raise ValueError("q, k and v must be device tensors [T, heads, D]")
-    if q.dtype not in _ELEMS or k.dtype != q.dtype or v.dtype != q.dtype:
+    dev = _device(q, "q")
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError("q, k and v must be [T, heads, D]")
+    if q.dtype not in _ELEMS or k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise TypeError("q, k and v must be float16 or bfloat16, all the same")
     T, Hq, D = q.shape
     Hkv, B = k.shape[1], cu_len.numel() - 1
     out = _out(q, out, out_dtype, stream)
-    _same_device(dev, k=k, v=v, cu_len=cu_len, out=out)
+    for t, name in ((k, "k"), (v, "v"), (out, "out")):
+        _on(t, name, dev)
     qp, qs = _rows(q, "q", T, Hq, D)
     kp, ks = _rows(k, "k", T, Hkv, D)
     vp, vs = _rows(v, "v", T, Hkv, D)
     op, os = _rows(out, "out", T, Hq, D)
-    with _on(dev):
-        rc = _lib.load().ifx_attn_prompt(
-            qp, qs, kp, ks, vp, vs, _DTYPES[q.dtype], _i32(cu_len, "cu_len", B + 1), B, T, Hq, Hkv,
-            D, max_len, int(bool(causal)), window, D ** -0.5 if scale is None else scale, op, os,
-            _DTYPES[out.dtype], _stream(dev, stream))
-    _check(rc, "ifx_attn_prompt")
+    _launch(_lib.load().ifx_attn_prompt, "ifx_attn_prompt", dev, stream, qp, qs, kp, ks, vp, vs,
+            _DTYPES[q.dtype], _i32(cu_len, "cu_len", B + 1, dev), B, T, Hq, Hkv, D, max_len,
+            1 if causal else 0, window, D ** -0.5 if scale is None else scale, op, os,
+            _DTYPES[out.dtype])
     return out

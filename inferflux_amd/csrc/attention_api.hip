@@ -83,13 +83,14 @@ PagedPlan plan_paged(int B, int T, int Hq, int Hkv, int D, int max_q, int max_kv
     busy = (full > B ? full : B) * Hkv;
     slot = attn_tile_slot_bytes(D);
   }
-  int64_t splits = p.rows ? (1024 + busy - 1) / busy : (512 + busy - 1) / busy;
+  static const int R_=getenv("TR")?atoi(getenv("TR")):1024, T_=getenv("TT")?atoi(getenv("TT")):512, C_=getenv("TC")?atoi(getenv("TC")):512;
+  int64_t splits = p.rows ? (R_ + busy - 1) / busy : (T_ + busy - 1) / busy;
   if (splits > 128) splits = 128;
   const int64_t fit = (IFX_ATTN_WORKSPACE_BYTES - kCntBytes) / (units * slot);
   if (splits > fit) splits = fit;
   if (units > kMaxUnits || splits < 1) splits = 1;
   p.chunk = round_up((max_kv + splits - 1) / splits, unit);
-  if (!p.rows && splits > 1 && p.chunk < 512) p.chunk = 512;
+  if (!p.rows && splits > 1 && p.chunk < C_) p.chunk = C_;
   p.splits = splits > 1 ? (max_kv + p.chunk - 1) / p.chunk : 1;
   p.bytes = p.splits > 1 ? kCntBytes + units * p.splits * slot : 0;
   return p;

@@ -96,6 +96,9 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
   const int tok_a = row0 / a.G, tok_z = (min(row0 + kRows, R) - 1) / a.G;
   const int kend = a.causal ? ctx + tok_z + 1 : kv;
   const int kbeg = a.window > 0 ? max(0, ctx + tok_a - a.window + 1) & ~(TK - 1) : 0;
+  // stages [full_a, full_z) all of its rows see whole
+  const int full_a = a.window > 0 ? (max(0, ctx + tok_z - a.window + 1) + TK - 1) & ~(TK - 1) : 0;
+  const int full_z = max(0, a.causal ? ctx + tok_a + 1 : kv) & ~(TK - 1);
   const int chunk = split_chunk(a, kend - kbeg, TK);
   const int ns = kend > kbeg ? (kend - kbeg + chunk - 1) / chunk : 1;
   if (z >= ns) return;
@@ -106,9 +109,8 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
   const int head = kvh * a.G + row - tok * a.G;
   const int hi = a.causal ? ctx + tok : kv - 1;
   const int lo = a.window > 0 ? max(0, ctx + tok - a.window + 1) : 0;
-  // over the wave's rows: all see [lo_z, hi_a], some [lo_a, hi_z]
-  const int hi_a = __builtin_amdgcn_readlane(hi, 0), hi_z = __builtin_amdgcn_readlane(hi, 31);
-  const int lo_a = __builtin_amdgcn_readlane(lo, 0), lo_z = __builtin_amdgcn_readlane(lo, 31);
+  const int hi_z = __builtin_amdgcn_readlane(hi, 31);  // some of the wave's rows see [lo_a, hi_z]
+  const int lo_a = __builtin_amdgcn_readlane(lo, 0);
 
   u32x4 qf[NS];
   {
@@ -336,22 +338,32 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
     if constexpr (PAGED) entry = entry_of(zbeg);
     load(zbeg, entry, 0);
     if constexpr (PAGED) entry = entry_of(zbeg + TK);
-    int buf = 0;
-    for (int k0 = zbeg; k0 < zend; k0 += TK, buf ^= 1) {
-      wait_own_memory();
-      __syncthreads();  // this stage is in LDS, and no wave reads the other one
-      if (k0 + TK < zend) {
-        load(k0 + TK, entry, buf ^ 1);
-        if constexpr (PAGED) entry = entry_of(k0 + 2 * TK);
+    int k0 = zbeg, buf = 0;
+    auto stages = [&](int until, auto edge_c) {
+      for (; k0 < until; k0 += TK, buf ^= 1) {
+        wait_own_memory();
+        __syncthreads();  // this stage is in LDS, and no wave reads the other one
+        if (k0 + TK < zend) {
+          load(k0 + TK, entry, buf ^ 1);
+          if constexpr (PAGED) entry = entry_of(k0 + 2 * TK);
+        }
+        const char *sk = reinterpret_cast<const char *>(lds + buf * 2 * kPieces);
+        const char *sv = sk + kPieces * 16;
+        if constexpr (decltype(edge_c)::value) {
+          if (k0 <= hi_z && k0 + TK > lo_a) step(k0, sk, sv, edge_c);
+        } else {
+          step(k0, sk, sv, edge_c);
+        }
       }
-      const char *sk = reinterpret_cast<const char *>(lds + buf * 2 * kPieces);
-      const char *sv = sk + kPieces * 16;
-      if (k0 <= hi_z && k0 + TK > lo_a) {
-        if (k0 >= lo_z && k0 + TK - 1 <= hi_a)
-          step(k0, sk, sv, std::false_type{});
-        else
-          step(k0, sk, sv, std::true_type{});
-      }
+    };
+    // stages that all rows of the workgroup see whole, between those that some
+    // see in part: where windows begin, and at the causal end
+    int until = a.window > 0 ? min(full_a, zend) : zbeg;
+    while (true) {
+      stages(until, std::true_type{});
+      if (k0 >= zend) break;
+      stages(min(full_z, zend), std::false_type{});
+      until = zend;
     }
   }
 
