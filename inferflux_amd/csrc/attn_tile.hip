@@ -23,7 +23,8 @@ constexpr int kNW = 4;             // waves of a workgroup
 constexpr int kRows = 32 * kNW;    // its query rows
 constexpr int TK = kTileKeys;
 
-// LDS places, in 16-byte pieces of 8 values.
+// LDS places, in 16-byte pieces of 8 values.  Copies go from memory to LDS
+// past the registers.
 //
 // A paged stage is a copy of the cache's order: K [D / 8][64 keys], V
 // [8 key groups][D].  Lanes read neighbouring pieces.
@@ -99,10 +100,13 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
   // stages [full_a, full_z) all of its rows see whole
   const int full_a = a.window > 0 ? (max(0, ctx + tok_z - a.window + 1) + TK - 1) & ~(TK - 1) : 0;
   const int full_z = max(0, a.causal ? ctx + tok_a + 1 : kv) & ~(TK - 1);
-  const int chunk = split_chunk(a, kend - kbeg, TK);
-  const int ns = kend > kbeg ? (kend - kbeg + chunk - 1) / chunk : 1;
-  if (z >= ns) return;
-  const int zbeg = kbeg + z * chunk, zend = min(zbeg + chunk, kend);
+  int ns = 1, zbeg = kbeg, zend = kend;  // prompts are not split
+  if constexpr (PAGED) {
+    const int chunk = split_chunk(a, kend - kbeg, TK);
+    if (kend > kbeg) ns = (kend - kbeg + chunk - 1) / chunk;
+    if (z >= ns) return;
+    zbeg = kbeg + z * chunk, zend = min(zbeg + chunk, kend);
+  }
 
   // this lane's row sees [lo, hi]; rows behind the last repeat it
   const int row = min(row0 + 32 * wave + n, R - 1), tok = row / a.G;
@@ -176,13 +180,12 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
         }
       }
     } else {
-      // Ranges of the stage's rows: rows behind the request's last read as 0.
-      // 64 places in order, each with the piece that belongs there.
+      // the stage's rows; those behind the request's last read as 0
       const int rows = min(kv - k0, TK);
       const rsrc_t rk = make_rsrc(K + k0 * a.k_stride, rows * k_row);
       const rsrc_t rv = make_rsrc(V + k0 * a.v_stride, rows * v_row);
 #pragma unroll
-      for (int i = 0; i < NL; ++i) {
+      for (int i = 0; i < NL; ++i) {  // 64 places in order, each with the piece that belongs there
         const int p0 = (i * kNW + wave) * 64;
         if constexpr (kSame) {
           to_lds(rk, k_off, i * (kNW * 64 / NP) * k_row, sk + p0);
@@ -198,19 +201,15 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
 
   // ---- operands from LDS
   // Byte offsets of this lane's pieces; what changes with the step, dim tile or
-  // key group is an immediate, or exclusive-ored in where pieces are exchanged.
+  // key group is an immediate, or XORed in where pieces are exchanged.
   const int kn = key_of_row(n), ti = lane & 15;
-  int k_lane, k_swap, v_lane, v_swap;
-  if constexpr (PAGED) {
-    k_lane = (h * TK + kn) * 16, k_swap = 0;
-    v_lane = (h * D + n) * 16, v_swap = 0;
-  } else {
-    k_lane = kn * NP * 16, k_swap = (h ^ swap_k<D>(n)) * 16;
-    // V is read transposing: each group of 16 lanes reads four rows of 16 dims
-    // and gets four keys of one dim a lane
-    v_lane = (8 * h + (ti >> 2)) * NP * 16 + ((lane & 16) >> 3) * 16 + (ti & 3) * 8;
-    v_swap = swap_v<D>(ti >> 2) * 16;
-  }
+  const int k_lane = PAGED ? (h * TK + kn) * 16 : kn * NP * 16;
+  const int k_swap = PAGED ? 0 : (h ^ swap_k<D>(n)) * 16;
+  // packed rows: V is read transposing: each group of 16 lanes reads four rows
+  // of 16 dims and gets four keys of one dim a lane
+  const int v_lane = PAGED ? (h * D + n) * 16
+                           : (8 * h + (ti >> 2)) * NP * 16 + ((lane & 16) >> 3) * 16 + (ti & 3) * 8;
+  const int v_swap = PAGED ? 0 : swap_v<D>(ti >> 2) * 16;
   auto k_at = [&](const char *sk, int sub, int s) {
     const char *p = PAGED ? sk + (k_lane + (2 * s * TK + 32 * sub) * 16)
                           : sk + ((k_swap ^ (32 * s)) + k_lane) + 32 * sub * NP * 16;
@@ -245,26 +244,9 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
     return T::value(reinterpret_cast<const uint16_t *>(sv + piece * 16)[PAGED ? key & 7 : dim & 7]);
   };
 
-  auto step = [&](int k0, const char *sk, const char *sv, auto edge_c) {
-    constexpr bool EDGE = decltype(edge_c)::value;
-    f32x16 s[2];
-#pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[sub][r] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < NS; ++i) s[sub] = T::mfma32(k_at(sk, sub, i), qf[i], s[sub]);
-      if constexpr (EDGE) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = k0 + 32 * sub + 16 * (r >> 3) + 8 * h + (r & 7);
-          s[sub][r] = key >= lo && key <= hi ? s[sub][r] : -__builtin_inff();
-        }
-      }
-    }
-    float mt = fmaxf(s[0][0], s[1][0]);
-#pragma unroll
-    for (int r = 1; r < 16; ++r) mt = fmaxf(fmaxf(mt, s[0][r]), s[1][r]);
+  // One stage. The matrix cores get the fragments of K, then of V, in one
+  // sequence (frag): fragment i + kAhead is on its way from LDS while i is used.
+  auto raise = [&](float mt) {  // the running maximum, where it is far enough behind
     mt = halves_max(mt);
     if (__any((mt - m) * a.c > kLag)) {
       const float mn = fmaxf(m, mt);
@@ -276,61 +258,134 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
         for (int r = 0; r < 16; ++r) acc[d][r] *= w;
       m = mn;
     }
-    const float mc = m == -__builtin_inff() ? 0.0f : m * a.c - T::kShift;
+    return m == -__builtin_inff() ? 0.0f : m * a.c - T::kShift;
+  };
+  auto step = [&](const char *sk, const char *sv) {
+    constexpr int kAhead = 4;
+    f32x16 s[2];
+    u32x4 f[4 * NS];  // K of both halves, V: at most kAhead + 1 are alive
+    auto frag = [&](int i) {
+      if (i < 2 * NS)
+        f[i] = k_at(sk, i / NS, i % NS);
+      else if (i < 4 * NS)
+        f[i] = v_at(sv, (i - 2 * NS) / ND, (i - 2 * NS) % ND);
+    };
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) frag(i);
+    __builtin_amdgcn_sched_barrier(0);
+    float mt = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < 2 * NS; ++i) {
+      frag(i + kAhead);
+      s[i / NS] = T::mfma32(f[i], qf[i % NS], s[i / NS]);
+      // the first half's maximum beside the second half's products
+      constexpr int kFrom = NS + NS / 4, kSteps = 2 * NS - kFrom;
+      if (i >= kFrom) {
+#pragma unroll
+        for (int r = (i - kFrom) * 8 / kSteps; r < (i - kFrom + 1) * 8 / kSteps; ++r)
+          mt = fmaxf(fmaxf(mt, s[0][2 * r]), s[0][2 * r + 1]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) mt = fmaxf(fmaxf(mt, s[1][r]), s[1][r + 1]);
+    const float mc = raise(mt);
     u32x4 pf[4];
-    float sum = 0.0f;
+    auto weigh = [&](int sub, int r) {  // keys 2r and 2r + 1 of a half
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][2 * r], a.c, -mc));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][2 * r + 1], a.c, -mc));
+      l += p0 + p1;
+      pf[2 * sub + (r >> 2)][r & 3] = T::pack(p0, p1);
+    };
+#pragma unroll
+    for (int r = 0; r < 8; ++r) weigh(0, r);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 2 * NS; ++i) {
+      frag(2 * NS + i + kAhead);
+      acc[i % ND] = T::mfma32(f[2 * NS + i], pf[i / ND], acc[i % ND]);
+      if (i < NS) {  // the second half's weights beside the first half's products
+#pragma unroll
+        for (int r = i * 8 / NS; r < (i + 1) * 8 / NS; ++r) weigh(1, r);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  // One stage of which some rows see only a part.
+  auto edge_step = [&](int k0, const char *sk, const char *sv) {
+    f32x16 s[2];
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[sub][r] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) s[sub] = T::mfma32(k_at(sk, sub, i), qf[i], s[sub]);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int key = k0 + 32 * sub + 16 * (r >> 3) + 8 * h + (r & 7);
+        s[sub][r] = key >= lo && key <= hi ? s[sub][r] : -__builtin_inff();
+      }
+    }
+    float mt = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mt = fmaxf(fmaxf(mt, s[0][r]), s[1][r]);
+    const float mc = raise(mt);
+    u32x4 pf[4];
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
       for (int r = 0; r < 16; r += 2) {
         const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][r], a.c, -mc));
         const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][r + 1], a.c, -mc));
-        sum += p0 + p1;
+        l += p0 + p1;
         pf[2 * sub + (r >> 3)][(r & 7) >> 1] = T::pack(p0, p1);
       }
-    l += sum;
 
-    if constexpr (EDGE) {
-      // A masked key's probability is 0, but 0 times an infinity or NaN is not:
-      // a product of V with zeros shows whether the stage holds one.  Then the
-      // stage is added key by key, so that a row takes only what it sees.
-      f32x16 probe;
+    __builtin_amdgcn_sched_barrier(0);
+
+    // A masked key's probability is 0, but 0 times an infinity or NaN is not: a
+    // product of V with zeros shows whether the stage holds one.  Then the
+    // stage is added key by key, so that a row takes only what it sees.
+    f32x16 probe;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) probe[r] = 0.0f;
-      const u32x4 zero = {0u, 0u, 0u, 0u};
+    for (int r = 0; r < 16; ++r) probe[r] = 0.0f;
+    const u32x4 zero = {0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
+    for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-        for (int d = 0; d < ND; ++d) probe = T::mfma32(v_in(k0, sv, ks, d), zero, probe);
-      float any = probe[0];
+      for (int d = 0; d < ND; ++d) probe = T::mfma32(v_in(k0, sv, ks, d), zero, probe);
+    __builtin_amdgcn_sched_barrier(0);
+    float any = probe[0];
 #pragma unroll
-      for (int r = 1; r < 16; ++r) any += probe[r];
-      if (__any(any != 0.0f)) {
+    for (int r = 1; r < 16; ++r) any += probe[r];
+    if (__any(any != 0.0f)) {
 #pragma unroll 1
-        for (int i = 0; i < TK; ++i) {
-          const int key = k0 + i, w = (i & 7) >> 1;
-          const u32x4 pk = i < 16 ? pf[0] : i < 32 ? pf[1] : i < 48 ? pf[2] : pf[3];
-          const uint32_t pd = w == 0 ? pk[0] : w == 1 ? pk[1] : w == 2 ? pk[2] : pk[3];
-          const uint32_t mine = (pd >> (16 * (i & 1))) & 0xFFFFu;
-          const float p = T::value(static_cast<uint32_t>(
-              __shfl(static_cast<int>(mine), n + 32 * ((i >> 3) & 1))));
-          const bool seen = key >= lo && key <= hi;
+      for (int i = 0; i < TK; ++i) {
+        const int key = k0 + i, w = (i & 7) >> 1;
+        const u32x4 pk = i < 16 ? pf[0] : i < 32 ? pf[1] : i < 48 ? pf[2] : pf[3];
+        const uint32_t pd = w == 0 ? pk[0] : w == 1 ? pk[1] : w == 2 ? pk[2] : pk[3];
+        const uint32_t mine = (pd >> (16 * (i & 1))) & 0xFFFFu;
+        const float p = T::value(static_cast<uint32_t>(
+            __shfl(static_cast<int>(mine), n + 32 * ((i >> 3) & 1))));
+        const bool seen = key >= lo && key <= hi;
 #pragma unroll
-          for (int d = 0; d < ND; ++d)
+        for (int d = 0; d < ND; ++d)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const float v = v_one(sv, i, 32 * d + 8 * (r >> 2) + 4 * h + (r & 3));
-              acc[d][r] = seen ? __builtin_fmaf(p, v, acc[d][r]) : acc[d][r];
-            }
-        }
-        return;
+          for (int r = 0; r < 16; ++r) {
+            const float v = v_one(sv, i, 32 * d + 8 * (r >> 2) + 4 * h + (r & 3));
+            acc[d][r] = seen ? __builtin_fmaf(p, v, acc[d][r]) : acc[d][r];
+            __builtin_amdgcn_sched_barrier(0);
+          }
       }
+      return;
     }
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-      for (int d = 0; d < ND; ++d)
-        acc[d] = T::mfma32(EDGE ? v_in(k0, sv, ks, d) : v_at(sv, ks, d), pf[ks], acc[d]);
+      for (int d = 0; d < ND; ++d) acc[d] = T::mfma32(v_in(k0, sv, ks, d), pf[ks], acc[d]);
   };
 
   if (zbeg < zend) {
@@ -350,9 +405,9 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
         const char *sk = reinterpret_cast<const char *>(lds + buf * 2 * kPieces);
         const char *sv = sk + kPieces * 16;
         if constexpr (decltype(edge_c)::value) {
-          if (k0 <= hi_z && k0 + TK > lo_a) step(k0, sk, sv, edge_c);
+          if (k0 <= hi_z && k0 + TK > lo_a) edge_step(k0, sk, sv);
         } else {
-          step(k0, sk, sv, edge_c);
+          step(sk, sv);
         }
       }
     };
@@ -383,7 +438,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
         store4(o, a.out_dtype, 32 * d + 8 * g + 4 * h, v);
       }
   };
-  if (ns == 1) return write(1.0f / l);
+  if (!PAGED || ns == 1) return write(1.0f / l);
 
   // split: this chunk's sums to its slot, every lane in its own places; the
   // last workgroup of the tile adds the chunks in their order, lane by lane
