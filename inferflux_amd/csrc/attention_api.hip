@@ -42,6 +42,7 @@ bool is_out(int dtype) { return dtype == IFX_ATTN_F32 || is_elem(dtype); }
 bool heads_ok(int B, int T, int Hq, int Hkv, int D) {
   if (B < 1 || B > IFX_ATTN_MAX_BATCH || T < 0 || Hkv < 1 || Hq < Hkv || Hq % Hkv) return false;
   if (D != 64 && D != 96 && D != 128 && D != 256) return false;
+  if (static_cast<int64_t>(Hkv) * D >= (1 << 22)) return false;  // bytes of a page: 32 bits
   const int64_t rows = static_cast<int64_t>(T) * (Hq / Hkv);
   return rows < (1 << 30) && (rows / 32 + B) * Hkv < (1 << 23);
 }
@@ -62,7 +63,7 @@ struct PagedPlan {
 
 int round_up(int64_t n, int to) { return static_cast<int>((n + to - 1) / to * to); }
 
-// How ifx_attn_paged's keys are split over workgroups.  attn_rows: about 1024
+// How ifx_attn_paged's keys are split over workgroups.  attn_rows: about 2048
 // workgroups (two a CU are resident), of 128 keys at least.  attn_tile: enough
 // for the 512 that are resident.  Fewer where the split sums would not fit
 // the largest workspace.
@@ -83,14 +84,13 @@ PagedPlan plan_paged(int B, int T, int Hq, int Hkv, int D, int max_q, int max_kv
     busy = (full > B ? full : B) * Hkv;
     slot = attn_tile_slot_bytes(D);
   }
-  static const int R_=getenv("TR")?atoi(getenv("TR")):1024, T_=getenv("TT")?atoi(getenv("TT")):512, C_=getenv("TC")?atoi(getenv("TC")):512;
-  int64_t splits = p.rows ? (R_ + busy - 1) / busy : (T_ + busy - 1) / busy;
+  int64_t splits = p.rows ? (2048 + busy - 1) / busy : (1024 + busy - 1) / busy;
   if (splits > 128) splits = 128;
   const int64_t fit = (IFX_ATTN_WORKSPACE_BYTES - kCntBytes) / (units * slot);
   if (splits > fit) splits = fit;
   if (units > kMaxUnits || splits < 1) splits = 1;
   p.chunk = round_up((max_kv + splits - 1) / splits, unit);
-  if (!p.rows && splits > 1 && p.chunk < C_) p.chunk = C_;
+  if (!p.rows && splits > 1 && p.chunk < 512) p.chunk = 512;
   p.splits = splits > 1 ? (max_kv + p.chunk - 1) / p.chunk : 1;
   p.bytes = p.splits > 1 ? kCntBytes + units * p.splits * slot : 0;
   return p;

@@ -134,7 +134,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
   const int sh = a.page_shift, P = 1 << sh;
   const int32_t *table = PAGED ? a.table + static_cast<int64_t>(b) * a.table_width : nullptr;
   const int wmax = a.table_width - 1, last_page = static_cast<int>(a.num_pages) - 1;
-  const int64_t page_elems = (static_cast<int64_t>(a.Hkv) * D) << sh;
+  const uint32_t page_bytes = static_cast<uint32_t>(a.Hkv * D * 2) << sh;
   const uint16_t *K = static_cast<const uint16_t *>(a.k) +
                       (PAGED ? (static_cast<int64_t>(kvh) * D) << sh
                              : q0 * a.k_stride + static_cast<int64_t>(kvh) * D);
@@ -152,50 +152,61 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
     k_off = key * k_row + (c ^ swap_k<D>(key_of_row(key))) * 16;
     v_off = key * v_row + (c ^ swap_v<D>(key)) * 16;
   }
-  // of key k0 + lane, as the table has it: it is read a stage ahead and looked
-  // at only when that stage's loads are issued
+  // the page of key k0 + lane, as the table has it: it is read a stage ahead and
+  // looked at only when that stage's copies are issued
   auto entry_of = [&](int k0) { return table[min((k0 + lane) >> sh, wmax)]; };
-  auto load = [&](int k0, int entry, int buf) {
-    const int page = min(max(entry, 0), last_page);
-    u32x4 *sk = lds + buf * 2 * kPieces, *sv = sk + kPieces;
+  auto page_of = [&](int entry) { return min(max(entry, 0), last_page); };
+  // One stage's copies: where they come from, and the i-th (of 2 NL) of this wave.
+  struct Source {
+    const char *kp;  // paged K: this lane's key
+    int page, k0, buf;
+    rsrc_t rk, rv;   // packed rows: those behind the request's last read as 0
+  };
+  auto source = [&](int k0, int entry, int buf) {
+    Source f;
+    f.k0 = k0, f.buf = buf;
     if constexpr (PAGED) {
-      const uint16_t *kp = K + page * page_elems + ((k0 + lane) & (P - 1)) * 8;
-#pragma unroll
-      for (int i = 0; i < NL; ++i) {  // the 64 keys' pieces of one dim group
-        const int c = i * kNW + wave;
-        to_lds(kp + (static_cast<int64_t>(c * 8) << sh), sk + c * TK);
-      }
-#pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        const int p0 = (i * kNW + wave) * 64;
-        if constexpr (D % 64 == 0) {  // 64 dims of one key group
-          const int g = p0 / D;
-          const int64_t e = __builtin_amdgcn_readlane(page, 8 * g) * page_elems;
-          const uint16_t *vp = V + e + ((k0 + 8 * g) & (P - 1)) * D + (p0 - g * D) * 8;
-          to_lds(vp + lane * 8, sv + p0);
-        } else {
-          const int p = p0 + lane, g = p / D, dim = p - g * D;
-          const int64_t e = __shfl(page, 8 * g) * page_elems;
-          to_lds(V + e + ((k0 + 8 * g) & (P - 1)) * D + dim * 8, sv + p0);
-        }
-      }
+      f.page = page_of(entry);
+      f.kp = reinterpret_cast<const char *>(K) +
+             static_cast<uint64_t>(static_cast<uint32_t>(f.page)) * page_bytes +
+             ((k0 + lane) & (P - 1)) * 16;
     } else {
-      // the stage's rows; those behind the request's last read as 0
       const int rows = min(kv - k0, TK);
-      const rsrc_t rk = make_rsrc(K + k0 * a.k_stride, rows * k_row);
-      const rsrc_t rv = make_rsrc(V + k0 * a.v_stride, rows * v_row);
-#pragma unroll
-      for (int i = 0; i < NL; ++i) {  // 64 places in order, each with the piece that belongs there
-        const int p0 = (i * kNW + wave) * 64;
-        if constexpr (kSame) {
-          to_lds(rk, k_off, i * (kNW * 64 / NP) * k_row, sk + p0);
-          to_lds(rv, v_off, i * (kNW * 64 / NP) * v_row, sv + p0);
-        } else {
-          const int p = p0 + lane, key = p / NP, c = p - key * NP;
-          to_lds(rk, key * k_row + (c ^ swap_k<D>(key_of_row(key & 31))) * 16, 0, sk + p0);
-          to_lds(rv, key * v_row + (c ^ swap_v<D>(key)) * 16, 0, sv + p0);
-        }
+      f.rk = make_rsrc(K + k0 * a.k_stride, rows * k_row);
+      f.rv = make_rsrc(V + k0 * a.v_stride, rows * v_row);
+    }
+    return f;
+  };
+  auto copy = [&](const Source &f, int j) {
+    const int i = j >> 1, n0 = i * kNW + wave;  // 64 pieces
+    u32x4 *sk = lds + f.buf * 2 * kPieces + n0 * 64, *sv = sk + kPieces;
+    if constexpr (PAGED) {
+      if ((j & 1) == 0) {  // K: the 64 keys' pieces of one dim group
+        to_lds(f.kp + ((n0 * 16) << sh), sk);
+      } else if constexpr (D % 64 == 0) {  // V: 64 dims of one key group
+        const int g = n0 * 64 / D;
+        const uint32_t pg = __builtin_amdgcn_readlane(f.page, 8 * g);
+        to_lds(reinterpret_cast<const char *>(V) + static_cast<uint64_t>(pg) * page_bytes +
+                   (((f.k0 + 8 * g) & (P - 1)) * D + (n0 * 64 - g * D) * 8) * 2 + lane * 16,
+               sv);
+      } else {
+        const int p = n0 * 64 + lane, g = p / D, dim = p - g * D;
+        const uint32_t pg = __shfl(f.page, 8 * g);
+        to_lds(reinterpret_cast<const char *>(V) + static_cast<uint64_t>(pg) * page_bytes +
+                   (((f.k0 + 8 * g) & (P - 1)) * D + dim * 8) * 2,
+               sv);
       }
+    } else if constexpr (kSame) {  // 64 places in order, each with the piece that belongs there
+      if ((j & 1) == 0)
+        to_lds(f.rk, k_off, i * (kNW * 64 / NP) * k_row, sk);
+      else
+        to_lds(f.rv, v_off, i * (kNW * 64 / NP) * v_row, sv);
+    } else {
+      const int p = n0 * 64 + lane, key = p / NP, c = p - key * NP;
+      if ((j & 1) == 0)
+        to_lds(f.rk, key * k_row + (c ^ swap_k<D>(key_of_row(key & 31))) * 16, 0, sk);
+      else
+        to_lds(f.rv, key * v_row + (c ^ swap_v<D>(key)) * 16, 0, sv);
     }
   };
 
@@ -210,9 +221,9 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
   const int v_lane = PAGED ? (h * D + n) * 16
                            : (8 * h + (ti >> 2)) * NP * 16 + ((lane & 16) >> 3) * 16 + (ti & 3) * 8;
   const int v_swap = PAGED ? 0 : swap_v<D>(ti >> 2) * 16;
-  auto k_at = [&](const char *sk, int sub, int s) {
+  auto k_at = [&](const char *sk, int sub, int s, int swap) {
     const char *p = PAGED ? sk + (k_lane + (2 * s * TK + 32 * sub) * 16)
-                          : sk + ((k_swap ^ (32 * s)) + k_lane) + 32 * sub * NP * 16;
+                          : sk + ((swap ^ (32 * s)) + k_lane) + 32 * sub * NP * 16;
     return *reinterpret_cast<const u32x4 *>(p);
   };
   auto v_at = [&](const char *sv, int ks, int d) -> u32x4 {
@@ -239,14 +250,9 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
     }
     return r;
   };
-  auto v_one = [&](const char *sv, int key, int dim) {  // one value, for the rare path
-    const int piece = PAGED ? (key >> 3) * D + dim : key * NP + ((dim >> 3) ^ swap_v<D>(key));
-    return T::value(reinterpret_cast<const uint16_t *>(sv + piece * 16)[PAGED ? key & 7 : dim & 7]);
-  };
-
-  // One stage. The matrix cores get the fragments of K, then of V, in one
-  // sequence (frag): fragment i + kAhead is on its way from LDS while i is used.
-  auto raise = [&](float mt) {  // the running maximum, where it is far enough behind
+  // Raises the running maximum where a stage's is far enough above it; what the
+  // exponents are then taken relative to.
+  auto raise = [&](float mt) {
     mt = halves_max(mt);
     if (__any((mt - m) * a.c > kLag)) {
       const float mn = fmaxf(m, mt);
@@ -260,43 +266,58 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
     }
     return m == -__builtin_inff() ? 0.0f : m * a.c - T::kShift;
   };
-  auto step = [&](const char *sk, const char *sv) {
+  // One stage.  The matrix cores get the fragments of K, then of V, in one
+  // sequence: fragment i + kAhead is on its way from LDS while i is multiplied.
+  // next(j), j < 2 NL, issues the next stage's copies, one at a time between the
+  // first products: a wave waits at its next copy until the last is under way.
+  const f32x16 none_yet = {};
+  auto step = [&](const char *sk, const char *sv, auto next) {
     constexpr int kAhead = 4;
     f32x16 s[2];
     u32x4 f[4 * NS];  // K of both halves, V: at most kAhead + 1 are alive
+    int swap = k_swap;
+    asm volatile("" : "+v"(swap));  // offsets formed anew in every stage, not kept in registers
     auto frag = [&](int i) {
       if (i < 2 * NS)
-        f[i] = k_at(sk, i / NS, i % NS);
+        f[i] = k_at(sk, i / NS, i % NS, swap);
       else if (i < 4 * NS)
         f[i] = v_at(sv, (i - 2 * NS) / ND, (i - 2 * NS) % ND);
     };
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.0f;
-#pragma unroll
     for (int i = 0; i < kAhead; ++i) frag(i);
+    if constexpr (!PAGED) {
+#pragma unroll
+      for (int j = 0; j < 2 * NL; ++j) next(j);
+    }
     __builtin_amdgcn_sched_barrier(0);
-    float mt = -__builtin_inff();
+    float mt[2] = {-__builtin_inff(), -__builtin_inff()};
 #pragma unroll
     for (int i = 0; i < 2 * NS; ++i) {
       frag(i + kAhead);
-      s[i / NS] = T::mfma32(f[i], qf[i % NS], s[i / NS]);
+      s[i / NS] = T::mfma32(f[i], qf[i % NS], i % NS ? s[i / NS] : none_yet);
+      if constexpr (PAGED) {
+#pragma unroll
+        for (int j = i * NL / NS; j < (i + 1) * NL / NS; ++j) next(j);
+      }
       // the first half's maximum beside the second half's products
       constexpr int kFrom = NS + NS / 4, kSteps = 2 * NS - kFrom;
       if (i >= kFrom) {
 #pragma unroll
         for (int r = (i - kFrom) * 8 / kSteps; r < (i - kFrom + 1) * 8 / kSteps; ++r)
-          mt = fmaxf(fmaxf(mt, s[0][2 * r]), s[0][2 * r + 1]);
+          mt[r & 1] = fmaxf(fmaxf(mt[r & 1], s[0][2 * r]), s[0][2 * r + 1]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int r = 0; r < 16; r += 2) mt = fmaxf(fmaxf(mt, s[1][r]), s[1][r + 1]);
-    const float mc = raise(mt);
+    for (int r = 0; r < 8; ++r) mt[r & 1] = fmaxf(fmaxf(mt[r & 1], s[1][2 * r]), s[1][2 * r + 1]);
+    const float mc = raise(fmaxf(mt[0], mt[1]));
     u32x4 pf[4];
+    float sum[2] = {l, 0.0f};
     auto weigh = [&](int sub, int r) {  // keys 2r and 2r + 1 of a half
       const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][2 * r], a.c, -mc));
       const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][2 * r + 1], a.c, -mc));
-      l += p0 + p1;
+      sum[0] += p0;
+      sum[1] += p1;
       pf[2 * sub + (r >> 2)][r & 3] = T::pack(p0, p1);
     };
 #pragma unroll
@@ -312,17 +333,19 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    l = sum[0] + sum[1];
   };
 
   // One stage of which some rows see only a part.
+  bool tainted = false;
   auto edge_step = [&](int k0, const char *sk, const char *sv) {
     f32x16 s[2];
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[sub][r] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < NS; ++i) s[sub] = T::mfma32(k_at(sk, sub, i), qf[i], s[sub]);
+      for (int i = 0; i < NS; ++i)
+        s[sub] = T::mfma32(k_at(sk, sub, i, k_swap), qf[i], i ? s[sub] : none_yet);
+      __builtin_amdgcn_sched_barrier(0);  // a few fragments at a time: registers
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int key = k0 + 32 * sub + 16 * (r >> 3) + 8 * h + (r & 7);
@@ -343,82 +366,122 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
         l += p0 + p1;
         pf[2 * sub + (r >> 3)][(r & 7) >> 1] = T::pack(p0, p1);
       }
-
-    __builtin_amdgcn_sched_barrier(0);
-
     // A masked key's probability is 0, but 0 times an infinity or NaN is not: a
-    // product of V with zeros shows whether the stage holds one.  Then the
-    // stage is added key by key, so that a row takes only what it sees.
-    f32x16 probe;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) probe[r] = 0.0f;
+    // product of V with zeros shows whether the stage holds one.
+    f32x16 probe = none_yet;
     const u32x4 zero = {0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
+    for (int ks = 0; ks < 4; ++ks) {
 #pragma unroll
-      for (int d = 0; d < ND; ++d) probe = T::mfma32(v_in(k0, sv, ks, d), zero, probe);
-    __builtin_amdgcn_sched_barrier(0);
+      for (int d = 0; d < ND; ++d) {
+        const u32x4 v = v_in(k0, sv, ks, d);
+        probe = T::mfma32(v, zero, probe);
+        acc[d] = T::mfma32(v, pf[ks], acc[d]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
     float any = probe[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) any += probe[r];
-    if (__any(any != 0.0f)) {
-#pragma unroll 1
-      for (int i = 0; i < TK; ++i) {
-        const int key = k0 + i, w = (i & 7) >> 1;
-        const u32x4 pk = i < 16 ? pf[0] : i < 32 ? pf[1] : i < 48 ? pf[2] : pf[3];
-        const uint32_t pd = w == 0 ? pk[0] : w == 1 ? pk[1] : w == 2 ? pk[2] : pk[3];
-        const uint32_t mine = (pd >> (16 * (i & 1))) & 0xFFFFu;
-        const float p = T::value(static_cast<uint32_t>(
-            __shfl(static_cast<int>(mine), n + 32 * ((i >> 3) & 1))));
-        const bool seen = key >= lo && key <= hi;
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float v = v_one(sv, i, 32 * d + 8 * (r >> 2) + 4 * h + (r & 3));
-            acc[d][r] = seen ? __builtin_fmaf(p, v, acc[d][r]) : acc[d][r];
-            __builtin_amdgcn_sched_barrier(0);
-          }
-      }
-      return;
-    }
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-      for (int d = 0; d < ND; ++d) acc[d] = T::mfma32(v_in(k0, sv, ks, d), pf[ks], acc[d]);
+    tainted |= __any(any != 0.0f) != 0;
   };
 
   if (zbeg < zend) {
-    int entry = 0;
+    int entry = 0, k0 = zbeg, buf = 0;
     if constexpr (PAGED) entry = entry_of(zbeg);
-    load(zbeg, entry, 0);
+    {
+      const Source f = source(zbeg, entry, 0);
+#pragma unroll
+      for (int j = 0; j < 2 * NL; ++j) copy(f, j);
+    }
     if constexpr (PAGED) entry = entry_of(zbeg + TK);
-    int k0 = zbeg, buf = 0;
-    auto stages = [&](int until, auto edge_c) {
+    // Stages up to `until`.  (`last`: a stage among them may have no successor.)
+    auto stages = [&](int until, auto edge_c, auto last_c) {
       for (; k0 < until; k0 += TK, buf ^= 1) {
         wait_own_memory();
         __syncthreads();  // this stage is in LDS, and no wave reads the other one
-        if (k0 + TK < zend) {
-          load(k0 + TK, entry, buf ^ 1);
-          if constexpr (PAGED) entry = entry_of(k0 + 2 * TK);
-        }
+        const bool more = !decltype(last_c)::value || k0 + TK < zend;
+        const Source f = source(more ? k0 + TK : zbeg, entry, buf ^ 1);
+        if constexpr (PAGED) entry = entry_of(k0 + 2 * TK);
+        auto next = [&](int j) {
+          if (more) copy(f, j);
+        };
         const char *sk = reinterpret_cast<const char *>(lds + buf * 2 * kPieces);
         const char *sv = sk + kPieces * 16;
         if constexpr (decltype(edge_c)::value) {
+#pragma unroll
+          for (int j = 0; j < 2 * NL; ++j) next(j);
           if (k0 <= hi_z && k0 + TK > lo_a) edge_step(k0, sk, sv);
         } else {
-          step(sk, sv);
+          step(sk, sv, next);
         }
       }
     };
     // stages that all rows of the workgroup see whole, between those that some
     // see in part: where windows begin, and at the causal end
+    using yes = std::true_type;
+    using no = std::false_type;
     int until = a.window > 0 ? min(full_a, zend) : zbeg;
     while (true) {
-      stages(until, std::true_type{});
+      stages(until, yes{}, yes{});
       if (k0 >= zend) break;
-      stages(min(full_z, zend), std::false_type{});
+      stages(min(full_z, zend - TK), no{}, no{});
+      stages(min(full_z, zend), no{}, yes{});
       until = zend;
+    }
+  }
+
+  // A wave that met an infinity or NaN in the values of a stage that its rows
+  // see in part takes its rows again, key by key from memory, each lane its
+  // row's half of the dims, so that a row takes only what it sees.  Rare and
+  // slow (about a microsecond a key).
+  if (tainted) {
+    auto dim_of = [&](int i) { return 32 * (i >> 4) + 8 * (i >> 2 & 3) + 4 * h; };  // of i .. i + 3
+    float q[ND * 16];
+    const uint16_t *qp = static_cast<const uint16_t *>(a.q) + (q0 + tok) * a.q_stride +
+                         static_cast<int64_t>(head) * D;
+#pragma unroll
+    for (int i = 0; i < ND * 16; ++i) q[i] = T::value(qp[dim_of(i) + (i & 3)]);
+#pragma unroll
+    for (int i = 0; i < ND * 16; ++i) acc[i >> 4][i & 15] = 0.0f;
+    m = -__builtin_inff(), l = 0.0f;
+#pragma unroll 1
+    for (int key = zbeg; key < zend; ++key) {
+      const char *kp, *vp;
+      if constexpr (PAGED) {
+        const uint64_t at = static_cast<uint64_t>(static_cast<uint32_t>(
+                                page_of(table[min(key >> sh, wmax)]))) * page_bytes;
+        kp = reinterpret_cast<const char *>(K) + at + (key & (P - 1)) * 16;
+        vp = reinterpret_cast<const char *>(V) + at + ((key & (P - 1) & ~7) * D + (key & 7)) * 2;
+      } else {
+        kp = reinterpret_cast<const char *>(K + key * a.k_stride);
+        vp = reinterpret_cast<const char *>(V + key * a.v_stride);
+      }
+      float x = 0.0f;
+#pragma unroll
+      for (int i = 0; i < ND * 16; i += 4) {
+        const int dim = dim_of(i);
+        const u32x2 k4 = ldg<u32x2>(kp + (PAGED ? ((dim & ~7) * 2 << sh) + (dim & 7) * 2 : dim * 2));
+        x = __builtin_fmaf(q[i], T::value(k4.x & 0xFFFFu), x);
+        x = __builtin_fmaf(q[i + 1], T::value(k4.x >> 16), x);
+        x = __builtin_fmaf(q[i + 2], T::value(k4.y & 0xFFFFu), x);
+        x = __builtin_fmaf(q[i + 3], T::value(k4.y >> 16), x);
+      }
+      x = halves_sum(x);
+      const bool seen = key >= lo && key <= hi;
+      const float mn = seen ? fmaxf(m, x) : m;
+      const float w = mn == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * a.c);
+      const float rel = mn == -__builtin_inff() ? 0.0f : mn * a.c - T::kShift;
+      const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(x, a.c, -rel));
+      m = mn;
+      l = l * w + (seen && h == 0 ? pr : 0.0f);  // the halves' are added below
+#pragma unroll
+      for (int i = 0; i < ND * 16; ++i) {
+        const float v = T::value(*reinterpret_cast<const uint16_t *>(
+            vp + (dim_of(i) + (i & 3)) * (PAGED ? 16 : 2)));
+        const float o = acc[i >> 4][i & 15] * w;
+        acc[i >> 4][i & 15] = seen ? __builtin_fmaf(pr, v, o) : o;
+      }
     }
   }
 
