@@ -55,44 +55,51 @@ constexpr int kMaxUnits = 8192;
 constexpr int64_t kCntBytes = kMaxUnits * 4;
 
 struct PagedPlan {
-  bool rows;  // attn_rows, else attn_tile
-  int tiles;  // attn_tile: row tiles of the launch
-  int chunk, splits;
-  int64_t bytes;  // of workspace
+  bool rows;          // attn_rows, else attn_tile
+  int chunk, splits;  // attn_rows
+  int tiles, goal;    // attn_tile: workgroups of a key/value head, those of split tiles
+  int64_t bytes;      // of workspace
 };
 
 int round_up(int64_t n, int to) { return static_cast<int>((n + to - 1) / to * to); }
 
-// How ifx_attn_paged's keys are split over workgroups.  attn_rows: about 2048
-// workgroups (two a CU are resident), of 128 keys at least.  attn_tile: enough
-// for the 512 that are resident.  Fewer where the split sums would not fit
-// the largest workspace.
+// How ifx_attn_paged's keys are split over workgroups.
+//
+// attn_rows: about 2048 workgroups of 128 keys at least, four rounds of the 512
+// that are resident, as requests differ in length (32 requests of 531 to 22591
+// keys, 40 / 8 heads of 128: 187 us; 1024: 204, 4096: 187, 8192: 199).
+//
+// attn_tile: the workgroups that are resident, two a CU (D = 64: three, D = 256: one), if the
+// row tiles are fewer; each finds its share (find_item).
+//
+// Fewer where the split sums would not fit the largest workspace.
 PagedPlan plan_paged(int B, int T, int Hq, int Hkv, int D, int max_q, int max_kv) {
   PagedPlan p{};
   const int G = Hq / Hkv;
   const int64_t rows = static_cast<int64_t>(max_q) * G;
+  constexpr int64_t space = IFX_ATTN_WORKSPACE_BYTES - kCntBytes;
   p.rows = rows <= kRowsMax;
-  const int unit = p.rows ? kRowKeys : kTileKeys;
-  int64_t units, busy, slot;
   if (p.rows) {
-    units = busy = static_cast<int64_t>(B) * Hkv;
-    slot = rows * (D + 4) * 4;
+    const int64_t units = static_cast<int64_t>(B) * Hkv, slot = rows * (D + 4) * 4;
+    int64_t splits = (2048 + units - 1) / units;
+    if (splits > 128) splits = 128;
+    if (splits > space / (units * slot)) splits = space / (units * slot);
+    if (units > kMaxUnits || splits < 1) splits = 1;
+    p.chunk = round_up((max_kv + splits - 1) / splits, kRowKeys);
+    p.splits = splits > 1 ? (max_kv + p.chunk - 1) / p.chunk : 1;
+    p.bytes = p.splits > 1 ? kCntBytes + units * p.splits * slot : 0;
   } else {
-    const int64_t full = static_cast<int64_t>(T) * G / attn_tile_rows(D);
-    p.tiles = static_cast<int>(full) + B;
-    units = static_cast<int64_t>(p.tiles) * Hkv;
-    busy = (full > B ? full : B) * Hkv;
-    slot = attn_tile_slot_bytes(D);
+    const int64_t rounds = static_cast<int64_t>(T) * G / attn_tile_rows(D) + B;
+    const int64_t slot = attn_tile_slot_bytes(D);
+    // 2 goal slots (find_item), a counter each
+    int64_t goal = (D == 256 ? 256 : D == 64 ? 768 : 512) / Hkv;
+    if (goal > space / slot / 2 / Hkv) goal = space / slot / 2 / Hkv;
+    const int64_t use = rounds * ((max_kv + attn_tile_min_keys() - 1) / attn_tile_min_keys());
+    p.goal = static_cast<int>(goal < use ? goal : use);
+    if (max_kv <= attn_tile_min_keys()) p.goal = 0;
+    p.tiles = static_cast<int>(rounds) + p.goal;
+    p.bytes = p.goal ? kCntBytes + 2 * p.goal * Hkv * slot : 0;
   }
-  int64_t splits = p.rows ? (2048 + busy - 1) / busy : (1024 + busy - 1) / busy;
-  if (splits > 128) splits = 128;
-  const int64_t fit = (IFX_ATTN_WORKSPACE_BYTES - kCntBytes) / (units * slot);
-  if (splits > fit) splits = fit;
-  if (units > kMaxUnits || splits < 1) splits = 1;
-  p.chunk = round_up((max_kv + splits - 1) / splits, unit);
-  if (!p.rows && splits > 1 && p.chunk < 512) p.chunk = 512;
-  p.splits = splits > 1 ? (max_kv + p.chunk - 1) / p.chunk : 1;
-  p.bytes = p.splits > 1 ? kCntBytes + units * p.splits * slot : 0;
   return p;
 }
 
@@ -191,7 +198,7 @@ int ifx_attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cac
   a.B = B, a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv;
   a.causal = 1, a.window = window, a.out_dtype = out_dtype;
   a.c = scale * kLog2e;
-  a.chunk = p.chunk, a.splits = p.splits;
+  a.chunk = p.chunk, a.splits = p.splits, a.goal = p.goal;
   if (p.bytes) {
     a.cnt = static_cast<uint32_t *>(workspace);
     a.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + kCntBytes);
@@ -224,7 +231,6 @@ int ifx_attn_prompt(const void *q, int64_t q_stride, const void *k, int64_t k_st
   a.B = B, a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv;
   a.causal = causal != 0, a.window = window, a.out_dtype = out_dtype;
   a.c = scale * kLog2e;
-  a.chunk = 1 << 30, a.splits = 1;
   const int tiles = static_cast<int>(static_cast<int64_t>(T) * a.G / attn_tile_rows(D)) + B;
   return status_of(launch_attn_tile(a, dtype, D, false, tiles, static_cast<hipStream_t>(stream)));
 }

@@ -56,7 +56,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const AttnArgs a, int lds_
   const int ctx = kv - nq;  // position of the first row; below 0 it sees nothing
   const int lo0 = a.window > 0 ? max(0, ctx - a.window + 1) : 0;
   const int kbeg = lo0 & ~(kRowKeys - 1), kend = kv;  // the last row sees kv - 1
-  const int chunk = split_chunk(a, kend - kbeg, kRowKeys);
+  const int chunk = split_chunk(a, kend - kbeg);
   const int ns = kend > kbeg ? (kend - kbeg + chunk - 1) / chunk : 1;
   if (z >= ns) return;
   const int zbeg = kbeg + z * chunk, zend = min(zbeg + chunk, kend);

@@ -54,42 +54,148 @@ __device__ __forceinline__ int swap_v(int key) {
   return D == 64 ? (key & 2) << 1 : D == 96 ? 0 : (key & 3) << 2;
 }
 
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(v, o);
+    v += lane >= o ? u : 0;
+  }
+  return v;
+}
+
+// A piece of paged work: item `item` (chunk major) of request b's `tiles` row
+// tiles x ns chunks of `chunk` stages.  chunk is 0 where there is no such item.
+struct Split {
+  int chunk, ns, slot;  // slot: of the split sums of the request's first tile
+  int b, item, tiles;
+};
+
+// Item i of the batch (for one key/value head), found by a wave from the
+// requests' {row tiles, stages}.  The work is cut so that about `goal` items
+// of one length come out: fewer leave compute units idle, more start a second
+// round.  Where the row tiles alone are more than that, only requests that are
+// longer than the average share are split.  At most 2 goal items belong to
+// split tiles: where a request of s > c stages is cut in chunks of c, they are
+// less than s / c + 1 < 2 s / c, and c is at least (sum of s) / goal.
+constexpr int kMinChunk = 8;  // stages: what a chunk costs beside its keys
+__device__ __forceinline__ Split find_item(const int2 *reqs, int B, int i, int goal, int lane) {
+  const int per = (B + 63) / 64, b0 = min(lane * per, B), b1 = min(b0 + per, B);
+  int chunk = 1 << 24;
+  if (goal > 0) {
+    float stages = 0.0f, tiles = 0.0f;
+#pragma unroll 1
+    for (int b = b0; b < b1; ++b) {
+      const int2 r = reqs[b];
+      tiles += static_cast<float>(r.x);
+      stages += static_cast<float>(r.x) * static_cast<float>(r.y);
+    }
+    tiles = wave_sum(tiles);
+    chunk = max(kMinChunk, static_cast<int>(min(ceilf(wave_sum(stages) / goal), 1e7f)));
+    for (int tries = 0; tries < 3 && tiles < goal; ++tries) {
+      float items = 0.0f;
+#pragma unroll 1
+      for (int b = b0; b < b1; ++b) {
+        const int2 r = reqs[b];
+        items += static_cast<float>(r.x * ((r.y + chunk - 1) / chunk));
+      }
+      items = wave_sum(items);
+      if (items <= goal) break;
+      chunk = max(chunk + 1, static_cast<int>(chunk * (items / goal)));
+    }
+    chunk = __builtin_amdgcn_readfirstlane(chunk);
+  }
+  int items = 0, slots = 0;
+#pragma unroll 1
+  for (int b = b0; b < b1; ++b) {
+    const int2 r = reqs[b];
+    const int ns = (r.y + chunk - 1) / chunk;
+    items += r.x * ns;
+    slots += ns > 1 ? r.x * ns : 0;
+  }
+  int at = wave_scan(items, lane) - items, slot = wave_scan(slots, lane) - slots;
+  Split f = {0, 0, 0, 0, 0, 0};
+  const uint64_t has = __ballot(i >= at && i < at + items);
+  if (!has) return f;
+  const int who = __builtin_ctzll(has);
+  at = __builtin_amdgcn_readlane(at, who), slot = __builtin_amdgcn_readlane(slot, who);
+  for (int b = who * per;; ++b) {
+    const int2 r = reqs[b];
+    const int ns = (r.y + chunk - 1) / chunk, n = r.x * ns;
+    if (i < at + n) {
+      f.chunk = __builtin_amdgcn_readfirstlane((r.y + ns - 1) / ns);  // of equal length
+      f.ns = __builtin_amdgcn_readfirstlane(ns);
+      f.slot = __builtin_amdgcn_readfirstlane(slot);
+      f.b = __builtin_amdgcn_readfirstlane(b);
+      f.item = __builtin_amdgcn_readfirstlane(i - at);
+      f.tiles = __builtin_amdgcn_readfirstlane(r.x);
+      return f;
+    }
+    at += n;
+    slot += ns > 1 ? n : 0;
+  }
+}
+
 }  // namespace
 
 template <int DT, int D, bool PAGED>
-__global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const AttnArgs a) {
+__global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_attn_tile(const AttnArgs a) {
   using T = Elem<DT>;
   constexpr int ND = D / 32, NS = D / 16, NP = D / 8;
   constexpr int kPieces = TK * NP;              // of K, and of V, a stage
   constexpr int NL = kPieces / (64 * kNW);      // pieces a thread loads, each
   extern __shared__ u32x4 lds[];                // [2 stages][K, V][kPieces]
-  __shared__ int found[3];
+  __shared__ int found[2];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kvh = blockIdx.x % a.Hkv, z = blockIdx.y;
+  const int kvh = blockIdx.x % a.Hkv;
 
-  // Which request's rows: request b owns the row tiles from
-  // floor(cu[b] G / kRows) + b on, at least as many as it needs, so that no
-  // tile list has to be built.  Late tiles (long key ranges) come first.
-  const int tile = (gridDim.x - 1 - blockIdx.x) / a.Hkv;
-  if (tid == 0) found[0] = -1;
-  __syncthreads();
-  for (int b = tid; b < a.B; b += 64 * kNW) {
-    const int c0 = min(max(a.cu[b], 0), a.T), c1 = min(max(a.cu[b + 1], 0), a.T);
-    const int t0 = c0 * a.G / kRows + b, t1 = c1 * a.G / kRows + b + 1;
-    if (t0 <= tile && tile < t1 && (tile - t0) * kRows < (c1 - c0) * a.G) {
-      found[0] = b;
-      found[1] = c0;
-      found[2] = c1;
+  // Which rows and keys.  No list of work is built beforehand: each workgroup
+  // finds its own.
+  int b, tile, z = 0;  // request, its row tile, its chunk of the keys
+  Split split = {1 << 24, 1, 0};
+  if constexpr (PAGED) {
+    int2 *reqs = reinterpret_cast<int2 *>(lds);
+    for (int i = tid; i < a.B; i += 64 * kNW) {
+      const int c0 = min(max(a.cu[i], 0), a.T), c1 = min(max(a.cu[i + 1], 0), a.T);
+      const int tiles = (max(c1 - c0, 0) * a.G + kRows - 1) / kRows;
+      int keys = min(max(a.kv_len[i], 0), a.table_width << a.page_shift);
+      if (a.window > 0) keys = min<int64_t>(keys, static_cast<int64_t>(a.window) + kRows + TK);
+      reqs[i] = make_int2(tiles, max(1, (keys + TK - 1) / TK));
     }
+    __syncthreads();
+    split = find_item(reqs, a.B, blockIdx.x / a.Hkv, a.goal, lane);
+    if (split.chunk == 0) return;
+    __syncthreads();  // reqs is read, stages may come
+    b = split.b, z = split.item / split.tiles;
+    tile = split.tiles - 1 - (split.item - z * split.tiles);  // late tiles first
+  } else {
+    // request b owns the row tiles from floor(cu[b] G / kRows) + b on, at least
+    // as many as it needs; late tiles (long key ranges) come first
+    const int t = (gridDim.x - 1 - blockIdx.x) / a.Hkv;
+    if (tid == 0) found[0] = -1;
+    __syncthreads();
+    for (int i = tid; i < a.B; i += 64 * kNW) {
+      const int c0 = min(max(a.cu[i], 0), a.T), c1 = min(max(a.cu[i + 1], 0), a.T);
+      const int t0 = c0 * a.G / kRows + i, t1 = c1 * a.G / kRows + i + 1;
+      if (t0 <= t && t < t1 && (t - t0) * kRows < (c1 - c0) * a.G) {
+        found[0] = i;
+        found[1] = t - t0;
+      }
+    }
+    __syncthreads();
+    b = __builtin_amdgcn_readfirstlane(found[0]);
+    if (b < 0) return;
+    tile = __builtin_amdgcn_readfirstlane(found[1]);
   }
-  __syncthreads();
-  const int b = __builtin_amdgcn_readfirstlane(found[0]);
-  if (b < 0) return;
-  const int q0 = __builtin_amdgcn_readfirstlane(found[1]);
-  const int nq = __builtin_amdgcn_readfirstlane(found[2]) - q0;
+  const int q0 = min(max(a.cu[b], 0), a.T);
+  const int nq = min(max(a.cu[b + 1], 0), a.T) - q0;
   const int R = nq * a.G;
-  const int row0 = (tile - (q0 * a.G / kRows + b)) * kRows;  // the workgroup's first
+  const int row0 = tile * kRows;  // the workgroup's first
   const int kv = PAGED ? min(max(a.kv_len[b], 0), a.table_width << a.page_shift) : nq;
   const int ctx = kv - nq;  // position of the request's first row
 
@@ -102,7 +208,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
   const int full_z = max(0, a.causal ? ctx + tok_a + 1 : kv) & ~(TK - 1);
   int ns = 1, zbeg = kbeg, zend = kend;  // prompts are not split
   if constexpr (PAGED) {
-    const int chunk = split_chunk(a, kend - kbeg, TK);
+    const int chunk = split.chunk * TK;
     if (kend > kbeg) ns = (kend - kbeg + chunk - 1) / chunk;
     if (z >= ns) return;
     zbeg = kbeg + z * chunk, zend = min(zbeg + chunk, kend);
@@ -115,6 +221,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
   const int lo = a.window > 0 ? max(0, ctx + tok - a.window + 1) : 0;
   const int hi_z = __builtin_amdgcn_readlane(hi, 31);  // some of the wave's rows see [lo_a, hi_z]
   const int lo_a = __builtin_amdgcn_readlane(lo, 0);
+  const bool idle = row0 + 32 * wave >= R;  // the wave has no rows, it only copies
 
   u32x4 qf[NS];
   {
@@ -408,10 +515,11 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
         };
         const char *sk = reinterpret_cast<const char *>(lds + buf * 2 * kPieces);
         const char *sv = sk + kPieces * 16;
-        if constexpr (decltype(edge_c)::value) {
+        if (decltype(edge_c)::value || idle) {
 #pragma unroll
           for (int j = 0; j < 2 * NL; ++j) next(j);
-          if (k0 <= hi_z && k0 + TK > lo_a) edge_step(k0, sk, sv);
+          if constexpr (decltype(edge_c)::value)
+            if (!idle && k0 <= hi_z && k0 + TK > lo_a) edge_step(k0, sk, sv);
         } else {
           step(sk, sv, next);
         }
@@ -507,9 +615,9 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
   // last workgroup of the tile adds the chunks in their order, lane by lane
   const rsrc_t part = make_rsrc(a.part, a.part_bytes);
   constexpr uint32_t kWaveBytes = 32 * D * 4 + 64 * 4 * 2, kSlotBytes = kNW * kWaveBytes;
-  const uint32_t unit = static_cast<uint32_t>(tile) * a.Hkv + kvh;
-  const uint32_t mine = unit * a.splits * kSlotBytes + wave * kWaveBytes + lane * 16;
-  const uint32_t mine_ml = unit * a.splits * kSlotBytes + wave * kWaveBytes + 32 * D * 4 + lane * 8;
+  const uint32_t first = split.slot * a.Hkv + (tile * a.Hkv + kvh) * split.ns;  // the tile's slots
+  const uint32_t mine = first * kSlotBytes + wave * kWaveBytes + lane * 16;
+  const uint32_t mine_ml = first * kSlotBytes + wave * kWaveBytes + 32 * D * 4 + lane * 8;
   {
     const uint32_t at = mine + z * kSlotBytes;
 #pragma unroll
@@ -522,7 +630,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : 2) void k_attn_tile(const 
         __builtin_bit_cast(u32x2, make_float2(m, l)), part, mine_ml + z * kSlotBytes, 0, kAuxDevice);
   }
   wait_own_memory();
-  uint32_t *cnt = a.cnt + unit;
+  uint32_t *cnt = a.cnt + first;
   if (!split_arrive_last(cnt, ns)) return;
   float top = -__builtin_inff(), total = 0.0f;
   for (int y = 0; y < ns; ++y) {
@@ -566,7 +674,7 @@ hipError_t launch_tile(const AttnArgs &a, int tiles, hipStream_t s) {
       if (e != hipSuccess) return e;
     }
   }
-  IFX_LAUNCH(k_attn_tile, (DT, D, PAGED), dim3(a.Hkv * tiles, a.splits), dim3(64 * kNW), bytes, s, a);
+  IFX_LAUNCH(k_attn_tile, (DT, D, PAGED), dim3(a.Hkv * tiles), dim3(64 * kNW), bytes, s, a);
   return last_error();
 }
 template <int DT>
@@ -581,6 +689,7 @@ hipError_t launch_tile(const AttnArgs &a, int D, bool paged, int tiles, hipStrea
 }  // namespace
 
 int attn_tile_rows(int) { return kRows; }
+int attn_tile_min_keys() { return kMinChunk * TK; }
 int64_t attn_tile_slot_bytes(int D) { return kNW * (32 * D * 4 + 64 * 4 * 2); }
 
 hipError_t launch_attn_tile(const AttnArgs &a, int dtype, int D, bool paged, int tiles,

@@ -160,8 +160,9 @@ struct AttnArgs {
   int B, T, Hq, Hkv, G;
   int causal, window, out_dtype;
   float c;     // scale * log2(e)
-  int chunk;   // keys of a split
-  int splits;  // most splits of a request: grid and workspace slots
+  int chunk;   // attn_rows: keys of a split
+  int splits;  // attn_rows: most splits of a request, grid and workspace slots
+  int goal;    // attn_tile: about this many workgroups for a key/value head
   uint32_t *cnt;
   float *part;
   uint32_t part_bytes;
@@ -173,17 +174,18 @@ constexpr int kRowsMax = 32;   // rows of a request that attn_rows takes
 constexpr int kRowKeys = 128;  // attn_rows: keys that a workgroup's waves take at a time
 constexpr int kTileKeys = 64;  // attn_tile: keys of a stage
 
-// Keys of a split: the plan's, or more where a request is longer than the plan
+// attn_rows: keys of a split, the plan's, or more where a request is longer than the plan
 // was told, so that a.splits of them always suffice.
-__device__ __forceinline__ int split_chunk(const AttnArgs &a, int keys, int unit) {
+__device__ __forceinline__ int split_chunk(const AttnArgs &a, int keys) {
   if (keys <= static_cast<int64_t>(a.chunk) * a.splits) return a.chunk;
-  return (keys / a.splits / unit + 1) * unit;
+  return (keys / a.splits / kRowKeys + 1) * kRowKeys;
 }
 
 hipError_t launch_attn_rows(const AttnArgs &a, int dtype, int D, int max_rows, hipStream_t s);
 hipError_t launch_attn_tile(const AttnArgs &a, int dtype, int D, bool paged, int tiles,
                             hipStream_t s);
 int attn_tile_rows(int D);
+int attn_tile_min_keys();  // of a split
 int64_t attn_tile_slot_bytes(int D);
 
 }  // namespace ifx
