@@ -54,18 +54,28 @@ __device__ __forceinline__ int swap_v(int key) {
   return D == 64 ? (key & 2) << 1 : D == 96 ? 0 : (key & 3) << 2;
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  return v;
+// Inclusive sums over the lanes, in the vector unit's own lane moves: shifts by
+// 1, 2, 4, 8 within 16 lanes, then the last lane of each 16 to the next, and of
+// the first 32 to the others.
+__device__ __forceinline__ int add_of(int a, int b) { return a + b; }
+__device__ __forceinline__ float add_of(float a, float b) { return a + b; }
+template <int CTRL, int ROWS, class V>
+__device__ __forceinline__ V add_moved(V v) {
+  return add_of(v, __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(
+                       0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, false)));
 }
-__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(v, o);
-    v += lane >= o ? u : 0;
-  }
-  return v;
+template <class V>
+__device__ __forceinline__ V wave_scan(V v) {
+  v = add_moved<0x111, 0xF>(v);
+  v = add_moved<0x112, 0xF>(v);
+  v = add_moved<0x114, 0xF>(v);
+  v = add_moved<0x118, 0xF>(v);
+  v = add_moved<0x142, 0xA>(v);
+  return add_moved<0x143, 0xC>(v);
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(v)), 63));
 }
 
 // A piece of paged work: item `item` (chunk major) of request b's `tiles` row
@@ -77,11 +87,9 @@ struct Split {
 
 // Item i of the batch (for one key/value head), found by a wave from the
 // requests' {row tiles, stages}.  The work is cut so that about `goal` items
-// of one length come out: fewer leave compute units idle, more start a second
-// round.  Where the row tiles alone are more than that, only requests that are
-// longer than the average share are split.  At most 2 goal items belong to
-// split tiles: where a request of s > c stages is cut in chunks of c, they are
-// less than s / c + 1 < 2 s / c, and c is at least (sum of s) / goal.
+// of one length come out.  At most `goal` items belong to split tiles: all
+// items are no more, or else chunks are so long that a request of s > c stages,
+// cut in less than s / c + 1 < 2 s / c of them, leaves no more.
 constexpr int kMinChunk = 8;  // stages: what a chunk costs beside its keys
 __device__ __forceinline__ Split find_item(const int2 *reqs, int B, int i, int goal, int lane) {
   const int per = (B + 63) / 64, b0 = min(lane * per, B), b1 = min(b0 + per, B);
@@ -94,19 +102,23 @@ __device__ __forceinline__ Split find_item(const int2 *reqs, int B, int i, int g
       tiles += static_cast<float>(r.x);
       stages += static_cast<float>(r.x) * static_cast<float>(r.y);
     }
-    tiles = wave_sum(tiles);
-    chunk = max(kMinChunk, static_cast<int>(min(ceilf(wave_sum(stages) / goal), 1e7f)));
-    for (int tries = 0; tries < 3 && tiles < goal; ++tries) {
-      float items = 0.0f;
+    const float share = min(wave_sum(stages) / goal, 5e6f);
+    chunk = max(kMinChunk, static_cast<int>(share) + 1);
+    bool fits = false;
+    if (wave_sum(tiles) < goal) {
+      for (int tries = 0; tries < 3 && !fits; ++tries) {
+        float items = 0.0f;
 #pragma unroll 1
-      for (int b = b0; b < b1; ++b) {
-        const int2 r = reqs[b];
-        items += static_cast<float>(r.x * ((r.y + chunk - 1) / chunk));
+        for (int b = b0; b < b1; ++b) {
+          const int2 r = reqs[b];
+          items += static_cast<float>(r.x * ((r.y + chunk - 1) / chunk));
+        }
+        items = wave_sum(items);
+        fits = items <= goal;
+        if (!fits) chunk = max(chunk + 1, static_cast<int>(chunk * (items / goal)));
       }
-      items = wave_sum(items);
-      if (items <= goal) break;
-      chunk = max(chunk + 1, static_cast<int>(chunk * (items / goal)));
     }
+    if (!fits) chunk = max(chunk, static_cast<int>(2.0f * share) + 1);
     chunk = __builtin_amdgcn_readfirstlane(chunk);
   }
   int items = 0, slots = 0;
@@ -117,7 +129,7 @@ __device__ __forceinline__ Split find_item(const int2 *reqs, int B, int i, int g
     items += r.x * ns;
     slots += ns > 1 ? r.x * ns : 0;
   }
-  int at = wave_scan(items, lane) - items, slot = wave_scan(slots, lane) - slots;
+  int at = wave_scan(items) - items, slot = wave_scan(slots) - slots;
   Split f = {0, 0, 0, 0, 0, 0};
   const uint64_t has = __ballot(i >= at && i < at + items);
   if (!has) return f;
@@ -215,8 +227,8 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
   }
 
   // this lane's row sees [lo, hi]; rows behind the last repeat it
-  const int row = min(row0 + 32 * wave + n, R - 1), tok = row / a.G;
-  const int head = kvh * a.G + row - tok * a.G;
+  int row = min(row0 + 32 * wave + n, R - 1), tok = row / a.G;
+  int head = kvh * a.G + row - tok * a.G;
   const int hi = a.causal ? ctx + tok : kv - 1;
   const int lo = a.window > 0 ? max(0, ctx + tok - a.window + 1) : 0;
   const int hi_z = __builtin_amdgcn_readlane(hi, 31);  // some of the wave's rows see [lo_a, hi_z]
@@ -594,30 +606,38 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
   }
 
   l = halves_sum(l);
-  const bool none = hi < lo;  // the row sees no key
-  auto write = [&](float inv) {
-    if (row0 + 32 * wave + n >= R) return;
+  bool none = hi < lo;  // the row sees no key
+  bool own = row0 + 32 * wave + n < R;
+  auto write_dims = [&](int d, const f32x4 *v, float scale) {  // of one dim tile
+    if (!own) return;
     char *o = static_cast<char *>(a.out) +
               ((q0 + tok) * a.out_stride + static_cast<int64_t>(head) * D) * dtype_bytes(a.out_dtype);
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+    for (int g = 0; g < 4; ++g)
+      store4(o, a.out_dtype, 32 * d + 8 * g + 4 * h, none ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : v[g] * scale);
+  };
+  auto write = [&](float scale) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        f32x4 v;
+    for (int d = 0; d < ND; ++d) {
+      f32x4 v[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = none ? 0.0f : acc[d][4 * g + r] * inv;
-        store4(o, a.out_dtype, 32 * d + 8 * g + 4 * h, v);
-      }
+      for (int i = 0; i < 16; ++i) v[i >> 2][i & 3] = acc[d][i];
+      write_dims(d, v, scale);
+    }
   };
   if (!PAGED || ns == 1) return write(1.0f / l);
 
   // split: this chunk's sums to its slot, every lane in its own places; the
-  // last workgroup of the tile adds the chunks in their order, lane by lane
+  // last workgroup of the tile adds the chunks in their order, lane by lane.
+  // Lanes without a row have their places behind the buffer's end: they write
+  // nothing and read zeros.
   const rsrc_t part = make_rsrc(a.part, a.part_bytes);
   constexpr uint32_t kWaveBytes = 32 * D * 4 + 64 * 4 * 2, kSlotBytes = kNW * kWaveBytes;
   const uint32_t first = split.slot * a.Hkv + (tile * a.Hkv + kvh) * split.ns;  // the tile's slots
-  const uint32_t mine = first * kSlotBytes + wave * kWaveBytes + lane * 16;
-  const uint32_t mine_ml = first * kSlotBytes + wave * kWaveBytes + 32 * D * 4 + lane * 8;
+  constexpr uint32_t kOut = 1u << 30;
+  const uint32_t out = row0 + 32 * wave + n < R ? 0 : kOut;
+  uint32_t mine = (first * kSlotBytes + wave * kWaveBytes + lane * 16) | out;
+  uint32_t mine_ml = (first * kSlotBytes + wave * kWaveBytes + 32 * D * 4 + lane * 8) | out;
   {
     const uint32_t at = mine + z * kSlotBytes;
 #pragma unroll
@@ -632,31 +652,87 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
   wait_own_memory();
   uint32_t *cnt = a.cnt + first;
   if (!split_arrive_last(cnt, ns)) return;
+  const bool few = R - row0 <= 32;  // all rows are the first wave's: the waves share the dims
+  if (few) {
+    row = min(row0 + n, R - 1), tok = row / a.G, head = kvh * a.G + row - tok * a.G;
+    own = row0 + n < R;
+    none = a.causal && ctx + tok < 0;  // a row that sees any sees itself
+    const uint32_t at = first * kSlotBytes | (own ? 0 : kOut);
+    mine = at + lane * 16, mine_ml = at + 32 * D * 4 + lane * 8;
+  }
+  auto ml_of = [&](int y) {  // of chunk y, and past the last of none
+    return __builtin_bit_cast(
+        float2, __builtin_amdgcn_raw_buffer_load_b64(
+                    part, y < ns ? mine_ml + y * kSlotBytes : kOut, 0, kAuxDevice));
+  };
+  // Reads past the L2 take a microsecond: several at a time
   float top = -__builtin_inff(), total = 0.0f;
-  for (int y = 0; y < ns; ++y) {
-    const float2 ml = __builtin_bit_cast(
-        float2, __builtin_amdgcn_raw_buffer_load_b64(part, mine_ml + y * kSlotBytes, 0, kAuxDevice));
-    const float mn = fmaxf(top, ml.x);
-    total = total * weight(top, mn, a.c) + ml.y * weight(ml.x, mn, a.c);
-    top = mn;
+  for (int y0 = 0; y0 < ns; y0 += 8) {
+    float2 ml[8];
+#pragma unroll
+    for (int y = 0; y < 8; ++y) ml[y] = ml_of(y0 + y);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int y = 0; y < 8; ++y) {
+      const float my = y0 + y < ns ? ml[y].x : -__builtin_inff();
+      const float mn = fmaxf(top, my);
+      total = total * weight(top, mn, a.c) + ml[y].y * weight(my, mn, a.c);
+      top = mn;
+    }
+  }
+  if (few) {
+#pragma unroll 1
+    for (int d = wave; d < ND; d += kNW) {
+      f32x4 o[4] = {};
+      for (int y0 = 0; y0 < ns; y0 += 4) {
+        float2 ml[4];
+        f32x4 v[4][4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          ml[y] = ml_of(y0 + y);
+          const uint32_t at = y0 + y < ns ? mine + (y0 + y) * kSlotBytes + d * 4096 : kOut;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) v[y][g] = ld_dev4(part, at + g * 1024);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const float w = y0 + y < ns ? weight(ml[y].x, top, a.c) : 0.0f;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) o[g] += v[y][g] * w;
+        }
+      }
+      write_dims(d, o, 1.0f / total);
+    }
+    return split_reset(cnt);
   }
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
-  for (int y = 0; y < ns; ++y) {
-    const float2 ml = __builtin_bit_cast(
-        float2, __builtin_amdgcn_raw_buffer_load_b64(part, mine_ml + y * kSlotBytes, 0, kAuxDevice));
-    const float w = weight(ml.x, top, a.c);
-    const uint32_t at = mine + y * kSlotBytes;
+  for (int y = 0; y < ns; y += 2) {
+    constexpr int kAtOnce = ND < 4 ? ND : 4;  // dim tiles
+    const float2 ml0 = ml_of(y), ml1 = ml_of(y + 1);
+    const uint32_t at0 = mine + y * kSlotBytes;
+    const uint32_t at1 = y + 1 < ns ? at0 + kSlotBytes : kOut;
+    const float w0 = weight(ml0.x, top, a.c), w1 = y + 1 < ns ? weight(ml1.x, top, a.c) : 0.0f;
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+    for (int d0 = 0; d0 < ND; d0 += kAtOnce) {
+      f32x4 v0[4 * kAtOnce], v1[4 * kAtOnce];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 v = ld_dev4(part, at + (4 * d + g) * 1024);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[d][4 * g + r] += v[r] * w;
+      for (int i = 0; i < 4 * kAtOnce && 4 * d0 + i < 4 * ND; ++i) {
+        v0[i] = ld_dev4(part, at0 + (4 * d0 + i) * 1024);
+        v1[i] = ld_dev4(part, at1 + (4 * d0 + i) * 1024);
       }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 4 * kAtOnce && 4 * d0 + i < 4 * ND; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int d = d0 + (i >> 2), j = 4 * (i & 3) + r;
+          acc[d][j] = (acc[d][j] + v0[i][r] * w0) + v1[i][r] * w1;
+        }
+    }
   }
   write(1.0f / total);
   split_reset(cnt);
