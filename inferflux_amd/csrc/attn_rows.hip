@@ -87,10 +87,18 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const AttnArgs a, int lds_
   const uint16_t *V = static_cast<const uint16_t *>(a.v) + ((static_cast<int64_t>(kvh) * D) << sh);
   const int wmax = a.table_width - 1;
 
+  // The pages of a tile's two 16-key halves, as the table has them: read a tile
+  // ahead, looked at when that tile's loads are issued.
+  int next0 = 0, next1 = 0;
+  auto entries = [&](int k0) {
+    next0 = table[min(k0 >> sh, wmax)];
+    next1 = table[min((k0 + 16) >> sh, wmax)];
+  };
+  entries(zbeg + 32 * wave);
   for (int k0 = zbeg + 32 * wave; k0 < zend; k0 += 32 * kWaves) {
-    // the pages of the tile's two 16-key halves
-    const int pg0 = min(max(table[min(k0 >> sh, wmax)], 0), last_page);
-    const int pg1 = min(max(table[min((k0 + 16) >> sh, wmax)], 0), last_page);
+    const int pg0 = min(max(next0, 0), last_page);
+    const int pg1 = min(max(next1, 0), last_page);
+    entries(k0 + 32 * kWaves);
     const int64_t e0 = pg0 * page_elems, e1 = pg1 * page_elems;
     u32x4 kf[NS], vf[2][ND];
     {

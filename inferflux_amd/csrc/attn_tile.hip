@@ -19,6 +19,9 @@ namespace ifx {
 
 namespace {
 
+// Lambdas that are calls would keep what they capture in memory.
+#define IFX_INLINE __attribute__((always_inline))
+
 constexpr int kNW = 4;             // waves of a workgroup
 constexpr int kRows = 32 * kNW;    // its query rows
 constexpr int TK = kTileKeys;
@@ -281,7 +284,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
     int page, k0, buf;
     rsrc_t rk, rv;   // packed rows: those behind the request's last read as 0
   };
-  auto source = [&](int k0, int entry, int buf) {
+  auto source = [&](int k0, int entry, int buf) IFX_INLINE {
     Source f;
     f.k0 = k0, f.buf = buf;
     if constexpr (PAGED) {
@@ -296,7 +299,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
     }
     return f;
   };
-  auto copy = [&](const Source &f, int j) {
+  auto copy = [&](const Source &f, int j) IFX_INLINE {
     const int i = j >> 1, n0 = i * kNW + wave;  // 64 pieces
     u32x4 *sk = lds + f.buf * 2 * kPieces + n0 * 64, *sv = sk + kPieces;
     if constexpr (PAGED) {
@@ -340,12 +343,12 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
   const int v_lane = PAGED ? (h * D + n) * 16
                            : (8 * h + (ti >> 2)) * NP * 16 + ((lane & 16) >> 3) * 16 + (ti & 3) * 8;
   const int v_swap = PAGED ? 0 : swap_v<D>(ti >> 2) * 16;
-  auto k_at = [&](const char *sk, int sub, int s, int swap) {
+  auto k_at = [&](const char *sk, int sub, int s, int swap) IFX_INLINE {
     const char *p = PAGED ? sk + (k_lane + (2 * s * TK + 32 * sub) * 16)
                           : sk + ((swap ^ (32 * s)) + k_lane) + 32 * sub * NP * 16;
     return *reinterpret_cast<const u32x4 *>(p);
   };
-  auto v_at = [&](const char *sv, int ks, int d) -> u32x4 {
+  auto v_at = [&](const char *sv, int ks, int d) IFX_INLINE -> u32x4 {
     if constexpr (PAGED) {
       return *reinterpret_cast<const u32x4 *>(sv + (v_lane + (2 * ks * D + 32 * d) * 16));
     } else {
@@ -359,7 +362,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
     }
   };
   // the same without what lies behind the last token: a page's unwritten slots
-  auto v_in = [&](int k0, const char *sv, int ks, int d) -> u32x4 {
+  auto v_in = [&](int k0, const char *sv, int ks, int d) IFX_INLINE -> u32x4 {
     u32x4 r = v_at(sv, ks, d);
     if constexpr (PAGED) {
       const int key = k0 + 16 * ks + 8 * h;
@@ -371,7 +374,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
   };
   // Raises the running maximum where a stage's is far enough above it; what the
   // exponents are then taken relative to.
-  auto raise = [&](float mt) {
+  auto raise = [&](float mt) IFX_INLINE {
     mt = halves_max(mt);
     if (__any((mt - m) * a.c > kLag)) {
       const float mn = fmaxf(m, mt);
@@ -390,7 +393,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
   // next(j), j < 2 NL, issues the next stage's copies, one at a time between the
   // first products: a wave waits at its next copy until the last is under way.
   const f32x16 none_yet = {};
-  auto step = [&](const char *sk, const char *sv, auto next) {
+  auto step = [&](const char *sk, const char *sv, auto next) IFX_INLINE {
     constexpr int kAhead = 4;
     f32x16 s[2];
     u32x4 f[4 * NS];  // K of both halves, V: at most kAhead + 1 are alive
@@ -457,7 +460,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
 
   // One stage of which some rows see only a part.
   bool tainted = false;
-  auto edge_step = [&](int k0, const char *sk, const char *sv) {
+  auto edge_step = [&](int k0, const char *sk, const char *sv) IFX_INLINE {
     f32x16 s[2];
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
@@ -515,7 +518,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
     }
     if constexpr (PAGED) entry = entry_of(zbeg + TK);
     // Stages up to `until`.  (`last`: a stage among them may have no successor.)
-    auto stages = [&](int until, auto edge_c, auto last_c) {
+    auto stages = [&](int until, auto edge_c, auto last_c) IFX_INLINE {
       for (; k0 < until; k0 += TK, buf ^= 1) {
         wait_own_memory();
         __syncthreads();  // this stage is in LDS, and no wave reads the other one
@@ -608,7 +611,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
   l = halves_sum(l);
   bool none = hi < lo;  // the row sees no key
   bool own = row0 + 32 * wave + n < R;
-  auto write_dims = [&](int d, const f32x4 *v, float scale) {  // of one dim tile
+  auto write_dims = [&](int d, const f32x4 *v, float scale) IFX_INLINE {  // of one dim tile
     if (!own) return;
     char *o = static_cast<char *>(a.out) +
               ((q0 + tok) * a.out_stride + static_cast<int64_t>(head) * D) * dtype_bytes(a.out_dtype);
@@ -616,7 +619,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
     for (int g = 0; g < 4; ++g)
       store4(o, a.out_dtype, 32 * d + 8 * g + 4 * h, none ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : v[g] * scale);
   };
-  auto write = [&](float scale) {
+  auto write = [&](float scale) IFX_INLINE {
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       f32x4 v[4];
