@@ -55,52 +55,45 @@ constexpr int kMaxUnits = 8192;
 constexpr int64_t kCntBytes = kMaxUnits * 4;
 
 struct PagedPlan {
-  bool rows;          // attn_rows, else attn_tile
-  int chunk, splits;  // attn_rows
-  int tiles, goal;    // attn_tile: workgroups of a key/value head, those of split tiles
-  int64_t bytes;      // of workspace
+  bool rows;         // attn_rows, else attn_tile
+  int goal, items;   // AttnArgs; workgroups of a key/value head
+  int64_t bytes;     // of workspace
 };
 
-int round_up(int64_t n, int to) { return static_cast<int>((n + to - 1) / to * to); }
-
-// How ifx_attn_paged's keys are split over workgroups.
+// How ifx_attn_paged's keys are split over workgroups: about `goal` work items
+// for each key/value head, whose lengths the workgroups find (find_item).
 //
-// attn_rows: about 2048 workgroups of 128 keys at least, four rounds of the 512
-// that are resident, as requests differ in length (32 requests of 531 to 22591
-// keys, 40 / 8 heads of 128: 187 us; 1024: 204, 4096: 187, 8192: 199).
+// attn_tile: as many as are resident, two a CU (D = 64: three, D = 256: one).
+// A chunk of 512 tokens over 7430 keys, 40 / 8 heads of 128: 114 us with 512,
+// 116 with 768, 124 with 1000.
 //
-// attn_tile: as many workgroups as are resident, two a CU (D = 64: three,
-// D = 256: one); each finds its share (find_item).  A chunk of 512 tokens over
-// 7430 keys, 40 / 8 heads of 128: 114 us with 512, 116 with 768, 124 with 1000.
+// attn_rows: two rounds of those that are resident, as requests differ in
+// length.  32 requests of 531 to 22591 keys, 40 / 8 heads of 128: 167 us with
+// 512, 152 with 768, 151 with 1024, 156 with 1536, 160 with 2048.
 //
 // Fewer where the split sums would not fit the largest workspace.
 PagedPlan plan_paged(int B, int T, int Hq, int Hkv, int D, int max_q, int max_kv) {
   PagedPlan p{};
   const int G = Hq / Hkv;
   const int64_t rows = static_cast<int64_t>(max_q) * G;
-  constexpr int64_t space = IFX_ATTN_WORKSPACE_BYTES - kCntBytes;
   p.rows = rows <= kRowsMax;
-  if (p.rows) {
-    const int64_t units = static_cast<int64_t>(B) * Hkv, slot = rows * (D + 4) * 4;
-    int64_t splits = (2048 + units - 1) / units;
-    if (splits > 128) splits = 128;
-    if (splits > space / (units * slot)) splits = space / (units * slot);
-    if (units > kMaxUnits || splits < 1) splits = 1;
-    p.chunk = round_up((max_kv + splits - 1) / splits, kRowKeys);
-    p.splits = splits > 1 ? (max_kv + p.chunk - 1) / p.chunk : 1;
-    p.bytes = p.splits > 1 ? kCntBytes + units * p.splits * slot : 0;
-  } else {
-    const int64_t rounds = static_cast<int64_t>(T) * G / attn_tile_rows(D) + B;
-    const int64_t slot = attn_tile_slot_bytes(D);
-    // `goal` items of a key/value head have a slot and a counter (find_item)
-    int64_t goal = (D == 256 ? 256 : D == 64 ? 768 : 512) / Hkv;
-    if (goal > space / slot / Hkv) goal = space / slot / Hkv;
-    const int64_t use = rounds * ((max_kv + attn_tile_min_keys() - 1) / attn_tile_min_keys());
-    p.goal = static_cast<int>(goal < use ? goal : use);
-    if (max_kv <= attn_tile_min_keys()) p.goal = 0;
-    p.tiles = static_cast<int>(rounds) + p.goal;
-    p.bytes = p.goal ? kCntBytes + p.goal * Hkv * slot : 0;
-  }
+  // row tiles, stages of the longest request that a split must have, bytes of a slot
+  const int64_t tiles = p.rows ? B : static_cast<int64_t>(T) * G / attn_tile_rows(D) + B;
+  const int unit = p.rows ? kRowKeys : attn_tile_min_keys();
+  const int64_t slot = p.rows ? rows * (D + 4) * 4 : attn_tile_slot_bytes(D);
+  const int all = p.rows ? 1024 : D == 256 ? 256 : D == 64 ? 768 : 512;
+  int64_t goal = all / Hkv;
+  const int64_t use = tiles * ((static_cast<int64_t>(max_kv) + unit - 1) / unit);
+  const int64_t fit = (IFX_ATTN_WORKSPACE_BYTES - kCntBytes) / slot / Hkv;
+  if (goal > use) goal = use;
+  if (goal > fit) goal = fit;
+  if (goal > kMaxUnits / Hkv) goal = kMaxUnits / Hkv;
+  if (p.rows && goal > attn_rows_max_goal(static_cast<int>(rows)))
+    goal = attn_rows_max_goal(static_cast<int>(rows));
+  if (max_kv <= unit) goal = 0;
+  p.goal = static_cast<int>(goal);
+  p.items = static_cast<int>(tiles + goal);
+  p.bytes = goal ? kCntBytes + goal * Hkv * slot : 0;
   return p;
 }
 
@@ -199,15 +192,15 @@ int ifx_attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cac
   a.B = B, a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv;
   a.causal = 1, a.window = window, a.out_dtype = out_dtype;
   a.c = scale * kLog2e;
-  a.chunk = p.chunk, a.splits = p.splits, a.goal = p.goal;
+  a.goal = p.goal;
   if (p.bytes) {
     a.cnt = static_cast<uint32_t *>(workspace);
     a.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + kCntBytes);
     a.part_bytes = static_cast<uint32_t>(p.bytes - kCntBytes);
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (p.rows) return status_of(launch_attn_rows(a, dtype, D, max_q * a.G, s));
-  return status_of(launch_attn_tile(a, dtype, D, true, p.tiles, s));
+  if (p.rows) return status_of(launch_attn_rows(a, dtype, D, max_q * a.G, p.items, s));
+  return status_of(launch_attn_tile(a, dtype, D, true, p.items, s));
 }
 
 int ifx_attn_prompt(const void *q, int64_t q_stride, const void *k, int64_t k_stride,

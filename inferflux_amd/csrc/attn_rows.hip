@@ -21,6 +21,7 @@ namespace ifx {
 namespace {
 
 constexpr int kWaves = 4;
+constexpr uint32_t kOut = 1u << 30;  // an offset past the workspace's end: reads zeros
 
 // The four dwords of an 8-key piece with the keys outside [lo, hi] cleared.
 struct PieceMask {
@@ -39,24 +40,30 @@ __device__ __forceinline__ PieceMask piece_mask(int key, int lo, int hi) {
 }  // namespace
 
 template <int DT, int D>
-__global__ __launch_bounds__(256, 2) void k_attn_rows(const AttnArgs a, int lds_rows) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(const AttnArgs a, int lds_rows) {
   using T = Elem<DT>;
   constexpr int ND = D / 32, NS = D / 16;
-  extern __shared__ float red[];  // [wave][D / 4][row][4]
+  extern __shared__ float red[];  // [wave][D / 4][row][4]; at first the requests
   __shared__ float red_m[kWaves][32], red_l[kWaves][32];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kvh = blockIdx.x, b = blockIdx.y, z = blockIdx.z;
+  const int kvh = blockIdx.x % a.Hkv;
   const int sh = a.page_shift, P = 1 << sh;
 
-  const int q0 = min(max(a.cu[b], 0), a.T), q1 = min(max(a.cu[b + 1], 0), a.T);
-  const int kv = min(max(a.kv_len[b], 0), a.table_width << sh);
-  const int nq = q1 - q0, R = min(nq * a.G, lds_rows);
-  if (nq <= 0) return;
+  // the workgroup's request and chunk of its keys
+  const Split split = find_item<1>(
+      a, reinterpret_cast<int2 *>(red), blockIdx.x / a.Hkv, [&](const Request &r) {
+        int keys = r.kv;
+        if (a.window > 0) keys = min<int64_t>(keys, static_cast<int64_t>(a.window) + r.nq + kRowKeys);
+        return make_int2(r.nq > 0 ? 1 : 0, max(1, (keys + kRowKeys - 1) / kRowKeys));
+      });
+  if (split.chunk == 0) return;
+  const int b = split.b, z = split.item;
+  const int q0 = split.req.q0, nq = split.req.nq, kv = split.req.kv, R = min(nq * a.G, lds_rows);
   const int ctx = kv - nq;  // position of the first row; below 0 it sees nothing
   const int lo0 = a.window > 0 ? max(0, ctx - a.window + 1) : 0;
   const int kbeg = lo0 & ~(kRowKeys - 1), kend = kv;  // the last row sees kv - 1
-  const int chunk = split_chunk(a, kend - kbeg);
+  const int chunk = split.chunk * kRowKeys;
   const int ns = kend > kbeg ? (kend - kbeg + chunk - 1) / chunk : 1;
   if (z >= ns) return;
   const int zbeg = kbeg + z * chunk, zend = min(zbeg + chunk, kend);
@@ -264,7 +271,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const AttnArgs a, int lds_
   // split: this chunk's sums to its slot, (m, l) of its rows behind them
   const rsrc_t part = make_rsrc(a.part, a.part_bytes);
   const uint32_t slot_bytes = lds_rows * (D + 4) * 4;
-  const uint32_t slot0 = static_cast<uint32_t>((b * a.Hkv + kvh) * a.splits) * slot_bytes;
+  const uint32_t first = split.slot * a.Hkv + kvh * split.ns;  // the request's slots
+  const uint32_t slot0 = first * slot_bytes;
   const uint32_t slot = slot0 + z * slot_bytes;
   for (int i = tid; i < elems; i += 256) {
     const int r = i % R, d4 = i / R;
@@ -275,49 +283,81 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(const AttnArgs a, int lds_
   }
   if (tid < R) st_dev4(part, slot + (elems + tid) * 16, f32x4{red_m[0][tid], red_l[0][tid], 0.0f, 0.0f});
   wait_own_memory();
-  uint32_t *cnt = a.cnt + b * a.Hkv + kvh;
+  uint32_t *cnt = a.cnt + first;
   if (!split_arrive_last(cnt, ns)) return;
-  // every chunk's (m, l) to LDS, then each row's total and the chunks' weights
-  float *ml = red;  // [row + R * chunk][2]: the waves' sums are no longer needed
-  for (int i = tid; i < R * ns; i += 256) {
-    const int y = i / R;
-    const f32x4 v = ld_dev4(part, slot0 + y * slot_bytes + (elems + i - y * R) * 16);
-    ml[2 * i] = v.x;
-    ml[2 * i + 1] = v.y;
-  }
-  __syncthreads();
-  if (tid < R) {
+  // Reads past the L2 take a microsecond: a thread's first sums are on their way
+  // while the chunks' weights are formed.
+  constexpr int kAtOnce = 24;
+  f32x4 v[kAtOnce];
+  auto read = [&](int i, int y0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int y = 0; y < kAtOnce; ++y)
+      v[y] = ld_dev4(part, i < elems && y0 + y < ns ? slot0 + (y0 + y) * slot_bytes + i * 16 : kOut);
+  };
+  read(tid, 0);
+  __builtin_amdgcn_sched_barrier(0);
+  // [chunk][row] maximum, then weight, and sum: the waves' sums are no longer needed
+  float2 *ml = reinterpret_cast<float2 *>(red);
+  {
+    const int r = tid >> 3, j = tid & 7;  // eight lanes for a row
     float mx = -__builtin_inff(), sum = 0.0f;
-    for (int y = 0; y < ns; ++y) mx = fmaxf(mx, ml[2 * (y * R + tid)]);
-    for (int y = 0; y < ns; ++y) sum += ml[2 * (y * R + tid) + 1] * weight(ml[2 * (y * R + tid)], mx, a.c);
-    red_m[0][tid] = mx;
-    red_l[0][tid] = 1.0f / sum;
-  }
-  __syncthreads();
-  for (int i = tid; i < R * ns; i += 256) {
-    const int r = i % R;
-    ml[2 * i] = weight(ml[2 * i], red_m[0][r], a.c) * red_l[0][r];
+    if (r < R) {
+      for (int y0 = j; y0 < ns; y0 += 32) {
+        f32x4 u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int y = y0 + 8 * i;
+          u[i] = ld_dev4(part, y < ns ? slot0 + y * slot_bytes + (elems + r) * 16 : kOut);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int y = y0 + 8 * i;
+          if (y < ns) {
+            ml[y * R + r] = make_float2(u[i].x, u[i].y);
+            mx = fmaxf(mx, u[i].x);
+          }
+        }
+      }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+      for (int y = j; y < ns; y += 8) {
+        const float2 u = ml[y * R + r];
+        const float w = weight(u.x, mx, a.c);
+        ml[y * R + r].x = w;
+        sum += u.y * w;
+      }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor(sum, o);
+      if (j == 0) red_l[0][r] = 1.0f / sum;
+    }
   }
   __syncthreads();
   for (int i = tid; i < elems; i += 256) {
     const int r = i % R, d4 = i / R, t = r / a.G;
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int y = 0; y < ns; ++y) v += ld_dev4(part, slot0 + y * slot_bytes + i * 16) * ml[2 * (y * R + r)];
-    if (ctx + t < 0) v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    char *o = static_cast<char *>(a.out) +
-              ((q0 + t) * a.out_stride + static_cast<int64_t>(head0 + r % a.G) * D) *
-                  dtype_bytes(a.out_dtype);
-    store4(o, a.out_dtype, d4 * 4, v);
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int y0 = 0; y0 < ns; y0 += kAtOnce) {
+      if (i != tid || y0) read(i, y0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int y = 0; y < kAtOnce; ++y) o += v[y] * (y0 + y < ns ? ml[(y0 + y) * R + r].x : 0.0f);
+    }
+    o = ctx + t < 0 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : o * red_l[0][r];
+    char *to = static_cast<char *>(a.out) +
+               ((q0 + t) * a.out_stride + static_cast<int64_t>(head0 + r % a.G) * D) *
+                   dtype_bytes(a.out_dtype);
+    store4(to, a.out_dtype, d4 * 4, o);
   }
   split_reset(cnt);
 }
 
 namespace {
+constexpr int kMaxLds = 65536 - 2048;  // what a launch may ask for without more ado
+
 template <int DT, int D>
-hipError_t launch_rows(const AttnArgs &a, int max_rows, hipStream_t s) {
+hipError_t launch_rows(const AttnArgs &a, int max_rows, int items, hipStream_t s) {
   constexpr int row_bytes = kWaves * D * 4;  // LDS of a row: the waves' sums
-  if constexpr (row_bytes * kRowsMax > 65536) {
+  if constexpr (row_bytes * kRowsMax > kMaxLds) {
     static std::atomic<uint64_t> done{0};
     if (!dry_run()) {
       const hipError_t e = allow_lds(reinterpret_cast<const void *>(&k_attn_rows<DT, D>),
@@ -325,24 +365,30 @@ hipError_t launch_rows(const AttnArgs &a, int max_rows, hipStream_t s) {
       if (e != hipSuccess) return e;
     }
   }
-  IFX_LAUNCH(k_attn_rows, (DT, D), dim3(a.Hkv, a.B, a.splits), dim3(64 * kWaves),
-             static_cast<size_t>(row_bytes) * max_rows, s, a, max_rows);
+  // the waves' sums; before them the requests, after them the chunks' weights and sums
+  int bytes = row_bytes * max_rows;
+  if (bytes < a.B * 8) bytes = a.B * 8;
+  if (bytes < a.goal * max_rows * 8) bytes = a.goal * max_rows * 8;
+  IFX_LAUNCH(k_attn_rows, (DT, D), dim3(a.Hkv * items), dim3(64 * kWaves), bytes, s, a, max_rows);
   return last_error();
 }
 template <int DT>
-hipError_t launch_rows(const AttnArgs &a, int D, int max_rows, hipStream_t s) {
+hipError_t launch_rows(const AttnArgs &a, int D, int max_rows, int items, hipStream_t s) {
   switch (D) {
-    case 64: return launch_rows<DT, 64>(a, max_rows, s);
-    case 96: return launch_rows<DT, 96>(a, max_rows, s);
-    case 128: return launch_rows<DT, 128>(a, max_rows, s);
-    default: return launch_rows<DT, 256>(a, max_rows, s);
+    case 64: return launch_rows<DT, 64>(a, max_rows, items, s);
+    case 96: return launch_rows<DT, 96>(a, max_rows, items, s);
+    case 128: return launch_rows<DT, 128>(a, max_rows, items, s);
+    default: return launch_rows<DT, 256>(a, max_rows, items, s);
   }
 }
 }  // namespace
 
-hipError_t launch_attn_rows(const AttnArgs &a, int dtype, int D, int max_rows, hipStream_t s) {
-  return dtype == IFX_ATTN_F16 ? launch_rows<IFX_ATTN_F16>(a, D, max_rows, s)
-                               : launch_rows<IFX_ATTN_BF16>(a, D, max_rows, s);
+int attn_rows_max_goal(int max_rows) { return kMaxLds / 8 / max_rows; }
+
+hipError_t launch_attn_rows(const AttnArgs &a, int dtype, int D, int max_rows, int items,
+                            hipStream_t s) {
+  return dtype == IFX_ATTN_F16 ? launch_rows<IFX_ATTN_F16>(a, D, max_rows, items, s)
+                               : launch_rows<IFX_ATTN_BF16>(a, D, max_rows, items, s);
 }
 
 }  // namespace ifx

@@ -25,6 +25,7 @@ namespace {
 constexpr int kNW = 4;             // waves of a workgroup
 constexpr int kRows = 32 * kNW;    // its query rows
 constexpr int TK = kTileKeys;
+constexpr int kMinChunk = 8;  // stages: what a chunk costs beside its keys
 
 // LDS places, in 16-byte pieces of 8 values.  Copies go from memory to LDS
 // past the registers.
@@ -57,104 +58,6 @@ __device__ __forceinline__ int swap_v(int key) {
   return D == 64 ? (key & 2) << 1 : D == 96 ? 0 : (key & 3) << 2;
 }
 
-// Inclusive sums over the lanes, in the vector unit's own lane moves: shifts by
-// 1, 2, 4, 8 within 16 lanes, then the last lane of each 16 to the next, and of
-// the first 32 to the others.
-__device__ __forceinline__ int add_of(int a, int b) { return a + b; }
-__device__ __forceinline__ float add_of(float a, float b) { return a + b; }
-template <int CTRL, int ROWS, class V>
-__device__ __forceinline__ V add_moved(V v) {
-  return add_of(v, __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(
-                       0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, false)));
-}
-template <class V>
-__device__ __forceinline__ V wave_scan(V v) {
-  v = add_moved<0x111, 0xF>(v);
-  v = add_moved<0x112, 0xF>(v);
-  v = add_moved<0x114, 0xF>(v);
-  v = add_moved<0x118, 0xF>(v);
-  v = add_moved<0x142, 0xA>(v);
-  return add_moved<0x143, 0xC>(v);
-}
-__device__ __forceinline__ float wave_sum(float v) {
-  return __builtin_bit_cast(
-      float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(v)), 63));
-}
-
-// A piece of paged work: item `item` (chunk major) of request b's `tiles` row
-// tiles x ns chunks of `chunk` stages.  chunk is 0 where there is no such item.
-struct Split {
-  int chunk, ns, slot;  // slot: of the split sums of the request's first tile
-  int b, item, tiles;
-};
-
-// Item i of the batch (for one key/value head), found by a wave from the
-// requests' {row tiles, stages}.  The work is cut so that about `goal` items
-// of one length come out.  At most `goal` items belong to split tiles: all
-// items are no more, or else chunks are so long that a request of s > c stages,
-// cut in less than s / c + 1 < 2 s / c of them, leaves no more.
-constexpr int kMinChunk = 8;  // stages: what a chunk costs beside its keys
-__device__ __forceinline__ Split find_item(const int2 *reqs, int B, int i, int goal, int lane) {
-  const int per = (B + 63) / 64, b0 = min(lane * per, B), b1 = min(b0 + per, B);
-  int chunk = 1 << 24;
-  if (goal > 0) {
-    float stages = 0.0f, tiles = 0.0f;
-#pragma unroll 1
-    for (int b = b0; b < b1; ++b) {
-      const int2 r = reqs[b];
-      tiles += static_cast<float>(r.x);
-      stages += static_cast<float>(r.x) * static_cast<float>(r.y);
-    }
-    const float share = min(wave_sum(stages) / goal, 5e6f);
-    chunk = max(kMinChunk, static_cast<int>(share) + 1);
-    bool fits = false;
-    if (wave_sum(tiles) < goal) {
-      for (int tries = 0; tries < 3 && !fits; ++tries) {
-        float items = 0.0f;
-#pragma unroll 1
-        for (int b = b0; b < b1; ++b) {
-          const int2 r = reqs[b];
-          items += static_cast<float>(r.x * ((r.y + chunk - 1) / chunk));
-        }
-        items = wave_sum(items);
-        fits = items <= goal;
-        if (!fits) chunk = max(chunk + 1, static_cast<int>(chunk * (items / goal)));
-      }
-    }
-    if (!fits) chunk = max(chunk, static_cast<int>(2.0f * share) + 1);
-    chunk = __builtin_amdgcn_readfirstlane(chunk);
-  }
-  int items = 0, slots = 0;
-#pragma unroll 1
-  for (int b = b0; b < b1; ++b) {
-    const int2 r = reqs[b];
-    const int ns = (r.y + chunk - 1) / chunk;
-    items += r.x * ns;
-    slots += ns > 1 ? r.x * ns : 0;
-  }
-  int at = wave_scan(items) - items, slot = wave_scan(slots) - slots;
-  Split f = {0, 0, 0, 0, 0, 0};
-  const uint64_t has = __ballot(i >= at && i < at + items);
-  if (!has) return f;
-  const int who = __builtin_ctzll(has);
-  at = __builtin_amdgcn_readlane(at, who), slot = __builtin_amdgcn_readlane(slot, who);
-  for (int b = who * per;; ++b) {
-    const int2 r = reqs[b];
-    const int ns = (r.y + chunk - 1) / chunk, n = r.x * ns;
-    if (i < at + n) {
-      f.chunk = __builtin_amdgcn_readfirstlane((r.y + ns - 1) / ns);  // of equal length
-      f.ns = __builtin_amdgcn_readfirstlane(ns);
-      f.slot = __builtin_amdgcn_readfirstlane(slot);
-      f.b = __builtin_amdgcn_readfirstlane(b);
-      f.item = __builtin_amdgcn_readfirstlane(i - at);
-      f.tiles = __builtin_amdgcn_readfirstlane(r.x);
-      return f;
-    }
-    at += n;
-    slot += ns > 1 ? n : 0;
-  }
-}
-
 }  // namespace
 
 template <int DT, int D, bool PAGED>
@@ -169,23 +72,16 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kvh = blockIdx.x % a.Hkv;
 
-  // Which rows and keys.  No list of work is built beforehand: each workgroup
-  // finds its own.
   int b, tile, z = 0;  // request, its row tile, its chunk of the keys
-  Split split = {1 << 24, 1, 0};
+  Split split = {};
   if constexpr (PAGED) {
-    int2 *reqs = reinterpret_cast<int2 *>(lds);
-    for (int i = tid; i < a.B; i += 64 * kNW) {
-      const int c0 = min(max(a.cu[i], 0), a.T), c1 = min(max(a.cu[i + 1], 0), a.T);
-      const int tiles = (max(c1 - c0, 0) * a.G + kRows - 1) / kRows;
-      int keys = min(max(a.kv_len[i], 0), a.table_width << a.page_shift);
-      if (a.window > 0) keys = min<int64_t>(keys, static_cast<int64_t>(a.window) + kRows + TK);
-      reqs[i] = make_int2(tiles, max(1, (keys + TK - 1) / TK));
-    }
-    __syncthreads();
-    split = find_item(reqs, a.B, blockIdx.x / a.Hkv, a.goal, lane);
+    split = find_item<kMinChunk>(
+        a, reinterpret_cast<int2 *>(lds), blockIdx.x / a.Hkv, [&](const Request &r) {
+          int keys = r.kv;  // that a tile sees
+          if (a.window > 0) keys = min<int64_t>(keys, static_cast<int64_t>(a.window) + kRows + TK);
+          return make_int2((r.nq * a.G + kRows - 1) / kRows, max(1, (keys + TK - 1) / TK));
+        });
     if (split.chunk == 0) return;
-    __syncthreads();  // reqs is read, stages may come
     b = split.b, z = split.item / split.tiles;
     tile = split.tiles - 1 - (split.item - z * split.tiles);  // late tiles first
   } else {
@@ -206,12 +102,11 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
     b = __builtin_amdgcn_readfirstlane(found[0]);
     if (b < 0) return;
     tile = __builtin_amdgcn_readfirstlane(found[1]);
+    split.req.q0 = min(max(a.cu[b], 0), a.T);
+    split.req.kv = split.req.nq = min(max(a.cu[b + 1], 0), a.T) - split.req.q0;
   }
-  const int q0 = min(max(a.cu[b], 0), a.T);
-  const int nq = min(max(a.cu[b + 1], 0), a.T) - q0;
-  const int R = nq * a.G;
+  const int q0 = split.req.q0, nq = split.req.nq, kv = split.req.kv, R = nq * a.G;
   const int row0 = tile * kRows;  // the workgroup's first
-  const int kv = PAGED ? min(max(a.kv_len[b], 0), a.table_width << a.page_shift) : nq;
   const int ctx = kv - nq;  // position of the request's first row
 
   // keys that any row of the workgroup sees
@@ -743,7 +638,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
 
 namespace {
 template <int DT, int D, bool PAGED>
-hipError_t launch_tile(const AttnArgs &a, int tiles, hipStream_t s) {
+hipError_t launch_tile(const AttnArgs &a, int items, hipStream_t s) {
   constexpr int bytes = 2 * 2 * TK * D * 2;
   if constexpr (bytes > 65536 - 256) {
     static std::atomic<uint64_t> done{0};
@@ -753,16 +648,16 @@ hipError_t launch_tile(const AttnArgs &a, int tiles, hipStream_t s) {
       if (e != hipSuccess) return e;
     }
   }
-  IFX_LAUNCH(k_attn_tile, (DT, D, PAGED), dim3(a.Hkv * tiles), dim3(64 * kNW), bytes, s, a);
+  IFX_LAUNCH(k_attn_tile, (DT, D, PAGED), dim3(a.Hkv * items), dim3(64 * kNW), bytes, s, a);
   return last_error();
 }
 template <int DT>
-hipError_t launch_tile(const AttnArgs &a, int D, bool paged, int tiles, hipStream_t s) {
+hipError_t launch_tile(const AttnArgs &a, int D, bool paged, int items, hipStream_t s) {
   switch (D) {
-    case 64: return paged ? launch_tile<DT, 64, true>(a, tiles, s) : launch_tile<DT, 64, false>(a, tiles, s);
-    case 96: return paged ? launch_tile<DT, 96, true>(a, tiles, s) : launch_tile<DT, 96, false>(a, tiles, s);
-    case 128: return paged ? launch_tile<DT, 128, true>(a, tiles, s) : launch_tile<DT, 128, false>(a, tiles, s);
-    default: return paged ? launch_tile<DT, 256, true>(a, tiles, s) : launch_tile<DT, 256, false>(a, tiles, s);
+    case 64: return paged ? launch_tile<DT, 64, true>(a, items, s) : launch_tile<DT, 64, false>(a, items, s);
+    case 96: return paged ? launch_tile<DT, 96, true>(a, items, s) : launch_tile<DT, 96, false>(a, items, s);
+    case 128: return paged ? launch_tile<DT, 128, true>(a, items, s) : launch_tile<DT, 128, false>(a, items, s);
+    default: return paged ? launch_tile<DT, 256, true>(a, items, s) : launch_tile<DT, 256, false>(a, items, s);
   }
 }
 }  // namespace
@@ -771,10 +666,10 @@ int attn_tile_rows(int) { return kRows; }
 int attn_tile_min_keys() { return kMinChunk * TK; }
 int64_t attn_tile_slot_bytes(int D) { return kNW * (32 * D * 4 + 64 * 4 * 2); }
 
-hipError_t launch_attn_tile(const AttnArgs &a, int dtype, int D, bool paged, int tiles,
+hipError_t launch_attn_tile(const AttnArgs &a, int dtype, int D, bool paged, int items,
                             hipStream_t s) {
-  return dtype == IFX_ATTN_F16 ? launch_tile<IFX_ATTN_F16>(a, D, paged, tiles, s)
-                               : launch_tile<IFX_ATTN_BF16>(a, D, paged, tiles, s);
+  return dtype == IFX_ATTN_F16 ? launch_tile<IFX_ATTN_F16>(a, D, paged, items, s)
+                               : launch_tile<IFX_ATTN_BF16>(a, D, paged, items, s);
 }
 
 }  // namespace ifx

@@ -160,9 +160,7 @@ struct AttnArgs {
   int B, T, Hq, Hkv, G;
   int causal, window, out_dtype;
   float c;     // scale * log2(e)
-  int chunk;   // attn_rows: keys of a split
-  int splits;  // attn_rows: most splits of a request, grid and workspace slots
-  int goal;    // attn_tile: about this many workgroups for a key/value head
+  int goal;    // paged: work items of a key/value head (find_item)
   uint32_t *cnt;
   float *part;
   uint32_t part_bytes;
@@ -171,18 +169,162 @@ struct AttnArgs {
 // Query rows of one key/value head: row r of a request is query head r % G of
 // the group and new token r / G.
 constexpr int kRowsMax = 32;   // rows of a request that attn_rows takes
-constexpr int kRowKeys = 128;  // attn_rows: keys that a workgroup's waves take at a time
+constexpr int kRowKeys = 128;  // attn_rows: keys of a stage, 32 for each wave
 constexpr int kTileKeys = 64;  // attn_tile: keys of a stage
 
-// attn_rows: keys of a split, the plan's, or more where a request is longer than the plan
-// was told, so that a.splits of them always suffice.
-__device__ __forceinline__ int split_chunk(const AttnArgs &a, int keys) {
-  if (keys <= static_cast<int64_t>(a.chunk) * a.splits) return a.chunk;
-  return (keys / a.splits / kRowKeys + 1) * kRowKeys;
+// Inclusive sums over the lanes, in the vector unit's own lane moves: shifts by
+// 1, 2, 4, 8 within 16 lanes, then the last lane of each 16 to the next, and of
+// the first 32 to the others.
+__device__ __forceinline__ int add_of(int a, int b) { return a + b; }
+__device__ __forceinline__ float add_of(float a, float b) { return a + b; }
+template <int CTRL, int ROWS, class V>
+__device__ __forceinline__ V add_moved(V v) {
+  return add_of(v, __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(
+                       0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, false)));
+}
+template <class V>
+__device__ __forceinline__ V wave_scan(V v) {
+  v = add_moved<0x111, 0xF>(v);
+  v = add_moved<0x112, 0xF>(v);
+  v = add_moved<0x114, 0xF>(v);
+  v = add_moved<0x118, 0xF>(v);
+  v = add_moved<0x142, 0xA>(v);
+  return add_moved<0x143, 0xC>(v);
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(v)), 63));
 }
 
-hipError_t launch_attn_rows(const AttnArgs &a, int dtype, int D, int max_rows, hipStream_t s);
-hipError_t launch_attn_tile(const AttnArgs &a, int dtype, int D, bool paged, int tiles,
+struct Request {
+  int q0, nq, kv;  // first new token, new tokens, tokens
+};
+__device__ __forceinline__ Request request_of(const AttnArgs &a, int b) {
+  const int c0 = min(max(a.cu[b], 0), a.T), c1 = min(max(a.cu[b + 1], 0), a.T);
+  return {c0, max(c1 - c0, 0), min(max(a.kv_len[b], 0), a.table_width << a.page_shift)};
+}
+
+// ceil(x / d) for 0 <= x <= 2^24 with r = 1 / d: the product is off by less than 1.
+__device__ __forceinline__ int ceil_div(int x, int d, float r) {
+  const int q = static_cast<int>(static_cast<float>(x) * r), rest = x - q * d;
+  return q + (rest > 0) + (rest > d) - (rest <= -d);
+}
+
+// A piece of paged work: item `item` (chunk major) of request b's `tiles` row
+// tiles x ns chunks of `chunk` stages.  chunk is 0 where there is no such item.
+struct Split {
+  int chunk, ns, slot;  // ns: of the request; slot: of the split sums of its first tile
+  int b, item, tiles;
+  Request req;
+};
+
+// Item i of the batch (for one key/value head).  No list of work is built
+// beforehand: the workgroups' waves find it, each for itself, from the
+// requests' {row tiles, stages}, work(request); beyond 64 requests by way of
+// LDS (reqs).  The work is cut so that about a.goal items of one length come
+// out.  At most a.goal items belong to split tiles: all items are no more, or
+// else chunks are so long that a request of s > c stages, cut in less than
+// s / c + 1 < 2 s / c of them, leaves no more.
+template <int MIN_CHUNK, class Work>
+__device__ __forceinline__ Split find_item(const AttnArgs &a, int2 *reqs, int i, Work work) {
+  const int lane = threadIdx.x & 63, B = a.B, goal = a.goal;
+  const int per = (B + 63) / 64, b0 = min(lane * per, B), b1 = min(b0 + per, B);
+  Request req = {0, 0, 0};
+  int2 mine = {0, 1};  // the lane's first request
+  Split f = {};
+  if (B == 1) {  // nothing to be weighed against each other
+    f.req = request_of(a, 0);
+    const int2 r = work(f.req);
+    f.chunk = r.y, f.ns = 1, f.item = i, f.tiles = r.x;
+    if (goal >= r.x && r.x > 0) {
+      const int share = r.x == 1 ? goal : goal / r.x;  // chunks of a tile
+      f.chunk = max(MIN_CHUNK, ceil_div(r.y, share, __builtin_amdgcn_rcpf(static_cast<float>(share))));
+      f.ns = ceil_div(r.y, f.chunk, __builtin_amdgcn_rcpf(static_cast<float>(f.chunk)));
+    }
+    f.chunk = i < r.x * f.ns ? __builtin_amdgcn_readfirstlane(f.chunk) : 0;
+    f.ns = __builtin_amdgcn_readfirstlane(f.ns);
+    return f;
+  }
+  if (per == 1) {
+    if (lane < B) {
+      req = request_of(a, lane);
+      mine = work(req);
+    }
+  } else {
+    for (int b = threadIdx.x; b < B; b += blockDim.x) reqs[b] = work(request_of(a, b));
+    __syncthreads();
+    if (b0 < B) mine = reqs[b0];
+  }
+  auto each = [&](auto f) __attribute__((always_inline)) {
+    f(mine);
+#pragma unroll 1
+    for (int b = b0 + 1; b < b1; ++b) f(reqs[b]);
+  };
+  int chunk = 1 << 25;
+  float inv = 1.0f / chunk;
+  if (goal > 0) {
+    float stages = 0.0f, tiles = 0.0f;
+    each([&](int2 r) {
+      tiles += static_cast<float>(r.x);
+      stages += static_cast<float>(r.x) * static_cast<float>(r.y);
+    });
+    const float share = min(wave_sum(stages) / goal, 2e7f);
+    chunk = max(MIN_CHUNK, static_cast<int>(ceilf(share)));
+    bool fits = false;
+    if (wave_sum(tiles) < goal) {
+      for (int tries = 0; tries < 3 && !fits; ++tries) {
+        float items = 0.0f;
+        inv = __builtin_amdgcn_rcpf(static_cast<float>(chunk));
+        each([&](int2 r) { items += static_cast<float>(r.x * ceil_div(r.y, chunk, inv)); });
+        items = wave_sum(items);
+        fits = items <= goal;
+        if (!fits) chunk = max(chunk + 1, static_cast<int>(chunk * (items / goal)));
+      }
+    }
+    if (!fits) chunk = max(chunk, static_cast<int>(2.0f * share) + 1);
+    chunk = __builtin_amdgcn_readfirstlane(chunk);
+    inv = __builtin_amdgcn_rcpf(static_cast<float>(chunk));
+  }
+  int items = 0, slots = 0;
+  each([&](int2 r) {
+    const int ns = ceil_div(r.y, chunk, inv);
+    items += r.x * ns;
+    slots += ns > 1 ? r.x * ns : 0;
+  });
+  int at = wave_scan(items) - items, slot = wave_scan(slots) - slots;
+  const uint64_t has = __ballot(i >= at && i < at + items);
+  if (!has) return f;
+  const int who = __builtin_ctzll(has);
+  at = __builtin_amdgcn_readlane(at, who), slot = __builtin_amdgcn_readlane(slot, who);
+  int2 r = make_int2(__builtin_amdgcn_readlane(mine.x, who), __builtin_amdgcn_readlane(mine.y, who));
+  int b = who * per, ns = 0;
+  for (;; r = reqs[++b]) {
+    ns = ceil_div(r.y, chunk, inv);
+    if (i < at + r.x * ns) break;
+    at += r.x * ns;
+    slot += ns > 1 ? r.x * ns : 0;
+  }
+  ns = __builtin_amdgcn_readfirstlane(ns);
+  f.b = __builtin_amdgcn_readfirstlane(b);
+  f.tiles = __builtin_amdgcn_readfirstlane(r.x);
+  f.chunk = (__builtin_amdgcn_readfirstlane(r.y) + ns - 1) / ns;  // of equal length
+  f.ns = ns;
+  f.slot = __builtin_amdgcn_readfirstlane(slot);
+  f.item = i - __builtin_amdgcn_readfirstlane(at);
+  if (per == 1) {
+    f.req = {__builtin_amdgcn_readlane(req.q0, who), __builtin_amdgcn_readlane(req.nq, who),
+             __builtin_amdgcn_readlane(req.kv, who)};
+  } else {
+    f.req = request_of(a, f.b);
+    __syncthreads();  // reqs is read
+  }
+  return f;
+}
+
+hipError_t launch_attn_rows(const AttnArgs &a, int dtype, int D, int max_rows, int items,
+                            hipStream_t s);
+int attn_rows_max_goal(int max_rows);
+hipError_t launch_attn_tile(const AttnArgs &a, int dtype, int D, bool paged, int items,
                             hipStream_t s);
 int attn_tile_rows(int D);
 int attn_tile_min_keys();  // of a split
