@@ -14,44 +14,61 @@ namespace ifx {
 
 namespace {
 
+// Eight values of a row, as they lie in memory.
 template <int SRC>
-__device__ __forceinline__ void load8(const void *p, int64_t at, float (&x)[8]) {
-  if constexpr (SRC == IFX_ATTN_F32) {
-    const float *f = static_cast<const float *>(p) + at;
-    const f32x4 a = ldg<f32x4>(f), b = ldg<f32x4>(f + 4);
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-    x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  } else {
-    const u32x4 u = ldg<u32x4>(static_cast<const uint16_t *>(p) + at);
+struct Raw8 {
+  u32x4 u[SRC == IFX_ATTN_F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void *p, int64_t at) {
+    const char *c = static_cast<const char *>(p) + at * (SRC == IFX_ATTN_F32 ? 4 : 2);
+    u[0] = ldg<u32x4>(c);
+    if constexpr (SRC == IFX_ATTN_F32) u[1] = ldg<u32x4>(c + 16);
+  }
+  __device__ __forceinline__ void values(float (&x)[8]) const {
+    if constexpr (SRC == IFX_ATTN_F32) {
+      const f32x4 v = __builtin_bit_cast(f32x4, u[0]), w = __builtin_bit_cast(f32x4, u[1]);
+      x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+      x[4] = w.x, x[5] = w.y, x[6] = w.z, x[7] = w.w;
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = SRC == IFX_ATTN_F16 ? F16::value(u[i] & 0xFFFFu) : BF16::value(u[i] & 0xFFFFu);
-      x[2 * i + 1] = SRC == IFX_ATTN_F16 ? F16::value(u[i] >> 16) : BF16::value(u[i] >> 16);
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = SRC == IFX_ATTN_F16 ? F16::value(u[0][i] & 0xFFFFu) : BF16::value(u[0][i] & 0xFFFFu);
+        x[2 * i + 1] = SRC == IFX_ATTN_F16 ? F16::value(u[0][i] >> 16) : BF16::value(u[0][i] >> 16);
+      }
     }
   }
-}
+};
 
 template <class T>
 __device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
   return u32x4{T::pack(x[0], x[1]), T::pack(x[2], x[3]), T::pack(x[4], x[5]), T::pack(x[6], x[7])};
 }
 
+// Two neighbouring values of a row.
 template <int SRC>
-__device__ __forceinline__ float load1(const void *p, int64_t at) {
-  if constexpr (SRC == IFX_ATTN_F32) return static_cast<const float *>(p)[at];
-  const uint32_t u = static_cast<const uint16_t *>(p)[at];
-  return SRC == IFX_ATTN_F16 ? F16::value(u) : BF16::value(u);
+__device__ __forceinline__ float2 load2(const void *p, int64_t at) {
+  if constexpr (SRC == IFX_ATTN_F32) return ldg<float2>(static_cast<const float *>(p) + at);
+  const uint32_t u = ldg<uint32_t>(static_cast<const uint16_t *>(p) + at);
+  return SRC == IFX_ATTN_F16 ? make_float2(F16::value(u & 0xFFFFu), F16::value(u >> 16))
+                             : make_float2(BF16::value(u & 0xFFFFu), BF16::value(u >> 16));
+}
+
+// floor(x / d) for 0 <= x < 2^24 with r = 1 / d: the product is off by less than 1.
+__device__ __forceinline__ int quotient(int x, int d, float r) {
+  const int q = static_cast<int>(static_cast<float>(x) * r), rest = x - q * d;
+  return q + (rest >= d) - (rest < 0);
 }
 
 }  // namespace
 
-// A workgroup takes NTOK consecutive tokens.  Units of Q and K are pieces of 8
-// values (and their partners' piece where pairs lie half a rotation apart);
-// K's units run over the tokens first, so that neighbouring lanes write
-// neighbouring 16-byte pieces of the cache.  V's pieces hold 8 tokens of one
-// dim, so a lane gathers the tokens of one piece: the token that begins a run
-// of consecutive slots within a piece writes the whole run, from whichever
-// workgroup holds it, with one 16-byte store where the run fills the piece.
+// A workgroup takes NTOK consecutive tokens, and of them a part: K and V
+// (blockIdx.y 0) or some of Q's units.  Units of Q and K are pieces of 8 values
+// (and their partners' piece where pairs lie half a rotation apart); K's units
+// run over the tokens first, so that neighbouring lanes write neighbouring
+// 16-byte pieces of the cache.  A thread has two units' loads on their way at a
+// time.  V's pieces hold 8 tokens of one dim, so a lane gathers the tokens of
+// two dims' pieces: the token that begins a run of consecutive slots within a
+// piece writes the whole run, from whichever workgroup holds it, with 16-byte
+// stores where the run fills the piece.
 template <int DT, int SRC, int NTOK>
 __global__ __launch_bounds__(256) void k_rope_append(const AppendArgs a) {
   using T = Elem<DT>;
@@ -79,72 +96,78 @@ __global__ __launch_bounds__(256) void k_rope_append(const AppendArgs a) {
   }
   __syncthreads();
 
-  // Q and K: unit = (token, head, piece); a piece below rot_dim / 2 takes its
-  // partner along, the partner's own unit does nothing
-  const int heads = a.Hq + a.Hkv;
-  const int units = NTOK * heads * pieces;
-  for (int u = tid; u < units; u += 256) {
-    int t, head, pc;
-    if (u < NTOK * a.Hq * pieces) {  // Q: the row's order
-      pc = u % pieces;
-      head = u / pieces % a.Hq;
-      t = u / (pieces * a.Hq);
-    } else {  // K: tokens first
-      const int w = u - NTOK * a.Hq * pieces;
-      t = w % NTOK;
-      pc = w / NTOK % pieces;
-      head = a.Hq + w / (NTOK * pieces);
+  // Q and K: unit = (token, head, c): piece c and its partner, or behind the
+  // pairs a piece alone
+  const bool q_part = blockIdx.y > 0;
+  const int heads = q_part ? a.Hq : a.Hkv;
+  const int pairs = a.interleaved ? 0 : half >> 3, per_head = pieces - pairs;
+  const int units = NTOK * heads * per_head;
+  const int share = q_part ? (units + gridDim.y - 2) / (gridDim.y - 1) : units;
+  const int u_begin = q_part ? (blockIdx.y - 1) * share : 0, u_end = min(u_begin + share, units);
+  const float per_head_inv = 1.0f / per_head, heads_inv = 1.0f / heads;
+  constexpr int kAtOnce = 2;
+  for (int u0 = u_begin + tid; u0 < u_end; u0 += 256 * kAtOnce) {
+    Raw8<SRC> lo[kAtOnce], hi[kAtOnce];
+    int t[kAtOnce], head[kAtOnce], pc[kAtOnce], slot[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int u = u0 + 256 * j;
+      const int v = q_part ? u : u / NTOK, w = quotient(v, per_head, per_head_inv);
+      const int c = v - w * per_head;
+      t[j] = q_part ? quotient(w, heads, heads_inv) : u % NTOK;
+      head[j] = q_part ? w - t[j] * heads : w;
+      pc[j] = c < pairs ? c : c + pairs;
+      slot[j] = u < u_end ? slot_of[t[j] + 1] : -1;
+      if (slot[j] >= 0) {
+        const int64_t at = (t0 + t[j]) * (q_part ? a.q_stride : a.k_stride) +
+                           static_cast<int64_t>(head[j]) * a.D + pc[j] * 8;
+        lo[j].load(q_part ? a.q : a.k, at);
+        if (c < pairs) hi[j].load(q_part ? a.q : a.k, at + half);
+      }
     }
-    const int slot = slot_of[t + 1];
-    if (slot < 0) continue;
-    const bool is_q = head < a.Hq;
-    const int hh = is_q ? head : head - a.Hq;
-    const void *src = is_q ? a.q : a.k;
-    const int64_t at = (t0 + t) * (is_q ? a.q_stride : a.k_stride) +
-                       static_cast<int64_t>(hh) * a.D + pc * 8;
-    const float2 *tw = turn + t * half;
-    float x[8], y[8];
-    bool two = false;
-    if (a.interleaved || pc * 8 >= a.rot_dim) {
-      load8<SRC>(src, at, x);
-      if (pc * 8 < a.rot_dim) {
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      if (slot[j] < 0) continue;
+      const float2 *tw = turn + t[j] * half;
+      const bool two = pc[j] < pairs;
+      float x[8], y[8];
+      lo[j].values(x);
+      if (two) {
+        hi[j].values(y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 w = tw[pc[j] * 8 + i];
+          const float p = x[i], r = y[i];
+          x[i] = p * w.x - r * w.y;
+          y[i] = r * w.x + p * w.y;
+        }
+      } else if (pc[j] * 8 < a.rot_dim) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float2 w = tw[pc * 4 + i];
+          const float2 w = tw[pc[j] * 4 + i];
           const float p = x[2 * i], r = x[2 * i + 1];
           x[2 * i] = p * w.x - r * w.y;
           x[2 * i + 1] = r * w.x + p * w.y;
         }
       }
-    } else {
-      if (pc * 8 >= half) continue;
-      load8<SRC>(src, at, x);
-      load8<SRC>(src, at + half, y);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 w = tw[pc * 8 + i];
-        const float p = x[i], r = y[i];
-        x[i] = p * w.x - r * w.y;
-        y[i] = r * w.x + p * w.y;
+      if (q_part) {
+        uint16_t *o = static_cast<uint16_t *>(a.q_out) + (t0 + t[j]) * a.q_out_stride +
+                      static_cast<int64_t>(head[j]) * a.D + pc[j] * 8;
+        const u32x4 px = pack8<T>(x);
+        __builtin_memcpy(o, &px, 16);
+        if (two) {
+          const u32x4 py = pack8<T>(y);
+          __builtin_memcpy(o + half, &py, 16);
+        }
+      } else {
+        const int64_t chunk = static_cast<int64_t>(slot[j] >> sh) * a.Hkv + head[j];
+        u32x4 *o = static_cast<u32x4 *>(a.k_cache) + (chunk * pieces << sh) + (slot[j] & (P - 1));
+        o[pc[j] << sh] = pack8<T>(x);
+        if (two) o[(pc[j] + pairs) << sh] = pack8<T>(y);
       }
-      two = true;
-    }
-    if (is_q) {
-      uint16_t *o = static_cast<uint16_t *>(a.q_out) + (t0 + t) * a.q_out_stride +
-                    static_cast<int64_t>(hh) * a.D + pc * 8;
-      const u32x4 px = pack8<T>(x);
-      __builtin_memcpy(o, &px, 16);
-      if (two) {
-        const u32x4 py = pack8<T>(y);
-        __builtin_memcpy(o + half, &py, 16);
-      }
-    } else {
-      const int64_t chunk = static_cast<int64_t>(slot >> sh) * a.Hkv + hh;
-      u32x4 *o = static_cast<u32x4 *>(a.k_cache) + (chunk * pieces << sh) + (slot & (P - 1));
-      o[pc << sh] = pack8<T>(x);
-      if (two) o[(pc + (half >> 3)) << sh] = pack8<T>(y);
     }
   }
+  if (q_part) return;
 
   // V: unit = (run, head, dim), lanes along the dims
   for (int t = 0; t < NTOK; ++t) {
@@ -156,22 +179,28 @@ __global__ __launch_bounds__(256) void k_rope_append(const AppendArgs a) {
     while (((slot + n) & 7) != 0 && slot_of[t + 1 + n] == slot + n) ++n;
     const int64_t page = slot >> sh;
     const int in_page = slot & (P - 1);
-    for (int i = tid; i < a.Hkv * a.D; i += 256) {
+    for (int i = tid * 2; i < a.Hkv * a.D; i += 512) {
       const int hh = i / a.D, dim = i - hh * a.D;
       uint16_t *o = static_cast<uint16_t *>(a.v_cache) +
                     ((((page * a.Hkv + hh) << sh) + (in_page & ~7)) * a.D + dim * 8) +
                     (in_page & 7);
-      float x[8];
+      float x[8], y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        x[e] = e < n ? load1<SRC>(a.v, (t0 + t + e) * a.v_stride + i) : 0.0f;
-      const u32x4 p = pack8<T>(x);
+      for (int e = 0; e < 8; ++e) {
+        const float2 v = e < n ? load2<SRC>(a.v, (t0 + t + e) * a.v_stride + i) : make_float2(0.0f, 0.0f);
+        x[e] = v.x, y[e] = v.y;
+      }
+      const u32x4 p = pack8<T>(x), r = pack8<T>(y);
       if (n == 8) {
         *reinterpret_cast<u32x4 *>(o) = p;
+        *reinterpret_cast<u32x4 *>(o + 8) = r;
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (e < n) o[e] = static_cast<uint16_t>(p[e >> 1] >> (16 * (e & 1)));
+          if (e < n) {
+            o[e] = static_cast<uint16_t>(p[e >> 1] >> (16 * (e & 1)));
+            o[8 + e] = static_cast<uint16_t>(r[e >> 1] >> (16 * (e & 1)));
+          }
       }
     }
   }
@@ -181,9 +210,9 @@ namespace {
 template <int DT, int SRC>
 void launch(const AppendArgs &a, hipStream_t s) {
   if (a.T >= 2048) {
-    IFX_LAUNCH(k_rope_append, (DT, SRC, 8), dim3((a.T + 7) / 8), dim3(256), 0, s, a);
+    IFX_LAUNCH(k_rope_append, (DT, SRC, 8), dim3((a.T + 7) / 8, 3), dim3(256), 0, s, a);
   } else {
-    IFX_LAUNCH(k_rope_append, (DT, SRC, 1), dim3(a.T), dim3(256), 0, s, a);
+    IFX_LAUNCH(k_rope_append, (DT, SRC, 1), dim3(a.T, 2), dim3(256), 0, s, a);
   }
 }
 template <int DT>

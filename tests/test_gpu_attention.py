@@ -372,6 +372,33 @@ def test_paged_chunks_split(dev, ws, dt, Hq, Hkv, D, P, kv, new):
     assert counters_clear(ws)
 
 
+@pytest.mark.parametrize("dt,Hq,Hkv,D,P,B,qhi,long", [
+    ("f16", 8, 2, 64, 16, 65, 1, 5000),    # one request more than the lanes of a wave
+    ("bf16", 4, 4, 96, 32, 200, 2, 3000),  # some without new tokens
+    ("f16", 5, 1, 128, 16, 300, 1, 700),
+    ("bf16", 4, 2, 64, 16, 70, 40, 4000),  # row tiles
+    ("f16", 2, 2, 128, 64, 130, 90, 2500),
+    ("f16", 24, 24, 128, 16, 40, 60, 2600),  # more row tiles than work items are wanted
+])
+def test_paged_large_batches(dev, ws, dt, Hq, Hkv, D, P, B, qhi, long):
+    """Work is found in batches of more requests than a wave has lanes, of very
+    different lengths."""
+    import torch
+    note(f"paged large batch {dt} Hq={Hq} Hkv={Hkv} D={D} P={P} B={B} qhi={qhi}")
+    r = random.Random(B)
+    new = [r.choice([0, 1, r.randint(1, qhi)]) for _ in range(B)]
+    kv = [n + r.randint(0, 150) for n in new]
+    for b in (B // 3, B - 1):
+        new[b], kv[b] = qhi, long + b
+    x = Batch(dev, kv, new, Hq, Hkv, D, P, dt, seed=B, extra_rows=1)
+    x.run(ws)
+    x.verify()
+    first = x.out.clone()
+    x.run(ws)
+    assert torch.equal(first, x.out)
+    assert counters_clear(ws)
+
+
 @pytest.mark.parametrize("window", [1, 5, 64, 100, 2 ** 31 - 1])
 @pytest.mark.parametrize("new", [[1, 1, 1], [3, 2, 1], [80, 33, 1]])
 def test_paged_window(dev, ws, window, new):
