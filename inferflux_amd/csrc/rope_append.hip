@@ -64,11 +64,10 @@ __device__ __forceinline__ int quotient(int x, int d, float r) {
 // (blockIdx.y 0) or some of Q's units.  Units of Q and K are pieces of 8 values
 // (and their partners' piece where pairs lie half a rotation apart); K's units
 // run over the tokens first, so that neighbouring lanes write neighbouring
-// 16-byte pieces of the cache.  A thread has two units' loads on their way at a
-// time.  V's pieces hold 8 tokens of one dim, so a lane gathers the tokens of
-// two dims' pieces: the token that begins a run of consecutive slots within a
-// piece writes the whole run, from whichever workgroup holds it, with 16-byte
-// stores where the run fills the piece.
+// 16-byte pieces of the cache.  V's pieces hold 8 tokens of one dim, so a lane
+// gathers the tokens of two dims' pieces: the token that begins a run of
+// consecutive slots within a piece writes the whole run, from whichever
+// workgroup holds it, with 16-byte stores where the run fills the piece.
 template <int DT, int SRC, int NTOK>
 __global__ __launch_bounds__(256) void k_rope_append(const AppendArgs a) {
   using T = Elem<DT>;
@@ -105,66 +104,54 @@ __global__ __launch_bounds__(256) void k_rope_append(const AppendArgs a) {
   const int share = q_part ? (units + gridDim.y - 2) / (gridDim.y - 1) : units;
   const int u_begin = q_part ? (blockIdx.y - 1) * share : 0, u_end = min(u_begin + share, units);
   const float per_head_inv = 1.0f / per_head, heads_inv = 1.0f / heads;
-  constexpr int kAtOnce = 2;
-  for (int u0 = u_begin + tid; u0 < u_end; u0 += 256 * kAtOnce) {
-    Raw8<SRC> lo[kAtOnce], hi[kAtOnce];
-    int t[kAtOnce], head[kAtOnce], pc[kAtOnce], slot[kAtOnce];
+  for (int u = u_begin + tid; u < u_end; u += 256) {
+    const int v = q_part ? u : u / NTOK, w = quotient(v, per_head, per_head_inv);
+    const int c = v - w * per_head;
+    const int t = q_part ? quotient(w, heads, heads_inv) : u % NTOK;
+    const int head = q_part ? w - t * heads : w, pc = c < pairs ? c : c + pairs;
+    const int slot = slot_of[t + 1];
+    if (slot < 0) continue;
+    const bool two = c < pairs;
+    Raw8<SRC> lo, hi;
+    const int64_t at = (t0 + t) * (q_part ? a.q_stride : a.k_stride) +
+                       static_cast<int64_t>(head) * a.D + pc * 8;
+    lo.load(q_part ? a.q : a.k, at);
+    if (two) hi.load(q_part ? a.q : a.k, at + half);
+    const float2 *tw = turn + t * half;
+    float x[8], y[8];
+    lo.values(x);
+    if (two) {
+      hi.values(y);
 #pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) {
-      const int u = u0 + 256 * j;
-      const int v = q_part ? u : u / NTOK, w = quotient(v, per_head, per_head_inv);
-      const int c = v - w * per_head;
-      t[j] = q_part ? quotient(w, heads, heads_inv) : u % NTOK;
-      head[j] = q_part ? w - t[j] * heads : w;
-      pc[j] = c < pairs ? c : c + pairs;
-      slot[j] = u < u_end ? slot_of[t[j] + 1] : -1;
-      if (slot[j] >= 0) {
-        const int64_t at = (t0 + t[j]) * (q_part ? a.q_stride : a.k_stride) +
-                           static_cast<int64_t>(head[j]) * a.D + pc[j] * 8;
-        lo[j].load(q_part ? a.q : a.k, at);
-        if (c < pairs) hi[j].load(q_part ? a.q : a.k, at + half);
+      for (int i = 0; i < 8; ++i) {
+        const float2 w = tw[pc * 8 + i];
+        const float p = x[i], r = y[i];
+        x[i] = p * w.x - r * w.y;
+        y[i] = r * w.x + p * w.y;
+      }
+    } else if (pc * 8 < a.rot_dim) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 w = tw[pc * 4 + i];
+        const float p = x[2 * i], r = x[2 * i + 1];
+        x[2 * i] = p * w.x - r * w.y;
+        x[2 * i + 1] = r * w.x + p * w.y;
       }
     }
-#pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) {
-      if (slot[j] < 0) continue;
-      const float2 *tw = turn + t[j] * half;
-      const bool two = pc[j] < pairs;
-      float x[8], y[8];
-      lo[j].values(x);
+    if (q_part) {
+      uint16_t *o = static_cast<uint16_t *>(a.q_out) + (t0 + t) * a.q_out_stride +
+                    static_cast<int64_t>(head) * a.D + pc * 8;
+      const u32x4 px = pack8<T>(x);
+      __builtin_memcpy(o, &px, 16);
       if (two) {
-        hi[j].values(y);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 w = tw[pc[j] * 8 + i];
-          const float p = x[i], r = y[i];
-          x[i] = p * w.x - r * w.y;
-          y[i] = r * w.x + p * w.y;
-        }
-      } else if (pc[j] * 8 < a.rot_dim) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 w = tw[pc[j] * 4 + i];
-          const float p = x[2 * i], r = x[2 * i + 1];
-          x[2 * i] = p * w.x - r * w.y;
-          x[2 * i + 1] = r * w.x + p * w.y;
-        }
+        const u32x4 py = pack8<T>(y);
+        __builtin_memcpy(o + half, &py, 16);
       }
-      if (q_part) {
-        uint16_t *o = static_cast<uint16_t *>(a.q_out) + (t0 + t[j]) * a.q_out_stride +
-                      static_cast<int64_t>(head[j]) * a.D + pc[j] * 8;
-        const u32x4 px = pack8<T>(x);
-        __builtin_memcpy(o, &px, 16);
-        if (two) {
-          const u32x4 py = pack8<T>(y);
-          __builtin_memcpy(o + half, &py, 16);
-        }
-      } else {
-        const int64_t chunk = static_cast<int64_t>(slot[j] >> sh) * a.Hkv + head[j];
-        u32x4 *o = static_cast<u32x4 *>(a.k_cache) + (chunk * pieces << sh) + (slot[j] & (P - 1));
-        o[pc[j] << sh] = pack8<T>(x);
-        if (two) o[(pc[j] + pairs) << sh] = pack8<T>(y);
-      }
+    } else {
+      const int64_t chunk = static_cast<int64_t>(slot >> sh) * a.Hkv + head;
+      u32x4 *o = static_cast<u32x4 *>(a.k_cache) + (chunk * pieces << sh) + (slot & (P - 1));
+      o[pc << sh] = pack8<T>(x);
+      if (two) o[(pc + pairs) << sh] = pack8<T>(y);
     }
   }
   if (q_part) return;
@@ -210,7 +197,7 @@ namespace {
 template <int DT, int SRC>
 void launch(const AppendArgs &a, hipStream_t s) {
   if (a.T >= 2048) {
-    IFX_LAUNCH(k_rope_append, (DT, SRC, 8), dim3((a.T + 7) / 8, 3), dim3(256), 0, s, a);
+    IFX_LAUNCH(k_rope_append, (DT, SRC, 8), dim3((a.T + 7) / 8, 6), dim3(256), 0, s, a);
   } else {
     IFX_LAUNCH(k_rope_append, (DT, SRC, 1), dim3(a.T, 2), dim3(256), 0, s, a);
   }
