@@ -67,7 +67,6 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
   constexpr int kPieces = TK * NP;              // of K, and of V, a stage
   constexpr int NL = kPieces / (64 * kNW);      // pieces a thread loads, each
   extern __shared__ u32x4 lds[];                // [2 stages][K, V][kPieces]
-  __shared__ int found[2];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kvh = blockIdx.x % a.Hkv;
@@ -85,27 +84,17 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
     b = split.b, z = split.item / split.tiles;
     tile = split.tiles - 1 - (split.item - z * split.tiles);  // late tiles first
   } else {
-    // request b owns the row tiles from floor(cu[b] G / kRows) + b on, at least
-    // as many as it needs; late tiles (long key ranges) come first
-    const int t = (gridDim.x - 1 - blockIdx.x) / a.Hkv;
-    if (tid == 0) found[0] = -1;
-    __syncthreads();
-    for (int i = tid; i < a.B; i += 64 * kNW) {
-      const int c0 = min(max(a.cu[i], 0), a.T), c1 = min(max(a.cu[i + 1], 0), a.T);
-      const int t0 = c0 * a.G / kRows + i, t1 = c1 * a.G / kRows + i + 1;
-      if (t0 <= t && t < t1 && (t - t0) * kRows < (c1 - c0) * a.G) {
-        found[0] = i;
-        found[1] = t - t0;
-      }
-    }
-    __syncthreads();
-    b = __builtin_amdgcn_readfirstlane(found[0]);
-    if (b < 0) return;
-    tile = __builtin_amdgcn_readfirstlane(found[1]);
-    split.req.q0 = min(max(a.cu[b], 0), a.T);
-    split.req.kv = split.req.nq = min(max(a.cu[b + 1], 0), a.T) - split.req.q0;
+    const Tile found = find_tile(a, reinterpret_cast<int *>(lds), blockIdx.x / a.Hkv,
+                                 [&](const Request &r) { return (r.nq * a.G + kRows - 1) / kRows; });
+    if (found.b < 0) return;
+    b = found.b, tile = found.tile, split.req = found.req;
   }
-  const int q0 = split.req.q0, nq = split.req.nq, kv = split.req.kv, R = nq * a.G;
+  // the same in all lanes, and kept in scalar registers
+  b = __builtin_amdgcn_readfirstlane(b), tile = __builtin_amdgcn_readfirstlane(tile);
+  z = __builtin_amdgcn_readfirstlane(z);
+  const int q0 = __builtin_amdgcn_readfirstlane(split.req.q0);
+  const int nq = __builtin_amdgcn_readfirstlane(split.req.nq);
+  const int kv = __builtin_amdgcn_readfirstlane(split.req.kv), R = nq * a.G;
   const int row0 = tile * kRows;  // the workgroup's first
   const int ctx = kv - nq;  // position of the request's first row
 
@@ -118,7 +107,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
   const int full_z = max(0, a.causal ? ctx + tok_a + 1 : kv) & ~(TK - 1);
   int ns = 1, zbeg = kbeg, zend = kend;  // prompts are not split
   if constexpr (PAGED) {
-    const int chunk = split.chunk * TK;
+    const int chunk = __builtin_amdgcn_readfirstlane(split.chunk) * TK;
     if (kend > kbeg) ns = (kend - kbeg + chunk - 1) / chunk;
     if (z >= ns) return;
     zbeg = kbeg + z * chunk, zend = min(zbeg + chunk, kend);

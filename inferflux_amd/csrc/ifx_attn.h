@@ -175,25 +175,31 @@ constexpr int kTileKeys = 64;  // attn_tile: keys of a stage
 // Inclusive sums over the lanes, in the vector unit's own lane moves: shifts by
 // 1, 2, 4, 8 within 16 lanes, then the last lane of each 16 to the next, and of
 // the first 32 to the others.
-__device__ __forceinline__ int add_of(int a, int b) { return a + b; }
-__device__ __forceinline__ float add_of(float a, float b) { return a + b; }
-template <int CTRL, int ROWS, class V>
-__device__ __forceinline__ V add_moved(V v) {
-  return add_of(v, __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(
-                       0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, false)));
+struct Add {
+  template <class V>
+  __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
+};
+struct Max {
+  __device__ __forceinline__ int operator()(int a, int b) const { return max(a, b); }
+};
+template <int CTRL, int ROWS, class Op, class V>
+__device__ __forceinline__ V with_moved(V v) {  // lanes that get none: with 0
+  return Op()(v, __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(
+                     0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, false)));
 }
-template <class V>
+template <class Op = Add, class V>
 __device__ __forceinline__ V wave_scan(V v) {
-  v = add_moved<0x111, 0xF>(v);
-  v = add_moved<0x112, 0xF>(v);
-  v = add_moved<0x114, 0xF>(v);
-  v = add_moved<0x118, 0xF>(v);
-  v = add_moved<0x142, 0xA>(v);
-  return add_moved<0x143, 0xC>(v);
+  v = with_moved<0x111, 0xF, Op>(v);
+  v = with_moved<0x112, 0xF, Op>(v);
+  v = with_moved<0x114, 0xF, Op>(v);
+  v = with_moved<0x118, 0xF, Op>(v);
+  v = with_moved<0x142, 0xA, Op>(v);
+  return with_moved<0x143, 0xC, Op>(v);
 }
-__device__ __forceinline__ float wave_sum(float v) {
+template <class Op = Add, class V>
+__device__ __forceinline__ V wave_sum(V v) {
   return __builtin_bit_cast(
-      float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(v)), 63));
+      V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan<Op>(v)), 63));
 }
 
 struct Request {
@@ -316,6 +322,83 @@ __device__ __forceinline__ Split find_item(const AttnArgs &a, int2 *reqs, int i,
              __builtin_amdgcn_readlane(req.kv, who)};
   } else {
     f.req = request_of(a, f.b);
+    __syncthreads();  // reqs is read
+  }
+  return f;
+}
+
+// Row tile i of packed prompts (for one key/value head), found as above.
+// Causal: the requests' last tiles first, so the longest first, whichever
+// request they are of; N(t) = sum of max(tiles - t, 0) tiles have an index of t
+// or more, so tile i has the largest t of N(t) > i.  Not causal: in order.
+struct Tile {
+  int b, tile;  // b is -1 where there is no such tile
+  Request req;
+};
+template <class Tiles>
+__device__ __forceinline__ Tile find_tile(const AttnArgs &a, int *reqs, int i, Tiles tiles_of) {
+  const int lane = threadIdx.x & 63, B = a.B;
+  const int per = (B + 63) / 64, b0 = min(lane * per, B), b1 = min(b0 + per, B);
+  auto request = [&](int b) {
+    const int c0 = min(max(a.cu[b], 0), a.T), c1 = min(max(a.cu[b + 1], 0), a.T);
+    return Request{c0, max(c1 - c0, 0), max(c1 - c0, 0)};
+  };
+  Tile f = {-1, 0, {0, 0, 0}};
+  if (B == 1) {
+    f.req = request(0);
+    f.tile = tiles_of(f.req) - 1 - i;
+    f.b = f.tile < 0 ? -1 : 0;
+    return f;
+  }
+  int mine = 0;  // tiles of the lane's first request
+  if (per == 1) {
+    if (lane < B) {
+      f.req = request(lane);
+      mine = tiles_of(f.req);
+    }
+  } else {
+    for (int b = threadIdx.x; b < B; b += blockDim.x) reqs[b] = tiles_of(request(b));
+    __syncthreads();
+    if (b0 < B) mine = reqs[b0];
+  }
+  auto over = [&](int t) {  // the lane's tiles with an index of t or more
+    int n = max(mine - t, 0);
+#pragma unroll 1
+    for (int b = b0 + 1; b < b1; ++b) n += max(reqs[b] - t, 0);
+    return n;
+  };
+  int t = 0, has = over(0);  // the lane's candidates
+  if (a.causal) {
+    if (wave_sum(has) <= i) return f;
+    int most = mine;
+#pragma unroll 1
+    for (int b = b0 + 1; b < b1; ++b) most = max(most, reqs[b]);
+    most = wave_sum<Max>(most);
+    for (int bit = 1 << (31 - __builtin_clz(most)); bit; bit >>= 1)
+      if (wave_sum(over(t + bit)) > i) t += bit;
+    i -= wave_sum(over(t + 1));  // among the requests that have a tile t
+    has = over(t) - over(t + 1);
+  }
+  const int at = wave_scan(has) - has;
+  const uint64_t lanes = __ballot(i >= at && i < at + has);
+  if (!lanes) return f;
+  const int who = __builtin_ctzll(lanes);
+  i -= __builtin_amdgcn_readlane(at, who);
+  f.b = who * per;
+  f.tile = a.causal ? t : i;
+  if (per == 1) {
+    f.req = {__builtin_amdgcn_readlane(f.req.q0, who), __builtin_amdgcn_readlane(f.req.nq, who),
+             __builtin_amdgcn_readlane(f.req.kv, who)};
+  } else {
+    int b = f.b;
+    for (;; ++b) {
+      const int n = a.causal ? reqs[b] > t : reqs[b];
+      if (i < n) break;
+      i -= n;
+    }
+    f.b = __builtin_amdgcn_readfirstlane(b);
+    if (!a.causal) f.tile = i;
+    f.req = request(f.b);
     __syncthreads();  // reqs is read
   }
   return f;

@@ -557,6 +557,32 @@ def test_prompt(dev, dt, causal, window, Hq, Hkv, D, lens):
         a += n
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("Hq,Hkv,D,B,hi", [(4, 2, 64, 64, 300), (8, 1, 128, 65, 90), (3, 3, 64, 300, 40),
+                                           (10, 2, 96, 130, 60)])
+def test_prompt_large_batches(dev, causal, Hq, Hkv, D, B, hi):
+    """Row tiles are found in batches of as many requests as a wave has lanes,
+    and of more, some of them empty."""
+    import torch
+    from inferflux_amd import attention as at
+    note(f"prompt large batch causal={causal} Hq={Hq} Hkv={Hkv} D={D} B={B}")
+    r = random.Random(B)
+    lens = [r.choice([0, 1, r.randint(1, hi)]) for _ in range(B)]
+    lens[B // 2] = 700
+    g, T = gen(dev, B), sum(lens)
+    q, k, v = (torch.randn(T, h, D, generator=g, device=dev).half() for h in (Hq, Hkv, Hkv))
+    buf = torch.full((T + 1, Hq, D), 9.0, dtype=torch.float16, device=dev)
+    cu = i32([sum(lens[:b]) for b in range(B + 1)], dev)
+    got = at.prompt_attention(q, k, v, cu, max(lens), causal=causal, out=buf[:T])
+    assert bool((buf[T:] == 9).all())
+    a = 0
+    for n in lens:
+        if n:
+            ref, bound = attend(q[a:a + n], k[a:a + n], v[a:a + n], 0, D ** -0.5, causal, 0)
+            check(got[a:a + n], ref, bound, f"prompt of {n}")
+        a += n
+
+
 @pytest.mark.parametrize("dt", ["f16", "bf16"])
 @pytest.mark.parametrize("D", [64, 96, 128, 256])
 def test_prompt_non_finite(dev, dt, D):
