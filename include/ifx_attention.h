@@ -96,9 +96,11 @@ int ifx_rope_append(const void *q, int64_t q_stride, const void *k, int64_t k_st
  * with V; the result is rounded once to out_dtype (fp32, fp16 or bf16; rows
  * out_stride elements apart).
  *
- * max_q and max_kv bound the requests' rows and kv_len: they plan the launch
- * (how the keys are split over workgroups); a longer request is still
- * computed whole.  Lengths outside [0, table_width * page_size] and page
+ * max_q and max_kv bound the requests' new rows and kv_len, and plan the
+ * launch: which kernel takes it, how many workgroups there are and what
+ * workspace they need.  Of a request with more than max_q rows only the first
+ * max_q are sure to be computed; one with more than max_kv keys is computed
+ * whole, if not as fast.  Lengths outside [0, table_width * page_size] and page
  * numbers outside [0, num_pages) are clamped, so that no memory outside the
  * cache is touched.
  *
@@ -108,7 +110,7 @@ int ifx_rope_append(const void *q, int64_t q_stride, const void *k, int64_t k_st
  * sums are added in order: the same bits on every call.  Calls that share a
  * workspace must not overlap.  May be NULL with 0 bytes where none is needed.
  *
- * D: 64, 96, 128 or 256.  Hq a multiple of Hkv.  scale > 0.
+ * D: 64, 96, 128 or 256.  Hq a multiple of Hkv, Hkv * D < 2^22.  scale > 0.
  * table_width * page_size <= 2^30. */
 #define IFX_ATTN_WORKSPACE_BYTES (64 << 20)
 int64_t ifx_attn_paged_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int max_q,
@@ -124,8 +126,8 @@ int ifx_attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cac
  * q [T][Hq][D], k and v [T][Hkv][D], rows cu_len[b] .. cu_len[b + 1] - 1 are
  * prompt b.  Row i of a prompt of n sees its rows j < n, and j <= i where
  * causal, and j > i - window where causal and window > 0.  Otherwise as
- * ifx_attn_paged; k_stride, v_stride < 2^23.  max_len bounds the prompts' lengths (0 < max_len): the
- * launch is planned for it. */
+ * ifx_attn_paged; k_stride, v_stride < 2^23.  max_len > 0 bounds the prompts'
+ * lengths. */
 int ifx_attn_prompt(const void *q, int64_t q_stride, const void *k, int64_t k_stride,
                     const void *v, int64_t v_stride, int dtype, const int32_t *cu_len, int B,
                     int T, int Hq, int Hkv, int D, int max_len, int causal, int window,

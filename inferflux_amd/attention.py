@@ -222,7 +222,7 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_q, kv_len, max_q, max_k
     """Attention of the new tokens q [T, Hq, D] over the paged cache, which
     holds them already (ifx_attn_paged).  cu_q [B + 1]: the requests' first
     rows; kv_len [B]: their tokens, the new ones included; max_q, max_kv: bounds
-    of both.  A query sees its own position and what is before it, the last
+    of a request's rows (those past max_q may be left out) and tokens.  A query sees its own position and what is before it, the last
     `window` keys of it where window > 0.  scale: head_dim ** -0.5 if None.
     Returns out [T, Hq, D] (out_dtype: fp32, fp16 or bf16, q's type if None);
     its rows from cu_q[B] on are left as they were.  workspace: see

@@ -10,10 +10,14 @@
 // each wave reads its 32 keys' K and V straight into operand registers with
 // contiguous 16-byte loads, 16 KB a wave at D = 128, and nothing passes
 // through LDS.  Waves take tiles of 32 keys in turn, each with its own running
-// maximum and sums; they meet once, in LDS, at the end.  The keys of a request
-// are split over workgroups in chunks of a length that is the same for all
-// requests (long ones get more workgroups, not longer ones); the last
+// maximum and sums; they meet once, in LDS, at the end.  The keys of all
+// requests are cut into chunks of about one length (find_item); the last
 // workgroup of a request and head to finish adds the chunks in their order.
+//
+// Measured: 32 requests of 531 to 22591 keys, 40 query and 8 key/value heads of
+// 128 (796 MB), 148 us, 5.4 TB/s; with chunks as long as the longest request's
+// eighth, 187.  One request of 3000 keys, 16 and 2 heads: 9.6 us, of them 1 to
+// find the work, 1.4 for the keys, 1.7 for the waves' and 4 for the chunks' sums.
 #include "ifx_attn.h"
 
 namespace ifx {

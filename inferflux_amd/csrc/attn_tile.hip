@@ -13,6 +13,15 @@
 // O^T = V^T P^T): a lane then holds one row's scores, its maximum and sum need
 // no more than one exchange between lane halves, and the probabilities are the
 // next product's operand as they stand (key_of_row).
+//
+// Measured at 40 query and 8 key/value heads of 128: a causal prompt of 8111
+// tokens in 645 us, 1.04 PFLOP/s (a large 16-bit matrix product reaches 1.2 on
+// the same card); a chunk of 512 tokens over 7430 cached ones in 95 us.  What
+// took longer, for that prompt: K and V through registers 785 us with their
+// fragments read as they are needed, 657 with kAhead of them on their way; V
+// transposed in registers 800; 64 rows a wave 2600, as no 512 registers hold
+// them without moves; 8 waves in two groups half a stage apart 671; a head's
+// row sum as a dot product of the rounded probabilities no less.
 #include "ifx_attn.h"
 
 namespace ifx {
@@ -22,10 +31,12 @@ namespace {
 // Lambdas that are calls would keep what they capture in memory.
 #define IFX_INLINE __attribute__((always_inline))
 
-constexpr int kNW = 4;             // waves of a workgroup
-constexpr int kRows = 32 * kNW;    // its query rows
+constexpr int kNW = 4;           // waves of a workgroup
+constexpr int kRows = 32 * kNW;  // its query rows
 constexpr int TK = kTileKeys;
-constexpr int kMinChunk = 8;  // stages: what a chunk costs beside its keys
+// Stages of a chunk at least: beside them it takes 6 us for its first loads and
+// its sums' exchange, as much as 5 stages.
+constexpr int kMinChunk = 8;
 
 // LDS places, in 16-byte pieces of 8 values.  Copies go from memory to LDS
 // past the registers.
@@ -38,6 +49,7 @@ constexpr int kMinChunk = 8;  // stages: what a chunk costs beside its keys
 // lanes that a read serves at a time reach 16 different piece columns (256
 // bytes: all banks).  K's lanes differ in the row, V's transposing reads take
 // four rows of four neighbouring pieces.
+
 // 16 bytes a lane from memory to 64 consecutive places in LDS.
 __device__ __forceinline__ void to_lds(const void *from, u32x4 *to) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,

@@ -8,6 +8,10 @@
 // formed in fp64 as turns and reduced to half a turn there (a position of
 // 10^5 would leave an fp32 angle 10^-2 off), its sine and cosine in fp32: one
 // pair per position and frequency, shared by all heads through LDS.
+//
+// Measured: 5299 tokens of 40 query and 8 key/value heads of 128, fp16 (152 MB):
+// 43 us from memory, 3.5 TB/s, and 29 where the rows are still in the caches; 8
+// tokens of 16 and 2 heads, fp32: a kernel of 3.9 us.
 #include "ifx_attn.h"
 
 namespace ifx {
@@ -197,6 +201,7 @@ namespace {
 template <int DT, int SRC>
 void launch(const AppendArgs &a, hipStream_t s) {
   if (a.T >= 2048) {
+    // 5299 tokens as above: 54 us with one part for all, 45 with 2 for Q, 43 with 5
     IFX_LAUNCH(k_rope_append, (DT, SRC, 8), dim3((a.T + 7) / 8, 6), dim3(256), 0, s, a);
   } else {
     IFX_LAUNCH(k_rope_append, (DT, SRC, 1), dim3(a.T, 2), dim3(256), 0, s, a);
