@@ -579,61 +579,41 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
       top = mn;
     }
   }
-  if (few) {
-#pragma unroll 1
-    for (int d = wave; d < ND; d += kNW) {
-      f32x4 o[4] = {};
-      for (int y0 = 0; y0 < ns; y0 += 4) {
-        float2 ml[4];
-        f32x4 v[4][4];
+  // N dim tiles from d on, four chunks at a time
+  auto add_chunks = [&](int d, auto n_c) IFX_INLINE {
+    constexpr int N = decltype(n_c)::value;
+    f32x4 o[4 * N] = {};
+    for (int y0 = 0; y0 < ns; y0 += 4) {
+      float2 ml[4];
+      f32x4 v[4][4 * N];
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          ml[y] = ml_of(y0 + y);
-          const uint32_t at = y0 + y < ns ? mine + (y0 + y) * kSlotBytes + d * 4096 : kOut;
+      for (int y = 0; y < 4; ++y) {
+        ml[y] = ml_of(y0 + y);
+        const uint32_t at = y0 + y < ns ? mine + (y0 + y) * kSlotBytes + d * 4096 : kOut;
 #pragma unroll
-          for (int g = 0; g < 4; ++g) v[y][g] = ld_dev4(part, at + g * 1024);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const float w = y0 + y < ns ? weight(ml[y].x, top, a.c) : 0.0f;
-#pragma unroll
-          for (int g = 0; g < 4; ++g) o[g] += v[y][g] * w;
-        }
-      }
-      write_dims(d, o, 1.0f / total);
-    }
-    return split_reset(cnt);
-  }
-#pragma unroll
-  for (int d = 0; d < ND; ++d)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
-  for (int y = 0; y < ns; y += 2) {
-    constexpr int kAtOnce = ND < 4 ? ND : 4;  // dim tiles
-    const float2 ml0 = ml_of(y), ml1 = ml_of(y + 1);
-    const uint32_t at0 = mine + y * kSlotBytes;
-    const uint32_t at1 = y + 1 < ns ? at0 + kSlotBytes : kOut;
-    const float w0 = weight(ml0.x, top, a.c), w1 = y + 1 < ns ? weight(ml1.x, top, a.c) : 0.0f;
-#pragma unroll
-    for (int d0 = 0; d0 < ND; d0 += kAtOnce) {
-      f32x4 v0[4 * kAtOnce], v1[4 * kAtOnce];
-#pragma unroll
-      for (int i = 0; i < 4 * kAtOnce && 4 * d0 + i < 4 * ND; ++i) {
-        v0[i] = ld_dev4(part, at0 + (4 * d0 + i) * 1024);
-        v1[i] = ld_dev4(part, at1 + (4 * d0 + i) * 1024);
+        for (int g = 0; g < 4 * N; ++g) v[y][g] = ld_dev4(part, at + g * 1024);
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < 4 * kAtOnce && 4 * d0 + i < 4 * ND; ++i)
+      for (int y = 0; y < 4; ++y) {
+        const float w = y0 + y < ns ? weight(ml[y].x, top, a.c) : 0.0f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int d = d0 + (i >> 2), j = 4 * (i & 3) + r;
-          acc[d][j] = (acc[d][j] + v0[i][r] * w0) + v1[i][r] * w1;
-        }
+        for (int g = 0; g < 4 * N; ++g) o[g] += v[y][g] * w;
+      }
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i) write_dims(d + i, o + 4 * i, 1.0f / total);
+  };
+  using one = std::integral_constant<int, 1>;
+  using two = std::integral_constant<int, 2>;
+  if (few || D == 64) {  // (D = 64: registers of three waves a SIMD)
+#pragma unroll 1
+    for (int d = few ? wave : 0; d < ND; d += few ? kNW : 1) add_chunks(d, one{});
+  } else {
+#pragma unroll 1
+    for (int d = 0; d + 1 < ND; d += 2) add_chunks(d, two{});
+    if constexpr (ND % 2) add_chunks(ND - 1, one{});
   }
-  write(1.0f / total);
   split_reset(cnt);
 }
 

@@ -100,7 +100,8 @@ PAGED = dict(q=F, qs=2048, dt=1, kc=F, vc=F, pages=100, page=64, table=F, width=
     (dict(scale=float("nan")), GEOM), (dict(scale=float("inf")), GEOM), (dict(window=-1), GEOM),
     (dict(qs=2047), GEOM), (dict(os=2047), GEOM), (dict(q=None), NULL), (dict(kv=None), NULL),
     (dict(ws=None, wsn=0), NULL), (dict(wsn=4096), GEOM), (dict(ws=ctypes.c_void_p(0x10010)), GEOM),
-    (dict(vc=ctypes.c_void_p(0x10002)), GEOM), (dict(T=1 << 28), GEOM)])
+    (dict(vc=ctypes.c_void_p(0x10002)), GEOM), (dict(T=1 << 28), GEOM),
+    (dict(Hq=1 << 15, Hkv=1 << 15, qs=1 << 22, os=1 << 22, T=4), GEOM)])
 def test_paged_refusals(lib, change, want):
     with dry(lib) as d:
         assert lib.ifx_attn_paged(*{**PAGED, **change}.values()) == want

@@ -376,6 +376,7 @@ def test_paged_chunks_split(dev, ws, dt, Hq, Hkv, D, P, kv, new):
     ("f16", 8, 2, 64, 16, 65, 1, 5000),    # one request more than the lanes of a wave
     ("bf16", 4, 4, 96, 32, 200, 2, 3000),  # some without new tokens
     ("f16", 5, 1, 128, 16, 300, 1, 700),
+    ("f16", 24, 24, 64, 16, 70, 1, 4000),  # more requests than work items are wanted
     ("bf16", 4, 2, 64, 16, 70, 40, 4000),  # row tiles
     ("f16", 2, 2, 128, 64, 130, 90, 2500),
     ("f16", 24, 24, 128, 16, 40, 60, 2600),  # more row tiles than work items are wanted
