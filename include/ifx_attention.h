@@ -94,7 +94,7 @@ int ifx_rope_append(const void *q, int64_t q_stride, const void *k, int64_t k_st
  * from cu_q[B] on are left as they were.  Scores, their maximum and their sum
  * are fp32; the probabilities are rounded to the cache's type for the product
  * with V; the result is rounded once to out_dtype (fp32, fp16 or bf16; rows
- * out_stride elements apart).
+ * out_stride elements apart, which must not overlap the keys and values).
  *
  * max_q and max_kv bound the requests' new rows and kv_len, and plan the
  * launch: which kernel takes it, how many workgroups there are and what

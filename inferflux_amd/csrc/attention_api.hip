@@ -47,6 +47,10 @@ bool heads_ok(int B, int T, int Hq, int Hkv, int D) {
   return rows < (1 << 30) && (rows / 32 + B) * Hkv < (1 << 23);
 }
 
+// Positions are below 2^30: a window as wide is none, and position - window
+// stays within 32 bits, also of rows before the first key (above -2^30).
+int window_of(int window) { return window < (1 << 30) ? window : 0; }
+
 // Split sums: units (a request's or row tile's key/value head) that can be
 // split, their counters at the start of the workspace.  The counters' place is
 // the same for every shape, as one workspace serves calls of many shapes and
@@ -90,7 +94,7 @@ PagedPlan plan_paged(int B, int T, int Hq, int Hkv, int D, int max_q, int max_kv
   if (goal > kMaxUnits / Hkv) goal = kMaxUnits / Hkv;
   if (p.rows && goal > attn_rows_max_goal(static_cast<int>(rows)))
     goal = attn_rows_max_goal(static_cast<int>(rows));
-  if (max_kv <= unit) goal = 0;
+  if (max_kv <= (p.rows ? unit : 2 * unit - kTileKeys)) goal = 0;  // one chunk each
   p.goal = static_cast<int>(goal);
   p.items = static_cast<int>(tiles + goal);
   p.bytes = goal ? kCntBytes + goal * Hkv * slot : 0;
@@ -190,7 +194,7 @@ int ifx_attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cac
   a.table = block_table, a.cu = cu_q, a.kv_len = kv_len;
   a.num_pages = num_pages, a.table_width = table_width, a.page_shift = sh;
   a.B = B, a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv;
-  a.causal = 1, a.window = window, a.out_dtype = out_dtype;
+  a.causal = 1, a.window = window_of(window), a.out_dtype = out_dtype;
   a.c = scale * kLog2e;
   a.goal = p.goal;
   if (p.bytes) {
@@ -223,7 +227,7 @@ int ifx_attn_prompt(const void *q, int64_t q_stride, const void *k, int64_t k_st
   a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride, a.out_stride = out_stride;
   a.cu = cu_len;
   a.B = B, a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv;
-  a.causal = causal != 0, a.window = window, a.out_dtype = out_dtype;
+  a.causal = causal != 0, a.window = window_of(window), a.out_dtype = out_dtype;
   a.c = scale * kLog2e;
   const int tiles = static_cast<int>(static_cast<int64_t>(T) * a.G / attn_tile_rows(D)) + B;
   return status_of(launch_attn_tile(a, dtype, D, false, tiles, static_cast<hipStream_t>(stream)));

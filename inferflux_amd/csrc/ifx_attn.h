@@ -216,6 +216,12 @@ __device__ __forceinline__ int ceil_div(int x, int d, float r) {
   return q + (rest > 0) + (rest > d) - (rest <= -d);
 }
 
+// Chunks of a request of x stages: of `chunk` (r = 1 / chunk), or of least at least.
+template <int LEAST>
+__device__ __forceinline__ int chunks_of(int x, int chunk, float r) {
+  return min(ceil_div(x, chunk, r), max(x / LEAST, 1));
+}
+
 // A piece of paged work: item `item` (chunk major) of request b's `tiles` row
 // tiles x ns chunks of `chunk` stages.  chunk is 0 where there is no such item.
 struct Split {
@@ -245,7 +251,8 @@ __device__ __forceinline__ Split find_item(const AttnArgs &a, int2 *reqs, int i,
     if (goal >= r.x && r.x > 0) {
       const int share = r.x == 1 ? goal : goal / r.x;  // chunks of a tile
       f.chunk = max(MIN_CHUNK, ceil_div(r.y, share, __builtin_amdgcn_rcpf(static_cast<float>(share))));
-      f.ns = ceil_div(r.y, f.chunk, __builtin_amdgcn_rcpf(static_cast<float>(f.chunk)));
+      f.ns = chunks_of<MIN_CHUNK>(r.y, f.chunk, __builtin_amdgcn_rcpf(static_cast<float>(f.chunk)));
+      f.chunk = (r.y + f.ns - 1) / f.ns;  // of equal length
     }
     f.chunk = i < r.x * f.ns ? __builtin_amdgcn_readfirstlane(f.chunk) : 0;
     f.ns = __builtin_amdgcn_readfirstlane(f.ns);
@@ -281,7 +288,7 @@ __device__ __forceinline__ Split find_item(const AttnArgs &a, int2 *reqs, int i,
       for (int tries = 0; tries < 3 && !fits; ++tries) {
         float items = 0.0f;
         inv = __builtin_amdgcn_rcpf(static_cast<float>(chunk));
-        each([&](int2 r) { items += static_cast<float>(r.x * ceil_div(r.y, chunk, inv)); });
+        each([&](int2 r) { items += static_cast<float>(r.x * chunks_of<MIN_CHUNK>(r.y, chunk, inv)); });
         items = wave_sum(items);
         fits = items <= goal;
         if (!fits) chunk = max(chunk + 1, static_cast<int>(chunk * (items / goal)));
@@ -293,7 +300,7 @@ __device__ __forceinline__ Split find_item(const AttnArgs &a, int2 *reqs, int i,
   }
   int items = 0, slots = 0;
   each([&](int2 r) {
-    const int ns = ceil_div(r.y, chunk, inv);
+    const int ns = chunks_of<MIN_CHUNK>(r.y, chunk, inv);
     items += r.x * ns;
     slots += ns > 1 ? r.x * ns : 0;
   });
@@ -305,7 +312,7 @@ __device__ __forceinline__ Split find_item(const AttnArgs &a, int2 *reqs, int i,
   int2 r = make_int2(__builtin_amdgcn_readlane(mine.x, who), __builtin_amdgcn_readlane(mine.y, who));
   int b = who * per, ns = 0;
   for (;; r = reqs[++b]) {
-    ns = ceil_div(r.y, chunk, inv);
+    ns = chunks_of<MIN_CHUNK>(r.y, chunk, inv);
     if (i < at + r.x * ns) break;
     at += r.x * ns;
     slot += ns > 1 ? r.x * ns : 0;

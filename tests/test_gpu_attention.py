@@ -410,6 +410,16 @@ def test_paged_window(dev, ws, window, new):
     assert counters_clear(ws)
 
 
+@pytest.mark.parametrize("window", [2, 2 ** 30 - 1, 2 ** 30, 2 ** 31 - 1])
+@pytest.mark.parametrize("new,kv", [([9, 4], [3, 70]), ([90, 60], [41, 300])])
+def test_paged_window_rows_before_the_first_key(dev, ws, window, new, kv):
+    """Positions below 0 less the widest windows."""
+    note(f"paged window {window} new={new} kv={kv}")
+    x = Batch(dev, kv, new, 6, 2, 128, 16, "f16", seed=3)
+    x.run(ws, window=window)
+    x.verify(window=window)
+
+
 @pytest.mark.parametrize("out_dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("new,kv", [([1, 1], [70, 3000]), ([60, 5], [60, 2000])])
 def test_paged_output_types(dev, ws, out_dtype, new, kv):
