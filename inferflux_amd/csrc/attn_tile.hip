@@ -17,11 +17,15 @@
 // Measured at 40 query and 8 key/value heads of 128: a causal prompt of 8111
 // tokens in 645 us, 1.04 PFLOP/s (a large 16-bit matrix product reaches 1.2 on
 // the same card); a chunk of 512 tokens over 7430 cached ones in 95 us.  What
-// took longer, for that prompt: K and V through registers 785 us with their
-// fragments read as they are needed, 657 with kAhead of them on their way; V
-// transposed in registers 800; 64 rows a wave 2600, as no 512 registers hold
-// them without moves; 8 waves in two groups half a stage apart 671; a head's
-// row sum as a dot product of the rounded probabilities no less.
+// took longer, for that prompt: stages through registers 3207 us, as they
+// spill; fragments read where they are needed 701, when kAhead of them on their
+// way took 657; V transposed in registers 800; 64 rows a wave 2600, for the
+// moves between the halves of the register file; 8 waves in two groups half a
+// stage apart 671.
+//
+// Registers: 256 a wave, two workgroups a CU.  D = 64 does with 168, three a
+// CU: 8111 tokens of 40 / 8 heads in 370 us, two 387, four 1330 (spills).
+// D = 256 needs 512.
 #include "ifx_attn.h"
 
 namespace ifx {
