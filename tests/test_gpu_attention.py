@@ -377,6 +377,8 @@ def test_paged_chunks_split(dev, ws, dt, Hq, Hkv, D, P, kv, new):
     ("bf16", 4, 4, 96, 32, 200, 2, 3000),  # some without new tokens
     ("f16", 5, 1, 128, 16, 300, 1, 700),
     ("f16", 24, 24, 64, 16, 70, 1, 4000),  # more requests than work items are wanted
+    ("f16", 2, 1, 64, 16, 4096, 1, 2000),  # the largest batch
+    ("f16", 2, 1, 64, 16, 4096, 17, 1500),
     ("bf16", 4, 2, 64, 16, 70, 40, 4000),  # row tiles
     ("f16", 2, 2, 128, 64, 130, 90, 2500),
     ("f16", 24, 24, 128, 16, 40, 60, 2600),  # more row tiles than work items are wanted
@@ -570,7 +572,7 @@ def test_prompt(dev, dt, causal, window, Hq, Hkv, D, lens):
 
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("Hq,Hkv,D,B,hi", [(4, 2, 64, 64, 300), (8, 1, 128, 65, 90), (3, 3, 64, 300, 40),
-                                           (10, 2, 96, 130, 60)])
+                                           (10, 2, 96, 130, 60), (2, 1, 64, 4096, 3)])
 def test_prompt_large_batches(dev, causal, Hq, Hkv, D, B, hi):
     """Row tiles are found in batches of as many requests as a wave has lanes,
     and of more, some of them empty."""
