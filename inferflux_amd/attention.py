@@ -16,7 +16,8 @@ Whole prompts that no cache is kept for (scoring, embedding) go through
 prompt_attention instead.  Integers are int32, caches and rows of Q fp16 or
 bf16.  Nothing here synchronises the host, and with outputs given nothing
 allocates, so every call can be captured into a graph.  Calls run on the
-current stream of the tensors' device, or on `stream`, one of that device.
+current stream of the tensors' device, or on `stream`, one of that device; what
+they return there is read elsewhere only after a wait for `stream`.
 Errors are those of `ops`: NotHandled, HipError, ValueError, TypeError.
 """
 from collections import namedtuple
@@ -65,11 +66,16 @@ def _device(t, name):
 
 
 def _new(shape, dtype, like, stream):
-    """An output of a call: the allocator is told of a stream that is not the
-    current one, so that it does not hand the memory out while in use there."""
-    t = torch.empty(shape, dtype=dtype, device=like.device)
-    if stream is not None:
-        t.record_stream(stream)
+    """An output of a call.  On a given stream it is that stream's own memory:
+    the current one's may be a block just freed there, with work on it still
+    pending that `stream` does not wait for.  The caller goes on with it on the
+    current stream, so the allocator is told of that one."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    user = torch.cuda.current_stream(like.device)
+    with torch.cuda.stream(stream):
+        t = torch.empty(shape, dtype=dtype, device=like.device)
+    t.record_stream(user)
     return t
 
 

@@ -168,3 +168,38 @@ def test_wrapper_refusals_without_a_gpu():
     with pytest.raises(ValueError, match=r"must be \[3, 2, 8\]"):
         at._rows(torch.zeros(3, 2, 16), "q", 3, 2, 8)
     assert at._rows(torch.zeros(3, 40)[:, 8:24].view(3, 2, 8), "q", 3, 2, 8)[1] == 40
+
+
+def test_outputs_are_allocated_on_the_stream_of_the_call(monkeypatch):
+    """An output that a call makes for a given stream comes from that stream's
+    own memory, which nothing pending on another stream still uses, and the
+    current stream, where the caller goes on with it, is known to use it too."""
+    import contextlib
+
+    import torch
+    from inferflux_amd import attention as at
+    now, log = ["current"], []
+
+    class Out:
+        def record_stream(self, s):
+            log.append(("used on", s))
+
+    @contextlib.contextmanager
+    def on(s):
+        now.append(s)
+        yield
+        now.pop()
+
+    def empty(*a, **k):
+        log.append(("made on", now[-1]))
+        return Out()
+
+    like = torch.zeros(1)
+    monkeypatch.setattr(torch.cuda, "stream", on)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: now[-1])
+    monkeypatch.setattr(torch, "empty", empty)
+    at._new((2, 3), torch.float16, like, None)
+    assert log == [("made on", "current")]
+    log.clear()
+    at._new((2, 3), torch.float16, like, "given")
+    assert log == [("made on", "given"), ("used on", "current")]

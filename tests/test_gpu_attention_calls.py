@@ -1,0 +1,50 @@
+"""The attention operators in calls that a serving program makes beside the
+plain ones: on other streams without a wait, next to memory that holds
+nonsense, with windows inside long chunks."""
+import pytest
+
+from tests.attn_ref import attend, check
+from tests.test_gpu_attention import Batch, dev, dt_of, gen, i32, ws  # noqa: F401
+from tests.test_gpu_parity import note
+
+pytestmark = pytest.mark.gpu
+
+
+def test_outputs_on_a_stream_that_waits_for_nothing(dev, ws):
+    """Inputs are of stream s, and the current stream still has work to do on
+    blocks of the outputs' sizes that were freed there: it writes to none of
+    the outputs made on s."""
+    import torch
+    from inferflux_amd import attention as at
+    note("outputs on another stream")
+    x = Batch(dev, [300, 90], [40, 1], 8, 2, 128, 16, "f16", seed=2)
+    ctx, new = i32([260, 89], dev), i32([40, 1], dev)
+    free, count = i32([0], dev), i32([1], dev)
+    table = torch.zeros_like(x.table)
+    kc, vc = at.kv_cache(64, 2, 128, 16, torch.float16, dev)
+    slots = torch.arange(x.T, dtype=torch.int32, device=dev)
+    calls = {
+        "plan": lambda s: at.plan_batch(ctx, new, table, free, count, 16, x.T, stream=s),
+        "append": lambda s: at.rope_append(x.q, x.q[:, :2], x.q[:, 2:4], slots, slots, kc, vc, stream=s),
+        "paged": lambda s: at.paged_attention(x.q, x.kc, x.vc, x.table, x.cu, x.kvt, 40, 300, workspace=ws,
+                                              stream=s),
+        "prompt": lambda s: at.prompt_attention(x.q, x.q[:, :2], x.q[:, 2:4], x.cu, 40, stream=s),
+    }
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for what, call in calls.items():
+        want = call(None)  # and the sizes of the blocks that a call asks for
+        torch.cuda.synchronize()
+        want = [w.clone() for w in want] if what == "plan" else [want.clone()]
+        n = sum(w.numel() * w.element_size() for w in want)
+        blocks = [torch.empty(n, dtype=torch.uint8, device=dev) for _ in range(4)]
+        torch.cuda.synchronize()
+        torch.cuda._sleep(20_000_000)
+        for b in blocks:
+            b.fill_(77)
+        del blocks, b  # free for the current stream, with the fills pending
+        got = call(s)
+        s.synchronize()
+        torch.cuda.synchronize()  # the fills are done
+        for g, w in zip(got if what == "plan" else [got], want):
+            assert torch.equal(g, w), what
