@@ -19,7 +19,7 @@ def test_outputs_on_a_stream_that_waits_for_nothing(dev, ws):
     note("outputs on another stream")
     x = Batch(dev, [300, 90], [40, 1], 8, 2, 128, 16, "f16", seed=2)
     ctx, new = i32([260, 89], dev), i32([40, 1], dev)
-    free, count = i32([0], dev), i32([1], dev)
+    free, count = i32([3, 1, 2, 0], dev), i32([4], dev)
     table = torch.zeros_like(x.table)
     kc, vc = at.kv_cache(64, 2, 128, 16, torch.float16, dev)
     slots = torch.arange(x.T, dtype=torch.int32, device=dev)
