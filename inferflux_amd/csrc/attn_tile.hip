@@ -62,9 +62,11 @@ __device__ __forceinline__ void to_lds(const void *from, u32x4 *to) {
                                    (__attribute__((address_space(3))) void *)to, 16, 0, 0);
 }
 
-__device__ __forceinline__ void to_lds(rsrc_t from, int voff, int soff, u32x4 *to) {
+// The same from a range of memory; places behind its end get 0.  The whole
+// offset is the lanes': the range check does not count a scalar one.
+__device__ __forceinline__ void to_lds(rsrc_t from, int off, u32x4 *to) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)to, 16,
-                                           voff, soff, 0, 0);
+                                           off, 0, 0, 0);
 }
 
 template <int D>
@@ -221,16 +223,16 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
                sv);
       }
     } else if constexpr (kSame) {  // 64 places in order, each with the piece that belongs there
-      if ((j & 1) == 0)
-        to_lds(f.rk, k_off, i * (kNW * 64 / NP) * k_row, sk);
-      else
-        to_lds(f.rv, v_off, i * (kNW * 64 / NP) * v_row, sv);
+      const bool is_k = (j & 1) == 0;
+      int off = is_k ? k_off : v_off;
+      if (i) asm volatile("" : "+v"(off));  // the sum is formed here, not kept in a register
+      to_lds(is_k ? f.rk : f.rv, off + i * (kNW * 64 / NP) * (is_k ? k_row : v_row), is_k ? sk : sv);
     } else {
       const int p = n0 * 64 + lane, key = p / NP, c = p - key * NP;
       if ((j & 1) == 0)
-        to_lds(f.rk, key * k_row + (c ^ swap_k<D>(key_of_row(key & 31))) * 16, 0, sk);
+        to_lds(f.rk, key * k_row + (c ^ swap_k<D>(key_of_row(key & 31))) * 16, sk);
       else
-        to_lds(f.rv, key * v_row + (c ^ swap_v<D>(key)) * 16, 0, sv);
+        to_lds(f.rv, key * v_row + (c ^ swap_v<D>(key)) * 16, sv);
     }
   };
 

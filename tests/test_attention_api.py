@@ -203,3 +203,16 @@ def test_outputs_are_allocated_on_the_stream_of_the_call(monkeypatch):
     log.clear()
     at._new((2, 3), torch.float16, like, "given")
     assert log == [("made on", "given"), ("used on", "current")]
+
+
+def test_loads_of_packed_rows_are_bounded_by_the_lanes_offsets(tmp_path):
+    """Stages of packed rows rely on the buffer's end for the rows behind a
+    prompt's last.  The range check counts a lane's offset and not the scalar
+    one, so no such load may have a scalar offset."""
+    from inferflux_amd import build
+    out = tmp_path / "attn_tile.s"
+    subprocess.run([build.HIPCC] + build.COMMON + ["-S", "--cuda-device-only", "-x", "hip",
+                    os.path.join(build.CSRC, "attn_tile.hip"), "-o", str(out)], check=True,
+                   capture_output=True)
+    loads = re.findall(r"buffer_load_dwordx4 \S+ \S+ (\S+) offen.* lds", out.read_text())
+    assert len(loads) > 64 and set(loads) == {"0"}

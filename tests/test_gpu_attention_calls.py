@@ -48,3 +48,35 @@ def test_outputs_on_a_stream_that_waits_for_nothing(dev, ws):
         torch.cuda.synchronize()  # the fills are done
         for g, w in zip(got if what == "plan" else [got], want):
             assert torch.equal(g, w), what
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (True, 40)])
+@pytest.mark.parametrize("Hq,Hkv,D", [(4, 2, 64), (3, 1, 96), (4, 2, 128), (2, 1, 256)])
+@pytest.mark.parametrize("lens", [(70, 33, 1), (127, 64, 200), (16, 129, 33)])
+def test_prompt_rows_around_a_prompt_are_not_read(dev, dt, causal, window, Hq, Hkv, D, lens):
+    """K and V rows behind a prompt's last, its neighbour's or no prompt's, hold
+    NaN and infinities: the outer prompts have the same bits as beside zeros.
+    (A value read there would meet a probability of 0, and the wave would take
+    its rows again in another order of sums.)"""
+    import torch
+    from inferflux_amd import attention as at
+    note(f"prompt neighbours {dt} causal={causal} window={window} D={D} lens={lens}")
+    g = gen(dev, D + lens[0])
+    stray, T = 5, sum(lens) + 10
+    a, b, c, d = (stray + sum(lens[:i]) for i in range(4))
+    q, k, v = (torch.randn(T, h, D, generator=g, device=dev).to(dt_of(dt)) for h in (Hq, Hkv, Hkv))
+    cu = i32([a, b, c, d], dev)
+    outs = []
+    for fill in ((0.0, 0.0), (float("nan"), float("inf"))):
+        for t in (k, v):
+            t[:a], t[b:c], t[d:] = fill[0], fill[1], fill[0]
+            t[b:c:2] = fill[0]
+        out = torch.full((T, Hq, D), 9.0, dtype=dt_of(dt), device=dev)
+        at.prompt_attention(q, k, v, cu, max(lens), causal=causal, window=window, out=out)
+        assert bool((out[:a] == 9).all()) and bool((out[d:] == 9).all())
+        outs.append(out)
+    for lo, hi in ((a, b), (c, d)):
+        assert torch.equal(outs[0][lo:hi], outs[1][lo:hi])
+        check(outs[1][lo:hi], *attend(q[lo:hi], k[lo:hi], v[lo:hi], 0, D ** -0.5, causal, window))
+    assert bool(torch.isnan(outs[1][b:c]).any())
