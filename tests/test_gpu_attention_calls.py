@@ -4,7 +4,7 @@ nonsense, with windows inside long chunks."""
 import pytest
 
 from tests.attn_ref import attend, check
-from tests.test_gpu_attention import Batch, dev, dt_of, gen, i32, ws  # noqa: F401
+from tests.test_gpu_attention import Batch, counters_clear, dev, dt_of, gen, i32, ws  # noqa: F401
 from tests.test_gpu_parity import note
 
 pytestmark = pytest.mark.gpu
@@ -80,3 +80,73 @@ def test_prompt_rows_around_a_prompt_are_not_read(dev, dt, causal, window, Hq, H
         assert torch.equal(outs[0][lo:hi], outs[1][lo:hi])
         check(outs[1][lo:hi], *attend(q[lo:hi], k[lo:hi], v[lo:hi], 0, D ** -0.5, causal, window))
     assert bool(torch.isnan(outs[1][b:c]).any())
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("window", [300, 1501, 2944])
+@pytest.mark.parametrize("Hq,Hkv,D,P,kv,new", [
+    (4, 2, 64, 16, [4300, 700, 40], [200, 130, 1]), (6, 2, 96, 32, [4100], [131]),
+    (8, 2, 128, 64, [4500, 4001, 90], [100, 33, 90]), (2, 1, 256, 16, [4200, 650], [150, 7])])
+def test_paged_chunks_in_windows(dev, ws, dt, window, Hq, Hkv, D, P, kv, new):
+    """Row tiles that see stages in part where their windows begin, whole ones
+    behind them and their causal end: cut into chunks, whose number differs
+    between the tiles of a request, and not; then with nonsense in the pages
+    before the window."""
+    import torch
+    from inferflux_amd import attention as at
+    note(f"paged tile window={window} {dt} Hq={Hq} Hkv={Hkv} D={D} P={P} kv={kv} new={new}")
+    assert at.paged_workspace_bytes(len(kv), sum(new), Hq, Hkv, D, max(new), max(kv)) > 0
+    x = Batch(dev, kv, new, Hq, Hkv, D, P, dt, seed=D + window, extra_rows=2)
+    x.run(ws, window=window)
+    first = x.out.clone()
+    x.verify(window=window)
+    for _ in range(2):
+        x.out.fill_(9.0)
+        x.run(ws, window=window)
+        assert torch.equal(first, x.out)
+    x.run(ws, window=window, max_kv=600)  # needs no workspace: not split
+    x.verify(window=window)
+    for b, (n, L) in enumerate(zip(new, kv)):
+        gone = x.table[b, :max(0, (L - n - window + 1) // P)].long()  # pages that no row sees
+        x.kc[gone], x.vc[gone] = float("nan"), float("inf")
+    x.run(ws, window=window)
+    x.verify(window=window)
+    assert counters_clear(ws)
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("kv,new", [([5000], [70]), ([2300, 3000, 1], [64, 129, 1])])
+def test_paged_chunks_split_heads_of_96(dev, ws, dt, kv, new):
+    """Split sums of an odd number of dim tiles."""
+    import torch
+    from inferflux_amd import attention as at
+    note(f"paged tile split {dt} D=96 kv={kv} new={new}")
+    assert at.paged_workspace_bytes(len(kv), sum(new), 6, 2, 96, max(new), max(kv)) > 0
+    x = Batch(dev, kv, new, 6, 2, 96, 16, dt, seed=5)
+    x.run(ws)
+    first = x.out.clone()
+    x.verify()
+    x.run(ws)
+    assert torch.equal(first, x.out)
+    assert counters_clear(ws)
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("window", [129, 400, 1000])
+@pytest.mark.parametrize("Hq,Hkv,D,lens", [
+    (4, 2, 64, [1201, 500]), (3, 1, 96, [1100]), (4, 2, 128, [30, 1333]), (2, 1, 256, [1050, 401])])
+def test_prompt_in_windows(dev, dt, window, Hq, Hkv, D, lens):
+    """Prompts longer than their window."""
+    import torch
+    from inferflux_amd import attention as at
+    note(f"prompt window={window} {dt} Hq={Hq} Hkv={Hkv} D={D} lens={lens}")
+    g, T = gen(dev, D + window), sum(lens)
+    q, k, v = (torch.randn(T, h, D, generator=g, device=dev).to(dt_of(dt)) for h in (Hq, Hkv, Hkv))
+    cu = i32([sum(lens[:b]) for b in range(len(lens) + 1)], dev)
+    got = at.prompt_attention(q, k, v, cu, max(lens), window=window)
+    assert torch.equal(got, at.prompt_attention(q, k, v, cu, max(lens), window=window))
+    a = 0
+    for n in lens:
+        check(got[a:a + n], *attend(q[a:a + n], k[a:a + n], v[a:a + n], 0, D ** -0.5, True, window),
+              f"prompt of {n}")
+        a += n
