@@ -79,6 +79,14 @@ def _new(shape, dtype, like, stream):
     return t
 
 
+def _count(v, name):
+    """A size or length as the C entries take it: ctypes would drop the bits
+    that do not fit."""
+    if not 0 <= v < 1 << 31:
+        raise ValueError(f"{name} must be from 0 to 2^31 - 1, got {v}")
+    return v
+
+
 def _on(t, name, device):
     if t.get_device() != device:
         raise ValueError(f"{name} must be on cuda:{device}")
@@ -153,6 +161,7 @@ def plan_batch(ctx_len, new_len, block_table, free_pages, free_count, page_size,
       NO_PAGES, NARROW, NO_ROOM, BAD_LENGTH: then nothing is taken, cu_q is 0
       and every slot -1)."""
     dev, B = _device(ctx_len, "ctx_len"), ctx_len.numel()
+    page_size, max_tokens = _count(page_size, "page_size"), _count(max_tokens, "max_tokens")
     if block_table.dim() != 2 or block_table.shape[0] != B:
         raise ValueError("block_table must be [B, pages]")
     if out is None:
@@ -220,7 +229,9 @@ def _out(q, out, out_dtype, stream):
 def paged_workspace_bytes(B, T, Hq, Hkv, head_dim, max_q, max_kv):
     """Bytes of workspace that paged_attention needs for this shape (0: none;
     WORKSPACE_BYTES is enough for all)."""
-    return int(_lib.load().ifx_attn_paged_workspace_bytes(B, T, Hq, Hkv, head_dim, max_q, max_kv))
+    return int(_lib.load().ifx_attn_paged_workspace_bytes(
+        _count(B, "B"), _count(T, "T"), _count(Hq, "Hq"), _count(Hkv, "Hkv"),
+        _count(head_dim, "head_dim"), _count(max_q, "max_q"), _count(max_kv, "max_kv")))
 
 
 def paged_attention(q, k_cache, v_cache, block_table, cu_q, kv_len, max_q, max_kv, scale=None,
@@ -257,8 +268,9 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_q, kv_len, max_q, max_k
     _launch(_lib.load().ifx_attn_paged, "ifx_attn_paged", dev, stream, qp, qs, _DTYPES[q.dtype],
             k_cache.data_ptr(), v_cache.data_ptr(), n, P,
             _i32(block_table, "block_table", B * W, dev), W, _i32(cu_q, "cu_q", B + 1, dev),
-            _i32(kv_len, "kv_len", B, dev), B, T, Hq, Hkv, D, max_q, max_kv,
-            D ** -0.5 if scale is None else scale, window, op, os, _DTYPES[out.dtype], wp, wn)
+            _i32(kv_len, "kv_len", B, dev), B, T, Hq, Hkv, D, _count(max_q, "max_q"),
+            _count(max_kv, "max_kv"), D ** -0.5 if scale is None else scale,
+            _count(window, "window"), op, os, _DTYPES[out.dtype], wp, wn)
     return out
 
 
@@ -285,7 +297,7 @@ def prompt_attention(q, k, v, cu_len, max_len, causal=True, window=0, scale=None
     vp, vs = _rows(v, "v", T, Hkv, D)
     op, os = _rows(out, "out", T, Hq, D)
     _launch(_lib.load().ifx_attn_prompt, "ifx_attn_prompt", dev, stream, qp, qs, kp, ks, vp, vs,
-            _DTYPES[q.dtype], _i32(cu_len, "cu_len", B + 1, dev), B, T, Hq, Hkv, D, max_len,
-            1 if causal else 0, window, D ** -0.5 if scale is None else scale, op, os,
-            _DTYPES[out.dtype])
+            _DTYPES[q.dtype], _i32(cu_len, "cu_len", B + 1, dev), B, T, Hq, Hkv, D,
+            _count(max_len, "max_len"), 1 if causal else 0, _count(window, "window"),
+            D ** -0.5 if scale is None else scale, op, os, _DTYPES[out.dtype])
     return out

@@ -216,3 +216,16 @@ def test_loads_of_packed_rows_are_bounded_by_the_lanes_offsets(tmp_path):
                    capture_output=True)
     loads = re.findall(r"buffer_load_dwordx4 \S+ \S+ (\S+) offen.* lds", out.read_text())
     assert len(loads) > 64 and set(loads) == {"0"}
+
+
+def test_counts_that_pass_32_bits_are_refused():
+    """A window of 2^32 + 1 keys is not one of 1; sizes below 0 are refused as
+    every other bad size."""
+    from inferflux_amd import attention as at
+    for v in (0, 5, 2 ** 31 - 1):
+        assert at._count(v, "n") == v
+    for v in (-1, 2 ** 31, 2 ** 32 + 1, -2 ** 32):
+        with pytest.raises(ValueError, match="window"):
+            at._count(v, "window")
+    with pytest.raises(ValueError, match="max_kv"):
+        at.paged_workspace_bytes(1, 1, 16, 2, 128, 1, 2 ** 32 + 3000)

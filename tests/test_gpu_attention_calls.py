@@ -150,3 +150,18 @@ def test_prompt_in_windows(dev, dt, window, Hq, Hkv, D, lens):
         check(got[a:a + n], *attend(q[a:a + n], k[a:a + n], v[a:a + n], 0, D ** -0.5, True, window),
               f"prompt of {n}")
         a += n
+
+
+def test_counts_that_pass_32_bits(dev, ws):
+    from inferflux_amd import attention as at
+    note("counts past 32 bits")
+    x = Batch(dev, [20, 30], [1, 1], 8, 2, 128, 16, "f16")
+    for bad in (dict(window=2 ** 32 + 1), dict(max_q=2 ** 32 + 1), dict(max_kv=-1)):
+        with pytest.raises(ValueError):
+            x.run(ws, **bad)
+    with pytest.raises(ValueError):
+        at.prompt_attention(x.q, x.q[:, :2], x.q[:, 2:4], x.cu, 2, window=2 ** 32 + 1)
+    for bad in (dict(page_size=2 ** 32 + 16, max_tokens=2), dict(page_size=16, max_tokens=-1),
+                dict(page_size=16, max_tokens=2 ** 32)):
+        with pytest.raises(ValueError):
+            at.plan_batch(x.kvt, x.kvt, x.table, x.cu, x.cu, **bad)
