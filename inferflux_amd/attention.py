@@ -219,11 +219,10 @@ def rope_append(q, k, v, positions, slots, k_cache, v_cache, inv_freq=None, inte
 
 
 def _out(q, out, out_dtype, stream):
-    if out is None:
-        return _new(q.shape, out_dtype or q.dtype, q, stream)
-    if out.dtype not in _DTYPES or (out_dtype is not None and out.dtype != out_dtype):
+    want = out_dtype or (q.dtype if out is None else out.dtype)
+    if want not in _DTYPES or (out is not None and out.dtype is not want):
         raise TypeError("out must be float32, float16 or bfloat16, and of out_dtype if that is given")
-    return out
+    return _new(q.shape, want, q, stream) if out is None else out
 
 
 def paged_workspace_bytes(B, T, Hq, Hkv, head_dim, max_q, max_kv):

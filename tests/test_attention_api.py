@@ -229,3 +229,16 @@ def test_counts_that_pass_32_bits_are_refused():
             at._count(v, "window")
     with pytest.raises(ValueError, match="max_kv"):
         at.paged_workspace_bytes(1, 1, 16, 2, 128, 1, 2 ** 32 + 3000)
+
+
+def test_output_types_that_no_kernel_writes():
+    import torch
+    from inferflux_amd import attention as at
+    q = torch.zeros(2, 4, 64, dtype=torch.float16)
+    for dt in (torch.float64, torch.int8):
+        with pytest.raises(TypeError):
+            at._out(q, None, dt, None)
+        with pytest.raises(TypeError):
+            at._out(q, q.to(dt), None, None)
+    assert at._out(q, None, torch.float32, None).dtype is torch.float32
+    assert at._out(q, None, None, None).dtype is torch.float16
