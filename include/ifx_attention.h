@@ -57,7 +57,7 @@ enum ifx_plan_status {
  *                  every slot -1
  * Outputs must not overlap inputs (block_table apart, which is updated in
  * place).  Calling again with the same inputs gives the same results.
- * 1 <= B <= IFX_ATTN_MAX_BATCH, 1 <= table_width, 0 <= max_tokens. */
+ * 1 <= B <= IFX_ATTN_MAX_BATCH, 1 <= table_width, 0 <= max_tokens <= 2^30. */
 int ifx_plan_batch(const int32_t *ctx_len, const int32_t *new_len, int32_t *block_table,
                    int table_width, const int32_t *free_pages, int free_capacity,
                    const int32_t *free_count, int page_size, int B, int max_tokens, int32_t *cu_q,
@@ -75,7 +75,8 @@ int ifx_plan_batch(const int32_t *ctx_len, const int32_t *new_len, int32_t *bloc
  * [T][Hq][D] rows q_out_stride elements apart.  A token whose slot is outside
  * [0, num_pages * page_size) is left out: nothing of it is written, q_out's
  * row neither.  Slots of one call must differ.  D: a multiple of 8 up to 256;
- * rot_dim a multiple of 16 up to D; num_pages * page_size < 2^31. */
+ * rot_dim a multiple of 16 up to D; num_pages * page_size < 2^31; T up to
+ * 2^27 - 8, as many as a launch has workgroups for. */
 int ifx_rope_append(const void *q, int64_t q_stride, const void *k, int64_t k_stride,
                     const void *v, int64_t v_stride, int src_dtype, const int32_t *positions,
                     const int32_t *slots, const double *inv_freq, int rot_dim, int interleaved,

@@ -112,7 +112,7 @@ int ifx_plan_batch(const int32_t *ctx_len, const int32_t *new_len, int32_t *bloc
                    int32_t *status, void *stream) {
   const int sh = page_shift_of(page_size);
   if (sh < 0 || B < 1 || B > IFX_ATTN_MAX_BATCH || table_width < 1 || free_capacity < 0 ||
-      max_tokens < 0)
+      max_tokens < 0 || max_tokens > (1 << 30))
     return IFX_BAD_GEOMETRY;
   if (!ctx_len || !new_len || !block_table || !free_count || !cu_q || !kv_len || !free_left ||
       !status || (free_capacity && !free_pages) || (max_tokens && (!positions || !slots)))
@@ -138,8 +138,8 @@ int ifx_rope_append(const void *q, int64_t q_stride, const void *k, int64_t k_st
   if (!is_out(src_dtype) || !is_elem(cache_dtype)) return IFX_UNSUPPORTED_TYPE;
   const int sh = page_shift_of(page_size);
   if (sh < 0 || num_pages < 1 || num_pages > (INT_MAX >> sh)) return IFX_BAD_GEOMETRY;
-  if (T < 0 || Hq < 1 || Hkv < 1 || Hq > 65536 || Hkv > 65536 || D < 8 || D > 256 || D % 8 ||
-      rot_dim < 0 || rot_dim > D || rot_dim % 16)
+  if (T < 0 || T > (1 << 27) - 8 || Hq < 1 || Hkv < 1 || Hq > 65536 || Hkv > 65536 || D < 8 ||
+      D > 256 || D % 8 || rot_dim < 0 || rot_dim > D || rot_dim % 16)
     return IFX_BAD_GEOMETRY;
   const int64_t qn = static_cast<int64_t>(Hq) * D, kn = static_cast<int64_t>(Hkv) * D;
   if (q_stride < qn || k_stride < kn || v_stride < kn || q_out_stride < qn) return IFX_BAD_GEOMETRY;

@@ -242,3 +242,16 @@ def test_output_types_that_no_kernel_writes():
             at._out(q, q.to(dt), None, None)
     assert at._out(q, None, torch.float32, None).dtype is torch.float32
     assert at._out(q, None, None, None).dtype is torch.float16
+
+
+@pytest.mark.parametrize("T,want", [((1 << 30), OK), ((1 << 30) + 1, GEOM), (2 ** 31 - 1, GEOM)])
+def test_plan_rows_that_fit_the_grid(lib, T, want):
+    with dry(lib):
+        assert lib.ifx_plan_batch(*{**PLAN, "T": T}.values()) == want
+
+
+@pytest.mark.parametrize("T,want", [((1 << 27) - 8, OK), ((1 << 27) - 7, GEOM), (2 ** 31 - 1, GEOM)])
+def test_append_rows_that_fit_the_grid(lib, T, want):
+    """A launch has less than 2^32 threads: eight tokens a workgroup of 256."""
+    with dry(lib):
+        assert lib.ifx_rope_append(*{**APPEND, "T": T}.values()) == want
