@@ -111,7 +111,8 @@ int ifx_rope_append(const void *q, int64_t q_stride, const void *k, int64_t k_st
  * sums are added in order: the same bits on every call.  Calls that share a
  * workspace must not overlap.  May be NULL with 0 bytes where none is needed.
  *
- * D: 64, 96, 128 or 256.  Hq a multiple of Hkv, Hkv * D < 2^22.  scale > 0.
+ * D: 64, 96, 128 or 256.  Hq a multiple of Hkv, Hkv * D < 2^22.  scale > 0,
+ * and scale log2 e finite.
  * table_width * page_size <= 2^30. */
 #define IFX_ATTN_WORKSPACE_BYTES (64 << 20)
 int64_t ifx_attn_paged_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int max_q,

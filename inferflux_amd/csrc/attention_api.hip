@@ -47,6 +47,9 @@ bool heads_ok(int B, int T, int Hq, int Hkv, int D) {
   return rows < (1 << 30) && (rows / 32 + B) * Hkv < (1 << 23);
 }
 
+// scale log2 e is what the kernels multiply by.
+bool scale_ok(float scale) { return scale > 0.0f && std::isfinite(scale * kLog2e); }
+
 // Positions are below 2^30: a window as wide is none, and position - window
 // stays within 32 bits, also of rows before the first key (above -2^30).
 int window_of(int window) { return window < (1 << 30) ? window : 0; }
@@ -173,7 +176,7 @@ int ifx_attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cac
       table_width > ((1 << 30) >> sh))  // positions and the stages behind them fit an int
     return IFX_BAD_GEOMETRY;
   if (!heads_ok(B, T, Hq, Hkv, D) || max_q < 1 || max_kv < 1 || window < 0 ||
-      !(scale > 0.0f) || !std::isfinite(scale))
+      !scale_ok(scale))
     return IFX_BAD_GEOMETRY;
   const int64_t qn = static_cast<int64_t>(Hq) * D;
   if (q_stride < qn || out_stride < qn) return IFX_BAD_GEOMETRY;
@@ -213,7 +216,7 @@ int ifx_attn_prompt(const void *q, int64_t q_stride, const void *k, int64_t k_st
                     float scale, void *out, int64_t out_stride, int out_dtype, void *stream) {
   if (!is_elem(dtype) || !is_out(out_dtype)) return IFX_UNSUPPORTED_TYPE;
   if (!heads_ok(B, T, Hq, Hkv, D) || max_len < 1 || window < 0 || (window > 0 && !causal) ||
-      !(scale > 0.0f) || !std::isfinite(scale))
+      !scale_ok(scale))
     return IFX_BAD_GEOMETRY;
   const int64_t qn = static_cast<int64_t>(Hq) * D, kn = static_cast<int64_t>(Hkv) * D;
   // 64 rows of K or V are addressed by 32-bit offsets

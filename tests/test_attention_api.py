@@ -255,3 +255,12 @@ def test_append_rows_that_fit_the_grid(lib, T, want):
     """A launch has less than 2^32 threads: eight tokens a workgroup of 256."""
     with dry(lib):
         assert lib.ifx_rope_append(*{**APPEND, "T": T}.values()) == want
+
+
+@pytest.mark.parametrize("scale,want", [(2.3e38, OK), (2.4e38, GEOM), (3.4e38, GEOM)])
+def test_scales_that_pass_fp32_with_log2_e(lib, scale, want):
+    """The kernels' factor is scale log2 e: as an infinity it makes scores of 0
+    no numbers."""
+    with dry(lib):
+        assert lib.ifx_attn_paged(*{**PAGED, "scale": scale}.values()) == want
+        assert lib.ifx_attn_prompt(*{**PROMPT, "scale": scale}.values()) == want
