@@ -11,7 +11,8 @@
  * The paged cache.  A cache of one layer is num_pages pages of page_size
  * tokens (16, 32, 64, 128 or 256), 16-bit (fp16 or bf16), in the order in
  * which the MFMA instructions take their operands, so that a lane reads 16
- * contiguous bytes and a wave contiguous half kilobytes or more:
+ * contiguous bytes and half a wave half a kilobyte (of K at pages of 16 tokens
+ * two pages' 256 bytes):
  *   K  [page][kv head][D / 8][token in page][8]
  *   V  [page][kv head][token in page / 8][D][8]
  * Token i of a request lives in slot page * page_size + i % page_size, where
@@ -128,8 +129,9 @@ int ifx_attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cac
  * q [T][Hq][D], k and v [T][Hkv][D], rows cu_len[b] .. cu_len[b + 1] - 1 are
  * prompt b.  Row i of a prompt of n sees its rows j < n, and j <= i where
  * causal, and j > i - window where causal and window > 0.  Otherwise as
- * ifx_attn_paged; k_stride, v_stride < 2^23.  max_len > 0 bounds the prompts'
- * lengths. */
+ * ifx_attn_paged; k_stride, v_stride < 2^23.  max_len > 0 is a bound of the
+ * prompts' lengths; it is checked to be positive and plans nothing: prompts of
+ * any length up to T are computed whole. */
 int ifx_attn_prompt(const void *q, int64_t q_stride, const void *k, int64_t k_stride,
                     const void *v, int64_t v_stride, int dtype, const int32_t *cu_len, int B,
                     int T, int Hq, int Hkv, int D, int max_len, int causal, int window,

@@ -238,8 +238,9 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_q, kv_len, max_q, max_k
     """Attention of the new tokens q [T, Hq, D] over the paged cache, which
     holds them already (ifx_attn_paged).  cu_q [B + 1]: the requests' first
     rows; kv_len [B]: their tokens, the new ones included; max_q, max_kv: bounds
-    of a request's rows (those past max_q may be left out) and tokens.  A query sees its own position and what is before it, the last
-    `window` keys of it where window > 0.  scale: head_dim ** -0.5 if None.
+    of a request's rows (those past max_q may be left out) and tokens.  A query
+    sees its own position and what is before it, the last `window` keys of it
+    where window > 0.  scale: head_dim ** -0.5 if None.
     Returns out [T, Hq, D] (out_dtype: fp32, fp16 or bf16, q's type if None);
     its rows from cu_q[B] on are left as they were.  workspace: see
     `workspace` and paged_workspace_bytes."""
@@ -277,7 +278,8 @@ def prompt_attention(q, k, v, cu_len, max_len, causal=True, window=0, scale=None
                      out_dtype=None, stream=None):
     """Attention over whole prompts packed one after the other, without a cache
     (ifx_attn_prompt): q [T, Hq, D], k and v [T, Hkv, D] (fp16 or bf16), rows
-    cu_len[b] .. cu_len[b + 1] - 1 are prompt b, max_len bounds the lengths.
+    cu_len[b] .. cu_len[b + 1] - 1 are prompt b, max_len bounds the lengths
+    (checked to be positive, no launch depends on it).
     A row sees its prompt's rows; where causal those up to its own, the last
     `window` of them where window > 0.  Returns out [T, Hq, D] (out_dtype:
     fp32, fp16 or bf16, q's type if None)."""

@@ -71,12 +71,13 @@ struct PagedPlan {
 // for each key/value head, whose lengths the workgroups find (find_item).
 //
 // attn_tile: as many as are resident, two a CU (D = 64: three, D = 256: one).
-// A chunk of 512 tokens over 7430 keys, 40 / 8 heads of 128: 114 us with 512,
-// 116 with 768, 124 with 1000.
+// A chunk of 512 tokens over 7430 keys, 40 / 8 heads of 128: 143 us with 256,
+// 115 with 384, 95 with 512, 107 with 768, 101 with 1000.
 //
-// attn_rows: two rounds of those that are resident, as requests differ in
-// length.  32 requests of 531 to 22591 keys, 40 / 8 heads of 128: 167 us with
-// 512, 152 with 768, 151 with 1024, 156 with 1536, 160 with 2048.
+// attn_rows: two rounds of those that are resident at two a CU (D = 256: four
+// rounds at one), as requests differ in length.  32 requests of 531 to 22591
+// keys, 40 / 8 heads of 128: 162 us with 512, 150 with 768, 148 with 1024, 150
+// with 1536, 153 with 2048.
 //
 // Fewer where the split sums would not fit the largest workspace.
 PagedPlan plan_paged(int B, int T, int Hq, int Hkv, int D, int max_q, int max_kv) {

@@ -15,7 +15,8 @@
 // workgroup of a request and head to finish adds the chunks in their order.
 //
 // Measured: 32 requests of 531 to 22591 keys, 40 query and 8 key/value heads of
-// 128 (796 MB), 148 us, 5.4 TB/s; with chunks as long as the longest request's
+// 128 (796 MB), 148 us, 5.4 TB/s (matrix cores busy for 7 % of the time, vector
+// units for 13); with chunks as long as the longest request's
 // eighth, 187.  One request of 3000 keys, 16 and 2 heads: 9.6 us, of them 1 to
 // find the work, 1.4 for the keys, 1.7 for the waves' and 4 for the chunks' sums.
 #include "ifx_attn.h"

@@ -15,17 +15,20 @@
 // next product's operand as they stand (key_of_row).
 //
 // Measured at 40 query and 8 key/value heads of 128: a causal prompt of 8111
-// tokens in 645 us, 1.04 PFLOP/s (a large 16-bit matrix product reaches 1.2 on
-// the same card); a chunk of 512 tokens over 7430 cached ones in 95 us.  What
-// took longer, for that prompt: stages through registers 3207 us, as they
+// tokens in 630 us, 1.07 PFLOP/s (a large 16-bit matrix product reaches 1.2 on
+// the same card), and in up to 737 where the card has lowered its clock; there
+// the matrix cores are busy for 56 % of the time and the vector units for 47 %.
+// A chunk of 512 tokens over 7430 cached ones in 90 us.  What took longer, for
+// that prompt, on the way: stages through registers 3207 us, as they
 // spill; fragments read where they are needed 701, when kAhead of them on their
 // way took 657; V transposed in registers 800; 64 rows a wave 2600, for the
 // moves between the halves of the register file; 8 waves in two groups half a
 // stage apart 671.
 //
 // Registers: 256 a wave, two workgroups a CU.  D = 64 does with 168, three a
-// CU: 8111 tokens of 40 / 8 heads in 370 us, two 387, four 1330 (spills).
-// D = 256 needs 512.
+// CU: 8111 tokens of 40 / 8 heads took 370 us, with two 387, with four 1330
+// (spills).  D = 256 needs 512: 4111 tokens of 16 / 2 heads in 241 us (fp16) or
+// 276 (bf16).
 #include "ifx_attn.h"
 
 namespace ifx {
@@ -40,8 +43,8 @@ constexpr int kRows = 32 * kNW;  // its query rows
 constexpr int TK = kTileKeys;
 // Stages of a chunk at least: beside them it takes 6 us for its first loads and
 // its sums' exchange, as much as 5 stages.  A mixed batch (16 decode steps, 8
-// chunks): 33 us with 4 or 6, 29 with 8, 30 with 12; 60 tokens over 3000: 24,
-// 23, 25, 27.
+// chunks): 32 us with 4 or 6, 28 with 8, 30 with 12; 60 tokens over 3000: 23,
+// 23, 25, 30.
 constexpr int kMinChunk = 8;
 
 // LDS places, in 16-byte pieces of 8 values.  Copies go from memory to LDS

@@ -12,6 +12,13 @@ namespace ifx {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// Probabilities are rounded to the caches' type for the product with V: its
+// MFMA takes 16-bit operands, in fp32 it runs at a sixteenth of the rate, and
+// two 16-bit parts of each would be half as many products again.  The row sums
+// take them unrounded.  Against 64 bits an output is off by 0.0020 to 0.0023 of
+// its size in bf16 and 0.00023 to 0.00028 in fp16, where rounding the output
+// alone leaves 0.0017 and 0.0002.
+//
 // 16-bit element types: the MFMA operand, the conversion of two fp32 values
 // (round to nearest even) into one dword, and of one back.
 struct F16 {
@@ -168,7 +175,19 @@ struct AttnArgs {
 
 // Query rows of one key/value head: row r of a request is query head r % G of
 // the group and new token r / G.
-constexpr int kRowsMax = 32;   // rows of a request that attn_rows takes
+//
+// Rows of a request that attn_rows takes: what one of its MFMA tiles holds.  It
+// is made for decode steps, and drafts of many tokens would gain from a lower
+// bound where there are several requests.  us with attn_rows / attn_tile:
+//   16 / 2 heads of 128, rows     8          16         24         32
+//     1 request of 3000 keys  10.1/18.3  12.3/18.3  14.9/18.4  17.5/18.5
+//     8                       12.4/19.5  15.7/19.4  19.6/19.6  23.8/19.9
+//     32 of 6000              39.5/38.7  43.3/39.0  48.1/39.5  45.0/40.1
+//   40 / 8 heads, rows            5          15         20         30
+//     1 request of 3000 keys   9.6/18.1  12.3/18.3  14.5/18.4  17.3/18.6
+//     8                       26.1/26.6  29.6/26.8  33.0/26.9  37.3/27.6
+//     32 of 6000               144/152    150/152    155/154    162/154
+constexpr int kRowsMax = 32;
 constexpr int kRowKeys = 128;  // attn_rows: keys of a stage, 32 for each wave
 constexpr int kTileKeys = 64;  // attn_tile: keys of a stage
 
@@ -238,7 +257,7 @@ struct Split {
 // else chunks are so long that a request of s > c stages, cut in less than
 // s / c + 1 < 2 s / c of them, leaves no more.  Lane l has requests l, l + 64,
 // ...: their places in LDS are neighbours' (with consecutive ones a lane, 1024
-// prompts of 30 to 60 tokens took 283 us, not 168).
+// prompts of 30 to 60 tokens of 16 / 2 heads took 283 us; 177 now).
 template <int MIN_CHUNK, class Work>
 __device__ __forceinline__ Split find_item(const AttnArgs &a, int2 *reqs, int i, Work work) {
   const int lane = threadIdx.x & 63, B = a.B, goal = a.goal;

@@ -10,8 +10,8 @@
 //
 // Bound by latency: a launch, one dependent read of the lengths, one of the
 // tables.  So a single launch does it all: every workgroup scans the B
-// lengths itself (16 KB at most, from L2) instead of waiting for another to
-// do it, and then places its own span of tokens by a binary search among the
+// lengths itself (two arrays, 32 KB at most, from L2) instead of waiting for
+// another to do it, and then places its own span of tokens by a binary search among the
 // row offsets in LDS.  A new page's table entry is written by the thread that
 // places the page's first token: no thread reads an entry that another
 // writes, because entries below held_b are only read.  Measured: 32 decode

@@ -4,14 +4,19 @@
 //   y_i = x_i cos(a) - x_j sin(a),  y_j = x_j cos(a) + x_i sin(a),
 //   a = position * inv_freq
 //
-// Bound by HBM: every value is read once and written once.  The angle is
+// Every value is read once and written once, and at prompts' sizes HBM would be
+// the bound; what holds it up is that a workgroup's first rows are asked for
+// only behind its slots, positions, angles and a barrier, with two units a
+// thread to hide that, and that lanes of neighbouring pieces read their angles
+// from the same LDS banks (15 cycles an instruction).  The angle is
 // formed in fp64 as turns and reduced to half a turn there (a position of
 // 10^5 would leave an fp32 angle 10^-2 off), its sine and cosine in fp32: one
 // pair per position and frequency, shared by all heads through LDS.
 //
 // Measured: 5299 tokens of 40 query and 8 key/value heads of 128, fp16 (152 MB):
-// 43 us from memory, 3.5 TB/s, and 29 where the rows are still in the caches; 8
-// tokens of 16 and 2 heads, fp32: a kernel of 3.9 us.
+// 43 us from memory, 3.5 TB/s, and 27 where the rows are still in the caches
+// (vector units busy for 39 % of the time); 8 tokens of 16 and 2 heads, fp32: a
+// kernel of 3.9 us.
 #include "ifx_attn.h"
 
 namespace ifx {
@@ -200,8 +205,18 @@ __global__ __launch_bounds__(256) void k_rope_append(const AppendArgs a) {
 namespace {
 template <int DT, int SRC>
 void launch(const AppendArgs &a, hipStream_t s) {
+  // One token a workgroup hides its chain of dependent steps best, eight share
+  // K's and V's cache lines.  us with one / eight, rows in the caches, heads of 128:
+  //   tokens               32       256       512       1024       2048       5299
+  //   16 / 2, fp16     4.4/5.9   4.8/6.1   5.4/6.2   6.4/6.8  10.0/7.5  20.5/13.6
+  //   16 / 2, fp32     3.9/5.3   4.3/5.5   4.8/5.6   6.0/6.1   9.6/7.1  21.7/15.5
+  //   40 / 8, fp16     5.6/8.0   6.6/8.4   9.5/9.2  11.9/11.2 19.6/14.3 44.8/25.4
+  //   40 / 8, fp32     4.4/6.8   5.5/7.2   7.8/7.8  13.3/9.5  25.2/15.4 59.1/35.3
+  // They meet at 500 to 1200 tokens; from 2048 on eight are faster by a quarter
+  // at least for all of these.
   if (a.T >= 2048) {
-    // 5299 tokens as above: 54 us with one part for all, 45 with 2 for Q, 43 with 5
+    // 5299 tokens as above, from memory: 54 us with one part for all, 45 with 2 for
+    // Q, 43 with 5
     IFX_LAUNCH(k_rope_append, (DT, SRC, 8), dim3((a.T + 7) / 8, 6), dim3(256), 0, s, a);
   } else {
     IFX_LAUNCH(k_rope_append, (DT, SRC, 1), dim3(a.T, 2), dim3(256), 0, s, a);
