@@ -165,3 +165,54 @@ def test_counts_that_pass_32_bits(dev, ws):
                 dict(page_size=16, max_tokens=2 ** 32)):
         with pytest.raises(ValueError):
             at.plan_batch(x.kvt, x.kvt, x.table, x.cu, x.cu, **bad)
+
+
+def test_captured_calls_on_a_side_stream(dev, ws):
+    """Calls on a stream that a capture forks to, their outputs allocated in the
+    capture: replays with new inputs equal the eager results."""
+    import torch
+    from inferflux_amd import attention as at
+    note("capture with a side stream")
+    x = Batch(dev, [300, 90], [40, 1], 8, 2, 128, 16, "f16", seed=6)
+    side, ws2 = torch.cuda.Stream(), at.workspace(dev)
+
+    def both(stream, w):
+        o = at.paged_attention(x.q, x.kc, x.vc, x.table, x.cu, x.kvt, 40, 300, workspace=w, stream=stream)
+        return o, at.prompt_attention(x.q, x.q[:, :2], x.q[:, 2:4], x.cu, 40, stream=stream)
+
+    both(None, ws2)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        o, p = both(side, ws2)
+        here.wait_stream(side)
+        outs = o + 0, p + 0
+    for i in range(3):
+        x.q.copy_(torch.randn(x.q.shape, generator=gen(dev, i), device=dev))
+        gr.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in outs]
+        for a, b in zip(got, both(None, ws)):
+            assert torch.equal(a, b)
+        torch.cuda.synchronize()
+
+
+def test_two_calls_at_once(dev):
+    """Split calls on two streams, each with its workspace, at the same time."""
+    import torch
+    from inferflux_amd import attention as at
+    note("two streams")
+    xs = [Batch(dev, [6000, 50, 3000], [1, 1, 1], 16, 2, 128, 64, "f16", seed=1),
+          Batch(dev, [4000, 64], [70, 2], 8, 2, 128, 16, "f16", seed=2)]
+    wss = [at.workspace(dev) for _ in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for x, w, s in zip(xs, wss, streams):
+            x.run(w, stream=s)
+    torch.cuda.synchronize()
+    for x, w in zip(xs, wss):
+        x.verify()
+        assert counters_clear(w)
