@@ -110,6 +110,19 @@ SIGNATURES.update({
                          _i32, _i32, _i32, ctypes.c_float, _vp, _i64, _i32, _vp], _i32),
 })
 
+# Every symbol include/ifx_drafts.h declares.
+SIGNATURES.update({
+    "ifx_plan_tree": ([_vp] * 3 + [_i32, _i32] + [_vp] * 3, _i32),
+    "ifx_attn_tree": ([_vp, _i64, _i32, _vp, _vp, _i64, _i32, _vp, _i32, _vp, _vp, _vp] + [_i32] * 7 +
+                      [ctypes.c_float, _vp, _i64, _i32, _vp, _i64, _vp], _i32),
+    "ifx_verify_workspace_bytes": ([_i32, _i32], _i64),
+    "ifx_verify": ([_vp] * 3 + [_i32] * 3 + [_vp, _i64, _vp, _i64, _i32, _i32] + [_vp] * 6 +
+                   [_i64, _vp], _i32),
+    "ifx_keep_path": ([_vp] * 3 + [_i32, _i64, _i32, _i32, _i32, _vp, _i32] + [_vp] * 4 +
+                      [_i32] * 3 + [_vp], _i32),
+    "ifx_plan_kept": ([_vp] * 4 + [_i32, _vp, _i32, _vp, _i32, _i32] + [_vp] * 4, _i32),
+})
+
 _lib = None
 
 

@@ -33,6 +33,7 @@ EXACT = {"quantize.hip", "dequant.hip"}
 SOURCES = ["api.hip", "quantize.hip", "dequant.hip", "gemv.hip", "mmq_skinny.hip", "mmvq.hip", "gemm_mfma.hip", "gemv_lds.hip", "gemv_slot.hip", "gemm_f16.hip", "gemm_f16_q4.hip", "gemm_f16_q6.hip", "gemm_f16_q8.hip",
            "gemv_dq.hip", "packed.hip",
            "attention_api.hip", "kv_plan.hip", "rope_append.hip", "attn_rows.hip", "attn_tile.hip",
+           "drafts_api.hip", "draft_plan.hip", "verify_drafts.hip", "keep_path.hip",
            "../host/fused_quant_gemm.cpp", "../host/native_dispatch.cpp", "../host/gguf.cpp", "../host/gguf_model.cpp"]
 
 

@@ -1,9 +1,10 @@
-// attention_api.hip -- the C entry points of include/ifx_attention.h:
-// validation, the split of keys over workgroups, and the launches.
+// attention_api.hip -- the C entry points of include/ifx_attention.h, and the
+// attention's of include/ifx_drafts.h: validation, the split of keys over
+// workgroups, and the launches.
 #include <climits>
 #include <cmath>
 
-#include "ifx_attn.h"
+#include "ifx_drafts_impl.h"
 #include "ifx_qgemm.h"
 
 namespace ifx {
@@ -58,8 +59,8 @@ int window_of(int window) { return window < (1 << 30) ? window : 0; }
 // split, their counters at the start of the workspace.  The counters' place is
 // the same for every shape, as one workspace serves calls of many shapes and
 // only they have to be zero between calls.
-constexpr int kMaxUnits = 8192;
-constexpr int64_t kCntBytes = kMaxUnits * 4;
+constexpr int kMaxUnits = kSplitUnits;
+constexpr int64_t kCntBytes = kSplitCntBytes;
 
 struct PagedPlan {
   bool rows;         // attn_rows, else attn_tile
@@ -103,6 +104,54 @@ PagedPlan plan_paged(int B, int T, int Hq, int Hkv, int D, int max_q, int max_kv
   p.items = static_cast<int>(tiles + goal);
   p.bytes = goal ? kCntBytes + goal * Hkv * slot : 0;
   return p;
+}
+
+// masks: the nodes that rows of trees see, or null.
+int attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cache,
+               const void *v_cache, int64_t num_pages, int page_size, const int32_t *block_table,
+               int table_width, const int32_t *cu_q, const int32_t *kv_len, const uint64_t *masks,
+               int B, int T, int Hq, int Hkv, int D, int max_q, int max_kv, float scale,
+               int window, void *out, int64_t out_stride, int out_dtype, void *workspace,
+               int64_t workspace_bytes, void *stream) {
+  if (!is_elem(dtype) || !is_out(out_dtype)) return IFX_UNSUPPORTED_TYPE;
+  const int sh = page_shift_of(page_size);
+  if (sh < 0 || num_pages < 1 || num_pages > (INT_MAX >> sh) || table_width < 1 ||
+      table_width > ((1 << 30) >> sh))  // positions and the stages behind them fit an int
+    return IFX_BAD_GEOMETRY;
+  if (!heads_ok(B, T, Hq, Hkv, D) || max_q < 1 || max_kv < 1 || window < 0 ||
+      !scale_ok(scale))
+    return IFX_BAD_GEOMETRY;
+  const int64_t qn = static_cast<int64_t>(Hq) * D;
+  if (q_stride < qn || out_stride < qn) return IFX_BAD_GEOMETRY;
+  if (T == 0) return IFX_OK;
+  if (!q || !k_cache || !v_cache || !block_table || !cu_q || !kv_len || !out)
+    return IFX_NULL_POINTER;
+  if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15)
+    return IFX_BAD_GEOMETRY;
+  const PagedPlan p = plan_paged(B, T, Hq, Hkv, D, max_q, max_kv);
+  if (p.bytes) {
+    if (!workspace) return IFX_NULL_POINTER;
+    if (workspace_bytes < p.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255))
+      return IFX_BAD_GEOMETRY;
+  }
+  AttnArgs a{};
+  a.q = q, a.k = k_cache, a.v = v_cache, a.out = out;
+  a.q_stride = q_stride, a.out_stride = out_stride;
+  a.table = block_table, a.cu = cu_q, a.kv_len = kv_len;
+  a.num_pages = num_pages, a.table_width = table_width, a.page_shift = sh;
+  a.B = B, a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv;
+  a.causal = 1, a.window = window_of(window), a.out_dtype = out_dtype;
+  a.masks = masks;
+  a.c = scale * kLog2e;
+  a.goal = p.goal;
+  if (p.bytes) {
+    a.cnt = static_cast<uint32_t *>(workspace);
+    a.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + kCntBytes);
+    a.part_bytes = static_cast<uint32_t>(p.bytes - kCntBytes);
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (p.rows) return status_of(launch_attn_rows(a, dtype, D, max_q * a.G, p.items, s));
+  return status_of(launch_attn_tile(a, dtype, D, true, p.items, s));
 }
 
 }  // namespace
@@ -171,44 +220,22 @@ int ifx_attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cac
                    const int32_t *kv_len, int B, int T, int Hq, int Hkv, int D, int max_q,
                    int max_kv, float scale, int window, void *out, int64_t out_stride,
                    int out_dtype, void *workspace, int64_t workspace_bytes, void *stream) {
-  if (!is_elem(dtype) || !is_out(out_dtype)) return IFX_UNSUPPORTED_TYPE;
-  const int sh = page_shift_of(page_size);
-  if (sh < 0 || num_pages < 1 || num_pages > (INT_MAX >> sh) || table_width < 1 ||
-      table_width > ((1 << 30) >> sh))  // positions and the stages behind them fit an int
-    return IFX_BAD_GEOMETRY;
-  if (!heads_ok(B, T, Hq, Hkv, D) || max_q < 1 || max_kv < 1 || window < 0 ||
-      !scale_ok(scale))
-    return IFX_BAD_GEOMETRY;
-  const int64_t qn = static_cast<int64_t>(Hq) * D;
-  if (q_stride < qn || out_stride < qn) return IFX_BAD_GEOMETRY;
-  if (T == 0) return IFX_OK;
-  if (!q || !k_cache || !v_cache || !block_table || !cu_q || !kv_len || !out)
-    return IFX_NULL_POINTER;
-  if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15)
-    return IFX_BAD_GEOMETRY;
-  const PagedPlan p = plan_paged(B, T, Hq, Hkv, D, max_q, max_kv);
-  if (p.bytes) {
-    if (!workspace) return IFX_NULL_POINTER;
-    if (workspace_bytes < p.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255))
-      return IFX_BAD_GEOMETRY;
-  }
-  AttnArgs a{};
-  a.q = q, a.k = k_cache, a.v = v_cache, a.out = out;
-  a.q_stride = q_stride, a.out_stride = out_stride;
-  a.table = block_table, a.cu = cu_q, a.kv_len = kv_len;
-  a.num_pages = num_pages, a.table_width = table_width, a.page_shift = sh;
-  a.B = B, a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv;
-  a.causal = 1, a.window = window_of(window), a.out_dtype = out_dtype;
-  a.c = scale * kLog2e;
-  a.goal = p.goal;
-  if (p.bytes) {
-    a.cnt = static_cast<uint32_t *>(workspace);
-    a.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + kCntBytes);
-    a.part_bytes = static_cast<uint32_t>(p.bytes - kCntBytes);
-  }
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  if (p.rows) return status_of(launch_attn_rows(a, dtype, D, max_q * a.G, p.items, s));
-  return status_of(launch_attn_tile(a, dtype, D, true, p.items, s));
+  return attn_paged(q, q_stride, dtype, k_cache, v_cache, num_pages, page_size, block_table,
+                    table_width, cu_q, kv_len, nullptr, B, T, Hq, Hkv, D, max_q, max_kv, scale,
+                    window, out, out_stride, out_dtype, workspace, workspace_bytes, stream);
+}
+
+int ifx_attn_tree(const void *q, int64_t q_stride, int dtype, const void *k_cache,
+                  const void *v_cache, int64_t num_pages, int page_size,
+                  const int32_t *block_table, int table_width, const int32_t *cu_q,
+                  const int32_t *kv_len, const uint64_t *masks, int B, int T, int Hq, int Hkv,
+                  int D, int max_q, int max_kv, float scale, void *out, int64_t out_stride,
+                  int out_dtype, void *workspace, int64_t workspace_bytes, void *stream) {
+  if (max_q > IFX_TREE_MAX_NODES) return IFX_BAD_GEOMETRY;
+  if (T && !masks) return IFX_NULL_POINTER;
+  return attn_paged(q, q_stride, dtype, k_cache, v_cache, num_pages, page_size, block_table,
+                    table_width, cu_q, kv_len, masks, B, T, Hq, Hkv, D, max_q, max_kv, scale, 0,
+                    out, out_stride, out_dtype, workspace, workspace_bytes, stream);
 }
 
 int ifx_attn_prompt(const void *q, int64_t q_stride, const void *k, int64_t k_stride,

@@ -19,14 +19,13 @@
 // units for 13); with chunks as long as the longest request's
 // eighth, 187.  One request of 3000 keys, 16 and 2 heads: 9.6 us, of them 1 to
 // find the work, 1.4 for the keys, 1.7 for the waves' and 4 for the chunks' sums.
-#include "ifx_attn.h"
+#include "ifx_attn_rows.h"
 
 namespace ifx {
 
 namespace {
 
-constexpr int kWaves = 4;
-constexpr uint32_t kOut = 1u << 30;  // an offset past the workspace's end: reads zeros
+constexpr int kWaves = kRowWaves;
 
 // The four dwords of an 8-key piece with the keys outside [lo, hi] cleared.
 struct PieceMask {
@@ -44,12 +43,13 @@ __device__ __forceinline__ PieceMask piece_mask(int key, int lo, int hi) {
 
 }  // namespace
 
-template <int DT, int D>
+// TREE: rows see the cached tokens and the nodes of their masks.
+template <int DT, int D, bool TREE = false>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(const AttnArgs a, int lds_rows) {
   using T = Elem<DT>;
   constexpr int ND = D / 32, NS = D / 16;
   extern __shared__ float red[];  // [wave][D / 4][row][4]; at first the requests
-  __shared__ float red_m[kWaves][32], red_l[kWaves][32];
+  __shared__ RowSums sums;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kvh = blockIdx.x % a.Hkv;
@@ -75,7 +75,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(const AttnA
 
   // this lane's row: what it sees is [lo, hi]; rows behind the last repeat it
   const int row = min(n, R - 1), tok = row / a.G, head = kvh * a.G + row % a.G;
-  const int hi = ctx + tok, lo = a.window > 0 ? max(0, hi - a.window + 1) : 0;
+  Sight<TREE> sight = {0, ctx + tok, ctx, 0};
+  if constexpr (TREE)
+    sight.bits = node_bits(a, q0 + tok, nq);
+  else if (a.window > 0)
+    sight.lo = max(0, sight.hi - a.window + 1);
   u32x4 qf[NS];
   {
     const uint16_t *q = static_cast<const uint16_t *>(a.q) + (q0 + tok) * a.q_stride +
@@ -131,12 +135,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(const AttnA
 #pragma unroll
     for (int i = 0; i < NS; ++i) s = T::mfma32(kf[i], qf[i], s);
 
-    const bool edge = k0 + 31 > ctx || (a.window > 0 && k0 < ctx + nq - a.window);
+    const bool edge = k0 + 31 > ctx - TREE || (a.window > 0 && k0 < ctx + nq - a.window);
     if (edge) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int key = k0 + 16 * (r >> 3) + 8 * h + (r & 7);
-        s[r] = key >= lo && key <= hi ? s[r] : -__builtin_inff();
+        s[r] = sight.sees(key) ? s[r] : -__builtin_inff();
       }
       // values that no row sees: the pages' unwritten slots among them
 #pragma unroll
@@ -175,7 +179,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(const AttnA
     l += sum;
 
     bool apart = false;  // an infinity or NaN in V that some rows see and others do not
-    if (edge && nq > 1) {
+    if (edge && (TREE || nq > 1)) {
       f32x16 probe;
 #pragma unroll
       for (int r = 0; r < 16; ++r) probe[r] = 0.0f;
@@ -205,7 +209,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(const AttnA
         const float p = T::value(static_cast<uint32_t>(
             __shfl(static_cast<int>(mine), n + 32 * ((i >> 3) & 1))));
         if (key < lo0 || key >= kv) continue;
-        const bool seen = key >= lo && key <= hi;
+        const bool seen = sight.sees(key);
         const uint16_t *vp = V + (i < 16 ? e0 : e1) + ((key & (P - 1)) & ~7) * D + (key & 7);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
@@ -218,154 +222,24 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(const AttnA
     }
   }
 
-  // the four waves' sums, in the waves' order
-  l = halves_sum(l);
-  if (h == 0) {
-    red_m[wave][n] = m;
-    red_l[wave][n] = l;
-  }
-  __syncthreads();
-  float top = red_m[0][n];
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) top = fmaxf(top, red_m[w][n]);
-  const float scale = weight(m, top, a.c);
-  if (n < R) {
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        f32x4 v;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = acc[d][4 * g + r] * scale;
-        __builtin_memcpy(red + ((wave * (D / 4) + 8 * d + 2 * g + h) * R + n) * 4, &v, 16);
-      }
-  }
-  float lt = 0.0f;  // of row n
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const float mw = red_m[w][n];
-    lt += red_l[w][n] * weight(mw, top, a.c);
-  }
-  __syncthreads();  // all waves have read red_m / red_l
-  if (wave == 0 && h == 0) {
-    red_m[0][n] = top;
-    red_l[0][n] = lt;
-  }
-  __syncthreads();
-
-  const int elems = R * (D / 4);  // groups of four dims of a row
-  const int head0 = kvh * a.G;
-  if (ns == 1) {
-    for (int i = tid; i < elems; i += 256) {
-      const int r = i % R, d4 = i / R;
-      f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) v += ldg<f32x4>(red + ((w * (D / 4) + d4) * R + r) * 4);
-      const int t = r / a.G;
-      // a row that sees no key is 0; one whose keys all weigh nothing is not a number
-      const float inv = ctx + t < 0 ? 0.0f : 1.0f / red_l[0][r];
-      v = ctx + t < 0 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : v * inv;
-      char *o = static_cast<char *>(a.out) +
-                ((q0 + t) * a.out_stride + static_cast<int64_t>(head0 + r % a.G) * D) *
-                    dtype_bytes(a.out_dtype);
-      store4(o, a.out_dtype, d4 * 4, v);
-    }
-    return;
-  }
-
-  // split: this chunk's sums to its slot, (m, l) of its rows behind them
-  const rsrc_t part = make_rsrc(a.part, a.part_bytes);
-  const uint32_t slot_bytes = lds_rows * (D + 4) * 4;
-  const uint32_t first = split.slot * a.Hkv + kvh * split.ns;  // the request's slots
-  const uint32_t slot0 = first * slot_bytes;
-  const uint32_t slot = slot0 + z * slot_bytes;
-  for (int i = tid; i < elems; i += 256) {
-    const int r = i % R, d4 = i / R;
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) v += ldg<f32x4>(red + ((w * (D / 4) + d4) * R + r) * 4);
-    st_dev4(part, slot + i * 16, v);
-  }
-  if (tid < R) st_dev4(part, slot + (elems + tid) * 16, f32x4{red_m[0][tid], red_l[0][tid], 0.0f, 0.0f});
-  wait_own_memory();
-  uint32_t *cnt = a.cnt + first;
-  if (!split_arrive_last(cnt, ns)) return;
-  // Reads past the L2 take a microsecond: a thread's first sums are on their way
-  // while the chunks' weights are formed.
-  constexpr int kAtOnce = 24;
-  f32x4 v[kAtOnce];
-  auto read = [&](int i, int y0) __attribute__((always_inline)) {
-#pragma unroll
-    for (int y = 0; y < kAtOnce; ++y)
-      v[y] = ld_dev4(part, i < elems && y0 + y < ns ? slot0 + (y0 + y) * slot_bytes + i * 16 : kOut);
-  };
-  read(tid, 0);
-  __builtin_amdgcn_sched_barrier(0);
-  // [chunk][row] maximum, then weight, and sum: the waves' sums are no longer needed
-  float2 *ml = reinterpret_cast<float2 *>(red);
-  {
-    const int r = tid >> 3, j = tid & 7;  // eight lanes for a row
-    float mx = -__builtin_inff(), sum = 0.0f;
-    if (r < R) {
-      for (int y0 = j; y0 < ns; y0 += 32) {
-        f32x4 u[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int y = y0 + 8 * i;
-          u[i] = ld_dev4(part, y < ns ? slot0 + y * slot_bytes + (elems + r) * 16 : kOut);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int y = y0 + 8 * i;
-          if (y < ns) {
-            ml[y * R + r] = make_float2(u[i].x, u[i].y);
-            mx = fmaxf(mx, u[i].x);
-          }
-        }
-      }
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-      for (int y = j; y < ns; y += 8) {
-        const float2 u = ml[y * R + r];
-        const float w = weight(u.x, mx, a.c);
-        ml[y * R + r].x = w;
-        sum += u.y * w;
-      }
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor(sum, o);
-      if (j == 0) red_l[0][r] = 1.0f / sum;
-    }
-  }
-  __syncthreads();
-  for (int i = tid; i < elems; i += 256) {
-    const int r = i % R, d4 = i / R, t = r / a.G;
-    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int y0 = 0; y0 < ns; y0 += kAtOnce) {
-      if (i != tid || y0) read(i, y0);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int y = 0; y < kAtOnce; ++y) o += v[y] * (y0 + y < ns ? ml[(y0 + y) * R + r].x : 0.0f);
-    }
-    o = ctx + t < 0 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : o * red_l[0][r];
-    char *to = static_cast<char *>(a.out) +
-               ((q0 + t) * a.out_stride + static_cast<int64_t>(head0 + r % a.G) * D) *
-                   dtype_bytes(a.out_dtype);
-    store4(to, a.out_dtype, d4 * 4, o);
-  }
-  split_reset(cnt);
+  rows_finish<D>(a, split, red, sums, acc, m, l, a.c, lds_rows, R, ns, kvh, [&](int t) {
+    if constexpr (TREE)
+      return Sight<true>{0, 0, ctx, node_bits(a, q0 + t, nq)}.nothing();
+    else
+      return ctx + t < 0;
+  });
 }
 
 namespace {
 constexpr int kMaxLds = 65536 - 2048;  // what a launch may ask for without more ado
 
-template <int DT, int D>
+template <int DT, int D, bool TREE>
 hipError_t launch_rows(const AttnArgs &a, int max_rows, int items, hipStream_t s) {
   constexpr int row_bytes = kWaves * D * 4;  // LDS of a row: the waves' sums
   if constexpr (row_bytes * kRowsMax > kMaxLds) {
     static std::atomic<uint64_t> done{0};
     if (!dry_run()) {
-      const hipError_t e = allow_lds(reinterpret_cast<const void *>(&k_attn_rows<DT, D>),
+      const hipError_t e = allow_lds(reinterpret_cast<const void *>(&k_attn_rows<DT, D, TREE>),
                                      row_bytes * kRowsMax, done);
       if (e != hipSuccess) return e;
     }
@@ -374,17 +248,25 @@ hipError_t launch_rows(const AttnArgs &a, int max_rows, int items, hipStream_t s
   int bytes = row_bytes * max_rows;
   if (bytes < a.B * 8) bytes = a.B * 8;
   if (bytes < a.goal * max_rows * 8) bytes = a.goal * max_rows * 8;
-  IFX_LAUNCH(k_attn_rows, (DT, D), dim3(a.Hkv * items), dim3(64 * kWaves), bytes, s, a, max_rows);
+  if constexpr (TREE)
+    IFX_LAUNCH(k_attn_rows, (DT, D, true), dim3(a.Hkv * items), dim3(64 * kWaves), bytes, s, a, max_rows);
+  else
+    IFX_LAUNCH(k_attn_rows, (DT, D), dim3(a.Hkv * items), dim3(64 * kWaves), bytes, s, a, max_rows);
   return last_error();
+}
+template <int DT, bool TREE>
+hipError_t launch_rows(const AttnArgs &a, int D, int max_rows, int items, hipStream_t s) {
+  switch (D) {
+    case 64: return launch_rows<DT, 64, TREE>(a, max_rows, items, s);
+    case 96: return launch_rows<DT, 96, TREE>(a, max_rows, items, s);
+    case 128: return launch_rows<DT, 128, TREE>(a, max_rows, items, s);
+    default: return launch_rows<DT, 256, TREE>(a, max_rows, items, s);
+  }
 }
 template <int DT>
 hipError_t launch_rows(const AttnArgs &a, int D, int max_rows, int items, hipStream_t s) {
-  switch (D) {
-    case 64: return launch_rows<DT, 64>(a, max_rows, items, s);
-    case 96: return launch_rows<DT, 96>(a, max_rows, items, s);
-    case 128: return launch_rows<DT, 128>(a, max_rows, items, s);
-    default: return launch_rows<DT, 256>(a, max_rows, items, s);
-  }
+  return a.masks ? launch_rows<DT, true>(a, D, max_rows, items, s)
+                 : launch_rows<DT, false>(a, D, max_rows, items, s);
 }
 }  // namespace
 

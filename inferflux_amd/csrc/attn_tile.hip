@@ -29,7 +29,7 @@
 // CU: 8111 tokens of 40 / 8 heads took 370 us, with two 387, with four 1330
 // (spills).  D = 256 needs 512: 4111 tokens of 16 / 2 heads in 241 us (fp16) or
 // 276 (bf16).
-#include "ifx_attn.h"
+#include "ifx_attn_tile.h"
 
 namespace ifx {
 
@@ -38,8 +38,8 @@ namespace {
 // Lambdas that are calls would keep what they capture in memory.
 #define IFX_INLINE __attribute__((always_inline))
 
-constexpr int kNW = 4;           // waves of a workgroup
-constexpr int kRows = 32 * kNW;  // its query rows
+constexpr int kNW = kTileWaves;
+constexpr int kRows = kQueryRows;
 constexpr int TK = kTileKeys;
 // Stages of a chunk at least: beside them it takes 6 us for its first loads and
 // its sums' exchange, as much as 5 stages.  A mixed batch (16 decode steps, 8
@@ -83,7 +83,8 @@ __device__ __forceinline__ int swap_v(int key) {
 
 }  // namespace
 
-template <int DT, int D, bool PAGED>
+// TREE: rows see the cached tokens and the nodes of their masks.
+template <int DT, int D, bool PAGED, bool TREE = false>
 __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_attn_tile(const AttnArgs a) {
   using T = Elem<DT>;
   constexpr int ND = D / 32, NS = D / 16, NP = D / 8;
@@ -123,11 +124,11 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
 
   // keys that any row of the workgroup sees
   const int tok_a = row0 / a.G, tok_z = (min(row0 + kRows, R) - 1) / a.G;
-  const int kend = a.causal ? ctx + tok_z + 1 : kv;
+  const int kend = a.causal && !TREE ? ctx + tok_z + 1 : kv;
   const int kbeg = a.window > 0 ? max(0, ctx + tok_a - a.window + 1) & ~(TK - 1) : 0;
   // stages [full_a, full_z) all of its rows see whole
   const int full_a = a.window > 0 ? (max(0, ctx + tok_z - a.window + 1) + TK - 1) & ~(TK - 1) : 0;
-  const int full_z = max(0, a.causal ? ctx + tok_a + 1 : kv) & ~(TK - 1);
+  const int full_z = max(0, TREE ? ctx : a.causal ? ctx + tok_a + 1 : kv) & ~(TK - 1);
   int ns = 1, zbeg = kbeg, zend = kend;  // prompts are not split
   if constexpr (PAGED) {
     const int chunk = __builtin_amdgcn_readfirstlane(split.chunk) * TK;
@@ -137,12 +138,16 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
   }
 
   // this lane's row sees [lo, hi]; rows behind the last repeat it
-  int row = min(row0 + 32 * wave + n, R - 1), tok = row / a.G;
-  int head = kvh * a.G + row - tok * a.G;
-  const int hi = a.causal ? ctx + tok : kv - 1;
-  const int lo = a.window > 0 ? max(0, ctx + tok - a.window + 1) : 0;
-  const int hi_z = __builtin_amdgcn_readlane(hi, 31);  // some of the wave's rows see [lo_a, hi_z]
-  const int lo_a = __builtin_amdgcn_readlane(lo, 0);
+  const int row = min(row0 + 32 * wave + n, R - 1), tok = row / a.G;
+  const int head = kvh * a.G + row - tok * a.G;
+  Sight<TREE> sight = {0, a.causal ? ctx + tok : kv - 1, ctx, 0};
+  if constexpr (TREE)
+    sight.bits = node_bits(a, q0 + tok, nq);
+  else if (a.window > 0)
+    sight.lo = max(0, ctx + tok - a.window + 1);
+  // some of the wave's rows see [lo_a, hi_z]
+  const int hi_z = TREE ? kv - 1 : __builtin_amdgcn_readlane(sight.hi, 31);
+  const int lo_a = TREE ? 0 : __builtin_amdgcn_readlane(sight.lo, 0);
   const bool idle = row0 + 32 * wave >= R;  // the wave has no rows, it only copies
 
   u32x4 qf[NS];
@@ -378,7 +383,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int key = k0 + 32 * sub + 16 * (r >> 3) + 8 * h + (r & 7);
-        s[sub][r] = key >= lo && key <= hi ? s[sub][r] : -__builtin_inff();
+        s[sub][r] = sight.sees(key) ? s[sub][r] : -__builtin_inff();
       }
     }
     float mt = fmaxf(s[0][0], s[1][0]);
@@ -498,7 +503,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
         x = __builtin_fmaf(q[i + 3], T::value(k4.y >> 16), x);
       }
       x = halves_sum(x);
-      const bool seen = key >= lo && key <= hi;
+      const bool seen = sight.sees(key);
       const float mn = seen ? fmaxf(m, x) : m;
       const float w = mn == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * a.c);
       const float rel = mn == -__builtin_inff() ? 0.0f : mn * a.c - T::kShift;
@@ -515,141 +520,45 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
     }
   }
 
-  l = halves_sum(l);
-  bool none = hi < lo;  // the row sees no key
-  bool own = row0 + 32 * wave + n < R;
-  auto write_dims = [&](int d, const f32x4 *v, float scale) IFX_INLINE {  // of one dim tile
-    if (!own) return;
-    char *o = static_cast<char *>(a.out) +
-              ((q0 + tok) * a.out_stride + static_cast<int64_t>(head) * D) * dtype_bytes(a.out_dtype);
-#pragma unroll
-    for (int g = 0; g < 4; ++g)
-      store4(o, a.out_dtype, 32 * d + 8 * g + 4 * h, none ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : v[g] * scale);
-  };
-  auto write = [&](float scale) IFX_INLINE {
-#pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      f32x4 v[4];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i >> 2][i & 3] = acc[d][i];
-      write_dims(d, v, scale);
-    }
-  };
-  if (!PAGED || ns == 1) return write(1.0f / l);
-
-  // split: this chunk's sums to its slot, every lane in its own places; the
-  // last workgroup of the tile adds the chunks in their order, lane by lane.
-  // Lanes without a row have their places behind the buffer's end: they write
-  // nothing and read zeros.
-  const rsrc_t part = make_rsrc(a.part, a.part_bytes);
-  constexpr uint32_t kWaveBytes = 32 * D * 4 + 64 * 4 * 2, kSlotBytes = kNW * kWaveBytes;
-  const uint32_t first = split.slot * a.Hkv + (tile * a.Hkv + kvh) * split.ns;  // the tile's slots
-  constexpr uint32_t kOut = 1u << 30;
-  const uint32_t out = row0 + 32 * wave + n < R ? 0 : kOut;
-  uint32_t mine = (first * kSlotBytes + wave * kWaveBytes + lane * 16) | out;
-  uint32_t mine_ml = (first * kSlotBytes + wave * kWaveBytes + 32 * D * 4 + lane * 8) | out;
-  {
-    const uint32_t at = mine + z * kSlotBytes;
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        st_dev4(part, at + (4 * d + g) * 1024,
-                f32x4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]});
-    __builtin_amdgcn_raw_buffer_store_b64(
-        __builtin_bit_cast(u32x2, make_float2(m, l)), part, mine_ml + z * kSlotBytes, 0, kAuxDevice);
-  }
-  wait_own_memory();
-  uint32_t *cnt = a.cnt + first;
-  if (!split_arrive_last(cnt, ns)) return;
-  const bool few = R - row0 <= 32;  // all rows are the first wave's: the waves share the dims
-  if (few) {
-    row = min(row0 + n, R - 1), tok = row / a.G, head = kvh * a.G + row - tok * a.G;
-    own = row0 + n < R;
-    none = a.causal && ctx + tok < 0;  // a row that sees any sees itself
-    const uint32_t at = first * kSlotBytes | (own ? 0 : kOut);
-    mine = at + lane * 16, mine_ml = at + 32 * D * 4 + lane * 8;
-  }
-  auto ml_of = [&](int y) {  // of chunk y, and past the last of none
-    return __builtin_bit_cast(
-        float2, __builtin_amdgcn_raw_buffer_load_b64(
-                    part, y < ns ? mine_ml + y * kSlotBytes : kOut, 0, kAuxDevice));
-  };
-  // Reads past the L2 take a microsecond: several at a time
-  float top = -__builtin_inff(), total = 0.0f;
-  for (int y0 = 0; y0 < ns; y0 += 8) {
-    float2 ml[8];
-#pragma unroll
-    for (int y = 0; y < 8; ++y) ml[y] = ml_of(y0 + y);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int y = 0; y < 8; ++y) {
-      const float my = y0 + y < ns ? ml[y].x : -__builtin_inff();
-      const float mn = fmaxf(top, my);
-      total = total * weight(top, mn, a.c) + ml[y].y * weight(my, mn, a.c);
-      top = mn;
-    }
-  }
-  // N dim tiles from d on, four chunks at a time
-  auto add_chunks = [&](int d, auto n_c) IFX_INLINE {
-    constexpr int N = decltype(n_c)::value;
-    f32x4 o[4 * N] = {};
-    for (int y0 = 0; y0 < ns; y0 += 4) {
-      float2 ml[4];
-      f32x4 v[4][4 * N];
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        ml[y] = ml_of(y0 + y);
-        const uint32_t at = y0 + y < ns ? mine + (y0 + y) * kSlotBytes + d * 4096 : kOut;
-#pragma unroll
-        for (int g = 0; g < 4 * N; ++g) v[y][g] = ld_dev4(part, at + g * 1024);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const float w = y0 + y < ns ? weight(ml[y].x, top, a.c) : 0.0f;
-#pragma unroll
-        for (int g = 0; g < 4 * N; ++g) o[g] += v[y][g] * w;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) write_dims(d + i, o + 4 * i, 1.0f / total);
-  };
-  using one = std::integral_constant<int, 1>;
-  using two = std::integral_constant<int, 2>;
-  if (few || D == 64) {  // (D = 64: registers of three waves a SIMD)
-#pragma unroll 1
-    for (int d = few ? wave : 0; d < ND; d += few ? kNW : 1) add_chunks(d, one{});
-  } else {
-#pragma unroll 1
-    for (int d = 0; d + 1 < ND; d += 2) add_chunks(d, two{});
-    if constexpr (ND % 2) add_chunks(ND - 1, one{});
-  }
-  split_reset(cnt);
+  tile_finish<D, PAGED>(a, split, acc, m, l, a.c, tile, z, ns, kvh, R, [&](int t) {
+    if constexpr (TREE)
+      return Sight<true>{0, 0, ctx, node_bits(a, q0 + t, nq)}.nothing();
+    else
+      return a.causal && ctx + t < 0;
+  });
 }
 
 namespace {
-template <int DT, int D, bool PAGED>
+template <int DT, int D, bool PAGED, bool TREE>
 hipError_t launch_tile(const AttnArgs &a, int items, hipStream_t s) {
   constexpr int bytes = 2 * 2 * TK * D * 2;
   if constexpr (bytes > 65536 - 256) {
     static std::atomic<uint64_t> done{0};
     if (!dry_run()) {
       const hipError_t e =
-          allow_lds(reinterpret_cast<const void *>(&k_attn_tile<DT, D, PAGED>), bytes, done);
+          allow_lds(reinterpret_cast<const void *>(&k_attn_tile<DT, D, PAGED, TREE>), bytes, done);
       if (e != hipSuccess) return e;
     }
   }
-  IFX_LAUNCH(k_attn_tile, (DT, D, PAGED), dim3(a.Hkv * items), dim3(64 * kNW), bytes, s, a);
+  if constexpr (TREE)
+    IFX_LAUNCH(k_attn_tile, (DT, D, PAGED, true), dim3(a.Hkv * items), dim3(64 * kNW), bytes, s, a);
+  else
+    IFX_LAUNCH(k_attn_tile, (DT, D, PAGED), dim3(a.Hkv * items), dim3(64 * kNW), bytes, s, a);
   return last_error();
+}
+template <int DT, int D>
+hipError_t launch_tile(const AttnArgs &a, bool paged, int items, hipStream_t s) {
+  if (!paged) return launch_tile<DT, D, false, false>(a, items, s);
+  return a.masks ? launch_tile<DT, D, true, true>(a, items, s)
+                 : launch_tile<DT, D, true, false>(a, items, s);
 }
 template <int DT>
 hipError_t launch_tile(const AttnArgs &a, int D, bool paged, int items, hipStream_t s) {
   switch (D) {
-    case 64: return paged ? launch_tile<DT, 64, true>(a, items, s) : launch_tile<DT, 64, false>(a, items, s);
-    case 96: return paged ? launch_tile<DT, 96, true>(a, items, s) : launch_tile<DT, 96, false>(a, items, s);
-    case 128: return paged ? launch_tile<DT, 128, true>(a, items, s) : launch_tile<DT, 128, false>(a, items, s);
-    default: return paged ? launch_tile<DT, 256, true>(a, items, s) : launch_tile<DT, 256, false>(a, items, s);
+    case 64: return launch_tile<DT, 64>(a, paged, items, s);
+    case 96: return launch_tile<DT, 96>(a, paged, items, s);
+    case 128: return launch_tile<DT, 128>(a, paged, items, s);
+    default: return launch_tile<DT, 256>(a, paged, items, s);
   }
 }
 }  // namespace

@@ -171,7 +171,32 @@ struct AttnArgs {
   uint32_t *cnt;
   float *part;
   uint32_t part_bytes;
+  const uint64_t *masks;   // trees: per row, its request's nodes that it sees
+  const uint32_t *scales;  // 8-bit cache: K's and V's of a token and head
+  int q_dtype;             // 8-bit cache: type of the rows of Q
 };
+
+// What a row sees of its request's keys: [lo, hi], or of a tree of drafted
+// tokens the `ctx` cached ones before it and the nodes ctx + j whose bit j is set.
+template <bool TREE>
+struct Sight {
+  int lo, hi, ctx;
+  uint64_t bits;
+  __device__ __forceinline__ bool sees(int key) const {
+    if constexpr (!TREE) return key >= lo && key <= hi;
+    const int node = key - ctx;
+    return node < 0 || (node < 64 && (bits >> node & 1));
+  }
+  __device__ __forceinline__ bool nothing() const {
+    if constexpr (!TREE) return hi < lo;
+    return ctx <= 0 && (ctx <= -64 || bits >> -ctx == 0);
+  }
+};
+// The row of new token `tok` of a request of nq.
+__device__ __forceinline__ uint64_t node_bits(const AttnArgs &a, int row, int nq) {
+  const uint64_t bits = a.masks[row];
+  return nq < 64 ? bits & ((1ull << nq) - 1) : bits;
+}
 
 // Query rows of one key/value head: row r of a request is query head r % G of
 // the group and new token r / G.

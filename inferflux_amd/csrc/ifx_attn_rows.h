@@ -1,0 +1,170 @@
+// ifx_attn_rows.h -- what the attention kernels of requests with few query rows
+// (attn_rows.hip, attn_rows_q8.hip) do with their sums: the four waves' are
+// added in LDS, the chunks' of a request through the workspace.
+#pragma once
+
+#include "ifx_attn.h"
+
+namespace ifx {
+
+constexpr int kRowWaves = 4;
+
+// LDS of the waves' maxima and sums.
+struct RowSums {
+  float m[kRowWaves][32], l[kRowWaves][32];
+};
+
+// Lane n of each half of a wave holds row n: maximum m and sum l, and in acc
+// the dims 32 d + 8 (r / 4) + 4 h + r % 4.  Exponents are (s - m) c.  red:
+// [wave][D / 4][row][4], later [chunk][row].  none(t): whether the rows of new
+// token t see nothing.
+template <int D, class None>
+__device__ __forceinline__ void rows_finish(const AttnArgs &a, const Split &split, float *red,
+                                            RowSums &sums, const f32x16 (&acc)[D / 32], float m,
+                                            float l, float c, int lds_rows, int R, int ns, int kvh,
+                                            None none) {
+  constexpr int ND = D / 32;
+  constexpr uint32_t kOut = 1u << 30;  // an offset past the workspace's end: reads zeros
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int z = split.item, q0 = split.req.q0;
+
+  // the four waves' sums, in the waves' order
+  l = halves_sum(l);
+  if (h == 0) {
+    sums.m[wave][n] = m;
+    sums.l[wave][n] = l;
+  }
+  __syncthreads();
+  float top = sums.m[0][n];
+#pragma unroll
+  for (int w = 1; w < kRowWaves; ++w) top = fmaxf(top, sums.m[w][n]);
+  const float scale = weight(m, top, c);
+  if (n < R) {
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        f32x4 v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = acc[d][4 * g + r] * scale;
+        __builtin_memcpy(red + ((wave * (D / 4) + 8 * d + 2 * g + h) * R + n) * 4, &v, 16);
+      }
+  }
+  float lt = 0.0f;  // of row n
+#pragma unroll
+  for (int w = 0; w < kRowWaves; ++w) {
+    const float mw = sums.m[w][n];
+    lt += sums.l[w][n] * weight(mw, top, c);
+  }
+  __syncthreads();  // all waves have read sums.m / sums.l
+  if (wave == 0 && h == 0) {
+    sums.m[0][n] = top;
+    sums.l[0][n] = lt;
+  }
+  __syncthreads();
+
+  const int elems = R * (D / 4);  // groups of four dims of a row
+  const int head0 = kvh * a.G;
+  if (ns == 1) {
+    for (int i = tid; i < elems; i += 256) {
+      const int r = i % R, d4 = i / R;
+      f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < kRowWaves; ++w) v += ldg<f32x4>(red + ((w * (D / 4) + d4) * R + r) * 4);
+      const int t = r / a.G;
+      // a row that sees no key is 0; one whose keys all weigh nothing is not a number
+      const float inv = 1.0f / sums.l[0][r];
+      v = none(t) ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : v * inv;
+      char *o = static_cast<char *>(a.out) +
+                ((q0 + t) * a.out_stride + static_cast<int64_t>(head0 + r % a.G) * D) *
+                    dtype_bytes(a.out_dtype);
+      store4(o, a.out_dtype, d4 * 4, v);
+    }
+    return;
+  }
+
+  // split: this chunk's sums to its slot, (m, l) of its rows behind them
+  const rsrc_t part = make_rsrc(a.part, a.part_bytes);
+  const uint32_t slot_bytes = lds_rows * (D + 4) * 4;
+  const uint32_t first = split.slot * a.Hkv + kvh * split.ns;  // the request's slots
+  const uint32_t slot0 = first * slot_bytes;
+  const uint32_t slot = slot0 + z * slot_bytes;
+  for (int i = tid; i < elems; i += 256) {
+    const int r = i % R, d4 = i / R;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kRowWaves; ++w) v += ldg<f32x4>(red + ((w * (D / 4) + d4) * R + r) * 4);
+    st_dev4(part, slot + i * 16, v);
+  }
+  if (tid < R) st_dev4(part, slot + (elems + tid) * 16, f32x4{sums.m[0][tid], sums.l[0][tid], 0.0f, 0.0f});
+  wait_own_memory();
+  uint32_t *cnt = a.cnt + first;
+  if (!split_arrive_last(cnt, ns)) return;
+  // Reads past the L2 take a microsecond: a thread's first sums are on their way
+  // while the chunks' weights are formed.
+  constexpr int kAtOnce = 24;
+  f32x4 v[kAtOnce];
+  auto read = [&](int i, int y0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int y = 0; y < kAtOnce; ++y)
+      v[y] = ld_dev4(part, i < elems && y0 + y < ns ? slot0 + (y0 + y) * slot_bytes + i * 16 : kOut);
+  };
+  read(tid, 0);
+  __builtin_amdgcn_sched_barrier(0);
+  // [chunk][row] maximum, then weight, and sum: the waves' sums are no longer needed
+  float2 *ml = reinterpret_cast<float2 *>(red);
+  {
+    const int r = tid >> 3, j = tid & 7;  // eight lanes for a row
+    float mx = -__builtin_inff(), sum = 0.0f;
+    if (r < R) {
+      for (int y0 = j; y0 < ns; y0 += 32) {
+        f32x4 u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int y = y0 + 8 * i;
+          u[i] = ld_dev4(part, y < ns ? slot0 + y * slot_bytes + (elems + r) * 16 : kOut);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int y = y0 + 8 * i;
+          if (y < ns) {
+            ml[y * R + r] = make_float2(u[i].x, u[i].y);
+            mx = fmaxf(mx, u[i].x);
+          }
+        }
+      }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+      for (int y = j; y < ns; y += 8) {
+        const float2 u = ml[y * R + r];
+        const float w = weight(u.x, mx, c);
+        ml[y * R + r].x = w;
+        sum += u.y * w;
+      }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor(sum, o);
+      if (j == 0) sums.l[0][r] = 1.0f / sum;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < elems; i += 256) {
+    const int r = i % R, d4 = i / R, t = r / a.G;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int y0 = 0; y0 < ns; y0 += kAtOnce) {
+      if (i != tid || y0) read(i, y0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int y = 0; y < kAtOnce; ++y) o += v[y] * (y0 + y < ns ? ml[(y0 + y) * R + r].x : 0.0f);
+    }
+    o = none(t) ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : o * sums.l[0][r];
+    char *to = static_cast<char *>(a.out) +
+               ((q0 + t) * a.out_stride + static_cast<int64_t>(head0 + r % a.G) * D) *
+                   dtype_bytes(a.out_dtype);
+    store4(to, a.out_dtype, d4 * 4, o);
+  }
+  split_reset(cnt);
+}
+
+}  // namespace ifx
