@@ -123,6 +123,16 @@ SIGNATURES.update({
     "ifx_plan_kept": ([_vp] * 4 + [_i32, _vp, _i32, _vp, _i32, _i32] + [_vp] * 4, _i32),
 })
 
+# Every symbol include/ifx_attention_q8.h declares.
+SIGNATURES.update({
+    "ifx_rope_append_q8": ([_vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _i32,
+                            _i32, _i32, _i32, _vp, _i64, _i32, _vp, _vp, _vp, _i64, _i32, _vp], _i32),
+    "ifx_read_rows_q8": ([_vp, _vp, _vp, _i64, _i32, _vp, _i32, _i32, _i32, _vp, _i64, _vp, _i64,
+                          _i32, _vp], _i32),
+    "ifx_attn_paged_q8": ([_vp, _i64, _i32, _vp, _vp, _vp, _i64, _i32, _vp, _i32, _vp, _vp, _vp] +
+                          [_i32] * 7 + [ctypes.c_float, _i32, _vp, _i64, _i32, _vp, _i64, _vp], _i32),
+})
+
 _lib = None
 
 

@@ -34,6 +34,7 @@ SOURCES = ["api.hip", "quantize.hip", "dequant.hip", "gemv.hip", "mmq_skinny.hip
            "gemv_dq.hip", "packed.hip",
            "attention_api.hip", "kv_plan.hip", "rope_append.hip", "attn_rows.hip", "attn_tile.hip",
            "drafts_api.hip", "draft_plan.hip", "verify_drafts.hip", "keep_path.hip",
+           "rope_append_q8.hip", "attn_rows_q8.hip", "attn_tile_q8.hip",
            "../host/fused_quant_gemm.cpp", "../host/native_dispatch.cpp", "../host/gguf.cpp", "../host/gguf_model.cpp"]
 
 

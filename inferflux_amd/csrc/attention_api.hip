@@ -1,9 +1,10 @@
-// attention_api.hip -- the C entry points of include/ifx_attention.h, and the
-// attention's of include/ifx_drafts.h: validation, the split of keys over
-// workgroups, and the launches.
+// attention_api.hip -- the C entry points of include/ifx_attention.h and
+// include/ifx_attention_q8.h, and the attention's of include/ifx_drafts.h:
+// validation, the split of keys over workgroups, and the launches.
 #include <climits>
 #include <cmath>
 
+#include "ifx_attn_q8.h"
 #include "ifx_drafts_impl.h"
 #include "ifx_qgemm.h"
 
@@ -50,6 +51,26 @@ bool heads_ok(int B, int T, int Hq, int Hkv, int D) {
 
 // scale log2 e is what the kernels multiply by.
 bool scale_ok(float scale) { return scale > 0.0f && std::isfinite(scale * kLog2e); }
+
+// Geometry and pointers of an append; sets its number of slots.
+int append_args(AppendArgs &a, int64_t num_pages) {
+  const int sh = a.page_shift;
+  if (sh < 0 || num_pages < 1 || num_pages > (INT_MAX >> sh)) return IFX_BAD_GEOMETRY;
+  if (a.T < 0 || a.T > (1 << 27) - 8 || a.Hq < 1 || a.Hkv < 1 || a.Hq > 65536 || a.Hkv > 65536 ||
+      a.D < 8 || a.D > 256 || a.D % 8 || a.rot_dim < 0 || a.rot_dim > a.D || a.rot_dim % 16)
+    return IFX_BAD_GEOMETRY;
+  const int64_t qn = static_cast<int64_t>(a.Hq) * a.D, kn = static_cast<int64_t>(a.Hkv) * a.D;
+  if (a.q_stride < qn || a.k_stride < kn || a.v_stride < kn || a.q_out_stride < qn)
+    return IFX_BAD_GEOMETRY;
+  if (a.T == 0) return IFX_OK;
+  if (!a.q || !a.k || !a.v || !a.slots || !a.q_out || !a.k_cache || !a.v_cache ||
+      (a.rot_dim && (!a.positions || !a.inv_freq)))
+    return IFX_NULL_POINTER;
+  if ((reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache)) & 15)
+    return IFX_BAD_GEOMETRY;
+  a.num_slots = static_cast<int>(num_pages << sh);
+  return IFX_OK;
+}
 
 // Positions are below 2^30: a window as wide is none, and position - window
 // stays within 32 bits, also of rows before the first key (above -2^30).
@@ -106,11 +127,12 @@ PagedPlan plan_paged(int B, int T, int Hq, int Hkv, int D, int max_q, int max_kv
   return p;
 }
 
-// masks: the nodes that rows of trees see, or null.
+// masks: the nodes that rows of trees see, or null.  scales: of the 8-bit cache,
+// null for the 16-bit one.
 int attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cache,
-               const void *v_cache, int64_t num_pages, int page_size, const int32_t *block_table,
-               int table_width, const int32_t *cu_q, const int32_t *kv_len, const uint64_t *masks,
-               int B, int T, int Hq, int Hkv, int D, int max_q, int max_kv, float scale,
+               const void *v_cache, const void *scales, int64_t num_pages, int page_size,
+               const int32_t *block_table, int table_width, const int32_t *cu_q,
+               const int32_t *kv_len, const uint64_t *masks, int B, int T, int Hq, int Hkv, int D, int max_q, int max_kv, float scale,
                int window, void *out, int64_t out_stride, int out_dtype, void *workspace,
                int64_t workspace_bytes, void *stream) {
   if (!is_elem(dtype) || !is_out(out_dtype)) return IFX_UNSUPPORTED_TYPE;
@@ -141,7 +163,7 @@ int attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cache,
   a.num_pages = num_pages, a.table_width = table_width, a.page_shift = sh;
   a.B = B, a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv;
   a.causal = 1, a.window = window_of(window), a.out_dtype = out_dtype;
-  a.masks = masks;
+  a.masks = masks, a.scales = static_cast<const uint32_t *>(scales), a.q_dtype = dtype;
   a.c = scale * kLog2e;
   a.goal = p.goal;
   if (p.bytes) {
@@ -150,6 +172,9 @@ int attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cache,
     a.part_bytes = static_cast<uint32_t>(p.bytes - kCntBytes);
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
+  if (scales)
+    return status_of(p.rows ? launch_attn_rows_q8(a, D, max_q * a.G, p.items, s)
+                            : launch_attn_tile_q8(a, D, p.items, s));
   if (p.rows) return status_of(launch_attn_rows(a, dtype, D, max_q * a.G, p.items, s));
   return status_of(launch_attn_tile(a, dtype, D, true, p.items, s));
 }
@@ -189,23 +214,51 @@ int ifx_rope_append(const void *q, int64_t q_stride, const void *k, int64_t k_st
                     void *k_cache, void *v_cache, int cache_dtype, int64_t num_pages,
                     int page_size, void *stream) {
   if (!is_out(src_dtype) || !is_elem(cache_dtype)) return IFX_UNSUPPORTED_TYPE;
-  const int sh = page_shift_of(page_size);
-  if (sh < 0 || num_pages < 1 || num_pages > (INT_MAX >> sh)) return IFX_BAD_GEOMETRY;
-  if (T < 0 || T > (1 << 27) - 8 || Hq < 1 || Hkv < 1 || Hq > 65536 || Hkv > 65536 || D < 8 ||
-      D > 256 || D % 8 || rot_dim < 0 || rot_dim > D || rot_dim % 16)
-    return IFX_BAD_GEOMETRY;
-  const int64_t qn = static_cast<int64_t>(Hq) * D, kn = static_cast<int64_t>(Hkv) * D;
-  if (q_stride < qn || k_stride < kn || v_stride < kn || q_out_stride < qn) return IFX_BAD_GEOMETRY;
-  if (T == 0) return IFX_OK;
-  if (!q || !k || !v || !slots || !q_out || !k_cache || !v_cache ||
-      (rot_dim && (!positions || !inv_freq)))
-    return IFX_NULL_POINTER;
-  if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15)
-    return IFX_BAD_GEOMETRY;
-  const AppendArgs a{q, k, v, q_stride, k_stride, v_stride, q_out_stride, positions, slots,
-                     inv_freq, q_out, k_cache, v_cache, rot_dim, interleaved != 0, T, Hq, Hkv, D,
-                     sh, static_cast<int>(num_pages << sh)};
+  AppendArgs a{q, k, v, q_stride, k_stride, v_stride, q_out_stride, positions, slots, inv_freq,
+               q_out, k_cache, v_cache, rot_dim, interleaved != 0, T, Hq, Hkv, D,
+               page_shift_of(page_size), 0};
+  const int rc = append_args(a, num_pages);
+  if (rc || T == 0) return rc;
   return status_of(launch_rope_append(a, src_dtype, cache_dtype, static_cast<hipStream_t>(stream)));
+}
+
+int ifx_rope_append_q8(const void *q, int64_t q_stride, const void *k, int64_t k_stride,
+                       const void *v, int64_t v_stride, int src_dtype, const int32_t *positions,
+                       const int32_t *slots, const double *inv_freq, int rot_dim, int interleaved,
+                       int T, int Hq, int Hkv, int D, void *q_out, int64_t q_out_stride,
+                       int q_dtype, void *k_cache, void *v_cache, void *scales, int64_t num_pages,
+                       int page_size, void *stream) {
+  if (!is_out(src_dtype) || !is_elem(q_dtype)) return IFX_UNSUPPORTED_TYPE;
+  AppendQ8Args b{{q, k, v, q_stride, k_stride, v_stride, q_out_stride, positions, slots,
+                  inv_freq, q_out, k_cache, v_cache, rot_dim, interleaved != 0, T, Hq, Hkv, D,
+                  page_shift_of(page_size), 0},
+                 static_cast<uint32_t *>(scales)};
+  if (D % 32) return IFX_BAD_GEOMETRY;
+  const int rc = append_args(b.a, num_pages);
+  if (rc || T == 0) return rc;
+  if (!scales) return IFX_NULL_POINTER;
+  if (reinterpret_cast<uintptr_t>(scales) & 15) return IFX_BAD_GEOMETRY;
+  return status_of(launch_rope_append_q8(b, src_dtype, q_dtype, static_cast<hipStream_t>(stream)));
+}
+
+int ifx_read_rows_q8(const void *k_cache, const void *v_cache, const void *scales,
+                     int64_t num_pages, int page_size, const int32_t *slots, int N, int Hkv, int D,
+                     void *k_out, int64_t k_stride, void *v_out, int64_t v_stride, int out_dtype,
+                     void *stream) {
+  if (!is_out(out_dtype)) return IFX_UNSUPPORTED_TYPE;
+  const int sh = page_shift_of(page_size);
+  const int64_t row = static_cast<int64_t>(Hkv) * D;
+  if (sh < 0 || num_pages < 1 || num_pages > (INT_MAX >> sh) || N < 0 || N >= (1 << 27) ||
+      Hkv < 1 || Hkv > 65536 || D < 32 || D > 256 || D % 32 || k_stride < row || v_stride < row)
+    return IFX_BAD_GEOMETRY;
+  if (N == 0) return IFX_OK;
+  if (!k_cache || !v_cache || !scales || !slots || !k_out || !v_out) return IFX_NULL_POINTER;
+  if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) |
+       reinterpret_cast<uintptr_t>(scales)) & 15)
+    return IFX_BAD_GEOMETRY;
+  const ReadArgs a{k_cache, v_cache, static_cast<const uint32_t *>(scales), slots, k_out, v_out,
+                   k_stride, v_stride, N, Hkv, D, sh, static_cast<int>(num_pages << sh)};
+  return status_of(launch_read_rows_q8(a, out_dtype, static_cast<hipStream_t>(stream)));
 }
 
 int64_t ifx_attn_paged_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int max_q,
@@ -220,7 +273,7 @@ int ifx_attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cac
                    const int32_t *kv_len, int B, int T, int Hq, int Hkv, int D, int max_q,
                    int max_kv, float scale, int window, void *out, int64_t out_stride,
                    int out_dtype, void *workspace, int64_t workspace_bytes, void *stream) {
-  return attn_paged(q, q_stride, dtype, k_cache, v_cache, num_pages, page_size, block_table,
+  return attn_paged(q, q_stride, dtype, k_cache, v_cache, nullptr, num_pages, page_size, block_table,
                     table_width, cu_q, kv_len, nullptr, B, T, Hq, Hkv, D, max_q, max_kv, scale,
                     window, out, out_stride, out_dtype, workspace, workspace_bytes, stream);
 }
@@ -233,9 +286,24 @@ int ifx_attn_tree(const void *q, int64_t q_stride, int dtype, const void *k_cach
                   int out_dtype, void *workspace, int64_t workspace_bytes, void *stream) {
   if (max_q > IFX_TREE_MAX_NODES) return IFX_BAD_GEOMETRY;
   if (T && !masks) return IFX_NULL_POINTER;
-  return attn_paged(q, q_stride, dtype, k_cache, v_cache, num_pages, page_size, block_table,
+  return attn_paged(q, q_stride, dtype, k_cache, v_cache, nullptr, num_pages, page_size, block_table,
                     table_width, cu_q, kv_len, masks, B, T, Hq, Hkv, D, max_q, max_kv, scale, 0,
                     out, out_stride, out_dtype, workspace, workspace_bytes, stream);
+}
+
+int ifx_attn_paged_q8(const void *q, int64_t q_stride, int q_dtype, const void *k_cache,
+                      const void *v_cache, const void *scales, int64_t num_pages, int page_size,
+                      const int32_t *block_table, int table_width, const int32_t *cu_q,
+                      const int32_t *kv_len, const uint64_t *masks, int B, int T, int Hq, int Hkv,
+                      int D, int max_q, int max_kv, float scale, int window, void *out,
+                      int64_t out_stride, int out_dtype, void *workspace, int64_t workspace_bytes,
+                      void *stream) {
+  if (masks && (window || max_q > IFX_TREE_MAX_NODES)) return IFX_BAD_GEOMETRY;
+  if (T && !scales) return IFX_NULL_POINTER;
+  if (reinterpret_cast<uintptr_t>(scales) & 15) return IFX_BAD_GEOMETRY;
+  return attn_paged(q, q_stride, q_dtype, k_cache, v_cache, scales, num_pages, page_size,
+                    block_table, table_width, cu_q, kv_len, masks, B, T, Hq, Hkv, D, max_q, max_kv,
+                    scale, window, out, out_stride, out_dtype, workspace, workspace_bytes, stream);
 }
 
 int ifx_attn_prompt(const void *q, int64_t q_stride, const void *k, int64_t k_stride,

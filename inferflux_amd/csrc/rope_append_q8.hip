@@ -1,0 +1,284 @@
+// rope_append_q8.hip -- rotates the new tokens' Q and K, writes K and V into the
+// 8-bit paged cache (layout: ifx_attention_q8.h), and reads tokens back.
+//
+//   y_i = x_i cos(a) - x_j sin(a),  y_j = x_j cos(a) + x_i sin(a),
+//   a = position * inv_freq;  s = the smallest bf16 >= max |y| / 127,
+//   code_i = rint(y_i / s)
+//
+// K is rotated and both are divided in fp64, so that a code is that of the exact
+// value but for its last bits: an fp32 angle's error of 1e-7 would move one code
+// in 30000, and a value read back by a whole step.
+#include "ifx_attn_q8.h"
+#include "ifx_rope.h"
+
+namespace ifx {
+
+namespace {
+
+// The smallest fp32 that is no less than a non-negative x.
+__device__ __forceinline__ float not_below(double x) {
+  const float f = static_cast<float>(x);
+  return static_cast<double>(f) < x
+             ? __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, f) + 1)
+             : f;
+}
+
+// Bits of the smallest bf16 s with 127 s >= top (15 significant bits: exact in
+// fp32); of NaN where top is not finite.
+__device__ __forceinline__ uint32_t scale_bits(float top) {
+  if (!(top <= 3.4028234e38f)) return 0x7FC0u;
+  uint32_t s = __builtin_bit_cast(uint32_t, top / 127.0f) >> 16;
+  if (__builtin_bit_cast(float, s << 16) * 127.0f < top) ++s;
+  return s;
+}
+
+// max over the 16, 32 or 64 lanes that share a row; a NaN among them wins.
+template <int LANES>
+__device__ __forceinline__ float row_max(float v) {
+#pragma unroll
+  for (int d = 1; d < LANES; d <<= 1) {
+    const float o = __shfl_xor(v, d);
+    v = o > v || o != o ? o : v;
+  }
+  return v;
+}
+
+}  // namespace
+
+// A workgroup takes NTOK consecutive tokens, and of them a part: K and V
+// (blockIdx.y 0) or some of Q's units, pieces of 8 values (and their partners'
+// where pairs lie half a rotation apart).  A row of K or V is shared by LANES
+// lanes, four values each.
+template <int DT, int SRC, int LANES, int NTOK>
+__global__ __launch_bounds__(256) void k_rope_append_q8(const AppendQ8Args args) {
+  using T = Elem<DT>;
+  const AppendArgs &a = args.a;
+  __shared__ union {
+    float2 q[NTOK * 128];
+    double2 k[NTOK * 128];
+  } turn;
+  __shared__ int slot_of[NTOK];
+  const int tid = threadIdx.x, t0 = blockIdx.x * NTOK;
+  const int half = a.rot_dim >> 1, pieces = a.D >> 3, sh = a.page_shift, P = 1 << sh;
+  const bool q_part = blockIdx.y > 0;
+  if (tid < NTOK) {
+    const int t = t0 + tid, s = t < a.T ? a.slots[t] : -1;
+    slot_of[tid] = static_cast<uint32_t>(s) < static_cast<uint32_t>(a.num_slots) ? s : -1;
+  }
+  for (int i = tid; i < NTOK * half; i += 256) {
+    const int t = t0 + i / half;
+    if (t < a.T) {
+      const double turns = a.positions[t] * a.inv_freq[i % half] * 0.15915494309189533577;
+      const double x = 2.0 * (turns - rint(turns));
+      if (q_part) {
+        float sn, cs;
+        sincospif(static_cast<float>(x), &sn, &cs);
+        turn.q[i] = make_float2(cs, sn);
+      } else {
+        double sn, cs;
+        sincospi(x, &sn, &cs);
+        turn.k[i] = make_double2(cs, sn);
+      }
+    }
+  }
+  __syncthreads();
+
+  if (q_part) {
+    const int pairs = a.interleaved ? 0 : half >> 3, per_head = pieces - pairs;
+    const int units = NTOK * a.Hq * per_head, parts = gridDim.y - 1;
+    const int share = (units + parts - 1) / parts;
+    const int u0 = (blockIdx.y - 1) * share, u1 = min(u0 + share, units);
+    const float per_head_inv = 1.0f / per_head, heads_inv = 1.0f / a.Hq;
+    for (int u = u0 + tid; u < u1; u += 256) {
+      const int w = quotient(u, per_head, per_head_inv), c = u - w * per_head;
+      const int t = quotient(w, a.Hq, heads_inv), head = w - t * a.Hq;
+      if (slot_of[t] < 0) continue;
+      const int pc = c < pairs ? c : c + pairs;
+      const bool two = c < pairs;
+      Raw8<SRC> lo, hi;
+      const int64_t at = (t0 + t) * a.q_stride + static_cast<int64_t>(head) * a.D + pc * 8;
+      lo.load(a.q, at);
+      if (two) hi.load(a.q, at + half);
+      const float2 *tw = turn.q + t * half;
+      float x[8], y[8];
+      lo.values(x);
+      uint16_t *o = static_cast<uint16_t *>(a.q_out) + (t0 + t) * a.q_out_stride +
+                    static_cast<int64_t>(head) * a.D + pc * 8;
+      if (two) {
+        hi.values(y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 r = tw[pc * 8 + i];
+          const float p = x[i], s = y[i];
+          x[i] = p * r.x - s * r.y;
+          y[i] = s * r.x + p * r.y;
+        }
+        const u32x4 py = pack8<T>(y);
+        __builtin_memcpy(o + half, &py, 16);
+      } else if (pc * 8 < a.rot_dim) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 r = tw[pc * 4 + i];
+          const float p = x[2 * i], s = x[2 * i + 1];
+          x[2 * i] = p * r.x - s * r.y;
+          x[2 * i + 1] = s * r.x + p * r.y;
+        }
+      }
+      const u32x4 px = pack8<T>(x);
+      __builtin_memcpy(o, &px, 16);
+    }
+    return;
+  }
+
+  // K and V: row = (token, head, K or V), tokens fastest.  All lanes take as
+  // many turns, as rows are reduced across them.
+  const int sub = tid & (LANES - 1), dim = sub * 4, rows = NTOK * a.Hkv * 2;
+  for (int r0 = 0; r0 < rows; r0 += 256 / LANES) {
+    const int r = r0 + tid / LANES, t = r % NTOK, hv = r / NTOK, head = hv >> 1;
+    const bool is_v = hv & 1;
+    const int slot = r < rows ? slot_of[t] : -1;
+    const bool live = slot >= 0 && dim < a.D;
+    double y[4] = {0.0, 0.0, 0.0, 0.0};
+    if (live) {
+      const int64_t row = (t0 + t) * (is_v ? a.v_stride : a.k_stride) + static_cast<int64_t>(head) * a.D;
+      const void *src = is_v ? a.v : a.k;
+      const float2 p = load2<SRC>(src, row + dim), q = load2<SRC>(src, row + dim + 2);
+      const float x[4] = {p.x, p.y, q.x, q.y};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = x[i];
+      if (!is_v && dim < a.rot_dim) {
+        const double2 *tw = turn.k + t * half;
+        if (a.interleaved) {
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const double2 w = tw[(dim + i) >> 1];
+            y[i] = x[i] * w.x - x[i + 1] * w.y;
+            y[i + 1] = x[i + 1] * w.x + x[i] * w.y;
+          }
+        } else {
+          const bool first = dim < half;  // of its pair
+          const int other = first ? dim + half : dim - half;
+          const float2 u = load2<SRC>(src, row + other), v = load2<SRC>(src, row + other + 2);
+          const float z[4] = {u.x, u.y, v.x, v.y};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const double2 w = tw[(first ? dim : other) + i];
+            y[i] = first ? x[i] * w.x - z[i] * w.y : x[i] * w.x + z[i] * w.y;
+          }
+        }
+      }
+    }
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float m = not_below(fabs(y[i]));
+      top = m > top || m != m ? m : top;
+    }
+    top = row_max<LANES>(top);
+    const uint32_t bits = scale_bits(top);
+    const double s = __builtin_bit_cast(float, bits << 16);
+    uint32_t code[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)  // also where the scale is 0 or NaN
+      code[i] = s > 0.0 ? static_cast<uint32_t>(static_cast<int>(rint(y[i] / s))) & 0xFFu : 0u;
+    if (!live) continue;
+    const int64_t block = static_cast<int64_t>(slot >> sh) * a.Hkv + head;
+    const int tok = slot & (P - 1);
+    if (sub == 0)
+      reinterpret_cast<uint16_t *>(args.scales)[((block << sh) + tok) * 2 + is_v] =
+          static_cast<uint16_t>(bits);
+    if (is_v) {
+      uint8_t *o = static_cast<uint8_t *>(a.v_cache) +
+                   ((block << sh) + (tok & ~15)) * a.D + dim * 16 + (tok & 15);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i * 16] = static_cast<uint8_t>(code[i]);
+    } else {
+      uint8_t *o = static_cast<uint8_t *>(a.k_cache) + ((block * (a.D >> 4) + (dim >> 4)) << sh) * 16 +
+                   tok * 16 + (dim & 15);
+      *reinterpret_cast<uint32_t *>(o) = code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24;
+    }
+  }
+}
+
+// A thread reads 16 values of a row: K's as one piece, V's a byte each.
+template <int OUT>
+__global__ __launch_bounds__(256) void k_read_rows_q8(const ReadArgs a) {
+  const int units = a.Hkv * (a.D >> 4);  // of a token's K or V
+  const int sh = a.page_shift, P = 1 << sh;
+  for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < static_cast<int64_t>(a.N) * units * 2;
+       i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int u = static_cast<int>(i % units);
+    const int64_t w = i / units;
+    const bool is_v = w & 1;
+    const int row = static_cast<int>(w >> 1), head = u / (a.D >> 4), c = u - head * (a.D >> 4);
+    const int slot = a.slots[row];
+    float x[16] = {};
+    if (static_cast<uint32_t>(slot) < static_cast<uint32_t>(a.num_slots)) {
+      const int64_t block = static_cast<int64_t>(slot >> sh) * a.Hkv + head;
+      const int tok = slot & (P - 1);
+      const uint32_t s = a.scales[(block << sh) + tok];
+      const float scale = is_v ? v_scale(s) : k_scale(s);
+      if (is_v) {
+        const int8_t *p = static_cast<const int8_t *>(a.v) + ((block << sh) + (tok & ~15)) * a.D +
+                          c * 256 + (tok & 15);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = static_cast<float>(p[e * 16]) * scale;
+      } else {
+        const u32x4 p = static_cast<const u32x4 *>(a.k)[((block * (a.D >> 4) + c) << sh) + tok];
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          x[e] = static_cast<float>(static_cast<int8_t>(p[e >> 2] >> (8 * (e & 3)))) * scale;
+      }
+    }
+    char *o = static_cast<char *>(is_v ? a.v_out : a.k_out) +
+              (row * (is_v ? a.v_stride : a.k_stride) + static_cast<int64_t>(u) * 16) *
+                  (OUT == IFX_ATTN_F32 ? 4 : 2);
+#pragma unroll
+    for (int e = 0; e < 16; e += 4)
+      store4(o, OUT, e, f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]});
+  }
+}
+
+namespace {
+template <int DT, int SRC, int LANES>
+void launch(const AppendQ8Args &a, hipStream_t s) {
+  IFX_LAUNCH(k_rope_append_q8, (DT, SRC, LANES, 1), dim3(a.a.T, 2), dim3(256), 0, s, a);
+}
+template <int DT, int SRC>
+void launch(const AppendQ8Args &a, hipStream_t s) {
+  if (a.a.D <= 64) return launch<DT, SRC, 16>(a, s);
+  if (a.a.D <= 128) return launch<DT, SRC, 32>(a, s);
+  return launch<DT, SRC, 64>(a, s);
+}
+template <int DT>
+void launch(const AppendQ8Args &a, int src_dtype, hipStream_t s) {
+  switch (src_dtype) {
+    case IFX_ATTN_F32: return launch<DT, IFX_ATTN_F32>(a, s);
+    case IFX_ATTN_F16: return launch<DT, IFX_ATTN_F16>(a, s);
+    default: return launch<DT, IFX_ATTN_BF16>(a, s);
+  }
+}
+}  // namespace
+
+hipError_t launch_rope_append_q8(const AppendQ8Args &a, int src_dtype, int q_dtype, hipStream_t s) {
+  if (q_dtype == IFX_ATTN_F16)
+    launch<IFX_ATTN_F16>(a, src_dtype, s);
+  else
+    launch<IFX_ATTN_BF16>(a, src_dtype, s);
+  return last_error();
+}
+
+hipError_t launch_read_rows_q8(const ReadArgs &a, int out_dtype, hipStream_t s) {
+  const int64_t units = static_cast<int64_t>(a.N) * a.Hkv * (a.D >> 4) * 2;
+  const int64_t need = (units + 255) / 256;
+  const dim3 grid(static_cast<uint32_t>(need < 16384 ? need : 16384));
+  if (out_dtype == IFX_ATTN_F32)
+    IFX_LAUNCH(k_read_rows_q8, (IFX_ATTN_F32), grid, dim3(256), 0, s, a);
+  else if (out_dtype == IFX_ATTN_F16)
+    IFX_LAUNCH(k_read_rows_q8, (IFX_ATTN_F16), grid, dim3(256), 0, s, a);
+  else
+    IFX_LAUNCH(k_read_rows_q8, (IFX_ATTN_BF16), grid, dim3(256), 0, s, a);
+  return last_error();
+}
+
+}  // namespace ifx
