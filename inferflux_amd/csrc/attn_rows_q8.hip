@@ -23,12 +23,42 @@ __device__ __forceinline__ int key_of_row16(int m) {
   return (m & 3) | ((m >> 1) & 0xC) | ((m & 4) << 2);
 }
 
+constexpr int kStep = 32 * kRowWaves;  // keys from a wave's tile to its next
+constexpr int kDepth = 2;              // tiles that are on their way or worked on
+// 16-byte places of a tile in LDS: K, V, and 64 dwords of scales (32 keys', twice).
+template <int D>
+constexpr int tile_pieces() {
+  return 2 * (D / 32) * 64 + 16;
+}
+
+// 16 or 4 bytes a lane from memory to 64 consecutive places in LDS.
+__device__ __forceinline__ void to_lds16(const void *from, u32x4 *to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                   (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+}
+__device__ __forceinline__ void to_lds4(const void *from, u32x4 *to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                   (__attribute__((address_space(3))) void *)to, 4, 0, 0);
+}
+
+// Waits until at most N of this wave's loads are on their way: loads end in
+// order, so all before its last N have ended.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N < 64, "six bits count them");
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4 << 14));
+  __builtin_amdgcn_sched_barrier(0);
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+
 }  // namespace
 
 template <int D>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows_q8(const AttnArgs a, int lds_rows) {
   constexpr int ND = D / 32, NS = D / 16;
-  extern __shared__ float red[];  // [wave][D / 4][row][4]; at first the requests
+  // at first the requests, then [wave][tile][piece], then [wave][D / 4][row][4]
+  extern __shared__ float red[];
   __shared__ RowSums sums;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -76,52 +106,73 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows_q8(const At
   Level level;
   float l = 0.0f;
 
-  const int kn = key_of_row16(n);  // the key of a tile whose K this lane loads
+  // ---- tiles: memory to LDS past the registers, each lane's pieces to its own
+  // places, so that no wave waits for another
+  const int kn = key_of_row16(n);  // the key of a tile whose K this lane takes
   const int32_t *table = a.table + static_cast<int64_t>(b) * a.table_width;
   const int last_page = static_cast<int>(a.num_pages) - 1, wmax = a.table_width - 1;
   const int64_t page_bytes = (static_cast<int64_t>(a.Hkv) * D) << sh;
   const uint8_t *K = static_cast<const uint8_t *>(a.k) + ((static_cast<int64_t>(kvh) * D) << sh);
   const uint8_t *V = static_cast<const uint8_t *>(a.v) + ((static_cast<int64_t>(kvh) * D) << sh);
   const uint32_t *S = a.scales + (static_cast<int64_t>(kvh) << sh);
-
-  // A tile's codes and scales as they lie in the cache.
-  struct Raw {
-    u32x4 k[ND], v[ND], s[4];
-  };
-  // The pages of a tile's two 16-key halves, as the table has them: read a tile
-  // ahead, looked at when that tile's loads are issued.
-  int next0 = 0, next1 = 0;
-  auto entries = [&](int k0) {
-    next0 = table[min(k0 >> sh, wmax)];
-    next1 = table[min((k0 + 16) >> sh, wmax)];
-  };
-  auto load = [&](Raw &f, int k0) __attribute__((always_inline)) {
-    const int pg0 = min(max(next0, 0), last_page), pg1 = min(max(next1, 0), last_page);
-    entries(k0 + 32 * kRowWaves);
+  constexpr int kPieces = tile_pieces<D>(), kLoads = 2 * ND + 1;  // of a tile
+  u32x4 *ring = reinterpret_cast<u32x4 *>(red) + wave * kDepth * kPieces;
+  const int kfirst = zbeg + 32 * wave;
+  const int tiles = (zend - kfirst + kStep - 1) / kStep;
+  // The pages of the tiles' two 16-key halves, as the table has them: of 64 tiles
+  // at a time, a lane each.
+  int entry0 = 0, entry1 = 0;
+  auto issue = [&](int t) __attribute__((always_inline)) {
+    if ((t & 63) == 0) {
+      const int k = kfirst + (t + lane) * kStep;
+      entry0 = table[min(k >> sh, wmax)];
+      entry1 = table[min((k + 16) >> sh, wmax)];
+    }
+    const int k0 = kfirst + t * kStep;
+    const int pg0 = min(max(__builtin_amdgcn_readlane(entry0, t & 63), 0), last_page);
+    const int pg1 = min(max(__builtin_amdgcn_readlane(entry1, t & 63), 0), last_page);
+    u32x4 *to = ring + (t & (kDepth - 1)) * kPieces;
     const uint8_t *kp = K + (kn & 16 ? pg1 : pg0) * page_bytes +
                         ((((k0 + kn) & (P - 1)) + (h << sh)) * 16);
 #pragma unroll
-    for (int i = 0; i < ND; ++i) f.k[i] = ldg<u32x4>(kp + ((i * 32) << sh));
-    const int pg = h ? pg1 : pg0, at = (k0 + 16 * h) & (P - 1);
-    const uint32_t *sp = S + ((static_cast<int64_t>(pg) * a.Hkv) << sh) + at;
+    for (int i = 0; i < ND; ++i) to_lds16(kp + ((i * 32) << sh), to + i * 64);
+    const uint32_t *sp = S + ((static_cast<int64_t>(n & 16 ? pg1 : pg0) * a.Hkv) << sh) +
+                         ((k0 + n) & (P - 1));
+    to_lds4(sp, to + 2 * ND * 64);
+    const uint8_t *vp = V + (h ? pg1 : pg0) * page_bytes + ((k0 + 16 * h) & (P - 1)) * D + n * 16;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f.s[i] = ldg<u32x4>(sp + 4 * i);
-    const uint8_t *vp = V + pg * page_bytes + at * D + n * 16;
-#pragma unroll
-    for (int d = 0; d < ND; ++d) f.v[d] = ldg<u32x4>(vp + d * 512);
-    __builtin_amdgcn_sched_barrier(0);
+    for (int d = 0; d < ND; ++d) to_lds16(vp + d * 512, to + (ND + d) * 64);
   };
-  auto tile = [&](const Raw &f, int k0) __attribute__((always_inline)) {
+
+#pragma unroll
+  for (int t = 0; t < kDepth; ++t)
+    if (t < tiles) issue(t);
+#pragma unroll 1
+  for (int t = 0; t < tiles; ++t) {
+    const int k0 = kfirst + t * kStep;
+    const u32x4 *from = ring + (t & (kDepth - 1)) * kPieces;
+    if (t + 1 < tiles)
+      wait_loads<(kDepth - 1) * kLoads>();
+    else
+      wait_loads<0>();
     f32x16 s;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NS; ++i) s = F16::mfma32(codes_f16(f.k[i >> 1], i & 1), qf[i], s);
+    for (int i = 0; i < ND; ++i) {
+      const u32x4 k = from[i * 64 + lane];
+      s = F16::mfma32(codes_f16(k, 0), qf[2 * i], s);
+      s = F16::mfma32(codes_f16(k, 1), qf[2 * i + 1], s);
+    }
     float sv[16];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[r] *= k_scale(f.s[r >> 2][r & 3]);
-      sv[r] = v_scale(f.s[r >> 2][r & 3]);
+    for (int r = 0; r < 16; r += 4) {
+      const u32x4 f = from[2 * ND * 64 + 4 * h + (r >> 2)];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[r + j] *= k_scale(f[j]);
+        sv[r + j] = v_scale(f[j]);
+      }
     }
     if (k0 + 31 >= ctx + !tree || (a.window > 0 && k0 < ctx + nq - a.window)) {
       // what the row does not see, a page's unwritten slots among it
@@ -155,34 +206,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows_q8(const At
       pf[r >> 3][(r & 7) >> 1] = F16::pack(p0 * sv[r], p1 * sv[r + 1]);
     }
     l += sum;
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-      for (int d = 0; d < ND; ++d) acc[d] = F16::mfma32(codes_f16(f.v[d], ks), pf[ks], acc[d]);
-  };
-
-  constexpr int kStep = 32 * kRowWaves;
-  int k0 = zbeg + 32 * wave;
-  if (k0 < zend) {
-    Raw f, g;  // in turn: one's loads are on their way while the other is worked on
-    entries(k0);
-    load(f, k0);
-    while (true) {
-      if (k0 + kStep >= zend) {
-        tile(f, k0);
-        break;
-      }
-      load(g, k0 + kStep);
-      tile(f, k0);
-      k0 += kStep;
-      if (k0 + kStep >= zend) {
-        tile(g, k0);
-        break;
-      }
-      load(f, k0 + kStep);
-      tile(g, k0);
-      k0 += kStep;
+    for (int d = 0; d < ND; ++d) {
+      const u32x4 v = from[(ND + d) * 64 + lane];
+      acc[d] = F16::mfma32(codes_f16(v, 0), pf[0], acc[d]);
+      acc[d] = F16::mfma32(codes_f16(v, 1), pf[1], acc[d]);
     }
+    __builtin_amdgcn_sched_barrier(0);  // the tile's places are read
+    if (t + kDepth < tiles) issue(t + kDepth);
   }
 
   rows_finish<D>(a, split, red, sums, acc, level.of_sums(), l, 1.0f, lds_rows, R, ns, kvh, [&](int t) {
@@ -191,23 +223,23 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows_q8(const At
 }
 
 namespace {
-constexpr int kMaxLds = 65536 - 2048;  // what a launch may ask for without more ado
-
 template <int D>
 hipError_t launch_rows(const AttnArgs &a, int max_rows, int items, hipStream_t s) {
   constexpr int row_bytes = kRowWaves * D * 4;  // LDS of a row: the waves' sums
-  if constexpr (row_bytes * kRowsMax > kMaxLds) {
+  constexpr int ring_bytes = kRowWaves * kDepth * tile_pieces<D>() * 16;
+  constexpr int most = ring_bytes > row_bytes * kRowsMax ? ring_bytes : row_bytes * kRowsMax;
+  if constexpr (most > 65536 - 2048) {  // what a launch may ask for without more ado
     static std::atomic<uint64_t> done{0};
     if (!dry_run()) {
-      const hipError_t e = allow_lds(reinterpret_cast<const void *>(&k_attn_rows_q8<D>),
-                                     row_bytes * kRowsMax, done);
+      const hipError_t e = allow_lds(reinterpret_cast<const void *>(&k_attn_rows_q8<D>), most, done);
       if (e != hipSuccess) return e;
     }
   }
-  // the waves' sums; before them the requests, after them the chunks' weights and sums
-  int bytes = row_bytes * max_rows;
-  if (bytes < a.B * 8) bytes = a.B * 8;
-  if (bytes < a.goal * max_rows * 8) bytes = a.goal * max_rows * 8;
+  // the tiles; before them the requests, after them the waves' sums, and then the
+  // chunks' weights and sums
+  int bytes = ring_bytes;
+  for (const int need : {row_bytes * max_rows, a.B * 8, a.goal * max_rows * 8})
+    if (bytes < need) bytes = need;
   IFX_LAUNCH(k_attn_rows_q8, (D), dim3(a.Hkv * items), dim3(64 * kRowWaves), bytes, s, a, max_rows);
   return last_error();
 }
