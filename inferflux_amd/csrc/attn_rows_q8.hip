@@ -23,12 +23,36 @@ __device__ __forceinline__ int key_of_row16(int m) {
   return (m & 3) | ((m >> 1) & 0xC) | ((m & 4) << 2);
 }
 
+constexpr int kFewRows = 16;           // of the 16x16 products
 constexpr int kStep = 32 * kRowWaves;  // keys from a wave's tile to its next
 constexpr int kDepth = 2;              // tiles that are on their way or worked on
 // 16-byte places of a tile in LDS: K, V, and 64 dwords of scales (32 keys', twice).
 template <int D>
 constexpr int tile_pieces() {
   return 2 * (D / 32) * 64 + 16;
+}
+
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(F16::v8, a),
+                                                __builtin_bit_cast(F16::v8, b), c, 0, 0, 0);
+}
+
+// Over the four lanes of the same lane % 16.
+__device__ __forceinline__ void both_sixteens(float v, float &x, float &y) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  x = __builtin_bit_cast(float, static_cast<uint32_t>(r[0]));
+  y = __builtin_bit_cast(float, static_cast<uint32_t>(r[1]));
+}
+__device__ __forceinline__ float quarters_max(float v) {
+  float x, y;
+  both_sixteens(v, x, y);
+  return halves_max(fmaxf(x, y));
+}
+__device__ __forceinline__ float quarters_sum(float v) {
+  float x, y;
+  both_sixteens(v, x, y);
+  return halves_sum(x + y);
 }
 
 // 16 or 4 bytes a lane from memory to 64 consecutive places in LDS.
@@ -54,49 +78,103 @@ __device__ __forceinline__ void wait_loads() {
 
 }  // namespace
 
+namespace {
+
+// The workgroup's request and chunk of its keys, and what it sees of them.
+struct RowsWork {
+  Split split;
+  int b, q0, nq, kv, R, ctx, lo0, ns, zbeg, zend;
+  bool tree;
+};
+__device__ __forceinline__ bool rows_work(const AttnArgs &a, float *reqs, int lds_rows, RowsWork &w) {
+  w.split = find_item<1>(a, reinterpret_cast<int2 *>(reqs), blockIdx.x / a.Hkv, [&](const Request &r) {
+    int keys = r.kv;
+    if (a.window > 0) keys = min<int64_t>(keys, static_cast<int64_t>(a.window) + r.nq + kRowKeys);
+    return make_int2(r.nq > 0 ? 1 : 0, max(1, (keys + kRowKeys - 1) / kRowKeys));
+  });
+  if (w.split.chunk == 0) return false;
+  w.b = w.split.b, w.q0 = w.split.req.q0, w.nq = w.split.req.nq, w.kv = w.split.req.kv;
+  w.R = min(w.nq * a.G, lds_rows);
+  w.ctx = w.kv - w.nq;  // position of the first row; below 0 it sees nothing
+  w.tree = a.masks != nullptr;
+  w.lo0 = a.window > 0 ? max(0, w.ctx - a.window + 1) : 0;
+  const int kbeg = w.lo0 & ~(kRowKeys - 1), kend = w.kv, chunk = w.split.chunk * kRowKeys;
+  w.ns = kend > kbeg ? (kend - kbeg + chunk - 1) / chunk : 1;
+  if (w.split.item >= w.ns) return false;
+  w.zbeg = kbeg + w.split.item * chunk, w.zend = min(w.zbeg + chunk, kend);
+  return true;
+}
+
+// What a lane's row sees.
+struct RowSight {
+  bool tree;
+  Sight<false> line;
+  Sight<true> nodes;
+  __device__ __forceinline__ RowSight(const AttnArgs &a, const RowsWork &w, int tok)
+      : tree(w.tree), line{a.window > 0 ? max(0, w.ctx + tok - a.window + 1) : 0, w.ctx + tok, w.ctx, 0},
+        nodes{0, 0, w.ctx, 0} {
+    if (tree) nodes.bits = node_bits(a, w.q0 + tok, w.nq);
+  }
+  __device__ __forceinline__ bool sees(int key) const { return tree ? nodes.sees(key) : line.sees(key); }
+};
+// Whether some row may not see all of the 32 keys from k0 on.
+__device__ __forceinline__ bool in_part(const AttnArgs &a, const RowsWork &w, int k0) {
+  return k0 + 31 >= w.ctx + !w.tree || (a.window > 0 && k0 < w.ctx + w.nq - a.window);
+}
+// Whether the rows of new token t see nothing.
+__device__ __forceinline__ bool row_sees_nothing(const AttnArgs &a, const RowsWork &w, int t) {
+  return w.tree ? Sight<true>{0, 0, w.ctx, node_bits(a, w.q0 + t, w.nq)}.nothing() : w.ctx + t < 0;
+}
+
+// The pages of the two 16-key halves of a wave's tiles, as the table has them: of
+// 64 tiles at a time, a lane each.
+struct Pages {
+  const int32_t *table;
+  int sh, wmax, last, first, entry0, entry1;
+  __device__ __forceinline__ Pages(const AttnArgs &a, int b, int kfirst)
+      : table(a.table + static_cast<int64_t>(b) * a.table_width), sh(a.page_shift),
+        wmax(a.table_width - 1), last(static_cast<int>(a.num_pages) - 1), first(kfirst) {}
+  __device__ __forceinline__ void read(int t) {
+    const int64_t k = first + static_cast<int64_t>(t + (threadIdx.x & 63)) * kStep;
+    entry0 = table[min(k >> sh, static_cast<int64_t>(wmax))];
+    entry1 = table[min((k + 16) >> sh, static_cast<int64_t>(wmax))];
+    wait_loads<0>();  // here, so that no later use of them waits for tiles
+  }
+  __device__ __forceinline__ int page0(int t) const {
+    return min(max(__builtin_amdgcn_readlane(entry0, t & 63), 0), last);
+  }
+  __device__ __forceinline__ int page1(int t) const {
+    return min(max(__builtin_amdgcn_readlane(entry1, t & 63), 0), last);
+  }
+};
+
+}  // namespace
+
 template <int D>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows_q8(const AttnArgs a, int lds_rows) {
   constexpr int ND = D / 32, NS = D / 16;
-  // at first the requests, then [wave][tile][piece], then [wave][D / 4][row][4]
-  extern __shared__ float red[];
+  // At first the requests, then [wave][tile][piece], then [wave][D / 4][row][4].
+  // Aligned, as copies of 16 bytes a lane to LDS need it: behind 1028 bytes of
+  // other data they left parts of pieces wrong where many workgroups ran.
+  extern __shared__ __attribute__((aligned(16))) float red[];
   __shared__ RowSums sums;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kvh = blockIdx.x % a.Hkv;
   const int sh = a.page_shift, P = 1 << sh;
-
-  // the workgroup's request and chunk of its keys
-  const Split split = find_item<1>(
-      a, reinterpret_cast<int2 *>(red), blockIdx.x / a.Hkv, [&](const Request &r) {
-        int keys = r.kv;
-        if (a.window > 0) keys = min<int64_t>(keys, static_cast<int64_t>(a.window) + r.nq + kRowKeys);
-        return make_int2(r.nq > 0 ? 1 : 0, max(1, (keys + kRowKeys - 1) / kRowKeys));
-      });
-  if (split.chunk == 0) return;
-  const int b = split.b, z = split.item;
-  const int q0 = split.req.q0, nq = split.req.nq, kv = split.req.kv, R = min(nq * a.G, lds_rows);
-  const int ctx = kv - nq;  // position of the first row; below 0 it sees nothing
-  const bool tree = a.masks != nullptr;
-  const int lo0 = a.window > 0 ? max(0, ctx - a.window + 1) : 0;
-  const int kbeg = lo0 & ~(kRowKeys - 1), kend = kv;
-  const int chunk = split.chunk * kRowKeys;
-  const int ns = kend > kbeg ? (kend - kbeg + chunk - 1) / chunk : 1;
-  if (z >= ns) return;
-  const int zbeg = kbeg + z * chunk, zend = min(zbeg + chunk, kend);
+  RowsWork w;
+  if (!rows_work(a, red, lds_rows, w)) return;
 
   // this lane's row; rows behind the last repeat it
-  const int row = min(n, R - 1), tok = row / a.G, head = kvh * a.G + row % a.G;
-  const Sight<false> line = {a.window > 0 ? max(0, ctx + tok - a.window + 1) : 0, ctx + tok, ctx, 0};
-  Sight<true> nodes = {0, 0, ctx, 0};
-  if (tree) nodes.bits = node_bits(a, q0 + tok, nq);
+  const int row = min(n, w.R - 1), tok = row / a.G, head = kvh * a.G + row % a.G;
+  const RowSight sight(a, w, tok);
   u32x4 qf[NS];
   {  // of step s the dims 32 (s / 2) + 16 h + 8 (s % 2), as K's pieces hold them
-    const uint16_t *q = static_cast<const uint16_t *>(a.q) + (q0 + tok) * a.q_stride +
+    const uint16_t *q = static_cast<const uint16_t *>(a.q) + (w.q0 + tok) * a.q_stride +
                         static_cast<int64_t>(head) * D + 16 * h;
 #pragma unroll
     for (int s = 0; s < NS; ++s) qf[s] = ldg<u32x4>(q + 32 * (s >> 1) + 8 * (s & 1));
   }
-  const float c = row_to_f16(qf, a.q_dtype, a.c);
 
   f32x16 acc[ND];
 #pragma unroll
@@ -109,28 +187,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows_q8(const At
   // ---- tiles: memory to LDS past the registers, each lane's pieces to its own
   // places, so that no wave waits for another
   const int kn = key_of_row16(n);  // the key of a tile whose K this lane takes
-  const int32_t *table = a.table + static_cast<int64_t>(b) * a.table_width;
-  const int last_page = static_cast<int>(a.num_pages) - 1, wmax = a.table_width - 1;
   const int64_t page_bytes = (static_cast<int64_t>(a.Hkv) * D) << sh;
   const uint8_t *K = static_cast<const uint8_t *>(a.k) + ((static_cast<int64_t>(kvh) * D) << sh);
   const uint8_t *V = static_cast<const uint8_t *>(a.v) + ((static_cast<int64_t>(kvh) * D) << sh);
   const uint32_t *S = a.scales + (static_cast<int64_t>(kvh) << sh);
   constexpr int kPieces = tile_pieces<D>(), kLoads = 2 * ND + 1;  // of a tile
   u32x4 *ring = reinterpret_cast<u32x4 *>(red) + wave * kDepth * kPieces;
-  const int kfirst = zbeg + 32 * wave;
-  const int tiles = (zend - kfirst + kStep - 1) / kStep;
-  // The pages of the tiles' two 16-key halves, as the table has them: of 64 tiles
-  // at a time, a lane each.
-  int entry0 = 0, entry1 = 0;
+  const int kfirst = w.zbeg + 32 * wave, tiles = (w.zend - kfirst + kStep - 1) / kStep;
+  Pages pages(a, w.b, kfirst);
   auto issue = [&](int t) __attribute__((always_inline)) {
-    if ((t & 63) == 0) {
-      const int k = kfirst + (t + lane) * kStep;
-      entry0 = table[min(k >> sh, wmax)];
-      entry1 = table[min((k + 16) >> sh, wmax)];
-    }
-    const int k0 = kfirst + t * kStep;
-    const int pg0 = min(max(__builtin_amdgcn_readlane(entry0, t & 63), 0), last_page);
-    const int pg1 = min(max(__builtin_amdgcn_readlane(entry1, t & 63), 0), last_page);
+    if (t && (t & 63) == 0) pages.read(t);
+    const int k0 = kfirst + t * kStep, pg0 = pages.page0(t), pg1 = pages.page1(t);
     u32x4 *to = ring + (t & (kDepth - 1)) * kPieces;
     const uint8_t *kp = K + (kn & 16 ? pg1 : pg0) * page_bytes +
                         ((((k0 + kn) & (P - 1)) + (h << sh)) * 16);
@@ -144,6 +211,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows_q8(const At
     for (int d = 0; d < ND; ++d) to_lds16(vp + d * 512, to + (ND + d) * 64);
   };
 
+  pages.read(0);  // and the rows of Q are here
+  const float c = row_to_f16<32>(qf, a.q_dtype, a.c);
 #pragma unroll
   for (int t = 0; t < kDepth; ++t)
     if (t < tiles) issue(t);
@@ -174,12 +243,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows_q8(const At
         sv[r + j] = v_scale(f[j]);
       }
     }
-    if (k0 + 31 >= ctx + !tree || (a.window > 0 && k0 < ctx + nq - a.window)) {
-      // what the row does not see, a page's unwritten slots among it
+    if (in_part(a, w, k0)) {  // what the row does not see, a page's unwritten slots among it
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int key = k0 + 16 * h + r;
-        const bool sees = tree ? nodes.sees(key) : line.sees(key);
+        const bool sees = sight.sees(k0 + 16 * h + r);
         s[r] = sees ? s[r] : -__builtin_inff();
         sv[r] = sees ? sv[r] : 0.0f;
       }
@@ -189,12 +256,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows_q8(const At
     for (int r = 1; r < 16; ++r) mt = fmaxf(mt, s[r]), vt = fmaxf(vt, sv[r]);
     mt = halves_max(mt), vt = halves_max(vt);
     if (__any(level.above(mt, vt, c))) {
-      const float w = level.raise(mt, vt, c);
-      l *= w;
+      const float less = level.raise(mt, vt, c);
+      l *= less;
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[d][r] *= w;
+        for (int r = 0; r < 16; ++r) acc[d][r] *= less;
     }
     u32x4 pf[2];
     float sum = 0.0f;
@@ -217,21 +284,180 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows_q8(const At
     if (t + kDepth < tiles) issue(t + kDepth);
   }
 
-  rows_finish<D>(a, split, red, sums, acc, level.of_sums(), l, 1.0f, lds_rows, R, ns, kvh, [&](int t) {
-    return tree ? Sight<true>{0, 0, ctx, node_bits(a, q0 + t, nq)}.nothing() : ctx + t < 0;
-  });
+  l = halves_sum(l);
+  const auto put = [&](float scale) { put_rows32<D>(red, acc, scale, w.R); };
+  rows_finish<D>(a, w.split, red, sums, n, h == 0, level.of_sums(), l, 1.0f, lds_rows, w.R, w.ns, kvh,
+                 put, [&](int t) { return row_sees_nothing(a, w, t); });
+}
+
+// At most 16 rows: the same with 16x16 products, so that half as many scores are
+// weighed, and registers and LDS for twice as many workgroups.  Lane (m, g),
+// m = lane % 16, g = lane / 16, holds row m: of S^T the keys 8 g + 4 i + r
+// (register r of product i), which are the B operand of O^T = V^T P^T as they
+// stand; of O^T the dims 16 d + 4 g + r.
+template <int D>
+__global__ __launch_bounds__(256, D == 256 ? 2 : 4) void k_attn_rows16_q8(const AttnArgs a, int lds_rows) {
+  constexpr int ND = D / 32, NB = D / 16;
+  // at first the requests, then [wave][piece], then [wave][D / 4][row][4]
+  extern __shared__ __attribute__((aligned(16))) float red[];
+  __shared__ RowSums sums;
+  const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kvh = blockIdx.x % a.Hkv;
+  const int sh = a.page_shift, P = 1 << sh;
+  RowsWork w;
+  if (!rows_work(a, red, lds_rows, w)) return;
+
+  const int row = min(m, w.R - 1), tok = row / a.G, head = kvh * a.G + row % a.G;
+  const RowSight sight(a, w, tok);
+  u32x4 qf[ND];
+  {  // steps 2 i and 2 i + 1: the dims 64 i + 16 g + 0 .. 7 and + 8 .. 15, a piece of
+     // K; a last step alone: 8 g .. + 7 of the last 32
+    const uint16_t *q = static_cast<const uint16_t *>(a.q) + (w.q0 + tok) * a.q_stride +
+                        static_cast<int64_t>(head) * D;
+#pragma unroll
+    for (int s = 0; s < ND; ++s)
+      qf[s] = ldg<u32x4>(q + (s + 1 == ND && ND % 2 ? 32 * s + 8 * g : 64 * (s >> 1) + 16 * g + 8 * (s & 1)));
+  }
+  f32x4 acc[NB];
+#pragma unroll
+  for (int d = 0; d < NB; ++d) acc[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  Level level;
+  float l = 0.0f;
+
+  // ---- a tile: memory to LDS past the registers, K [D / 16][32 keys], in the
+  // order in which the products take them, V [2][D], scales [32]
+  const int64_t page_bytes = (static_cast<int64_t>(a.Hkv) * D) << sh;
+  const uint8_t *K = static_cast<const uint8_t *>(a.k) + ((static_cast<int64_t>(kvh) * D) << sh);
+  const uint8_t *V = static_cast<const uint8_t *>(a.v) + ((static_cast<int64_t>(kvh) * D) << sh);
+  const uint32_t *S = a.scales + (static_cast<int64_t>(kvh) << sh);
+  u32x4 *tk = reinterpret_cast<u32x4 *>(red) + wave * tile_pieces<D>(), *tv = tk + ND * 64;
+  u32x4 *ts = tv + ND * 64;
+  const int kfirst = w.zbeg + 32 * wave, tiles = (w.zend - kfirst + kStep - 1) / kStep;
+  Pages pages(a, w.b, kfirst);
+  const int kl = (lane >> 2 & 3) * 8 + (lane >> 4 & 1) * 4 + (lane & 3);  // the key that a lane copies
+  auto issue_k = [&](int t) __attribute__((always_inline)) {
+    if (t && (t & 63) == 0) pages.read(t);
+    const int k0 = kfirst + t * kStep, pg0 = pages.page0(t), pg1 = pages.page1(t);
+    const uint8_t *kp = K + (kl & 16 ? pg1 : pg0) * page_bytes +
+                        ((((k0 + kl) & (P - 1)) + ((lane >> 5) << sh)) * 16);
+#pragma unroll
+    for (int i = 0; i < ND; ++i) to_lds16(kp + ((i * 32) << sh), tk + i * 64);
+    const int n = lane & 31;
+    to_lds4(S + ((static_cast<int64_t>(n & 16 ? pg1 : pg0) * a.Hkv) << sh) + ((k0 + n) & (P - 1)), ts);
+  };
+  auto issue_v = [&](int t) __attribute__((always_inline)) {
+    const int k0 = kfirst + t * kStep, pg0 = pages.page0(t), pg1 = pages.page1(t);
+#pragma unroll
+    for (int i = 0; i < ND; ++i) {
+      const int p = i * 64 + lane, half = p >= D, dim = p - (half ? D : 0);
+      to_lds16(V + (half ? pg1 : pg0) * page_bytes + ((k0 + 16 * half) & (P - 1)) * D + dim * 16, tv + i * 64);
+    }
+  };
+
+  pages.read(0);  // and the rows of Q are here
+  const float c = row_to_f16<16>(qf, a.q_dtype, a.c);
+  if (tiles > 0) {
+    issue_k(0);
+    issue_v(0);
+  }
+#pragma unroll 1
+  for (int t = 0; t < tiles; ++t) {
+    const int k0 = kfirst + t * kStep;
+    const bool more = t + 1 < tiles;
+    wait_loads<ND>();  // K and the scales; V's are behind them
+    f32x4 s[2] = {};
+#pragma unroll
+    for (int i = 0; i < (ND + 1) / 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (2 * i + 1 < ND) {
+          const u32x4 k = tk[(4 * i + g) * 32 + 16 * e + m];
+          s[e] = mfma16(codes_f16(k, 0), qf[2 * i], s[e]);
+          s[e] = mfma16(codes_f16(k, 1), qf[2 * i + 1], s[e]);
+        } else {
+          const u32x2 k = reinterpret_cast<const u32x2 *>(tk + (4 * i + (g >> 1)) * 32 + 16 * e + m)[g & 1];
+          s[e] = mfma16(codes_f16(k), qf[2 * i], s[e]);
+        }
+      }
+    float sv[2][4];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const u32x4 f = ts[2 * g + e];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[e][r] *= k_scale(f[r]);
+        sv[e][r] = v_scale(f[r]);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);  // K's and the scales' places are read
+    if (more) issue_k(t + 1);
+    if (in_part(a, w, k0)) {  // what the row does not see, a page's unwritten slots among it
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const bool sees = sight.sees(k0 + 8 * g + 4 * e + r);
+          s[e][r] = sees ? s[e][r] : -__builtin_inff();
+          sv[e][r] = sees ? sv[e][r] : 0.0f;
+        }
+    }
+    float mt = s[0][0], vt = sv[0][0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) mt = fmaxf(mt, s[i >> 2][i & 3]), vt = fmaxf(vt, sv[i >> 2][i & 3]);
+    mt = quarters_max(mt), vt = quarters_max(vt);
+    if (__any(level.above(mt, vt, c))) {
+      const float less = level.raise(mt, vt, c);
+      l *= less;
+#pragma unroll
+      for (int d = 0; d < NB; ++d) acc[d] *= less;
+    }
+    u32x4 pf;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 1][2 * (i & 1)], c, -level.less));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 1][2 * (i & 1) + 1], c, -level.less));
+      l += p0 + p1;
+      pf[i] = F16::pack(p0 * sv[i >> 1][2 * (i & 1)], p1 * sv[i >> 1][2 * (i & 1) + 1]);
+    }
+    if (more)
+      wait_loads<ND + 1>();  // V; the next tile's K and scales are behind it
+    else
+      wait_loads<0>();
+#pragma unroll
+    for (int d = 0; d < NB; ++d) {
+      const u32x2 v = reinterpret_cast<const u32x2 *>(tv + (g >> 1) * D + 16 * d + m)[g & 1];
+      acc[d] = mfma16(codes_f16(v), pf, acc[d]);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // V's places are read
+    if (more) issue_v(t + 1);
+  }
+
+  l = quarters_sum(l);
+  const auto put = [&](float scale) {
+#pragma unroll
+    for (int d = 0; d < NB; ++d) {
+      const f32x4 v = acc[d] * scale;
+      __builtin_memcpy(red + ((wave * (D / 4) + 4 * d + g) * w.R + m) * 4, &v, 16);
+    }
+  };
+  rows_finish<D, 16>(a, w.split, red, sums, m, g == 0, level.of_sums(), l, 1.0f, lds_rows, w.R, w.ns, kvh,
+                 put, [&](int t) { return row_sees_nothing(a, w, t); });
 }
 
 namespace {
-template <int D>
+template <int D, bool FEW>
 hipError_t launch_rows(const AttnArgs &a, int max_rows, int items, hipStream_t s) {
   constexpr int row_bytes = kRowWaves * D * 4;  // LDS of a row: the waves' sums
-  constexpr int ring_bytes = kRowWaves * kDepth * tile_pieces<D>() * 16;
-  constexpr int most = ring_bytes > row_bytes * kRowsMax ? ring_bytes : row_bytes * kRowsMax;
+  constexpr int rows = FEW ? kFewRows : kRowsMax;
+  constexpr int ring_bytes = kRowWaves * (FEW ? 1 : kDepth) * tile_pieces<D>() * 16;
+  constexpr int most = ring_bytes > row_bytes * rows ? ring_bytes : row_bytes * rows;
   if constexpr (most > 65536 - 2048) {  // what a launch may ask for without more ado
     static std::atomic<uint64_t> done{0};
     if (!dry_run()) {
-      const hipError_t e = allow_lds(reinterpret_cast<const void *>(&k_attn_rows_q8<D>), most, done);
+      const void *kernel = FEW ? reinterpret_cast<const void *>(&k_attn_rows16_q8<D>)
+                               : reinterpret_cast<const void *>(&k_attn_rows_q8<D>);
+      const hipError_t e = allow_lds(kernel, most, done);
       if (e != hipSuccess) return e;
     }
   }
@@ -240,8 +466,17 @@ hipError_t launch_rows(const AttnArgs &a, int max_rows, int items, hipStream_t s
   int bytes = ring_bytes;
   for (const int need : {row_bytes * max_rows, a.B * 8, a.goal * max_rows * 8})
     if (bytes < need) bytes = need;
-  IFX_LAUNCH(k_attn_rows_q8, (D), dim3(a.Hkv * items), dim3(64 * kRowWaves), bytes, s, a, max_rows);
+  const dim3 grid(a.Hkv * items), block(64 * kRowWaves);
+  if constexpr (FEW)
+    IFX_LAUNCH(k_attn_rows16_q8, (D), grid, block, bytes, s, a, max_rows);
+  else
+    IFX_LAUNCH(k_attn_rows_q8, (D), grid, block, bytes, s, a, max_rows);
   return last_error();
+}
+template <int D>
+hipError_t launch_rows(const AttnArgs &a, int max_rows, int items, hipStream_t s) {
+  return max_rows <= kFewRows ? launch_rows<D, true>(a, max_rows, items, s)
+                              : launch_rows<D, false>(a, max_rows, items, s);
 }
 }  // namespace
 

@@ -80,7 +80,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void k_attn_tile_q8(con
 #pragma unroll
     for (int s = 0; s < NS; ++s) qf[s] = ldg<u32x4>(q + 16 * s);
   }
-  const float c = row_to_f16(qf, a.q_dtype, a.c);
+  const float c = row_to_f16<32>(qf, a.q_dtype, a.c);
   f32x16 acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d)

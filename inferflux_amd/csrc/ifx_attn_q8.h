@@ -41,16 +41,19 @@ __device__ __forceinline__ u32x2 codes_f16(uint32_t w) {
   const v2 hi = __builtin_bit_cast(v2, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) + less;
   return u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
 }
+__device__ __forceinline__ u32x4 codes_f16(u32x2 w) {
+  const u32x2 a = codes_f16(w.x), b = codes_f16(w.y);
+  return u32x4{a.x, a.y, b.x, b.y};
+}
 // Eight of a piece's sixteen: the first (i = 0) or the last.
 __device__ __forceinline__ u32x4 codes_f16(u32x4 p, int i) {
-  const u32x2 a = codes_f16(i ? p.z : p.x), b = codes_f16(i ? p.w : p.y);
-  return u32x4{a.x, a.y, b.x, b.y};
+  return codes_f16(i ? u32x2{p.z, p.w} : u32x2{p.x, p.y});
 }
 
 // Q of a row as fp16 operands: as it is, or of bf16 times a power of two that
-// takes the row's largest value to [2^13, 2^14).  f: the lane's part of the row,
-// its other half's the rest of it.  Returns what scores are multiplied by.
-template <int NS>
+// takes the row's largest value to [2^13, 2^14).  f: the lane's part of the row;
+// lanes LANES apart hold the rest of it.  Returns what scores are multiplied by.
+template <int LANES, int NS>
 __device__ __forceinline__ float row_to_f16(u32x4 (&f)[NS], int dtype, float c) {
   if (dtype == IFX_ATTN_F16) return c;
   float top = 0.0f;
@@ -59,7 +62,8 @@ __device__ __forceinline__ float row_to_f16(u32x4 (&f)[NS], int dtype, float c) 
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       top = fmaxf(top, fmaxf(fabsf(BF16::value(f[s][j] & 0xFFFFu)), fabsf(BF16::value(f[s][j] >> 16))));
-  top = halves_max(top);
+#pragma unroll
+  for (int d = LANES; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
   const int e = min(max(static_cast<int>(__builtin_bit_cast(uint32_t, top) >> 23), 64), 253);
   const float up = __builtin_bit_cast(float, static_cast<uint32_t>(267 - e) << 23);
 #pragma unroll
@@ -86,11 +90,14 @@ struct Level {
     float sn = size;
     if (vt > size)  // the next power of two
       sn = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, vt) + 0x7FFFFFu) & 0x7F800000u);
-    const float w = (mn == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c)) * (size / sn);
+    const float e = power(sn), was = power(size);
+    const float w = mn == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c + (was - e));
     m = mn, size = sn;
-    const int e = static_cast<int>(__builtin_bit_cast(uint32_t, sn) >> 23) - 127;
-    less = m == -__builtin_inff() ? 0.0f : m * c - F16::kShift + static_cast<float>(e);
+    less = m == -__builtin_inff() ? 0.0f : m * c - F16::kShift + e;
     return w;
+  }
+  static __device__ __forceinline__ float power(float size) {
+    return static_cast<float>(static_cast<int>(__builtin_bit_cast(uint32_t, size) >> 23) - 127);
   }
   // of sums that met nothing: -inf
   __device__ __forceinline__ float of_sums() const { return m == -__builtin_inff() ? m : less; }

@@ -14,24 +14,23 @@ struct RowSums {
   float m[kRowWaves][32], l[kRowWaves][32];
 };
 
-// Lane n of each half of a wave holds row n: maximum m and sum l, and in acc
-// the dims 32 d + 8 (r / 4) + 4 h + r % 4.  Exponents are (s - m) c.  red:
-// [wave][D / 4][row][4], later [chunk][row].  none(t): whether the rows of new
-// token t see nothing.
-template <int D, class None>
+// Of a wave the lanes with the same n hold row n, one of them (lead) besides the
+// others its maximum m and sum l; exponents are (s - m) c.  put(scale): the
+// lane writes its part of the row's sums, times scale, to red[wave][D / 4][R][4].
+// red later holds [chunk][row].  none(t): whether the rows of new token t see
+// nothing.  kAtOnce: chunks whose sums a thread reads at a time, 4 registers each.
+template <int D, int kAtOnce = 24, class Put, class None>
 __device__ __forceinline__ void rows_finish(const AttnArgs &a, const Split &split, float *red,
-                                            RowSums &sums, const f32x16 (&acc)[D / 32], float m,
-                                            float l, float c, int lds_rows, int R, int ns, int kvh,
+                                            RowSums &sums, int n, bool lead, float m, float l,
+                                            float c, int lds_rows, int R, int ns, int kvh, Put put,
                                             None none) {
-  constexpr int ND = D / 32;
   constexpr uint32_t kOut = 1u << 30;  // an offset past the workspace's end: reads zeros
-  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
+  const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int z = split.item, q0 = split.req.q0;
 
   // the four waves' sums, in the waves' order
-  l = halves_sum(l);
-  if (h == 0) {
+  if (lead) {
     sums.m[wave][n] = m;
     sums.l[wave][n] = l;
   }
@@ -39,18 +38,7 @@ __device__ __forceinline__ void rows_finish(const AttnArgs &a, const Split &spli
   float top = sums.m[0][n];
 #pragma unroll
   for (int w = 1; w < kRowWaves; ++w) top = fmaxf(top, sums.m[w][n]);
-  const float scale = weight(m, top, c);
-  if (n < R) {
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        f32x4 v;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = acc[d][4 * g + r] * scale;
-        __builtin_memcpy(red + ((wave * (D / 4) + 8 * d + 2 * g + h) * R + n) * 4, &v, 16);
-      }
-  }
+  if (n < R) put(weight(m, top, c));
   float lt = 0.0f;  // of row n
 #pragma unroll
   for (int w = 0; w < kRowWaves; ++w) {
@@ -58,7 +46,7 @@ __device__ __forceinline__ void rows_finish(const AttnArgs &a, const Split &spli
     lt += sums.l[w][n] * weight(mw, top, c);
   }
   __syncthreads();  // all waves have read sums.m / sums.l
-  if (wave == 0 && h == 0) {
+  if (wave == 0 && lead) {
     sums.m[0][n] = top;
     sums.l[0][n] = lt;
   }
@@ -103,7 +91,6 @@ __device__ __forceinline__ void rows_finish(const AttnArgs &a, const Split &spli
   if (!split_arrive_last(cnt, ns)) return;
   // Reads past the L2 take a microsecond: a thread's first sums are on their way
   // while the chunks' weights are formed.
-  constexpr int kAtOnce = 24;
   f32x4 v[kAtOnce];
   auto read = [&](int i, int y0) __attribute__((always_inline)) {
 #pragma unroll
@@ -165,6 +152,22 @@ __device__ __forceinline__ void rows_finish(const AttnArgs &a, const Split &spli
     store4(to, a.out_dtype, d4 * 4, o);
   }
   split_reset(cnt);
+}
+
+// put of 32-row accumulators: acc[d][r] of lane half h is dim 32 d + 8 (r / 4) + 4 h + r % 4.
+template <int D>
+__device__ __forceinline__ void put_rows32(float *red, const f32x16 (&acc)[D / 32], float scale, int R) {
+  const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      f32x4 v;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = acc[d][4 * g + r] * scale;
+      __builtin_memcpy(red + ((wave * (D / 4) + 8 * d + 2 * g + h) * R + n) * 4, &v, 16);
+    }
 }
 
 }  // namespace ifx
