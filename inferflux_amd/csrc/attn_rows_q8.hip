@@ -55,27 +55,6 @@ __device__ __forceinline__ float quarters_sum(float v) {
   return halves_sum(x + y);
 }
 
-// 16 or 4 bytes a lane from memory to 64 consecutive places in LDS.
-__device__ __forceinline__ void to_lds16(const void *from, u32x4 *to) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
-                                   (__attribute__((address_space(3))) void *)to, 16, 0, 0);
-}
-__device__ __forceinline__ void to_lds4(const void *from, u32x4 *to) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
-                                   (__attribute__((address_space(3))) void *)to, 4, 0, 0);
-}
-
-// Waits until at most N of this wave's loads are on their way: loads end in
-// order, so all before its last N have ended.
-template <int N>
-__device__ __forceinline__ void wait_loads() {
-  static_assert(N < 64, "six bits count them");
-  __atomic_signal_fence(__ATOMIC_SEQ_CST);
-  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4 << 14));
-  __builtin_amdgcn_sched_barrier(0);
-  __atomic_signal_fence(__ATOMIC_SEQ_CST);
-}
-
 }  // namespace
 
 namespace {

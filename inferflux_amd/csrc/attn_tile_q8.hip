@@ -21,6 +21,17 @@ namespace {
 constexpr int kThreads = 64 * kTileWaves;
 constexpr int TK = kTileKeys;
 constexpr int kMinChunk = 8;  // stages of a chunk at least (attn_tile)
+// Waits for this wave's LDS accesses and then for the workgroup's other waves;
+// copies from memory stay on their way.
+__device__ __forceinline__ void group_barrier() {
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+
+constexpr int kScales = 2 * TK + 4;  // of a stage: K's, V's, the largest of V's
 
 }  // namespace
 
@@ -30,10 +41,13 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void k_attn_tile_q8(con
   constexpr int kPieces = TK * D / 8;           // 16-byte pieces of fp16, of K and of V
   constexpr int kRaw = TK * D / 16;             // of codes
   constexpr int NL = (kRaw + kThreads - 1) / kThreads;
-  extern __shared__ u32x4 lds[];                // [2 stages][K, V][kPieces], [2][K, V scales][64]
-  float *scales = reinterpret_cast<float *>(lds + 4 * kPieces);
-  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  extern __shared__ u32x4 lds[];                // fp16 [K, V][kPieces], codes and scales as copied, kScales
+  u32x4 *raw = lds + 2 * kPieces;               // [K, V][kRaw], 64 dwords
+  float *scales = reinterpret_cast<float *>(raw + 2 * kRaw + 16);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // kept, and not the thread's number
+  const int n = lane & 31, h = lane >> 5;
   const int kvh = blockIdx.x % a.Hkv;
 
   const Split split = find_item<kMinChunk>(
@@ -99,77 +113,119 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void k_attn_tile_q8(con
   const uint32_t *S = a.scales + (static_cast<int64_t>(kvh) << sh);
   // the page of key k0 + lane, as the table has it: read a stage ahead
   auto entry_of = [&](int k0) { return table[min((k0 + lane) >> sh, wmax)]; };
-  u32x4 rk[NL], rv[NL];
-  uint32_t rs = 0;
-  auto load = [&](int k0, int entry) IFX_INLINE {
+  // Copies a stage's codes to LDS past the registers, each lane's pieces to its
+  // own places, and wave 0 the scales.
+  auto issue = [&](int k0, int entry) IFX_INLINE {
     const int page = min(max(entry, 0), last_page);
     const uint64_t at = static_cast<uint64_t>(static_cast<uint32_t>(page)) * page_bytes;
     const uint8_t *kp = K + at + ((k0 + lane) & (P - 1)) * 16;
     if (wave == 0)
-      rs = S[((static_cast<int64_t>(page) * a.Hkv) << sh) + ((k0 + lane) & (P - 1))];
+      to_lds4(S + ((static_cast<int64_t>(page) * a.Hkv) << sh) + ((k0 + lane) & (P - 1)), raw + 2 * kRaw);
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int p0 = (i * kTileWaves + wave) * 64, p = p0 + lane;  // 64 pieces
       if (kRaw % kThreads && p0 >= kRaw) break;
-      rk[i] = ldg<u32x4>(kp + ((p0 >> 6) << sh) * 16);
+      to_lds16(kp + ((p0 >> 6) << sh) * 16, raw + p0);
       const int g = p / D, dim = p - g * D;
       const uint32_t pg = static_cast<uint32_t>(__shfl(page, 16 * g));
-      rv[i] = ldg<u32x4>(V + static_cast<uint64_t>(pg) * page_bytes + ((k0 + 16 * g) & (P - 1)) * D + dim * 16);
+      to_lds16(V + static_cast<uint64_t>(pg) * page_bytes + ((k0 + 16 * g) & (P - 1)) * D + dim * 16,
+               raw + kRaw + p0);
     }
   };
-  auto store = [&](int buf) IFX_INLINE {
-    u32x4 *sk = lds + buf * 2 * kPieces, *sv = sk + kPieces;
+  // The codes that this wave copied as fp16.
+  auto convert = [&]() IFX_INLINE {
+    u32x4 *sk = lds, *sv = sk + kPieces;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int p0 = (i * kTileWaves + wave) * 64, p = p0 + lane;
       if (kRaw % kThreads && p0 >= kRaw) break;
       const int g = p / D, dim = p - g * D;
+      const u32x4 rk = raw[p], rv = raw[kRaw + p];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        sk[(p0 >> 6) * 2 * TK + e * TK + lane] = codes_f16(rk[i], e);
-        sv[(2 * g + e) * D + dim] = codes_f16(rv[i], e);
+        sk[(p0 >> 6) * 2 * TK + e * TK + lane] = codes_f16(rk, e);
+        sv[(2 * g + e) * D + dim] = codes_f16(rv, e);
       }
     }
     if (wave == 0) {
-      scales[buf * 2 * TK + lane] = k_scale(rs);
-      scales[buf * 2 * TK + TK + lane] = v_scale(rs);
+      const uint32_t rs = reinterpret_cast<const uint32_t *>(raw + 2 * kRaw)[lane];
+      scales[lane] = k_scale(rs);
+      scales[TK + lane] = v_scale(rs);
+      float top = v_scale(rs);
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+      if (lane == 0) scales[2 * TK] = top;
     }
   };
 
+  // One stage.  The matrix cores get the fragments of K, then of V, in one
+  // sequence: fragment i + kAhead is on its way from LDS while i is multiplied.
+  // edge: some rows see only a part of it.
   const int kn = key_of_row(n);
-  auto stage = [&](int k0, int buf, bool edge) IFX_INLINE {
-    const u32x4 *sk = lds + buf * 2 * kPieces, *sv = sk + kPieces;
-    const float *ks = scales + buf * 2 * TK, *vs = ks + TK;
+  const f32x16 none_yet = {};
+  auto stage = [&](int k0, auto edge_c) IFX_INLINE {
+    constexpr bool edge = decltype(edge_c)::value;
+    constexpr int kAhead = 3;
+    const u32x4 *sk = lds + h * TK + kn, *sv = lds + kPieces + h * D + n;
+    const float *ks = scales + 8 * h, *vs = ks + TK;
+    u32x4 f[4 * NS];  // K of both halves, V: at most kAhead + 1 are alive
+    auto frag = [&](int i) IFX_INLINE {
+      if (i < 2 * NS)
+        f[i] = sk[2 * (i % NS) * TK + 32 * (i / NS)];
+      else if (i < 4 * NS)
+        f[i] = sv[2 * ((i - 2 * NS) / ND) * D + 32 * ((i - 2 * NS) % ND)];
+    };
+    auto at = [](int sub, int r) { return 32 * sub + 16 * (r >> 3) + (r & 7); };  // key of register r, less 8 h
     f32x16 s[2];
-    float w[2][16];
-    float mt = -__builtin_inff(), vt = 0.0f;
+    float mt[2] = {-__builtin_inff(), -__builtin_inff()};
+    float vt = edge ? 0.0f : scales[2 * TK];
+    // what the lane's row sees of the keys of its half of the wave: bit 32 sub + 16 (r / 8) + r % 8
+    uint64_t sees = 0;
+    if constexpr (edge) sees = (tree ? nodes.of_64(k0) : line.of_64(k0)) >> (8 * h);
+    auto mask = [&](int key) IFX_INLINE {  // all bits where it sees it
+      const uint32_t half = static_cast<uint32_t>(key < 32 ? sees : sees >> 32);
+      return static_cast<uint32_t>(static_cast<int32_t>(half << (31 - (key & 31))) >> 31);
+    };
+    auto and_mask = [&](float v, uint32_t m) IFX_INLINE {
+      return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & m);
+    };
+    // four scores of a half, scaled and masked
+    auto scale4 = [&](int sub, int r) IFX_INLINE {
+      const f32x4 k4 = *reinterpret_cast<const f32x4 *>(ks + at(sub, r));
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[sub][r] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < NS; ++i)
-        s[sub] = F16::mfma32(sk[(2 * i + h) * TK + 32 * sub + kn], qf[i], s[sub]);
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int at = 32 * sub + 16 * (r >> 3) + 8 * h + (r & 7);
-        const f32x4 k4 = ldg<f32x4>(ks + at), v4 = ldg<f32x4>(vs + at);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[sub][r + j] *= k4[j];
-          w[sub][r + j] = v4[j];
-          if (edge) {
-            const bool sees = tree ? nodes.sees(k0 + at + j) : line.sees(k0 + at + j);
-            s[sub][r + j] = sees ? s[sub][r + j] : -__builtin_inff();
-            w[sub][r + j] = sees ? v4[j] : 0.0f;
-          }
-          mt = fmaxf(mt, s[sub][r + j]), vt = fmaxf(vt, w[sub][r + j]);
+      for (int j = 0; j < 4; ++j) {
+        float x = s[sub][r + j] * k4[j];
+        if constexpr (edge) {
+          const uint32_t m = mask(at(sub, r) + j);
+          x = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, x) & m) | (0xFF800000u & ~m));
+          vt = fmaxf(vt, and_mask(vs[at(sub, r) + j], m));
         }
+        s[sub][r + j] = x;
       }
+      mt[0] = fmaxf(fmaxf(mt[0], s[sub][r]), s[sub][r + 1]);
+      mt[1] = fmaxf(fmaxf(mt[1], s[sub][r + 2]), s[sub][r + 3]);
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) frag(i);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 2 * NS; ++i) {
+      frag(i + kAhead);
+      s[i / NS] = F16::mfma32(f[i], qf[i % NS], i % NS ? s[i / NS] : none_yet);
+      // the first half's scores beside the second half's products
+      constexpr int kFrom = NS + NS / 4, kSteps = 2 * NS - kFrom;
+      if (i >= kFrom) {
+#pragma unroll
+        for (int r = (i - kFrom) * 4 / kSteps; r < (i - kFrom + 1) * 4 / kSteps; ++r) scale4(0, 4 * r);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
-    mt = halves_max(mt), vt = halves_max(vt);
-    if (__any(level.above(mt, vt, c))) {
-      const float less = level.raise(mt, vt, c);
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) scale4(1, r);
+    const float top = halves_max(fmaxf(mt[0], mt[1]));
+    if constexpr (edge) vt = halves_max(vt);
+    if (__any(level.above(top, vt, c))) {
+      const float less = level.raise(top, vt, c);
       l *= less;
 #pragma unroll
       for (int d = 0; d < ND; ++d)
@@ -177,43 +233,65 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void k_attn_tile_q8(con
         for (int r = 0; r < 16; ++r) acc[d][r] *= less;
     }
     u32x4 pf[4];
-    float sum = 0.0f;
+    float sum[2] = {l, 0.0f};
+    auto weigh4 = [&](int sub, int r) IFX_INLINE {
+      f32x4 v4 = *reinterpret_cast<const f32x4 *>(vs + at(sub, r));
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][r], c, -level.less));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][r + 1], c, -level.less));
-        sum += p0 + p1;
-        pf[2 * sub + (r >> 3)][(r & 7) >> 1] = F16::pack(p0 * w[sub][r], p1 * w[sub][r + 1]);
+      for (int j = 0; j < 4; j += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][r + j], c, -level.less));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][r + j + 1], c, -level.less));
+        sum[0] += p0;
+        sum[1] += p1;
+        if constexpr (edge) {
+          v4[j] = and_mask(v4[j], mask(at(sub, r) + j));
+          v4[j + 1] = and_mask(v4[j + 1], mask(at(sub, r) + j + 1));
+        }
+        pf[2 * sub + (r >> 3)][((r & 7) + j) >> 1] = F16::pack(p0 * v4[j], p1 * v4[j + 1]);
       }
-    l += sum;
+    };
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
+    for (int r = 0; r < 16; r += 4) weigh4(0, r);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int d = 0; d < ND; ++d) acc[d] = F16::mfma32(sv[(2 * ks + h) * D + 32 * d + n], pf[ks], acc[d]);
+    for (int i = 0; i < 2 * NS; ++i) {
+      frag(2 * NS + i + kAhead);
+      acc[i % ND] = F16::mfma32(f[2 * NS + i], pf[i / ND], acc[i % ND]);
+      if (i < NS) {  // the second half's weights beside the first half's products
+#pragma unroll
+        for (int r = i * 4 / NS; r < (i + 1) * 4 / NS; ++r) weigh4(1, 4 * r);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    l = sum[0] + sum[1];
   };
 
   if (zbeg < zend) {
     int entry = entry_of(zbeg);
-    load(zbeg, entry);
+    issue(zbeg, entry);
     entry = entry_of(zbeg + TK);
-    store(0);
-    int buf = 0;
-    for (int k0 = zbeg; k0 < zend; k0 += TK, buf ^= 1) {
-      __syncthreads();  // this stage is in LDS, and no wave reads the other one
-      const bool more = k0 + TK < zend;
-      if (more) {
-        load(k0 + TK, entry);
-        entry = entry_of(k0 + 2 * TK);
+    int k0 = zbeg;
+    auto stages = [&](int until, auto edge_c) IFX_INLINE {
+      for (; k0 < until; k0 += TK) {
+        wait_loads<0>();
+        group_barrier();  // the stage before is multiplied
+        convert();
+        __builtin_amdgcn_sched_barrier(0);  // the codes' places are read
+        if (k0 + TK < zend) {
+          issue(k0 + TK, entry);
+          entry = entry_of(k0 + 2 * TK);
+        }
+        group_barrier();  // this stage is in LDS
+        if (!idle) stage(k0, edge_c);
       }
-      if (!idle) {
-        if (k0 < full_a || k0 >= full_z)
-          stage(k0, buf, true);
-        else
-          stage(k0, buf, false);
-      }
-      if (more) store(buf ^ 1);
+    };
+    // stages that all rows of the workgroup see whole, between those that some
+    // see in part: where windows begin, and at the causal end
+    int until = a.window > 0 ? min(full_a, zend) : zbeg;
+    while (true) {
+      stages(until, std::true_type{});
+      if (k0 >= zend) break;
+      stages(min(full_z, zend), std::false_type{});
+      until = zend;
     }
   }
 
@@ -225,7 +303,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void k_attn_tile_q8(con
 namespace {
 template <int D>
 hipError_t launch_tile(const AttnArgs &a, int items, hipStream_t s) {
-  constexpr int stages = 2 * 2 * TK * D * 2 + 2 * 2 * TK * 4, requests = IFX_ATTN_MAX_BATCH * 8;
+  constexpr int stages = 2 * TK * D * 3 + 256 + kScales * 4, requests = IFX_ATTN_MAX_BATCH * 8;
   constexpr int bytes = stages > requests ? stages : requests;
   if constexpr (bytes > 65536 - 256) {
     static std::atomic<uint64_t> done{0};

@@ -187,6 +187,17 @@ struct Sight {
     const int node = key - ctx;
     return node < 0 || (node < 64 && (bits >> node & 1));
   }
+  // Bit i: whether it sees key k0 + i.
+  __device__ __forceinline__ uint64_t of_64(int k0) const {
+    if constexpr (TREE) {
+      const int d = ctx - k0;  // cached tokens among them
+      const uint64_t before = d >= 64 ? ~0ull : d > 0 ? (1ull << d) - 1 : 0;
+      return before | (d >= 64 || d <= -64 ? 0 : d >= 0 ? bits << d : bits >> -d);
+    }
+    const int from = lo - k0, to = hi - k0;
+    const uint64_t up = to < 0 ? 0 : to >= 63 ? ~0ull : (2ull << to) - 1;
+    return from <= 0 ? up : from >= 64 ? 0 : up & (~0ull << from);
+  }
   __device__ __forceinline__ bool nothing() const {
     if constexpr (!TREE) return hi < lo;
     return ctx <= 0 && (ctx <= -64 || bits >> -ctx == 0);
