@@ -26,20 +26,29 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kStep = kThreads * 4;  // values that a workgroup reads at a time
+constexpr int kAhead = 4;            // such reads on their way
+constexpr int kAtOnce = 4;           // and where the token is looked for
 
-// Four values of a row from `at` on as they lie in memory; 0 past its end.
+// Four values of a row from `at` on.
+template <int DT>
+__device__ __forceinline__ f32x4 read4(const void *row, int at) {
+  if constexpr (DT == IFX_ATTN_F32) return ldg<f32x4>(static_cast<const float *>(row) + at);
+  const u32x2 u = ldg<u32x2>(static_cast<const uint16_t *>(row) + at);
+  using T = Elem<DT == IFX_ATTN_F32 ? IFX_ATTN_F16 : DT>;
+  return f32x4{T::value(u.x & 0xFFFFu), T::value(u.x >> 16), T::value(u.y & 0xFFFFu), T::value(u.y >> 16)};
+}
 // Negative values and NaN are 0.
+__device__ __forceinline__ f32x4 clean(f32x4 v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = v[i] > 0.0f ? v[i] : 0.0f;
+  return v;
+}
+// The same, and 0 past the row's end.
 template <int DT>
 __device__ __forceinline__ f32x4 probs4(const void *row, int at, int V) {
   f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
   if (at + 3 < V) {
-    if constexpr (DT == IFX_ATTN_F32) {
-      v = ldg<f32x4>(static_cast<const float *>(row) + at);
-    } else {
-      const u32x2 u = ldg<u32x2>(static_cast<const uint16_t *>(row) + at);
-      using T = Elem<DT>;
-      v = {T::value(u.x & 0xFFFFu), T::value(u.x >> 16), T::value(u.y & 0xFFFFu), T::value(u.y >> 16)};
-    }
+    v = read4<DT>(row, at);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -50,9 +59,7 @@ __device__ __forceinline__ f32x4 probs4(const void *row, int at, int V) {
           v[i] = Elem<DT>::value(static_cast<const uint16_t *>(row)[at + i]);
       }
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = v[i] > 0.0f ? v[i] : 0.0f;
-  return v;
+  return clean(v);
 }
 template <int DT>
 __device__ __forceinline__ float prob(const void *row, int at) {
@@ -74,30 +81,33 @@ __device__ __forceinline__ double lane64(double v, int lane) {
   const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(b >> 32), lane);
   return __builtin_bit_cast(double, (static_cast<uint64_t>(hi) << 32) | lo);
 }
-__device__ __forceinline__ double up64(double v, int d) {
+// Inclusive sums over the lanes, as wave_scan's, of 64 bits.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double add_moved(double v) {
   const uint64_t b = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = __shfl_up(static_cast<int>(b), d), hi = __shfl_up(static_cast<int>(b >> 32), d);
-  return __builtin_bit_cast(double, (static_cast<uint64_t>(hi) << 32) | lo);
+  const uint32_t lo = dpp<CTRL, ROWS>(0u, static_cast<uint32_t>(b));
+  const uint32_t hi = dpp<CTRL, ROWS>(0u, static_cast<uint32_t>(b >> 32));
+  return v + __builtin_bit_cast(double, (static_cast<uint64_t>(hi) << 32) | lo);
 }
-// Inclusive sums over the lanes.
 __device__ __forceinline__ double scan64(double v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const double o = up64(v, d);
-    if (lane >= d) v += o;
-  }
-  return v;
+  v = add_moved<0x111, 0xF>(v);
+  v = add_moved<0x112, 0xF>(v);
+  v = add_moved<0x114, 0xF>(v);
+  v = add_moved<0x118, 0xF>(v);
+  v = add_moved<0x142, 0xA>(v);
+  return add_moved<0x143, 0xC>(v);
 }
 
 // The workgroup's threads in order hold weights of `mine` each: the first at
-// which their sum passes `target`, or else the last that holds any; -1 if none
-// does.  before: the sum of those before it.
+// which their sum passes share * total + target, or else the last that holds any;
+// -1 if none does.  before: the sum of those before it.
 struct Place {
   int thread;
+  bool passed;
   double before, total;
 };
-__device__ __forceinline__ Place find_place(double mine, double target, double *sums, int *found) {
+__device__ __forceinline__ Place find_place(double mine, double share, double target, double *sums,
+                                            int *found) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const double to = scan64(mine);
   if (lane == 63) sums[wave] = to;
@@ -109,6 +119,7 @@ __device__ __forceinline__ Place find_place(double mine, double target, double *
     if (w == wave) before = total;
     total += sums[w];
   }
+  target += share * total;
   const bool over = mine > 0.0 && before + to > target, any = mine > 0.0;
   const uint64_t o = __ballot(over), s = __ballot(any);
   if (lane == 0) {
@@ -116,17 +127,17 @@ __device__ __forceinline__ Place find_place(double mine, double target, double *
     if (s) atomicMax(&found[1], 64 * wave + 63 - __builtin_clzll(s));
   }
   __syncthreads();
-  const int at = found[0] != INT_MAX ? found[0] : found[1];
-  double less = before + (to - mine);
-  if (tid == at) sums[kThreads / 64] = less;
+  const bool passed = found[0] != INT_MAX;
+  const int at = passed ? found[0] : found[1];
+  if (tid == at) sums[kThreads / 64] = before + (to - mine);
   __syncthreads();
-  return {at, sums[kThreads / 64], total};
+  return {at, passed, sums[kThreads / 64], total};
 }
 
 }  // namespace
 
 template <int DT>
-__global__ __launch_bounds__(kThreads) void k_verify(const VerifyArgs a) {
+__global__ __launch_bounds__(kThreads, 4) void k_verify(const VerifyArgs a) {
   __shared__ double sums[kThreads / 64 + 1], whole[kThreads / 64];
   __shared__ int found[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -181,14 +192,15 @@ __global__ __launch_bounds__(kThreads) void k_verify(const VerifyArgs a) {
   }
 
   // ---- the chunk's share of what the next token is drawn from
+  const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
   const void *pr = row_of<DT>(a.target, a.target_stride, r0 + last);
   const void *qr = nullptr;
   if (a.drafter && children) qr = row_of<DT>(a.drafter, a.drafter_stride, r0 + last);
   const uint64_t gone = a.drafter ? 0 : children;
   // weights of four tokens from `at` on; near: the children with tokens of the chunk
-  auto weights = [&](f32x4 v, int at, uint64_t near, double (&w)[4]) __attribute__((always_inline)) {
+  auto weights = [&](f32x4 v, f32x4 q, int at, uint64_t near,
+                     double (&w)[4]) __attribute__((always_inline)) {
     if (qr) {
-      const f32x4 q = probs4<DT>(qr, at, a.V);
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = fmax(static_cast<double>(v[i]) - static_cast<double>(q[i]), 0.0);
       return;
@@ -208,14 +220,27 @@ __global__ __launch_bounds__(kThreads) void k_verify(const VerifyArgs a) {
     const int from = z * a.chunk, to = min(from + a.chunk, a.V);
     const uint64_t near = near_of(from);
     double sum = 0.0, all = 0.0;
-    for (int at = from + tid * 4; at < to; at += kStep) {
-      const f32x4 v = probs4<DT>(pr, at, a.V);
+    auto add = [&](f32x4 v, f32x4 q, int at) __attribute__((always_inline)) {
       double w[4];
-      weights(v, at, near, w);
+      weights(v, q, at, near, w);
       sum += (w[0] + w[1]) + (w[2] + w[3]);
       all += (static_cast<double>(v[0]) + static_cast<double>(v[1])) +
              (static_cast<double>(v[2]) + static_cast<double>(v[3]));
+    };
+    int at = from + tid * 4;
+    for (; at - tid * 4 + kAhead * kStep <= to; at += kAhead * kStep) {  // several reads on their way
+      f32x4 v[kAhead], q[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) v[i] = read4<DT>(pr, at + i * kStep);
+      if (qr) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) q[i] = read4<DT>(qr, at + i * kStep);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) add(clean(v[i]), qr ? clean(q[i]) : none, at + i * kStep);
     }
+    for (; at < to; at += kStep)
+      add(probs4<DT>(pr, at, a.V), qr ? probs4<DT>(qr, at, a.V) : none, at);
     sum = scan64(sum), all = scan64(all);
     if (lane == 63) {
       sums[wave] = sum;
@@ -243,54 +268,69 @@ __global__ __launch_bounds__(kThreads) void k_verify(const VerifyArgs a) {
   }
   const bool some = __syncthreads_or(sum > 0.0);
   const double mine = some ? sum : all;
-  // the total in the order of find_place's sums
-  double total = 0.0;
-  {
-    const double to = scan64(mine);
-    if (lane == 63) whole[wave] = to;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kThreads / 64; ++w) total += whole[w];
-  }
-  const double target = fmax(static_cast<double>(a.sample_u[b]), 0.0) * total;
-  const Place chunk = find_place(mine, target, sums, found);
+  const double share = fmax(static_cast<double>(a.sample_u[b]), 0.0);
+  const Place chunk = find_place(mine, share, 0.0, sums, found);
   int drawn = -1;
   if (chunk.thread >= 0) {
-    const int from = chunk.thread * a.chunk, each = a.chunk / kThreads;  // values of a thread
+    const int from = chunk.thread * a.chunk, to = min(from + a.chunk, a.V);
     const uint64_t near = some ? near_of(from) : 0;
     if (!some) qr = nullptr;
-    const int at0 = from + tid * each, at1 = min(at0 + each, a.V);
-    double own = 0.0;
-    for (int at = at0; at < at1; at += 4) {
-      double w[4];
-      weights(probs4<DT>(pr, at, a.V), at, near, w);
-      own += w[0];
-      own += w[1];
-      own += w[2];
-      own += w[3];
-    }
-    const double rest = fmax(target - chunk.before, 0.0);
-    const Place place = find_place(own, rest, sums, found);
-    if (tid == place.thread) {
-      double to = place.before;
-      int v = -1;
-      bool done = false;
-      for (int at = at0; at < at1; at += 4) {
-        double w[4];
-        weights(probs4<DT>(pr, at, a.V), at, near, w);
+    const double rest = fmax(share * chunk.total - chunk.before, 0.0);
+    double run = 0.0;
+    bool passed = false;
+    // 32 tokens a thread, one behind the other, read all at once
+    for (int base = from; base < to && !passed; base += kThreads * 4 * kAtOnce) {
+      const int at = base + tid * 4 * kAtOnce;
+      f32x4 v[kAtOnce], q[kAtOnce];
+      if (base + kThreads * 4 * kAtOnce <= a.V) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          to += w[i];
-          if (!done && w[i] > 0.0) {
-            v = at + i;
-            done = to > rest;
-          }
+        for (int i = 0; i < kAtOnce; ++i) v[i] = read4<DT>(pr, at + 4 * i);
+        if (qr) {
+#pragma unroll
+          for (int i = 0; i < kAtOnce; ++i) q[i] = read4<DT>(qr, at + 4 * i);
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) v[i] = clean(v[i]), q[i] = qr ? clean(q[i]) : none;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+          v[i] = probs4<DT>(pr, at + 4 * i, a.V);
+          q[i] = qr ? probs4<DT>(qr, at + 4 * i, a.V) : none;
         }
       }
-      found[0] = v;
+      double own = 0.0;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        double w[4];
+        weights(v[i], q[i], at + 4 * i, near, w);
+        own += (w[0] + w[1]) + (w[2] + w[3]);
+      }
+      const Place place = find_place(own, 0.0, rest - run, sums, found);
+      if (tid == place.thread) {
+        double sum = place.before;
+        int token = -1;
+        bool done = false;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+          double w[4];
+          weights(v[i], q[i], at + 4 * i, near, w);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            sum += w[j];
+            if (!done && w[j] > 0.0) {
+              token = at + 4 * i + j;
+              done = sum > rest - run;
+            }
+          }
+        }
+        found[0] = token;
+      }
+      __syncthreads();
+      // rounding apart the sum passes `rest` in one of them; else the last weight's
+      if (place.thread >= 0) drawn = found[0];
+      passed = place.passed;
+      run += place.total;
     }
-    __syncthreads();
-    if (place.thread >= 0) drawn = found[0];
   }
   if (wave == 0) {
     const int accepted = __popcll(walked) - 1;
