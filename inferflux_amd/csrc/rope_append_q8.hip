@@ -15,14 +15,6 @@ namespace ifx {
 
 namespace {
 
-// The smallest fp32 that is no less than a non-negative x.
-__device__ __forceinline__ float not_below(double x) {
-  const float f = static_cast<float>(x);
-  return static_cast<double>(f) < x
-             ? __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, f) + 1)
-             : f;
-}
-
 // Bits of the smallest bf16 s with 127 s >= top (15 significant bits: exact in
 // fp32); of NaN where top is not finite.
 __device__ __forceinline__ uint32_t scale_bits(float top) {
@@ -32,62 +24,74 @@ __device__ __forceinline__ uint32_t scale_bits(float top) {
   return s;
 }
 
-// max over the 16, 32 or 64 lanes that share a row; a NaN among them wins.
+// The largest over the 8, 16 or 32 lanes that share a row.
 template <int LANES>
-__device__ __forceinline__ float row_max(float v) {
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+  v = max(v, dpp<0xB1>(0u, v));   // quad_perm [1,0,3,2]
+  v = max(v, dpp<0x4E>(0u, v));   // quad_perm [2,3,0,1]
+  v = max(v, dpp<0x141>(0u, v));  // row_half_mirror
+  if constexpr (LANES > 8) v = max(v, dpp<0x140>(0u, v));  // row_mirror
+  if constexpr (LANES > 16) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 16)));
+  return v;
+}
+template <int LANES>
+__device__ __forceinline__ double row_max(double v) {
 #pragma unroll
-  for (int d = 1; d < LANES; d <<= 1) {
-    const float o = __shfl_xor(v, d);
-    v = o > v || o != o ? o : v;
-  }
+  for (int d = 1; d < LANES; d <<= 1) v = fmax(v, __shfl_xor(v, d));
   return v;
 }
 
+// Scales below are divided by in fp64: their reciprocals pass fp32's range.
+constexpr float kLeast = 0x1p-100f;
+
 }  // namespace
 
-// A workgroup takes NTOK consecutive tokens, and of them a part: K and V
-// (blockIdx.y 0) or some of Q's units, pieces of 8 values (and their partners'
-// where pairs lie half a rotation apart).  A row of K or V is shared by LANES
-// lanes, four values each.
+// A workgroup takes NTOK consecutive tokens, and of them a part: K (blockIdx.y
+// 0), V (1) or some of Q's units, pieces of 8 values (and their partners' where
+// pairs lie half a rotation apart).  A row of K or V is shared by LANES lanes, a
+// piece of 8 values each.
 template <int DT, int SRC, int LANES, int NTOK>
 __global__ __launch_bounds__(256) void k_rope_append_q8(const AppendQ8Args args) {
   using T = Elem<DT>;
   const AppendArgs &a = args.a;
+  // cosine and sine: [token][i % 8][i / 8], so that neighbouring pieces' are neighbours
   __shared__ union {
     float2 q[NTOK * 128];
     double2 k[NTOK * 128];
   } turn;
   __shared__ int slot_of[NTOK];
   const int tid = threadIdx.x, t0 = blockIdx.x * NTOK;
-  const int half = a.rot_dim >> 1, pieces = a.D >> 3, sh = a.page_shift, P = 1 << sh;
-  const bool q_part = blockIdx.y > 0;
+  const int half = a.rot_dim >> 1, angles = half >> 3;  // half: a multiple of 8
+  const int pieces = a.D >> 3, sh = a.page_shift, P = 1 << sh;
+  const bool q_part = blockIdx.y > 1, is_v = blockIdx.y == 1;
   if (tid < NTOK) {
     const int t = t0 + tid, s = t < a.T ? a.slots[t] : -1;
     slot_of[tid] = static_cast<uint32_t>(s) < static_cast<uint32_t>(a.num_slots) ? s : -1;
   }
-  for (int i = tid; i < NTOK * half; i += 256) {
-    const int t = t0 + i / half;
+  for (int i = tid; i < NTOK * half && !is_v; i += 256) {
+    const int tok = i / half, t = t0 + tok, f = i - tok * half;
     if (t < a.T) {
-      const double turns = a.positions[t] * a.inv_freq[i % half] * 0.15915494309189533577;
+      const double turns = a.positions[t] * a.inv_freq[f] * 0.15915494309189533577;
       const double x = 2.0 * (turns - rint(turns));
+      const int to = tok * half + (f & 7) * angles + (f >> 3);
       if (q_part) {
         float sn, cs;
         sincospif(static_cast<float>(x), &sn, &cs);
-        turn.q[i] = make_float2(cs, sn);
+        turn.q[to] = make_float2(cs, sn);
       } else {
         double sn, cs;
         sincospi(x, &sn, &cs);
-        turn.k[i] = make_double2(cs, sn);
+        turn.k[to] = make_double2(cs, sn);
       }
     }
   }
   __syncthreads();
 
   if (q_part) {
-    const int pairs = a.interleaved ? 0 : half >> 3, per_head = pieces - pairs;
-    const int units = NTOK * a.Hq * per_head, parts = gridDim.y - 1;
+    const int pairs = a.interleaved ? 0 : angles, per_head = pieces - pairs;
+    const int units = NTOK * a.Hq * per_head, parts = gridDim.y - 2;
     const int share = (units + parts - 1) / parts;
-    const int u0 = (blockIdx.y - 1) * share, u1 = min(u0 + share, units);
+    const int u0 = (blockIdx.y - 2) * share, u1 = min(u0 + share, units);
     const float per_head_inv = 1.0f / per_head, heads_inv = 1.0f / a.Hq;
     for (int u = u0 + tid; u < u1; u += 256) {
       const int w = quotient(u, per_head, per_head_inv), c = u - w * per_head;
@@ -108,7 +112,7 @@ __global__ __launch_bounds__(256) void k_rope_append_q8(const AppendQ8Args args)
         hi.values(y);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float2 r = tw[pc * 8 + i];
+          const float2 r = tw[i * angles + pc];
           const float p = x[i], s = y[i];
           x[i] = p * r.x - s * r.y;
           y[i] = s * r.x + p * r.y;
@@ -118,7 +122,7 @@ __global__ __launch_bounds__(256) void k_rope_append_q8(const AppendQ8Args args)
       } else if (pc * 8 < a.rot_dim) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float2 r = tw[pc * 4 + i];
+          const float2 r = tw[((pc * 4 + i) & 7) * angles + (pc >> 1)];
           const float p = x[2 * i], s = x[2 * i + 1];
           x[2 * i] = p * r.x - s * r.y;
           x[2 * i + 1] = s * r.x + p * r.y;
@@ -130,72 +134,103 @@ __global__ __launch_bounds__(256) void k_rope_append_q8(const AppendQ8Args args)
     return;
   }
 
-  // K and V: row = (token, head, K or V), tokens fastest.  All lanes take as
-  // many turns, as rows are reduced across them.
-  const int sub = tid & (LANES - 1), dim = sub * 4, rows = NTOK * a.Hkv * 2;
-  for (int r0 = 0; r0 < rows; r0 += 256 / LANES) {
-    const int r = r0 + tid / LANES, t = r % NTOK, hv = r / NTOK, head = hv >> 1;
-    const bool is_v = hv & 1;
-    const int slot = r < rows ? slot_of[t] : -1;
-    const bool live = slot >= 0 && dim < a.D;
-    double y[4] = {0.0, 0.0, 0.0, 0.0};
-    if (live) {
-      const int64_t row = (t0 + t) * (is_v ? a.v_stride : a.k_stride) + static_cast<int64_t>(head) * a.D;
-      const void *src = is_v ? a.v : a.k;
-      const float2 p = load2<SRC>(src, row + dim), q = load2<SRC>(src, row + dim + 2);
-      const float x[4] = {p.x, p.y, q.x, q.y};
+  // K or V: row = (token, head), tokens fastest.  All lanes take as many turns, as
+  // rows are reduced across them.
+  constexpr int kRows = 256 / LANES;
+  const int c = tid & (LANES - 1), rows = NTOK * a.Hkv;
+  const void *src = is_v ? a.v : a.k;
+  const int64_t stride = is_v ? a.v_stride : a.k_stride;
+  const bool turned = !is_v && c * 8 < a.rot_dim, paired = turned && !a.interleaved;
+  const bool first = c < angles;  // of its pair
+  const int other = first ? c + angles : c - angles;
+  for (int r = tid / LANES; r - tid / LANES < rows; r += kRows) {
+    const int t = r % NTOK, head = r / NTOK;
+    const int slot = r < rows && c < pieces ? slot_of[t] : -1;
+    Raw8<SRC> lo = {}, hi = {};
+    if (slot >= 0) {
+      const int64_t row = (t0 + t) * stride + static_cast<int64_t>(head) * a.D;
+      lo.load(src, row + c * 8);
+      if (paired) hi.load(src, row + other * 8);
+    }
+    float v[8];
+    double y[8];  // of K
+    lo.values(v);
+    if (!is_v) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = x[i];
-      if (!is_v && dim < a.rot_dim) {
-        const double2 *tw = turn.k + t * half;
-        if (a.interleaved) {
+      for (int i = 0; i < 8; ++i) y[i] = v[i];
+      const double2 *tw = turn.k + t * half;
+      if (paired) {
+        float z[8];
+        hi.values(z);
 #pragma unroll
-          for (int i = 0; i < 4; i += 2) {
-            const double2 w = tw[(dim + i) >> 1];
-            y[i] = x[i] * w.x - x[i + 1] * w.y;
-            y[i + 1] = x[i + 1] * w.x + x[i] * w.y;
-          }
-        } else {
-          const bool first = dim < half;  // of its pair
-          const int other = first ? dim + half : dim - half;
-          const float2 u = load2<SRC>(src, row + other), v = load2<SRC>(src, row + other + 2);
-          const float z[4] = {u.x, u.y, v.x, v.y};
+        for (int i = 0; i < 8; ++i) {
+          const double2 w = tw[i * angles + (first ? c : other)];
+          y[i] = y[i] * w.x + (first ? -w.y : w.y) * static_cast<double>(z[i]);
+        }
+      } else if (turned) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const double2 w = tw[(first ? dim : other) + i];
-            y[i] = first ? x[i] * w.x - z[i] * w.y : x[i] * w.x + z[i] * w.y;
-          }
+        for (int i = 0; i < 8; i += 2) {
+          const double2 w = tw[((c * 4 + (i >> 1)) & 7) * angles + (c >> 1)];
+          const double p = y[i], q = y[i + 1];
+          y[i] = p * w.x - q * w.y;
+          y[i + 1] = q * w.x + p * w.y;
         }
       }
-    }
-    float top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float m = not_below(fabs(y[i]));
-      top = m > top || m != m ? m : top;
+      for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(y[i]);
     }
-    top = row_max<LANES>(top);
-    const uint32_t bits = scale_bits(top);
-    const double s = __builtin_bit_cast(float, bits << 16);
-    uint32_t code[4];
+    uint32_t most = 0;  // as bits: infinities and, above them, NaN win
 #pragma unroll
-    for (int i = 0; i < 4; ++i)  // also where the scale is 0 or NaN
-      code[i] = s > 0.0 ? static_cast<uint32_t>(static_cast<int>(rint(y[i] / s))) & 0xFFu : 0u;
-    if (!live) continue;
+    for (int i = 0; i < 8; ++i) most = max(most, __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu);
+    const float top = __builtin_bit_cast(float, row_max<LANES>(most));
+    uint32_t bits = scale_bits(top);
+    float s = __builtin_bit_cast(float, bits << 16);
+    if (!is_v && __any(127.0f * s == top)) {  // the value itself may be above that
+      double exact = 0.0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) exact = fmax(exact, fabs(y[i]));
+      exact = row_max<LANES>(exact);
+      if (127.0 * static_cast<double>(s) < exact && bits < 0x7F80u) s = __builtin_bit_cast(float, ++bits << 16);
+    }
+    const float inv = __builtin_amdgcn_rcpf(s);
+    int code[8];
+    bool near = s < kLeast;  // whether a value may lie on the other side of a border
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float q = v[i] * inv, n = rintf(q);
+      code[i] = static_cast<int>(n);
+      if (is_v) {
+        // what is left of v is exact in fp32: n s has 15 bits
+        const float left = fabsf(__builtin_fmaf(-n, s, v[i])), border = 0.5f * s;
+        if (left > border || (left == border && (code[i] & 1))) code[i] += v[i] > n * s ? 1 : -1;
+      } else {
+        near |= fabsf(q - n) > 0.4999f;
+      }
+    }
+    if (__any(near)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        code[i] = static_cast<int>(rint((is_v ? static_cast<double>(v[i]) : y[i]) / static_cast<double>(s)));
+    }
+    if (slot < 0) continue;
+    const bool some = s > 0.0f;  // not a row of zeros, nor one that reads as NaN
     const int64_t block = static_cast<int64_t>(slot >> sh) * a.Hkv + head;
     const int tok = slot & (P - 1);
-    if (sub == 0)
+    if (c == 0)
       reinterpret_cast<uint16_t *>(args.scales)[((block << sh) + tok) * 2 + is_v] =
           static_cast<uint16_t>(bits);
     if (is_v) {
-      uint8_t *o = static_cast<uint8_t *>(a.v_cache) +
-                   ((block << sh) + (tok & ~15)) * a.D + dim * 16 + (tok & 15);
+      uint8_t *o = static_cast<uint8_t *>(a.v_cache) + ((block << sh) + (tok & ~15)) * a.D + c * 128 +
+                   (tok & 15);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i * 16] = static_cast<uint8_t>(code[i]);
+      for (int i = 0; i < 8; ++i) o[i * 16] = static_cast<uint8_t>(some ? code[i] : 0);
     } else {
-      uint8_t *o = static_cast<uint8_t *>(a.k_cache) + ((block * (a.D >> 4) + (dim >> 4)) << sh) * 16 +
-                   tok * 16 + (dim & 15);
-      *reinterpret_cast<uint32_t *>(o) = code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24;
+      uint8_t *o = static_cast<uint8_t *>(a.k_cache) + ((block * (a.D >> 4) + (c >> 1)) << sh) * 16 +
+                   tok * 16 + (c & 1) * 8;
+      u32x2 w = {0u, 0u};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i >> 2] |= static_cast<uint32_t>(code[i] & 0xFF) << (8 * (i & 3));
+      *reinterpret_cast<u32x2 *>(o) = some ? w : u32x2{0u, 0u};
     }
   }
 }
@@ -242,13 +277,17 @@ __global__ __launch_bounds__(256) void k_read_rows_q8(const ReadArgs a) {
 namespace {
 template <int DT, int SRC, int LANES>
 void launch(const AppendQ8Args &a, hipStream_t s) {
-  IFX_LAUNCH(k_rope_append_q8, (DT, SRC, LANES, 1), dim3(a.a.T, 2), dim3(256), 0, s, a);
+  if (a.a.T >= 2048) {
+    IFX_LAUNCH(k_rope_append_q8, (DT, SRC, LANES, 8), dim3((a.a.T + 7) / 8, 7), dim3(256), 0, s, a);
+  } else {
+    IFX_LAUNCH(k_rope_append_q8, (DT, SRC, LANES, 1), dim3(a.a.T, 3), dim3(256), 0, s, a);
+  }
 }
 template <int DT, int SRC>
 void launch(const AppendQ8Args &a, hipStream_t s) {
-  if (a.a.D <= 64) return launch<DT, SRC, 16>(a, s);
-  if (a.a.D <= 128) return launch<DT, SRC, 32>(a, s);
-  return launch<DT, SRC, 64>(a, s);
+  if (a.a.D <= 64) return launch<DT, SRC, 8>(a, s);
+  if (a.a.D <= 128) return launch<DT, SRC, 16>(a, s);
+  return launch<DT, SRC, 32>(a, s);
 }
 template <int DT>
 void launch(const AppendQ8Args &a, int src_dtype, hipStream_t s) {
