@@ -41,6 +41,43 @@ __device__ __forceinline__ double row_max(double v) {
   return v;
 }
 
+// A dim's codes of N tokens to their slots: those that follow each other within a
+// piece together, in stores as wide as their places are aligned.  The slots are
+// the same for all lanes, and so are the branches.
+template <int N>
+__device__ __forceinline__ void store_tokens(uint8_t *dims, int D, int Hkv, int head, int sh,
+                                             const int *slot_of, const uint8_t *codes) {
+  const uint64_t all = *reinterpret_cast<const uint64_t *>(codes);
+  for (int t = 0; t < N;) {
+    const int slot = __builtin_amdgcn_readfirstlane(slot_of[t]);
+    if (slot < 0) {
+      ++t;
+      continue;
+    }
+    const int tok = slot & ((1 << sh) - 1);
+    uint8_t *o = dims + (((static_cast<int64_t>(slot >> sh) * Hkv + head) << sh) + (tok & ~15)) * D + (tok & 15);
+    auto follow = [&](int n) {  // whether n tokens from t on lie there, one behind the other
+      bool yes = t + n <= N && (slot & (n - 1)) == 0;
+      for (int i = 1; i < n && yes; ++i) yes = __builtin_amdgcn_readfirstlane(slot_of[t + i]) == slot + i;
+      return yes;
+    };
+    const uint64_t v = all >> (8 * t);
+    if (follow(8)) {
+      *reinterpret_cast<uint64_t *>(o) = v;
+      t += 8;
+    } else if (follow(4)) {
+      *reinterpret_cast<uint32_t *>(o) = static_cast<uint32_t>(v);
+      t += 4;
+    } else if (follow(2)) {
+      *reinterpret_cast<uint16_t *>(o) = static_cast<uint16_t>(v);
+      t += 2;
+    } else {
+      *o = static_cast<uint8_t>(v);
+      ++t;
+    }
+  }
+}
+
 // Scales below are divided by in fp64: their reciprocals pass fp32's range.
 constexpr float kLeast = 0x1p-100f;
 
@@ -136,7 +173,8 @@ __global__ __launch_bounds__(256) void k_rope_append_q8(const AppendQ8Args args)
 
   // K or V: row = (token, head), tokens fastest.  All lanes take as many turns, as
   // rows are reduced across them.
-  constexpr int kRows = 256 / LANES;
+  constexpr int kRows = 256 / LANES, kHeads = NTOK > 1 ? kRows / NTOK : 1;
+  uint8_t *by_dim = reinterpret_cast<uint8_t *>(&turn);  // V: [head][dim][token], of kHeads
   const int c = tid & (LANES - 1), rows = NTOK * a.Hkv;
   const void *src = is_v ? a.v : a.k;
   const int64_t stride = is_v ? a.v_stride : a.k_stride;
@@ -212,8 +250,28 @@ __global__ __launch_bounds__(256) void k_rope_append_q8(const AppendQ8Args args)
       for (int i = 0; i < 8; ++i)
         code[i] = static_cast<int>(rint((is_v ? static_cast<double>(v[i]) : y[i]) / static_cast<double>(s)));
     }
-    if (slot < 0) continue;
     const bool some = s > 0.0f;  // not a row of zeros, nor one that reads as NaN
+    if (NTOK > 1 && is_v) {
+      // by way of LDS, so that a lane has a dim's codes of all tokens
+      uint8_t *mine = by_dim + (head % kHeads) * LANES * 8 * NTOK + c * 8 * NTOK + t;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mine[i * NTOK] = static_cast<uint8_t>(some ? code[i] : 0);
+      if (slot >= 0 && c == 0)
+        reinterpret_cast<uint16_t *>(args.scales)[
+            (((static_cast<int64_t>(slot >> sh) * a.Hkv + head) << sh) + (slot & (P - 1))) * 2 + 1] =
+            static_cast<uint16_t>(bits);
+      __syncthreads();
+      const int head0 = (r - tid / LANES) / NTOK;
+      for (int i = tid; i < kHeads * LANES * 8; i += 256) {
+        const int h = i / (LANES * 8), dim = i - h * LANES * 8;
+        if (head0 + h >= a.Hkv || dim >= a.D) continue;
+        store_tokens<NTOK>(static_cast<uint8_t *>(a.v_cache) + dim * 16, a.D, a.Hkv, head0 + h, sh,
+                           slot_of, by_dim + i * NTOK);
+      }
+      __syncthreads();
+      continue;
+    }
+    if (slot < 0) continue;
     const int64_t block = static_cast<int64_t>(slot >> sh) * a.Hkv + head;
     const int tok = slot & (P - 1);
     if (c == 0)
@@ -235,17 +293,22 @@ __global__ __launch_bounds__(256) void k_rope_append_q8(const AppendQ8Args args)
   }
 }
 
-// A thread reads 16 values of a row: K's as one piece, V's a byte each.
+// A wave reads 16 tokens' K or V, 64 values of each: neighbouring lanes four
+// pieces of 16 values, so that a row is written in whole lines, and four lanes
+// further the next token, so that its codes, in V bytes of one piece, are near.
 template <int OUT>
 __global__ __launch_bounds__(256) void k_read_rows_q8(const ReadArgs a) {
-  const int units = a.Hkv * (a.D >> 4);  // of a token's K or V
-  const int sh = a.page_shift, P = 1 << sh;
-  for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < static_cast<int64_t>(a.N) * units * 2;
-       i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int u = static_cast<int>(i % units);
-    const int64_t w = i / units;
+  const int row_pieces = a.Hkv * (a.D >> 4), groups = (row_pieces + 3) >> 2;
+  const int sh = a.page_shift, P = 1 << sh, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t units = static_cast<int64_t>((a.N + 15) >> 4) * groups * 2;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + wave; i < units; i += static_cast<int64_t>(gridDim.x) * 4) {
+    const int64_t w = i / groups;
+    const int u = static_cast<int>(i - w * groups) * 4 + (lane & 3);  // piece of the row
     const bool is_v = w & 1;
-    const int row = static_cast<int>(w >> 1), head = u / (a.D >> 4), c = u - head * (a.D >> 4);
+    const int row = static_cast<int>(w >> 1) * 16 + (lane >> 2);
+    if (row >= a.N || u >= row_pieces) continue;
+    const int head = u / (a.D >> 4), c = u - head * (a.D >> 4);
     const int slot = a.slots[row];
     float x[16] = {};
     if (static_cast<uint32_t>(slot) < static_cast<uint32_t>(a.num_slots)) {
@@ -268,9 +331,18 @@ __global__ __launch_bounds__(256) void k_read_rows_q8(const ReadArgs a) {
     char *o = static_cast<char *>(is_v ? a.v_out : a.k_out) +
               (row * (is_v ? a.v_stride : a.k_stride) + static_cast<int64_t>(u) * 16) *
                   (OUT == IFX_ATTN_F32 ? 4 : 2);
+    if constexpr (OUT == IFX_ATTN_F32) {
 #pragma unroll
-    for (int e = 0; e < 16; e += 4)
-      store4(o, OUT, e, f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]});
+      for (int e = 0; e < 16; e += 4) store4(o, OUT, e, f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]});
+    } else {
+      using T = Elem<OUT == IFX_ATTN_F32 ? IFX_ATTN_F16 : OUT>;
+#pragma unroll
+      for (int e = 0; e < 16; e += 8) {
+        const u32x4 w8 = {T::pack(x[e], x[e + 1]), T::pack(x[e + 2], x[e + 3]),
+                          T::pack(x[e + 4], x[e + 5]), T::pack(x[e + 6], x[e + 7])};
+        __builtin_memcpy(o + e * 2, &w8, 16);
+      }
+    }
   }
 }
 
@@ -308,8 +380,8 @@ hipError_t launch_rope_append_q8(const AppendQ8Args &a, int src_dtype, int q_dty
 }
 
 hipError_t launch_read_rows_q8(const ReadArgs &a, int out_dtype, hipStream_t s) {
-  const int64_t units = static_cast<int64_t>(a.N) * a.Hkv * (a.D >> 4) * 2;
-  const int64_t need = (units + 255) / 256;
+  const int64_t units = static_cast<int64_t>((a.N + 15) >> 4) * ((a.Hkv * (a.D >> 4) + 3) >> 2) * 2;
+  const int64_t need = (units + 3) / 4;  // a wave each
   const dim3 grid(static_cast<uint32_t>(need < 16384 ? need : 16384));
   if (out_dtype == IFX_ATTN_F32)
     IFX_LAUNCH(k_read_rows_q8, (IFX_ATTN_F32), grid, dim3(256), 0, s, a);
