@@ -48,7 +48,8 @@ int ifx_read_rows_q8(const void *k_cache, const void *v_cache, const void *scale
 /* Attention of the new tokens over the 8-bit cache: as ifx_attn_paged on the
  * values that the cache stands for, q of q_dtype (fp16 or bf16).  With masks
  * [T], those of ifx_plan_tree (ifx_drafts.h), as ifx_attn_tree instead; window
- * must be 0 and max_q at most IFX_TREE_MAX_NODES then.
+ * must be 0 and max_q at most IFX_TREE_MAX_NODES then.  workspace: as
+ * ifx_attn_paged's, of ifx_attn_paged_workspace_bytes.
  *
  * Codes are exact in the products, which are summed in fp32.  Q of bf16 is
  * taken to fp16 with a power of two for each row, which loses nothing of what is

@@ -42,7 +42,10 @@ int ifx_plan_tree(const int32_t *parents, const int32_t *cu_q, const int32_t *kv
  * ifx_attn_paged without a window, but that row i of a request of n sees the
  * keys before its n new ones, and of these token kv_len - n + j where bit j of
  * masks[row] is set (j < n; the node itself too only where its bit is).
- * 1 <= max_q <= IFX_TREE_MAX_NODES; workspace: that of ifx_attn_paged. */
+ * 1 <= max_q <= IFX_TREE_MAX_NODES.  workspace: as ifx_attn_paged's, of
+ * ifx_attn_tree_workspace_bytes; one may serve both. */
+int64_t ifx_attn_tree_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int max_q,
+                                      int max_kv);
 int ifx_attn_tree(const void *q, int64_t q_stride, int dtype, const void *k_cache,
                   const void *v_cache, int64_t num_pages, int page_size,
                   const int32_t *block_table, int table_width, const int32_t *cu_q,

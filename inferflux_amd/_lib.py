@@ -115,6 +115,7 @@ SIGNATURES.update({
     "ifx_plan_tree": ([_vp] * 3 + [_i32, _i32] + [_vp] * 3, _i32),
     "ifx_attn_tree": ([_vp, _i64, _i32, _vp, _vp, _i64, _i32, _vp, _i32, _vp, _vp, _vp] + [_i32] * 7 +
                       [ctypes.c_float, _vp, _i64, _i32, _vp, _i64, _vp], _i32),
+    "ifx_attn_tree_workspace_bytes": ([_i32] * 7, _i64),
     "ifx_verify_workspace_bytes": ([_i32, _i32], _i64),
     "ifx_verify": ([_vp] * 3 + [_i32] * 3 + [_vp, _i64, _vp, _i64, _i32, _i32] + [_vp] * 6 +
                    [_i64, _vp], _i32),

@@ -102,11 +102,21 @@ struct PagedPlan {
 // with 1536, 153 with 2048.
 //
 // Fewer where the split sums would not fit the largest workspace.
-PagedPlan plan_paged(int B, int T, int Hq, int Hkv, int D, int max_q, int max_kv) {
+//
+// tree: drafts over the 16-bit cache, as many for every request.  From 17 rows on
+// attn_tile takes them, but for one or two requests of up to 24.  us with
+// attn_rows / attn_tile, with the plan's launch:
+//   16 / 2 heads of 128, 24 rows of 3000 keys  1 request 19.9/21.8, 4 21.3/22.8,
+//     8 25.4/23.1; 32 of 1000 to 9000 51/42.6
+//   40 / 8 heads, 20 rows  1 20.1/22.1, 2 24.4/23.0, 8 42.6/37.4, 32 114/112
+//     30 rows              1 23.1/22.3, 2 28.5/23.0, 8 48.1/36.9, 32 122/113
+// attn_rows_q8 is faster up to its 32 rows (30 rows of 40 / 8 heads: 1 request
+// 23.4/33.4, 8 38.6/39.5, 32 83/128).
+PagedPlan plan_paged(int B, int T, int Hq, int Hkv, int D, int max_q, int max_kv, bool tree) {
   PagedPlan p{};
   const int G = Hq / Hkv;
   const int64_t rows = static_cast<int64_t>(max_q) * G;
-  p.rows = rows <= kRowsMax;
+  p.rows = rows <= (!tree ? kRowsMax : B * Hkv <= 8 ? 24 : 16);
   // row tiles, stages of the longest request that a split must have, bytes of a slot
   const int64_t tiles = p.rows ? B : static_cast<int64_t>(T) * G / attn_tile_rows(D) + B;
   const int unit = p.rows ? kRowKeys : attn_tile_min_keys();
@@ -150,7 +160,7 @@ int attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cache,
     return IFX_NULL_POINTER;
   if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15)
     return IFX_BAD_GEOMETRY;
-  const PagedPlan p = plan_paged(B, T, Hq, Hkv, D, max_q, max_kv);
+  const PagedPlan p = plan_paged(B, T, Hq, Hkv, D, max_q, max_kv, masks && !scales);
   if (p.bytes) {
     if (!workspace) return IFX_NULL_POINTER;
     if (workspace_bytes < p.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255))
@@ -264,7 +274,7 @@ int ifx_read_rows_q8(const void *k_cache, const void *v_cache, const void *scale
 int64_t ifx_attn_paged_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int max_q,
                                        int max_kv) {
   if (!heads_ok(B, T, Hq, Hkv, D) || max_q < 1 || max_kv < 1) return 0;
-  return plan_paged(B, T, Hq, Hkv, D, max_q, max_kv).bytes;
+  return plan_paged(B, T, Hq, Hkv, D, max_q, max_kv, false).bytes;
 }
 
 int ifx_attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cache,
@@ -276,6 +286,12 @@ int ifx_attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cac
   return attn_paged(q, q_stride, dtype, k_cache, v_cache, nullptr, num_pages, page_size, block_table,
                     table_width, cu_q, kv_len, nullptr, B, T, Hq, Hkv, D, max_q, max_kv, scale,
                     window, out, out_stride, out_dtype, workspace, workspace_bytes, stream);
+}
+
+int64_t ifx_attn_tree_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int max_q,
+                                      int max_kv) {
+  if (!heads_ok(B, T, Hq, Hkv, D) || max_q < 1 || max_q > IFX_TREE_MAX_NODES || max_kv < 1) return 0;
+  return plan_paged(B, T, Hq, Hkv, D, max_q, max_kv, true).bytes;
 }
 
 int ifx_attn_tree(const void *q, int64_t q_stride, int dtype, const void *k_cache,

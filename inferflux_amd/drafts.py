@@ -105,6 +105,14 @@ def tree_attention(q, k_cache, v_cache, block_table, cu_q, kv_len, masks, max_q,
     return out
 
 
+def tree_workspace_bytes(B, T, Hq, Hkv, head_dim, max_q, max_kv):
+    """Bytes of workspace that tree_attention needs for this shape (0: none;
+    attention.WORKSPACE_BYTES is enough for all)."""
+    return int(_lib.load().ifx_attn_tree_workspace_bytes(
+        _count(B, "B"), _count(T, "T"), _count(Hq, "Hq"), _count(Hkv, "Hkv"),
+        _count(head_dim, "head_dim"), _count(max_q, "max_q"), _count(max_kv, "max_kv")))
+
+
 def _workspace(t, device):
     if t is None:
         return None, 0

@@ -23,7 +23,7 @@ def test_exports_what_the_header_declares(lib):
     from inferflux_amd import _lib
     text = open(os.path.join(ROOT, "include", "ifx_drafts.h")).read()
     syms = set(re.findall(r"^\s*(?:int|int64_t)\s+(ifx_\w+)\s*\(", text, re.M))
-    assert syms == {"ifx_plan_tree", "ifx_attn_tree", "ifx_verify_workspace_bytes", "ifx_verify",
+    assert syms == {"ifx_plan_tree", "ifx_attn_tree", "ifx_attn_tree_workspace_bytes", "ifx_verify_workspace_bytes", "ifx_verify",
                     "ifx_keep_path", "ifx_plan_kept"}
     assert syms <= set(_lib.SIGNATURES)
     out = subprocess.run(["nm", "-D", "--defined-only", _lib.LIB_PATH], capture_output=True,
@@ -58,7 +58,9 @@ ATTN = dict(q=F, qs=2048, dt=1, kc=F, vc=F, pages=100, page=64, table=F, width=5
 
 
 @pytest.mark.parametrize("change,want", [
-    ({}, "k_attn_rows<1,128,1>"), (dict(max_q=5), "k_attn_tile<1,128,1,1>"), (dict(dt=2), "k_attn_rows<2,128,1>"),
+    ({}, "k_attn_tile<1,128,1,1>"), (dict(max_q=2), "k_attn_rows<1,128,1>"), (dict(max_q=3), "k_attn_rows<1,128,1>"),
+    (dict(max_q=3, B=5), "k_attn_tile<1,128,1,1>"), (dict(max_q=2, B=5), "k_attn_rows<1,128,1>"),
+    (dict(dt=2, max_q=1), "k_attn_rows<2,128,1>"), (dict(dt=2), "k_attn_tile<2,128,1,1>"),
     (dict(max_q=64), "k_attn_tile<1,128,1,1>"), (dict(max_q=65), GEOM), (dict(max_q=0), GEOM),
     (dict(masks=None), NULL), (dict(T=0, masks=None), OK), (dict(dt=0), TYPE), (dict(odt=3), TYPE),
     (dict(page=24), GEOM), (dict(D=80), GEOM), (dict(Hq=15), GEOM), (dict(scale=0.0), GEOM),
@@ -67,6 +69,20 @@ def test_attn_tree_kernels_and_refusals(lib, change, want):
     with dry(lib) as d:
         rc = lib.ifx_attn_tree(*{**ATTN, **change}.values())
     assert (d.text, rc) == (want, OK) if isinstance(want, str) else (rc, d.text) == (want, "")
+
+
+@pytest.mark.parametrize("B,T,Hq,Hkv,D,max_q,max_kv", [
+    (1, 1, 16, 2, 128, 1, 3000), (4, 24, 16, 2, 128, 6, 3000), (16, 96, 40, 8, 128, 6, 9000), (1, 61, 16, 2, 128, 61, 3000),
+    (4096, 4096, 8, 8, 256, 64, 1 << 20), (1, 64, 64, 1, 256, 64, 1 << 30)])
+def test_attn_tree_workspace(lib, B, T, Hq, Hkv, D, max_q, max_kv):
+    """As many bytes as it says are enough, one less is not."""
+    n = lib.ifx_attn_tree_workspace_bytes(B, T, Hq, Hkv, D, max_q, max_kv)
+    assert 0 < n <= 64 << 20
+    change = dict(B=B, T=T, Hq=Hq, Hkv=Hkv, D=D, max_q=max_q, max_kv=max_kv, qs=Hq * D, os=Hq * D)
+    for have, want in ((n, OK), (n - 1, GEOM)):
+        with dry(lib) as d:
+            assert lib.ifx_attn_tree(*{**ATTN, **change, "wn": have}.values()) == want
+        assert d.text.startswith("k_attn_") == (want == OK)
 
 
 VERIFY = dict(tokens=ptr(0), parents=ptr(1), cu=ptr(2), B=4, T=32, max_q=8, p=ptr(3), ps=1000, q=None, qs=0,
