@@ -49,7 +49,7 @@ int ifx_read_rows_q8(const void *k_cache, const void *v_cache, const void *scale
  * values that the cache stands for, q of q_dtype (fp16 or bf16).  With masks
  * [T], those of ifx_plan_tree (ifx_drafts.h), as ifx_attn_tree instead; window
  * must be 0 and max_q at most IFX_TREE_MAX_NODES then.  workspace: as
- * ifx_attn_paged's, of ifx_attn_paged_workspace_bytes.
+ * ifx_attn_paged's, of ifx_attn_paged_q8_workspace_bytes; one may serve both.
  *
  * Codes are exact in the products, which are summed in fp32.  Q of bf16 is
  * taken to fp16 with a power of two for each row, which loses nothing of what is
@@ -57,6 +57,8 @@ int ifx_read_rows_q8(const void *k_cache, const void *v_cache, const void *scale
  * rounded to fp16, relative to the largest scale among the keys that the row has
  * met: what weighs 2^-20 of that and less loses bits.  Scales of V count as
  * 2^-80 at least in this. */
+int64_t ifx_attn_paged_q8_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int max_q,
+                                          int max_kv);
 int ifx_attn_paged_q8(const void *q, int64_t q_stride, int q_dtype, const void *k_cache,
                       const void *v_cache, const void *scales, int64_t num_pages, int page_size,
                       const int32_t *block_table, int table_width, const int32_t *cu_q,

@@ -130,6 +130,7 @@ SIGNATURES.update({
                             _i32, _i32, _i32, _vp, _i64, _i32, _vp, _vp, _vp, _i64, _i32, _vp], _i32),
     "ifx_read_rows_q8": ([_vp, _vp, _vp, _i64, _i32, _vp, _i32, _i32, _i32, _vp, _i64, _vp, _i64,
                           _i32, _vp], _i32),
+    "ifx_attn_paged_q8_workspace_bytes": ([_i32] * 7, _i64),
     "ifx_attn_paged_q8": ([_vp, _i64, _i32, _vp, _vp, _vp, _i64, _i32, _vp, _i32, _vp, _vp, _vp] +
                           [_i32] * 7 + [ctypes.c_float, _i32, _vp, _i64, _i32, _vp, _i64, _vp], _i32),
 })

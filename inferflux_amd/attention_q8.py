@@ -113,11 +113,19 @@ def read_rows(cache, slots, dtype=torch.float16, k_out=None, v_out=None, stream=
     return k_out, v_out
 
 
+def paged_workspace_bytes(B, T, Hq, Hkv, head_dim, max_q, max_kv):
+    """Bytes of workspace that paged_attention needs for this shape (0: none;
+    attention.WORKSPACE_BYTES is enough for all)."""
+    return int(_lib.load().ifx_attn_paged_q8_workspace_bytes(
+        _count(B, "B"), _count(T, "T"), _count(Hq, "Hq"), _count(Hkv, "Hkv"),
+        _count(head_dim, "head_dim"), _count(max_q, "max_q"), _count(max_kv, "max_kv")))
+
+
 def paged_attention(q, cache, block_table, cu_q, kv_len, max_q, max_kv, scale=None, window=0, masks=None,
                     out=None, out_dtype=None, workspace=None, stream=None):
     """attention.paged_attention over an 8-bit cache (ifx_attn_paged_q8), q
     float16 or bfloat16.  masks: of drafted trees, as drafts.tree_attention's
-    (window 0 then).  workspace: as attention's."""
+    (window 0 then).  workspace: attention.workspace, or paged_workspace_bytes of it."""
     n, Hkv, P, D = _q8_caches(cache)
     dev = _device(q, "q")
     if q.dim() != 3:

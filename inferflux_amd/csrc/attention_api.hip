@@ -85,6 +85,7 @@ constexpr int64_t kCntBytes = kSplitCntBytes;
 
 struct PagedPlan {
   bool rows;         // attn_rows, else attn_tile
+  int row_slots;     // attn_rows: rows of a workgroup
   int goal, items;   // AttnArgs; workgroups of a key/value head
   int64_t bytes;     // of workspace
 };
@@ -103,24 +104,41 @@ struct PagedPlan {
 //
 // Fewer where the split sums would not fit the largest workspace.
 //
-// tree: drafts over the 16-bit cache, as many for every request.  From 17 rows on
-// attn_tile takes them, but for one or two requests of up to 24.  us with
-// attn_rows / attn_tile, with the plan's launch:
+// Trees over the 16-bit cache go to attn_tile from 17 rows on, but for a few
+// units (requests times key/value heads) of up to 24.  us with attn_rows /
+// attn_tile, with the plan's launch:
 //   16 / 2 heads of 128, 24 rows of 3000 keys  1 request 19.9/21.8, 4 21.3/22.8,
 //     8 25.4/23.1; 32 of 1000 to 9000 51/42.6
 //   40 / 8 heads, 20 rows  1 20.1/22.1, 2 24.4/23.0, 8 42.6/37.4, 32 114/112
 //     30 rows              1 23.1/22.3, 2 28.5/23.0, 8 48.1/36.9, 32 122/113
-// attn_rows_q8 is faster up to its 32 rows (30 rows of 40 / 8 heads: 1 request
-// 23.4/33.4, 8 38.6/39.5, 32 83/128).
-PagedPlan plan_paged(int B, int T, int Hq, int Hkv, int D, int max_q, int max_kv, bool tree) {
+// The 8-bit cache's attn_rows is faster up to its 32 rows (30 rows of 40 / 8
+// heads: 1 request 23.4/33.4, 8 38.6/39.5, 32 83/128).
+//
+// More rows as blocks of 32 of attn_rows, where there are so few units that
+// attn_tile's workgroups would leave most of the chip idle (both read the keys
+// once for each block or tile).  us in blocks / with attn_tile, 3000 keys:
+//   16-bit  16 / 2 heads, 160 rows  1 request 23.6/33, 2 29.4/34, 8 37.5/35
+//                         480 rows  1 26.4/33.4, 2 31/34.3, 8 47/48
+//           40 / 8 heads,  60 rows  1 25.5/30.2, 2 34.4/31.1, 8 58/50
+//   8-bit   16 / 2 heads, 160 rows  1 23.5/35.8, 4 28.6/36.9, 16 41.5/51
+//           40 / 8 heads,  60 rows  1 25/34, 2 32/35, 4 37/35.4, 16 65/55
+//                         300 rows  1 34.8/37, 2 50/49, 4 64/55
+enum PagedKind { kPaged16, kTree16, kPaged8 };
+PagedPlan plan_paged(PagedKind kind, int B, int T, int Hq, int Hkv, int D, int max_q, int max_kv) {
   PagedPlan p{};
   const int G = Hq / Hkv;
-  const int64_t rows = static_cast<int64_t>(max_q) * G;
-  p.rows = rows <= (!tree ? kRowsMax : B * Hkv <= 8 ? 24 : 16);
+  const int64_t rows = static_cast<int64_t>(max_q) * G, units = static_cast<int64_t>(B) * Hkv;
+  p.rows = rows <= (kind != kTree16 ? kRowsMax : units <= 8 ? 24 : 16);
+  const bool blocks =
+      !p.rows && kind != kPaged16 && units * ((rows + 31) / 32) <= (kind == kTree16 ? 30 : 60) && rows > kRowsMax;
+  p.rows |= blocks;
   // row tiles, stages of the longest request that a split must have, bytes of a slot
-  const int64_t tiles = p.rows ? B : static_cast<int64_t>(T) * G / attn_tile_rows(D) + B;
+  const int64_t tiles = p.rows && !blocks
+                            ? B
+                            : static_cast<int64_t>(T) * G / (blocks ? kRowsMax : attn_tile_rows(D)) + B;
   const int unit = p.rows ? kRowKeys : attn_tile_min_keys();
-  const int64_t slot = p.rows ? rows * (D + 4) * 4 : attn_tile_slot_bytes(D);
+  p.row_slots = static_cast<int>(rows < kRowsMax ? rows : kRowsMax);
+  const int64_t slot = p.rows ? p.row_slots * (D + 4) * 4 : attn_tile_slot_bytes(D);
   const int all = p.rows ? 1024 : D == 256 ? 256 : D == 64 ? 768 : 512;
   int64_t goal = all / Hkv;
   const int64_t use = tiles * ((static_cast<int64_t>(max_kv) + unit - 1) / unit);
@@ -128,8 +146,8 @@ PagedPlan plan_paged(int B, int T, int Hq, int Hkv, int D, int max_q, int max_kv
   if (goal > use) goal = use;
   if (goal > fit) goal = fit;
   if (goal > kMaxUnits / Hkv) goal = kMaxUnits / Hkv;
-  if (p.rows && goal > attn_rows_max_goal(static_cast<int>(rows)))
-    goal = attn_rows_max_goal(static_cast<int>(rows));
+  if (p.rows && goal > attn_rows_max_goal(p.row_slots))
+    goal = attn_rows_max_goal(p.row_slots);
   if (max_kv <= (p.rows ? unit : 2 * unit - kTileKeys)) goal = 0;  // one chunk each
   p.goal = static_cast<int>(goal);
   p.items = static_cast<int>(tiles + goal);
@@ -160,7 +178,8 @@ int attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cache,
     return IFX_NULL_POINTER;
   if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15)
     return IFX_BAD_GEOMETRY;
-  const PagedPlan p = plan_paged(B, T, Hq, Hkv, D, max_q, max_kv, masks && !scales);
+  const PagedPlan p = plan_paged(scales ? kPaged8 : masks ? kTree16 : kPaged16, B, T, Hq, Hkv, D,
+                                 max_q, max_kv);
   if (p.bytes) {
     if (!workspace) return IFX_NULL_POINTER;
     if (workspace_bytes < p.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255))
@@ -183,9 +202,9 @@ int attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cache,
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (scales)
-    return status_of(p.rows ? launch_attn_rows_q8(a, D, max_q * a.G, p.items, s)
+    return status_of(p.rows ? launch_attn_rows_q8(a, D, p.row_slots, p.items, s)
                             : launch_attn_tile_q8(a, D, p.items, s));
-  if (p.rows) return status_of(launch_attn_rows(a, dtype, D, max_q * a.G, p.items, s));
+  if (p.rows) return status_of(launch_attn_rows(a, dtype, D, p.row_slots, p.items, s));
   return status_of(launch_attn_tile(a, dtype, D, true, p.items, s));
 }
 
@@ -274,7 +293,7 @@ int ifx_read_rows_q8(const void *k_cache, const void *v_cache, const void *scale
 int64_t ifx_attn_paged_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int max_q,
                                        int max_kv) {
   if (!heads_ok(B, T, Hq, Hkv, D) || max_q < 1 || max_kv < 1) return 0;
-  return plan_paged(B, T, Hq, Hkv, D, max_q, max_kv, false).bytes;
+  return plan_paged(kPaged16, B, T, Hq, Hkv, D, max_q, max_kv).bytes;
 }
 
 int ifx_attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cache,
@@ -291,7 +310,7 @@ int ifx_attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cac
 int64_t ifx_attn_tree_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int max_q,
                                       int max_kv) {
   if (!heads_ok(B, T, Hq, Hkv, D) || max_q < 1 || max_q > IFX_TREE_MAX_NODES || max_kv < 1) return 0;
-  return plan_paged(B, T, Hq, Hkv, D, max_q, max_kv, true).bytes;
+  return plan_paged(kTree16, B, T, Hq, Hkv, D, max_q, max_kv).bytes;
 }
 
 int ifx_attn_tree(const void *q, int64_t q_stride, int dtype, const void *k_cache,
@@ -305,6 +324,12 @@ int ifx_attn_tree(const void *q, int64_t q_stride, int dtype, const void *k_cach
   return attn_paged(q, q_stride, dtype, k_cache, v_cache, nullptr, num_pages, page_size, block_table,
                     table_width, cu_q, kv_len, masks, B, T, Hq, Hkv, D, max_q, max_kv, scale, 0,
                     out, out_stride, out_dtype, workspace, workspace_bytes, stream);
+}
+
+int64_t ifx_attn_paged_q8_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int max_q,
+                                          int max_kv) {
+  if (!heads_ok(B, T, Hq, Hkv, D) || max_q < 1 || max_kv < 1) return 0;
+  return plan_paged(kPaged8, B, T, Hq, Hkv, D, max_q, max_kv).bytes;
 }
 
 int ifx_attn_paged_q8(const void *q, int64_t q_stride, int q_dtype, const void *k_cache,

@@ -43,7 +43,8 @@ __device__ __forceinline__ PieceMask piece_mask(int key, int lo, int hi) {
 
 }  // namespace
 
-// TREE: rows see the cached tokens and the nodes of their masks.
+// TREE: rows see the cached tokens and the nodes of their masks; more than 32
+// are blocks of 32, the keys of each split by themselves.
 template <int DT, int D, bool TREE = false>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(const AttnArgs a, int lds_rows) {
   using T = Elem<DT>;
@@ -60,11 +61,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(const AttnA
       a, reinterpret_cast<int2 *>(red), blockIdx.x / a.Hkv, [&](const Request &r) {
         int keys = r.kv;
         if (a.window > 0) keys = min<int64_t>(keys, static_cast<int64_t>(a.window) + r.nq + kRowKeys);
-        return make_int2(r.nq > 0 ? 1 : 0, max(1, (keys + kRowKeys - 1) / kRowKeys));
+        const int blocks = TREE ? (r.nq * a.G + 31) / 32 : r.nq > 0 ? 1 : 0;
+        return make_int2(blocks, max(1, (keys + kRowKeys - 1) / kRowKeys));
       });
   if (split.chunk == 0) return;
-  const int b = split.b, z = split.item;
-  const int q0 = split.req.q0, nq = split.req.nq, kv = split.req.kv, R = min(nq * a.G, lds_rows);
+  const int b = split.b, z = TREE ? split.item / split.tiles : split.item;
+  const int block = TREE ? split.item - z * split.tiles : 0, row0 = 32 * block;
+  const int q0 = split.req.q0, nq = split.req.nq, kv = split.req.kv, R = min(nq * a.G - row0, lds_rows);
   const int ctx = kv - nq;  // position of the first row; below 0 it sees nothing
   const int lo0 = a.window > 0 ? max(0, ctx - a.window + 1) : 0;
   const int kbeg = lo0 & ~(kRowKeys - 1), kend = kv;  // the last row sees kv - 1
@@ -74,7 +77,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(const AttnA
   const int zbeg = kbeg + z * chunk, zend = min(zbeg + chunk, kend);
 
   // this lane's row: what it sees is [lo, hi]; rows behind the last repeat it
-  const int row = min(n, R - 1), tok = row / a.G, head = kvh * a.G + row % a.G;
+  const int row = row0 + min(n, R - 1), tok = row / a.G, head = kvh * a.G + row % a.G;
   Sight<TREE> sight = {0, ctx + tok, ctx, 0};
   if constexpr (TREE)
     sight.bits = node_bits(a, q0 + tok, nq);
@@ -224,7 +227,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(const AttnA
 
   l = halves_sum(l);
   const auto put = [&](float scale) { put_rows32<D>(red, acc, scale, R); };
-  rows_finish<D>(a, split, red, sums, n, h == 0, m, l, a.c, lds_rows, R, ns, kvh, put, [&](int t) {
+  rows_finish<D>(a, split, red, sums, n, h == 0, m, l, a.c, lds_rows, R, block, z, ns, kvh, put, [&](int t) {
     if constexpr (TREE)
       return Sight<true>{0, 0, ctx, node_bits(a, q0 + t, nq)}.nothing();
     else

@@ -59,28 +59,29 @@ __device__ __forceinline__ float quarters_sum(float v) {
 
 namespace {
 
-// The workgroup's request and chunk of its keys, and what it sees of them.
+// The workgroup's request, block of 32 of its rows and chunk of its keys.
 struct RowsWork {
   Split split;
-  int b, q0, nq, kv, R, ctx, lo0, ns, zbeg, zend;
+  int b, q0, nq, kv, R, ctx, lo0, block, z, ns, zbeg, zend;  // R: rows of the block
   bool tree;
 };
 __device__ __forceinline__ bool rows_work(const AttnArgs &a, float *reqs, int lds_rows, RowsWork &w) {
   w.split = find_item<1>(a, reinterpret_cast<int2 *>(reqs), blockIdx.x / a.Hkv, [&](const Request &r) {
     int keys = r.kv;
     if (a.window > 0) keys = min<int64_t>(keys, static_cast<int64_t>(a.window) + r.nq + kRowKeys);
-    return make_int2(r.nq > 0 ? 1 : 0, max(1, (keys + kRowKeys - 1) / kRowKeys));
+    return make_int2((r.nq * a.G + 31) / 32, max(1, (keys + kRowKeys - 1) / kRowKeys));
   });
   if (w.split.chunk == 0) return false;
   w.b = w.split.b, w.q0 = w.split.req.q0, w.nq = w.split.req.nq, w.kv = w.split.req.kv;
-  w.R = min(w.nq * a.G, lds_rows);
+  w.z = w.split.item / w.split.tiles, w.block = w.split.item - w.z * w.split.tiles;
+  w.R = min(w.nq * a.G - 32 * w.block, lds_rows);
   w.ctx = w.kv - w.nq;  // position of the first row; below 0 it sees nothing
   w.tree = a.masks != nullptr;
   w.lo0 = a.window > 0 ? max(0, w.ctx - a.window + 1) : 0;
   const int kbeg = w.lo0 & ~(kRowKeys - 1), kend = w.kv, chunk = w.split.chunk * kRowKeys;
   w.ns = kend > kbeg ? (kend - kbeg + chunk - 1) / chunk : 1;
-  if (w.split.item >= w.ns) return false;
-  w.zbeg = kbeg + w.split.item * chunk, w.zend = min(w.zbeg + chunk, kend);
+  if (w.z >= w.ns) return false;
+  w.zbeg = kbeg + w.z * chunk, w.zend = min(w.zbeg + chunk, kend);
   return true;
 }
 
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows_q8(const At
   if (!rows_work(a, red, lds_rows, w)) return;
 
   // this lane's row; rows behind the last repeat it
-  const int row = min(n, w.R - 1), tok = row / a.G, head = kvh * a.G + row % a.G;
+  const int row = 32 * w.block + min(n, w.R - 1), tok = row / a.G, head = kvh * a.G + row % a.G;
   const RowSight sight(a, w, tok);
   u32x4 qf[NS];
   {  // of step s the dims 32 (s / 2) + 16 h + 8 (s % 2), as K's pieces hold them
@@ -265,7 +266,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows_q8(const At
 
   l = halves_sum(l);
   const auto put = [&](float scale) { put_rows32<D>(red, acc, scale, w.R); };
-  rows_finish<D>(a, w.split, red, sums, n, h == 0, level.of_sums(), l, 1.0f, lds_rows, w.R, w.ns, kvh,
+  rows_finish<D>(a, w.split, red, sums, n, h == 0, level.of_sums(), l, 1.0f, lds_rows, w.R, w.block, w.z, w.ns, kvh,
                  put, [&](int t) { return row_sees_nothing(a, w, t); });
 }
 
@@ -287,7 +288,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void k_attn_rows16_q8(const 
   RowsWork w;
   if (!rows_work(a, red, lds_rows, w)) return;
 
-  const int row = min(m, w.R - 1), tok = row / a.G, head = kvh * a.G + row % a.G;
+  const int row = 32 * w.block + min(m, w.R - 1), tok = row / a.G, head = kvh * a.G + row % a.G;
   const RowSight sight(a, w, tok);
   u32x4 qf[ND];
   {  // steps 2 i and 2 i + 1: the dims 64 i + 16 g + 0 .. 7 and + 8 .. 15, a piece of
@@ -420,7 +421,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void k_attn_rows16_q8(const 
       __builtin_memcpy(red + ((wave * (D / 4) + 4 * d + g) * w.R + m) * 4, &v, 16);
     }
   };
-  rows_finish<D, 16>(a, w.split, red, sums, m, g == 0, level.of_sums(), l, 1.0f, lds_rows, w.R, w.ns, kvh,
+  rows_finish<D, 16>(a, w.split, red, sums, m, g == 0, level.of_sums(), l, 1.0f, lds_rows, w.R, w.block, w.z, w.ns, kvh,
                  put, [&](int t) { return row_sees_nothing(a, w, t); });
 }
 

@@ -17,17 +17,18 @@ struct RowSums {
 // Of a wave the lanes with the same n hold row n, one of them (lead) besides the
 // others its maximum m and sum l; exponents are (s - m) c.  put(scale): the
 // lane writes its part of the row's sums, times scale, to red[wave][D / 4][R][4].
-// red later holds [chunk][row].  none(t): whether the rows of new token t see
-// nothing.  kAtOnce: chunks whose sums a thread reads at a time, 4 registers each.
+// red later holds [chunk][row].  The R rows are those from row0 on of the
+// request, its row block number `block`, whose keys are cut into ns chunks, this
+// one z.  none(t): whether the rows of new token t see nothing.  kAtOnce: chunks whose sums a thread reads at a time, 4 registers each.
 template <int D, int kAtOnce = 24, class Put, class None>
 __device__ __forceinline__ void rows_finish(const AttnArgs &a, const Split &split, float *red,
                                             RowSums &sums, int n, bool lead, float m, float l,
-                                            float c, int lds_rows, int R, int ns, int kvh, Put put,
-                                            None none) {
+                                            float c, int lds_rows, int R, int block, int z, int ns,
+                                            int kvh, Put put, None none) {
   constexpr uint32_t kOut = 1u << 30;  // an offset past the workspace's end: reads zeros
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int z = split.item, q0 = split.req.q0;
+  const int q0 = split.req.q0, row0 = block * 32;
 
   // the four waves' sums, in the waves' order
   if (lead) {
@@ -60,12 +61,12 @@ __device__ __forceinline__ void rows_finish(const AttnArgs &a, const Split &spli
       f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int w = 0; w < kRowWaves; ++w) v += ldg<f32x4>(red + ((w * (D / 4) + d4) * R + r) * 4);
-      const int t = r / a.G;
+      const int row = row0 + r, t = row / a.G;
       // a row that sees no key is 0; one whose keys all weigh nothing is not a number
       const float inv = 1.0f / sums.l[0][r];
       v = none(t) ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : v * inv;
       char *o = static_cast<char *>(a.out) +
-                ((q0 + t) * a.out_stride + static_cast<int64_t>(head0 + r % a.G) * D) *
+                ((q0 + t) * a.out_stride + static_cast<int64_t>(head0 + row % a.G) * D) *
                     dtype_bytes(a.out_dtype);
       store4(o, a.out_dtype, d4 * 4, v);
     }
@@ -75,7 +76,7 @@ __device__ __forceinline__ void rows_finish(const AttnArgs &a, const Split &spli
   // split: this chunk's sums to its slot, (m, l) of its rows behind them
   const rsrc_t part = make_rsrc(a.part, a.part_bytes);
   const uint32_t slot_bytes = lds_rows * (D + 4) * 4;
-  const uint32_t first = split.slot * a.Hkv + kvh * split.ns;  // the request's slots
+  const uint32_t first = split.slot * a.Hkv + (block * a.Hkv + kvh) * split.ns;  // the block's slots
   const uint32_t slot0 = first * slot_bytes;
   const uint32_t slot = slot0 + z * slot_bytes;
   for (int i = tid; i < elems; i += 256) {
@@ -137,7 +138,7 @@ __device__ __forceinline__ void rows_finish(const AttnArgs &a, const Split &spli
   }
   __syncthreads();
   for (int i = tid; i < elems; i += 256) {
-    const int r = i % R, d4 = i / R, t = r / a.G;
+    const int r = i % R, d4 = i / R, row = row0 + r, t = row / a.G;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int y0 = 0; y0 < ns; y0 += kAtOnce) {
       if (i != tid || y0) read(i, y0);
@@ -147,7 +148,7 @@ __device__ __forceinline__ void rows_finish(const AttnArgs &a, const Split &spli
     }
     o = none(t) ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : o * sums.l[0][r];
     char *to = static_cast<char *>(a.out) +
-               ((q0 + t) * a.out_stride + static_cast<int64_t>(head0 + r % a.G) * D) *
+               ((q0 + t) * a.out_stride + static_cast<int64_t>(head0 + row % a.G) * D) *
                    dtype_bytes(a.out_dtype);
     store4(to, a.out_dtype, d4 * 4, o);
   }

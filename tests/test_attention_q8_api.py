@@ -24,7 +24,8 @@ def test_exports_what_the_header_declares(lib):
     from inferflux_amd import _lib
     text = open(os.path.join(ROOT, "include", "ifx_attention_q8.h")).read()
     syms = set(re.findall(r"^\s*(?:int|int64_t)\s+(ifx_\w+)\s*\(", text, re.M))
-    assert syms == {"ifx_rope_append_q8", "ifx_read_rows_q8", "ifx_attn_paged_q8"}
+    assert syms == {"ifx_rope_append_q8", "ifx_read_rows_q8", "ifx_attn_paged_q8_workspace_bytes",
+                    "ifx_attn_paged_q8"}
     assert syms <= set(_lib.SIGNATURES)
     out = subprocess.run(["nm", "-D", "--defined-only", _lib.LIB_PATH], capture_output=True,
                          text=True, check=True).stdout
@@ -76,9 +77,12 @@ ATTN = dict(q=F, qs=2048, dt=1, kc=F, vc=F, s=F, pages=100, page=64, table=F, wi
 
 
 @pytest.mark.parametrize("change,want", [
-    ({}, "k_attn_rows_q8<128>"), (dict(max_q=5), "k_attn_tile_q8<128>"), (dict(dt=2), "k_attn_rows_q8<128>"),
+    ({}, "k_attn_rows_q8<128>"), (dict(max_q=2), "k_attn_rows16_q8<128>"), (dict(dt=2), "k_attn_rows_q8<128>"),
+    # blocks of rows: 4 requests x 2 heads x 7 blocks, and row tiles from 8 on
+    (dict(max_q=28), "k_attn_rows_q8<128>"), (dict(max_q=29), "k_attn_tile_q8<128>"),
+    (dict(max_q=5, B=15), "k_attn_rows_q8<128>"), (dict(max_q=5, B=16), "k_attn_tile_q8<128>"),
     (dict(D=64, qs=1024, os=1024), "k_attn_rows_q8<64>"), (dict(D=96), "k_attn_rows_q8<96>"),
-    (dict(D=256, qs=4096, os=4096, max_q=9), "k_attn_tile_q8<256>"), (dict(masks=F), "k_attn_rows_q8<128>"),
+    (dict(D=256, qs=4096, os=4096, max_q=90), "k_attn_tile_q8<256>"), (dict(masks=F), "k_attn_rows_q8<128>"),
     (dict(masks=F, max_q=64), "k_attn_tile_q8<128>"), (dict(masks=F, max_q=65), GEOM),
     (dict(masks=F, window=9), GEOM), (dict(window=9), "k_attn_rows_q8<128>"), (dict(window=-1), GEOM),
     (dict(T=0, s=None), OK), (dict(s=None), NULL), (dict(s=ODD), GEOM), (dict(kc=ODD), GEOM), (dict(dt=0), TYPE),
@@ -88,6 +92,20 @@ def test_attention_kernels_and_refusals(lib, change, want):
     with dry(lib) as d:
         rc = lib.ifx_attn_paged_q8(*{**ATTN, **change}.values())
     assert (d.text, rc) == (want, OK) if isinstance(want, str) else (rc, d.text) == (want, "")
+
+
+@pytest.mark.parametrize("B,T,Hq,Hkv,D,max_q,max_kv", [
+    (1, 1, 16, 2, 128, 1, 3000), (4, 24, 16, 2, 128, 6, 3000), (16, 96, 40, 8, 128, 6, 9000), (1, 61, 16, 2, 128, 61, 3000),
+    (1, 512, 40, 8, 128, 512, 8000), (4096, 4096, 8, 8, 256, 64, 1 << 20), (1, 64, 64, 1, 256, 64, 1 << 30)])
+def test_attention_workspace(lib, B, T, Hq, Hkv, D, max_q, max_kv):
+    """As many bytes as it says are enough, one less is not."""
+    n = lib.ifx_attn_paged_q8_workspace_bytes(B, T, Hq, Hkv, D, max_q, max_kv)
+    assert 0 < n <= 64 << 20
+    change = dict(B=B, T=T, Hq=Hq, Hkv=Hkv, D=D, max_q=max_q, max_kv=max_kv, qs=Hq * D, os=Hq * D)
+    for have, want in ((n, OK), (n - 1, GEOM)):
+        with dry(lib) as d:
+            assert lib.ifx_attn_paged_q8(*{**ATTN, **change, "wn": have}.values()) == want
+        assert d.text.startswith("k_attn_") == (want == OK)
 
 
 def test_python_refusals():

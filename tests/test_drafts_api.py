@@ -58,7 +58,8 @@ ATTN = dict(q=F, qs=2048, dt=1, kc=F, vc=F, pages=100, page=64, table=F, width=5
 
 
 @pytest.mark.parametrize("change,want", [
-    ({}, "k_attn_tile<1,128,1,1>"), (dict(max_q=2), "k_attn_rows<1,128,1>"), (dict(max_q=3), "k_attn_rows<1,128,1>"),
+    ({}, "k_attn_tile<1,128,1,1>"), (dict(max_q=12, B=3), "k_attn_rows<1,128,1>"), (dict(max_q=20, B=3), "k_attn_rows<1,128,1>"),
+    (dict(max_q=21, B=3), "k_attn_tile<1,128,1,1>"), (dict(max_q=2), "k_attn_rows<1,128,1>"), (dict(max_q=3), "k_attn_rows<1,128,1>"),
     (dict(max_q=3, B=5), "k_attn_tile<1,128,1,1>"), (dict(max_q=2, B=5), "k_attn_rows<1,128,1>"),
     (dict(dt=2, max_q=1), "k_attn_rows<2,128,1>"), (dict(dt=2), "k_attn_tile<2,128,1,1>"),
     (dict(max_q=64), "k_attn_tile<1,128,1,1>"), (dict(max_q=65), GEOM), (dict(max_q=0), GEOM),

@@ -229,10 +229,11 @@ def test_decode(dev, qdt, Hq, Hkv, D, P, lens):
 
 @pytest.mark.parametrize("qdt", ["f16", "bf16"])
 @pytest.mark.parametrize("Hq,Hkv,D,P", SHAPES)
-@pytest.mark.parametrize("lens", ["prompt", "chunk", "mixed"])
+@pytest.mark.parametrize("lens", ["prompt", "chunk", "mixed", "crowd"])
 def test_chunks(dev, qdt, Hq, Hkv, D, P, lens):
     note(f"q8 chunks {qdt} {Hq}/{Hkv} D={D} P={P} {lens}")
-    ctx, new = {"prompt": ([0, 0], [150, 33]), "chunk": ([1500], [70]), "mixed": ([900, 0, 17, 130, 64], [1, 65, 0, 40, 7])}[lens]
+    ctx, new = {"prompt": ([0, 0], [150, 33]), "chunk": ([1500], [70]), "mixed": ([900, 0, 17, 130, 64], [1, 65, 0, 40, 7]),
+                "crowd": ([i * 37 % 400 for i in range(34)], [(1, 2, 70)[i % 3] for i in range(34)])}[lens]
     run_paged(dev, qdt, ctx, new, Hq, Hkv, D, P, seed=D + P, side=8)
 
 
@@ -245,11 +246,12 @@ def test_windows(dev, n, Hq, Hkv, D, window):
 
 @pytest.mark.parametrize("qdt", ["f16", "bf16"])
 @pytest.mark.parametrize("Hq,Hkv,D,P", SHAPES)
-@pytest.mark.parametrize("shape", ["few", "wide"])
+@pytest.mark.parametrize("shape", ["few", "wide", "crowd"])
 def test_trees(dev, qdt, Hq, Hkv, D, P, shape):
     note(f"q8 tree {qdt} {Hq}/{Hkv} D={D} P={P} {shape}")
     rng = random.Random(Hq * 131 + D + P + len(shape))
-    ctx, new = {"few": ([0, 5, 300, 64], [4, 1, 3, 4]), "wide": ([700, 63, 0], [64, 33, 9])}[shape]
+    ctx, new = {"few": ([0, 5, 300, 64], [4, 1, 3, 4]), "wide": ([700, 63, 0], [64, 33, 9]),
+                "crowd": ([rng.randint(0, 400) for _ in range(34)], [rng.choice([1, 2, 40]) for _ in range(33)] + [40])}[shape]
     run_paged(dev, qdt, ctx, new, Hq, Hkv, D, P, masks=tree_masks(rng, new), seed=D + P)
 
 
@@ -330,6 +332,27 @@ def test_split_keys_repeat(dev, B, n, Hq, Hkv, D):
     a = run_paged(dev, "f16", ctx, [n] * B, Hq, Hkv, D, 16, workspace=ws)
     b = run_paged(dev, "f16", ctx, [n] * B, Hq, Hkv, D, 16, workspace=ws)
     assert torch.equal(a, b)
+
+
+def test_every_kernel_is_reached(dev):
+    """The shapes above go through all kernels and head sizes."""
+    import torch
+    from inferflux_amd import _lib, attention as at, attention_q8 as q8, drafts
+    note("q8 kernels")
+    lib = _lib.load()
+    lib.ifx_launch_log_begin(0)
+    for Hq, Hkv, D, P in SHAPES[:5]:
+        for B, n in ((1, 1), (1, 64), (34, 40)):
+            cache = q8.kv_cache(4, Hkv, D, P, device=dev)
+            table = torch.zeros(B, 4, dtype=torch.int32, device=dev)
+            q = torch.zeros(B * n, Hq, D, dtype=torch.float16, device=dev)
+            cu, kv = i32([i * n for i in range(B + 1)], dev), i32([n] * B, dev)
+            q8.paged_attention(q, cache, table, cu, kv, n, 60, workspace=at.workspace(dev))
+    torch.cuda.synchronize()
+    log = lib.ifx_launch_log_end().decode()
+    for D in (64, 96, 128, 256):
+        for k in ("rows16_q8", "rows_q8", "tile_q8"):
+            assert f"k_attn_{k}<{D}>" in log, (k, D)
 
 
 def test_bounds_below_the_lengths(dev):

@@ -164,12 +164,13 @@ def tree_masks(rng, new, reach=4):
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("Hq,Hkv,D,P", [(16, 2, 128, 64), (40, 8, 128, 16), (6, 6, 64, 32), (9, 3, 96, 16), (8, 2, 256, 128),
                                         (7, 1, 128, 256)])
-@pytest.mark.parametrize("shape", ["one", "few", "wide", "mixed"])
+@pytest.mark.parametrize("shape", ["one", "few", "wide", "mixed", "crowd"])
 def test_tree_attention(dev, dtype, Hq, Hkv, D, P, shape):
     note(f"tree {dtype} {Hq}/{Hkv} D={D} P={P} {shape}")
     rng = random.Random(Hq * 131 + D + P + len(shape))
     ctx, new = {"one": ([1700], [3]), "few": ([0, 5, 300, 64], [4, 1, 3, 4]), "wide": ([700, 63], [64, 33]),
-                "mixed": ([900, 0, 17, 130, 64], [1, 20, 0, 61, 7])}[shape]
+                "mixed": ([900, 0, 17, 130, 64], [1, 20, 0, 61, 7]),
+                "crowd": ([rng.randint(0, 400) for _ in range(34)], [rng.choice([1, 2, 40]) for _ in range(33)] + [40])}[shape]
     run_tree(dev, dtype, ctx, new, tree_masks(rng, new), Hq, Hkv, D, P, seed=D + P)
 
 
