@@ -23,7 +23,7 @@ import torch
 from . import _lib
 from .attention import (_DTYPES, _ELEMS, PAGE_SIZES, _count, _device, _i32, _launch, _new, _on, _out,
                         _rows)
-from .drafts import _masks, _table, _workspace
+from .drafts import _all_on, _masks, _table, _workspace
 
 Q8Cache = namedtuple("Q8Cache", "k v scales")
 
@@ -33,9 +33,10 @@ def _q8_caches(c):
     k, v, s = c
     if k.dtype is not torch.int8 or v.dtype is not torch.int8 or s.dtype is not torch.bfloat16:
         raise TypeError("an 8-bit cache has int8 codes and bfloat16 scales")
-    if k.dim() == 5 and v.dim() == 5 and s.dim() == 4:
-        n, h, d16, p, e = k.shape
-        if e == 16 and tuple(v.shape) == (n, h, p // 16, d16 * 16, 16) and tuple(s.shape) == (n, h, p, 2):
+    shape = k.shape
+    if len(shape) == 5:
+        n, h, d16, p, e = shape
+        if e == 16 and v.shape == (n, h, p // 16, d16 * 16, 16) and s.shape == (n, h, p, 2):
             if not (k.is_contiguous() and v.is_contiguous() and s.is_contiguous()):
                 raise ValueError("the cache must be contiguous")
             return n, h, p, d16 * 16
@@ -79,9 +80,7 @@ def rope_append(q, k, v, positions, slots, cache, inv_freq=None, interleaved=Fal
         rot, freq = 2 * inv_freq.numel(), _on(inv_freq, "inv_freq", dev).data_ptr()
     if q_out is None:
         q_out = _new((T, Hq, D), want, cache.k, stream)
-    for t, name in ((q, "q"), (k, "k"), (v, "v"), (cache.v, "cache.v"), (cache.scales, "cache.scales"),
-                    (q_out, "q_out")):
-        _on(t, name, dev)
+    _all_on(dev, q, k, v, cache.v, cache.scales, q_out)
     qp, qs = _rows(q, "q", T, Hq, D)
     kp, ks = _rows(k, "k", T, Hkv, D)
     vp, vs = _rows(v, "v", T, Hkv, D)
@@ -103,8 +102,7 @@ def read_rows(cache, slots, dtype=torch.float16, k_out=None, v_out=None, stream=
     v_out = _new((N, Hkv, D), k_out.dtype, cache.k, stream) if v_out is None else v_out
     if k_out.dtype not in _DTYPES or v_out.dtype is not k_out.dtype:
         raise TypeError("k_out and v_out must be float32, float16 or bfloat16, both the same")
-    for t, name in ((cache.v, "cache.v"), (cache.scales, "cache.scales"), (k_out, "k_out"), (v_out, "v_out")):
-        _on(t, name, dev)
+    _all_on(dev, cache.v, cache.scales, k_out, v_out)
     kp, ks = _rows(k_out, "k_out", N, Hkv, D)
     vp, vs = _rows(v_out, "v_out", N, Hkv, D)
     _launch(_lib.load().ifx_read_rows_q8, "ifx_read_rows_q8", dev, stream, cache.k.data_ptr(),
@@ -136,8 +134,7 @@ def paged_attention(q, cache, block_table, cu_q, kv_len, max_q, max_kv, scale=No
     B = kv_len.numel()
     W = _table(block_table, B)
     out = _out(q, out, out_dtype, stream)
-    for t, name in ((cache.k, "cache.k"), (cache.v, "cache.v"), (cache.scales, "cache.scales"), (out, "out")):
-        _on(t, name, dev)
+    _all_on(dev, cache.k, cache.v, cache.scales, out)
     qp, qs = _rows(q, "q", T, Hq, D)
     op, os = _rows(out, "out", T, Hq, D)
     wp, wn = _workspace(workspace, dev)

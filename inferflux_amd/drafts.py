@@ -45,6 +45,12 @@ def _masks(t, n, device):
     return _on(t, "masks", device).data_ptr()
 
 
+def _all_on(device, *tensors):
+    for t in tensors:
+        if t.get_device() != device:
+            raise ValueError(f"all tensors of a call must be on cuda:{device}")
+
+
 def _f32(t, name, n, device):
     if t.dtype is not torch.float32:
         raise TypeError(f"{name} must be float32")
@@ -91,8 +97,7 @@ def tree_attention(q, k_cache, v_cache, block_table, cu_q, kv_len, masks, max_q,
     B = kv_len.numel()
     W = _table(block_table, B)
     out = _out(q, out, out_dtype, stream)
-    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache"), (out, "out")):
-        _on(t, name, dev)
+    _all_on(dev, k_cache, v_cache, out)
     qp, qs = _rows(q, "q", T, Hq, D)
     op, os = _rows(out, "out", T, Hq, D)
     wp, wn = _workspace(workspace, dev)
@@ -193,8 +198,7 @@ def keep_path(cache, block_table, cu_q, kv_len, path, accepted, max_q, stream=No
     else:
         n, Hkv, P, D = _caches(*cache)
     dev, B, T = _device(cache[0], "k_cache"), kv_len.numel(), path.numel()
-    for t, name in zip(cache[1:], ("v_cache", "scales")):
-        _on(t, name, dev)
+    _all_on(dev, *cache)
     W = _table(block_table, B)
     _launch(_lib.load().ifx_keep_path, "ifx_keep_path", dev, stream, cache[0].data_ptr(),
             cache[1].data_ptr(), cache[2].data_ptr() if len(cache) == 3 else None,
