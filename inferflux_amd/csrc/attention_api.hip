@@ -117,9 +117,13 @@ struct PagedPlan {
 // More rows as blocks of 32 of attn_rows, where there are so few units that
 // attn_tile's workgroups would leave most of the chip idle (both read the keys
 // once for each block or tile).  us in blocks / with attn_tile, 3000 keys:
-//   16-bit  16 / 2 heads, 160 rows  1 request 23.6/33, 2 29.4/34, 8 37.5/35
-//                         480 rows  1 26.4/33.4, 2 31/34.3, 8 47/48
-//           40 / 8 heads,  60 rows  1 25.5/30.2, 2 34.4/31.1, 8 58/50
+//   16-bit  16 / 1 heads, 640 rows  1 request 24/33, 2 27.5/34, 4 33.5/35
+//                        1024 rows  1 26/33.4, 2 33/34.6, 4 48/36
+//           16 / 2 heads, 160 rows  1 23.5/33, 2 29.7/34.2, 4 31.7/34.8
+//                         512 rows  1 26/33.3, 2 31.5/34.7, 4 38.9/36
+//           16 / 4 heads,  80 rows  1 25/30.5, 2 32.5/31.8, 4 35.7/32.5
+//           40 / 8 heads, 100 rows  1 30.4/32.2, 2 35.4/33.7, 4 47.5/35.1
+//                         200 rows  1 34.7/33.3, 2 39.7/35.2
 //   8-bit   16 / 2 heads, 160 rows  1 23.5/35.8, 4 28.6/36.9, 16 41.5/51
 //           40 / 8 heads,  60 rows  1 25/34, 2 32/35, 4 37/35.4, 16 65/55
 //                         300 rows  1 34.8/37, 2 50/49, 4 64/55
@@ -129,8 +133,9 @@ PagedPlan plan_paged(PagedKind kind, int B, int T, int Hq, int Hkv, int D, int m
   const int G = Hq / Hkv;
   const int64_t rows = static_cast<int64_t>(max_q) * G, units = static_cast<int64_t>(B) * Hkv;
   p.rows = rows <= (kind != kTree16 ? kRowsMax : units <= 8 ? 24 : 16);
-  const bool blocks =
-      !p.rows && kind != kPaged16 && units * ((rows + 31) / 32) <= (kind == kTree16 ? 30 : 60) && rows > kRowsMax;
+  const int most = kind == kPaged8 ? 60 : units <= 4 ? 80 : 32;
+  const bool blocks = !p.rows && kind != kPaged16 && rows > kRowsMax &&
+                      units * ((rows + kRowsMax - 1) / kRowsMax) <= most;
   p.rows |= blocks;
   // row tiles, stages of the longest request that a split must have, bytes of a slot
   const int64_t tiles = p.rows && !blocks
@@ -160,8 +165,8 @@ PagedPlan plan_paged(PagedKind kind, int B, int T, int Hq, int Hkv, int D, int m
 int attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cache,
                const void *v_cache, const void *scales, int64_t num_pages, int page_size,
                const int32_t *block_table, int table_width, const int32_t *cu_q,
-               const int32_t *kv_len, const uint64_t *masks, int B, int T, int Hq, int Hkv, int D, int max_q, int max_kv, float scale,
-               int window, void *out, int64_t out_stride, int out_dtype, void *workspace,
+               const int32_t *kv_len, const uint64_t *masks, int B, int T, int Hq, int Hkv, int D,
+               int max_q, int max_kv, float scale, int window, void *out, int64_t out_stride, int out_dtype, void *workspace,
                int64_t workspace_bytes, void *stream) {
   if (!is_elem(dtype) || !is_out(out_dtype)) return IFX_UNSUPPORTED_TYPE;
   const int sh = page_shift_of(page_size);
