@@ -278,7 +278,7 @@ __global__ __launch_bounds__(kThreads, 4) void k_verify(const VerifyArgs a) {
     const double rest = fmax(share * chunk.total - chunk.before, 0.0);
     double run = 0.0;
     bool passed = false;
-    // 32 tokens a thread, one behind the other, read all at once
+    // 16 tokens a thread, one behind the other, read all at once
     for (int base = from; base < to && !passed; base += kThreads * 4 * kAtOnce) {
       const int at = base + tid * 4 * kAtOnce;
       f32x4 v[kAtOnce], q[kAtOnce];
@@ -298,6 +298,9 @@ __global__ __launch_bounds__(kThreads, 4) void k_verify(const VerifyArgs a) {
           q[i] = qr ? probs4<DT>(qr, at + 4 * i, a.V) : none;
         }
       }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i)  // the next chunk's, whose children `near` has not
+        if (at + 4 * i >= to) v[i] = q[i] = none;
       double own = 0.0;
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i) {
@@ -353,16 +356,21 @@ __global__ __launch_bounds__(kThreads, 4) void k_verify(const VerifyArgs a) {
   split_reset(a.cnt + b);
 }
 
-// Chunks of a row: enough workgroups for four a CU, of whole steps, as many
-// as a workgroup has threads at most.  us for 1 / 48 rows of 151936 values:
+// Chunks of a row: enough workgroups for four a CU, of whole rounds of kAhead
+// steps, as many as a workgroup has threads at most.  us for 1 / 4 / 16 / 32 / 48 /
+// 64 rows of 151936 values:
+//   for 512 workgroups   7.9 / 9.3 / 13.9 / 16.8 / 20.7 / 24.8
+//       1024             7.9 / 9.3 / 15.0 / 15.9 / 18.4 / 21.1
+//       1024, of steps   9.0 / 14.2 / 17.7 / 19.1 / 18.5 / 21.7
 void verify_split(int B, int V, int *chunks, int *chunk) {
-  const int64_t steps = (static_cast<int64_t>(V) + kStep - 1) / kStep;
+  constexpr int kRound = kAhead * kStep;
+  const int64_t rounds = (static_cast<int64_t>(V) + kRound - 1) / kRound;
   int64_t want = 1024 / B;
   if (want < 1) want = 1;
   if (want > kThreads) want = kThreads;
-  const int64_t each = (steps + want - 1) / want;
-  *chunk = static_cast<int>(each * kStep);
-  *chunks = static_cast<int>((steps + each - 1) / each);
+  const int64_t each = (rounds + want - 1) / want;
+  *chunk = static_cast<int>(each * kRound);
+  *chunks = static_cast<int>((rounds + each - 1) / each);
 }
 
 hipError_t launch_verify(const VerifyArgs &a, int prob_dtype, hipStream_t s) {
