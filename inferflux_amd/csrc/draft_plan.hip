@@ -3,9 +3,10 @@
 //
 //   mask_i = {i} + mask_parent(i),  position_i = ctx + |mask_i| - 1
 //
-// Bound by latency: a launch, the reads of the lengths, then of the parents.  A
-// request is a wave, its nodes the lanes: the masks of all nodes grow twice as
-// far towards the root with each of six exchanges between lanes.
+// Bound by latency: a launch, the reads of the lengths, then of the parents; 5 us
+// for one tree of 61 nodes as for 24 of 40.  A request is a wave, its nodes the
+// lanes: the masks of all nodes grow twice as far towards the root with each of
+// six exchanges between lanes, where a walk would take a node's depth of them.
 #include "ifx_drafts_impl.h"
 
 namespace ifx {
@@ -67,8 +68,9 @@ hipError_t launch_plan_tree(const TreeArgs &a, hipStream_t s) {
 // One workgroup: a page's place among the free ones depends on how many all
 // requests behind its own give back.
 __global__ __launch_bounds__(1024) void k_plan_kept(const KeptArgs a) {
+  constexpr int kEach = IFX_ATTN_MAX_BATCH / 1024;  // requests of a thread
   __shared__ int64_t part[16];
-  __shared__ int given[IFX_ATTN_MAX_BATCH];  // pages of the requests
+  __shared__ int given[IFX_ATTN_MAX_BATCH], behind[IFX_ATTN_MAX_BATCH];  // pages of a request, of those behind it
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, sh = a.page_shift, P = 1 << sh;
   const int room = a.table_width << sh;
   auto of = [&](int b, int &kept, int &held) {  // tokens kept, pages held
@@ -78,22 +80,31 @@ __global__ __launch_bounds__(1024) void k_plan_kept(const KeptArgs a) {
     held = (kv + P - 1) >> sh;
     return held - ((kept + P - 1) >> sh);
   };
-  int64_t sum = 0;
-  for (int b = tid; b < a.B; b += 1024) {
-    int kept, held;
-    const int give = of(b, kept, held);
-    a.ctx_len[b] = kept;
-    given[b] = give;
-    sum += give;
+  int give[kEach];
+  int64_t own = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int b = tid * kEach + i;
+    give[i] = 0;
+    if (b < a.B) {
+      int kept, held;
+      give[i] = of(b, kept, held);
+      a.ctx_len[b] = kept;
+    }
+    own += give[i];
   }
+  int64_t to = own;  // of the wave's threads up to this one
   for (int d = 1; d < 64; d <<= 1) {
-    const int lo = __shfl_xor(static_cast<int>(sum), d), hi = __shfl_xor(static_cast<int>(sum >> 32), d);
-    sum += (static_cast<int64_t>(hi) << 32) | static_cast<uint32_t>(lo);
+    const int lo = __shfl_up(static_cast<int>(to), d), hi = __shfl_up(static_cast<int>(to >> 32), d);
+    if (lane >= d) to += (static_cast<int64_t>(hi) << 32) | static_cast<uint32_t>(lo);
   }
-  if (lane == 0) part[wave] = sum;
+  if (lane == 63) part[wave] = to;
   __syncthreads();
   int64_t total = 0;
-  for (int w = 0; w < 16; ++w) total += part[w];
+  for (int w = 0; w < 16; ++w) {
+    if (w < wave) to += part[w];
+    total += part[w];
+  }
   const int count = min(max(a.free_count[0], 0), a.free_capacity);
   const bool fits = total <= a.free_capacity - count;
   if (tid == 0) {
@@ -101,18 +112,22 @@ __global__ __launch_bounds__(1024) void k_plan_kept(const KeptArgs a) {
     a.status[0] = fits ? 0 : IFX_KEPT_NO_SPACE;
   }
   if (!fits) return;
-  // The last request's last page first.  Requests in turn over the waves, the
-  // pages before each summed by its wave.
+  to -= own;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    to += give[i];
+    given[tid * kEach + i] = give[i];
+    behind[tid * kEach + i] = static_cast<int>(total - to);
+  }
+  __syncthreads();
+  // the last request's last page first; a wave takes a request
   for (int b = wave; b < a.B; b += 16) {
-    const int give = given[b];
-    if (!give) continue;
-    int behind = 0;
-    for (int o = b + 1 + lane; o < a.B; o += 64) behind += given[o];
-    behind = wave_sum(behind);
+    const int n = given[b];
+    if (!n) continue;
     int kept, held;
     of(b, kept, held);
-    for (int i = lane; i < give; i += 64)
-      a.free_pages[count + behind + i] = a.table[static_cast<int64_t>(b) * a.table_width + held - 1 - i];
+    for (int i = lane; i < n; i += 64)
+      a.free_pages[count + behind[b] + i] = a.table[static_cast<int64_t>(b) * a.table_width + held - 1 - i];
   }
 }
 
