@@ -27,8 +27,10 @@ extern "C" {
  * V, for each token and head, the scale is the smallest bf16 that is no less
  * than max |x| / 127, and a code is x / scale rounded to nearest, ties to even:
  * a value is off by at most half a scale.  A head's row of zeros has scale 0;
- * one that holds an infinity or NaN has scale NaN and codes 0, so that all of
- * it reads back as NaN.  D: a multiple of 32 up to 256; scales 16-byte aligned. */
+ * one that holds an infinity or NaN, or a rotated K past fp32's range, has scale
+ * NaN and codes 0, so that all of it reads back as NaN.  Slots within the cache
+ * must differ: what two tokens write to one is codes and scales of either.
+ * D: a multiple of 32 up to 256; scales 16-byte aligned. */
 int ifx_rope_append_q8(const void *q, int64_t q_stride, const void *k, int64_t k_stride,
                        const void *v, int64_t v_stride, int src_dtype, const int32_t *positions,
                        const int32_t *slots, const double *inv_freq, int rot_dim, int interleaved,

@@ -266,7 +266,7 @@ int ifx_rope_append_q8(const void *q, int64_t q_stride, const void *k, int64_t k
   AppendQ8Args b{{q, k, v, q_stride, k_stride, v_stride, q_out_stride, positions, slots,
                   inv_freq, q_out, k_cache, v_cache, rot_dim, interleaved != 0, T, Hq, Hkv, D,
                   page_shift_of(page_size), 0},
-                 static_cast<uint32_t *>(scales)};
+                 static_cast<uint32_t *>(scales), 0};
   if (D % 32) return IFX_BAD_GEOMETRY;
   const int rc = append_args(b.a, num_pages);
   if (rc || T == 0) return rc;

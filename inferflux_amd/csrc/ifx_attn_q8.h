@@ -10,6 +10,7 @@ namespace ifx {
 struct AppendQ8Args {
   AppendArgs a;
   uint32_t *scales;
+  int kv_parts;  // parts that K's and V's heads are each shared out in
 };
 hipError_t launch_rope_append_q8(const AppendQ8Args &a, int src_dtype, int q_dtype, hipStream_t s);
 

@@ -5,9 +5,18 @@
 //   a = position * inv_freq;  s = the smallest bf16 >= max |y| / 127,
 //   code_i = rint(y_i / s)
 //
-// K is rotated and both are divided in fp64, so that a code is that of the exact
-// value but for its last bits: an fp32 angle's error of 1e-7 would move one code
-// in 30000, and a value read back by a whole step.
+// K is rotated in fp64, and a code is that of the exact value but for fp64's last
+// bits: an fp32 angle's error of 1e-7 would move one code in 30000, and a value read
+// back by a whole step.  The quotients are first taken in fp32, by a reciprocal,
+// which is off by less than 1e-4 of a step; only a wave in which a value of K lies
+// within that of a border divides in fp64, and what is left of V after the nearest
+// code is exact in fp32.
+//
+// Few tokens: bound by latency, 4.6 us for 8 tokens of 16 / 2 heads of 128, the
+// read of them 3.3.  Many: 5299 tokens of fp16, 40 / 8 heads of 128, take 33 us for
+// 130 MB and the read of them 11 us for 44 MB, where a copy of as many bytes takes
+// 25 and 8.4: what keeps the append from that is V's transposed bytes and K's
+// fp64, angles among it.
 #include "ifx_attn_q8.h"
 #include "ifx_rope.h"
 
@@ -83,9 +92,9 @@ constexpr float kLeast = 0x1p-100f;
 
 }  // namespace
 
-// A workgroup takes NTOK consecutive tokens, and of them a part: K (blockIdx.y
-// 0), V (1) or some of Q's units, pieces of 8 values (and their partners' where
-// pairs lie half a rotation apart).  A row of K or V is shared by LANES lanes, a
+// A workgroup takes NTOK consecutive tokens, and of them a part: some of K's
+// heads (blockIdx.y below kv_parts), of V's (the next kv_parts) or of Q's units,
+// pieces of 8 values (and their partners' where pairs lie half a rotation apart).  A row of K or V is shared by LANES lanes, a
 // piece of 8 values each.
 template <int DT, int SRC, int LANES, int NTOK>
 __global__ __launch_bounds__(256) void k_rope_append_q8(const AppendQ8Args args) {
@@ -100,7 +109,8 @@ __global__ __launch_bounds__(256) void k_rope_append_q8(const AppendQ8Args args)
   const int tid = threadIdx.x, t0 = blockIdx.x * NTOK;
   const int half = a.rot_dim >> 1, angles = half >> 3;  // half: a multiple of 8
   const int pieces = a.D >> 3, sh = a.page_shift, P = 1 << sh;
-  const bool q_part = blockIdx.y > 1, is_v = blockIdx.y == 1;
+  const int kv_parts = args.kv_parts, y = blockIdx.y;
+  const bool q_part = y >= 2 * kv_parts, is_v = !q_part && y >= kv_parts;
   if (tid < NTOK) {
     const int t = t0 + tid, s = t < a.T ? a.slots[t] : -1;
     slot_of[tid] = static_cast<uint32_t>(s) < static_cast<uint32_t>(a.num_slots) ? s : -1;
@@ -126,9 +136,9 @@ __global__ __launch_bounds__(256) void k_rope_append_q8(const AppendQ8Args args)
 
   if (q_part) {
     const int pairs = a.interleaved ? 0 : angles, per_head = pieces - pairs;
-    const int units = NTOK * a.Hq * per_head, parts = gridDim.y - 2;
+    const int units = NTOK * a.Hq * per_head, parts = gridDim.y - 2 * kv_parts;
     const int share = (units + parts - 1) / parts;
-    const int u0 = (blockIdx.y - 2) * share, u1 = min(u0 + share, units);
+    const int u0 = (y - 2 * kv_parts) * share, u1 = min(u0 + share, units);
     const float per_head_inv = 1.0f / per_head, heads_inv = 1.0f / a.Hq;
     for (int u = u0 + tid; u < u1; u += 256) {
       const int w = quotient(u, per_head, per_head_inv), c = u - w * per_head;
@@ -176,12 +186,14 @@ __global__ __launch_bounds__(256) void k_rope_append_q8(const AppendQ8Args args)
   constexpr int kRows = 256 / LANES, kHeads = NTOK > 1 ? kRows / NTOK : 1;
   uint8_t *by_dim = reinterpret_cast<uint8_t *>(&turn);  // V: [head][dim][token], of kHeads
   const int c = tid & (LANES - 1), rows = NTOK * a.Hkv;
+  const int part_rows = ((rows + kRows - 1) / kRows + kv_parts - 1) / kv_parts * kRows;  // whole turns
+  const int from = (is_v ? y - kv_parts : y) * part_rows, until = min(from + part_rows, rows);
   const void *src = is_v ? a.v : a.k;
   const int64_t stride = is_v ? a.v_stride : a.k_stride;
   const bool turned = !is_v && c * 8 < a.rot_dim, paired = turned && !a.interleaved;
   const bool first = c < angles;  // of its pair
   const int other = first ? c + angles : c - angles;
-  for (int r = tid / LANES; r - tid / LANES < rows; r += kRows) {
+  for (int r = from + tid / LANES; r - tid / LANES < until; r += kRows) {
     const int t = r % NTOK, head = r / NTOK;
     const int slot = r < rows && c < pieces ? slot_of[t] : -1;
     Raw8<SRC> lo = {}, hi = {};
@@ -347,12 +359,32 @@ __global__ __launch_bounds__(256) void k_read_rows_q8(const ReadArgs a) {
 }
 
 namespace {
+// Eight tokens a workgroup, whose V is written eight bytes at a time rather than
+// byte by byte, from where there are workgroups enough for the chip.  us of an
+// append and a read with one token / with eight, heads of 128, fp16 rows:
+//    8 /  1 heads  256 tokens 7.5/8.0, 512 9.2/8.2, 1024 13.3/8.5, 2048 21.4/10.0
+//   16 /  2        256 8.0/8.2, 512 10.0/8.6, 1024 14.7/9.2, 4096 40.5/17.3
+//   40 /  8        128 7.8/8.3, 192 8.9/8.6, 512 13.4/11.1, 4096 62.8/40.2
+//   48 / 16         64 8.3/8.3, 128 9.0/8.7, 512 17.8/14.3, 2048 46.7/32.6
+//   32 / 32         64 10.8/8.5, 256 16.3/13.3, 1024 41.0/29.8, 2048 86.6/50.0
+// Of K's and V's heads as few a workgroup as fill the chip, as each makes the
+// angles anew: with a turn / two / four of the workgroup's lanes over them
+//   40 /  8 heads  512 tokens 11.1/13.3/19.2, 2048 24.1/22.5/24.6, 4096 44.5/41.7/40.2
+//   32 / 32        512 19.7/20.3/24.1, 1024 31.2/29.8/31.7, 2048 58.7/52.8/50.0
 template <int DT, int SRC, int LANES>
-void launch(const AppendQ8Args &a, hipStream_t s) {
-  if (a.a.T >= 2048) {
-    IFX_LAUNCH(k_rope_append_q8, (DT, SRC, LANES, 8), dim3((a.a.T + 7) / 8, 7), dim3(256), 0, s, a);
+void launch(AppendQ8Args a, hipStream_t s) {
+  const AppendArgs &p = a.a;
+  if (static_cast<int64_t>(p.T) * (p.Hq + 2 * p.Hkv) >= 7168) {
+    const int turns = (8 * p.Hkv * LANES + 255) / 256;  // of K's heads
+    const int64_t groups = static_cast<int64_t>(p.T + 7) / 8 * turns;
+    const int each = groups < 1024 ? 1 : groups < 2048 ? 2 : 4;
+    const int units = 8 * p.Hq * ((p.D >> 3) - (p.interleaved ? 0 : p.rot_dim >> 4));
+    a.kv_parts = (turns + each - 1) / each;
+    IFX_LAUNCH(k_rope_append_q8, (DT, SRC, LANES, 8),
+               dim3((p.T + 7) / 8, 2 * a.kv_parts + (units + 511) / 512), dim3(256), 0, s, a);
   } else {
-    IFX_LAUNCH(k_rope_append_q8, (DT, SRC, LANES, 1), dim3(a.a.T, 3), dim3(256), 0, s, a);
+    a.kv_parts = 1;
+    IFX_LAUNCH(k_rope_append_q8, (DT, SRC, LANES, 1), dim3(p.T, 3), dim3(256), 0, s, a);
   }
 }
 template <int DT, int SRC>
