@@ -1,15 +1,23 @@
 // attn_rows_q8.hip -- attention over the 8-bit paged cache of requests with few
-// query rows (at most 32 = new tokens x query heads of a group: decode steps,
-// drafts).
+// query rows (at most 32 = new tokens x query heads of a group, or some blocks of
+// 32: decode steps, drafts).
 //
 //   s_j = sk_j q . ck_j,  p_j = 2^(c s_j - m),  l = sum p_j,
 //   o = sum (p_j sv_j) cv_j / l;  ck, cv: codes, sk, sv: scales
 //
-// Bound by HBM: as attn_rows, with half its bytes.  The codes go from the cache
-// into registers, half a kilobyte a half-wave, and are taken to fp16 operands
-// there, one vector instruction a code; K's scales meet the scores, V's the
-// probabilities, of which there are 32 times fewer than codes.  The next
-// tile's loads are on their way during a tile's products.
+// Bound by HBM, at half the 16-bit cache's bytes, or for few requests by latency.
+// As in attn_rows a wave takes every fourth 32 keys of a chunk, and the rows of the
+// key/value head are the columns of both products, transposed.  Codes go from the
+// cache to LDS past the registers, each lane's to places that it alone reads, so
+// that no wave waits for another; from there they are taken to fp16, exactly, half
+// a vector instruction a code.  K's scales meet the scores, V's the probabilities,
+// of which there are 32 times fewer than codes.
+//
+// Codes held in registers until their turn instead spilled: 270 us for 32 requests
+// of 404.5 MB (40 / 8 heads of 128, 531 to 22591 keys) against 99, and 85 with the
+// 16x16 products below: 4.8 TB/s, where a kernel that only copied the tiles took
+// 82 and the 16-bit cache's takes 148.  One request of 3000 keys, 16 / 2 heads:
+// 10.3 us.  768 to 3072 work items instead of 1024: the same.
 #include "ifx_attn_q8.h"
 #include "ifx_attn_rows.h"
 
@@ -23,7 +31,9 @@ __device__ __forceinline__ int key_of_row16(int m) {
   return (m & 3) | ((m >> 1) & 0xC) | ((m & 4) << 2);
 }
 
-constexpr int kFewRows = 16;           // of the 16x16 products
+// Rows of the 16x16 products, which take half the 32x32 ones' work and room: 32
+// requests of 5 rows, 404.5 MB, 82 us with them and 99 without.
+constexpr int kFewRows = 16;
 constexpr int kStep = 32 * kRowWaves;  // keys from a wave's tile to its next
 constexpr int kDepth = 2;              // tiles that are on their way or worked on
 // 16-byte places of a tile in LDS: K, V, and 64 dwords of scales (32 keys', twice).
@@ -54,10 +64,6 @@ __device__ __forceinline__ float quarters_sum(float v) {
   both_sixteens(v, x, y);
   return halves_sum(x + y);
 }
-
-}  // namespace
-
-namespace {
 
 // The workgroup's request, block of 32 of its rows and chunk of its keys.
 struct RowsWork {
@@ -266,8 +272,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows_q8(const At
 
   l = halves_sum(l);
   const auto put = [&](float scale) { put_rows32<D>(red, acc, scale, w.R); };
-  rows_finish<D>(a, w.split, red, sums, n, h == 0, level.of_sums(), l, 1.0f, lds_rows, w.R, w.block, w.z, w.ns, kvh,
-                 put, [&](int t) { return row_sees_nothing(a, w, t); });
+  rows_finish<D>(a, w.split, red, sums, n, h == 0, level.of_sums(), l, 1.0f, lds_rows, w.R, w.block,
+                 w.z, w.ns, kvh, put, [&](int t) { return row_sees_nothing(a, w, t); });
 }
 
 // At most 16 rows: the same with 16x16 products, so that half as many scores are
@@ -421,8 +427,8 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void k_attn_rows16_q8(const 
       __builtin_memcpy(red + ((wave * (D / 4) + 4 * d + g) * w.R + m) * 4, &v, 16);
     }
   };
-  rows_finish<D, 16>(a, w.split, red, sums, m, g == 0, level.of_sums(), l, 1.0f, lds_rows, w.R, w.block, w.z, w.ns, kvh,
-                 put, [&](int t) { return row_sees_nothing(a, w, t); });
+  rows_finish<D, 16>(a, w.split, red, sums, m, g == 0, level.of_sums(), l, 1.0f, lds_rows, w.R, w.block,
+                     w.z, w.ns, kvh, put, [&](int t) { return row_sees_nothing(a, w, t); });
 }
 
 namespace {

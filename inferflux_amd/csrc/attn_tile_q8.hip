@@ -4,11 +4,18 @@
 //   s_j = sk_j q . ck_j,  p_j = 2^(c s_j - m),  l = sum p_j,
 //   o = sum (p_j sv_j) cv_j / l;  ck, cv: codes, sk, sv: scales
 //
-// Bound by the vector units beside the matrix cores.  Work is shared as in
-// attn_tile: 128 rows of a key/value head a workgroup, 32 a wave, stages of 64
-// keys in LDS, both products transposed.  A stage's codes are taken to fp16
-// once for all four waves, on their way from registers, where they have waited
-// for the stage before, to LDS.
+// Work is shared as in attn_tile: 128 rows of a key/value head a workgroup, 32 a
+// wave, stages of 64 keys in LDS, both products transposed.  A stage's codes are
+// copied to LDS past the registers while the stage before is multiplied; then each
+// wave takes a quarter of them to fp16, in LDS too, for all four.
+//
+// Bound by the vector units and LDS beside the matrix cores: 375 vector
+// instructions and 32 products of 32x32x16 for a wave's stage, LDS read and written
+// for about as long.  512 tokens behind 7430, 40 / 8 heads of 128: 124 us, 650
+// TFLOP/s (the 16-bit cache's: 100).  Tried: codes in registers instead of LDS 133
+// to 146, stages of 32 keys 145, three workgroups a CU of 168 registers 213 (they
+// spill), codes taken to fp16 between the products 126; the same without any scales
+// (which is no attention, but a bound) 119.
 #include "ifx_attn_q8.h"
 #include "ifx_attn_tile.h"
 
@@ -21,6 +28,7 @@ namespace {
 constexpr int kThreads = 64 * kTileWaves;
 constexpr int TK = kTileKeys;
 constexpr int kMinChunk = 8;  // stages of a chunk at least (attn_tile)
+
 // Waits for this wave's LDS accesses and then for the workgroup's other waves;
 // copies from memory stay on their way.
 __device__ __forceinline__ void group_barrier() {
@@ -103,7 +111,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void k_attn_tile_q8(con
   Level level;
   float l = 0.0f;
 
-  // ---- stages: memory to registers, and from there as fp16 to LDS
+  // ---- stages: codes from memory to LDS, and from there as fp16 to LDS
   const int sh = a.page_shift, P = 1 << sh;
   const int32_t *table = a.table + static_cast<int64_t>(b) * a.table_width;
   const int wmax = a.table_width - 1, last_page = static_cast<int>(a.num_pages) - 1;

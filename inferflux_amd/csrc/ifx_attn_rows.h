@@ -19,7 +19,8 @@ struct RowSums {
 // lane writes its part of the row's sums, times scale, to red[wave][D / 4][R][4].
 // red later holds [chunk][row].  The R rows are those from row0 on of the
 // request, its row block number `block`, whose keys are cut into ns chunks, this
-// one z.  none(t): whether the rows of new token t see nothing.  kAtOnce: chunks whose sums a thread reads at a time, 4 registers each.
+// one z.  none(t): whether the rows of new token t see nothing.  kAtOnce: chunks
+// whose sums a thread reads at a time, 4 registers each.
 template <int D, int kAtOnce = 24, class Put, class None>
 __device__ __forceinline__ void rows_finish(const AttnArgs &a, const Split &split, float *red,
                                             RowSums &sums, int n, bool lead, float m, float l,
