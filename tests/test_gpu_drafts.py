@@ -357,6 +357,26 @@ def test_verify_corners(dev):
     run_verify(dev, [0, 2, 0], None, [0, 5], p[:2], [0.5] * 2, [0.7] * 3)
 
 
+@pytest.mark.parametrize("V", [4095, 4096, 4097, 8193, 20000])
+@pytest.mark.parametrize("B", [1, 30, 700])
+def test_verify_at_the_ends_of_chunks(dev, V, B):
+    """A few equal weights around multiples of 4096, where rows are cut: numbers
+    exactly at their sums and next to them, children among them."""
+    import torch
+    note(f"verify chunks V={V} B={B}")
+    rng = random.Random(V + B)
+    at = sorted({x for c in range(0, V + 1, 4096) for x in (c - 1, c, c + 1) if 0 <= x < V} | {V - 1})[:16]
+    p = torch.zeros(2 * B, V, device=dev)
+    p[:, at] = 0.0625
+    trees = [[-1, 0]] * B
+    tokens = [rng.choice(at) for _ in range(2 * B)]
+    total = len(at) * 0.0625
+    numbers = [x / 16 / total for x in range(len(at))]
+    au = [rng.choice([0.0, 0.0625, 0.9]) for _ in range(2 * B)]
+    su = [max(rng.choice(numbers) + rng.choice([0.0, 2.0 ** -20, -2.0 ** -20]), 0.0) for _ in range(B)]
+    run_verify(dev, [2] * B, sum(trees, []), tokens, p, au, su)
+
+
 def test_verify_accepts_as_often_as_the_target_says(dev):
     """The token behind the root, accepted or drawn, has the target's
     probabilities: 4000 requests, each count within six of its deviations."""
