@@ -177,7 +177,7 @@ def verify(tokens, cu_q, target_probs, accept_u, sample_u, max_q, parents=None, 
         raise ValueError("verify needs a workspace")
     wp, wn = _workspace(workspace, dev)
     if out is None:
-        out = Verified(*_new(B + 2 * T, torch.int32, tokens, stream).split((B, T, T)))
+        out = Verified(*_new(B + 2 * T, torch.int32, tokens, stream).split_with_sizes((B, T, T)))
     _launch(_lib.load().ifx_verify, "ifx_verify", dev, stream, _i32(tokens, "tokens", T, dev),
             None if parents is None else _i32(parents, "parents", T, dev),
             _i32(cu_q, "cu_q", B + 1, dev), B, T, _count(max_q, "max_q"), tp, ts, dp, ds,
@@ -218,7 +218,7 @@ def plan_kept(cu_q, kv_len, accepted, block_table, free_pages, free_count, page_
     dev, B = _device(kv_len, "kv_len"), kv_len.numel()
     W = _table(block_table, B)
     if out is None:
-        out = KeptPlan(*_new(B + 2, torch.int32, kv_len, stream).split((B, 1, 1)))
+        out = KeptPlan(*_new(B + 2, torch.int32, kv_len, stream).split_with_sizes((B, 1, 1)))
     _launch(_lib.load().ifx_plan_kept, "ifx_plan_kept", dev, stream, _i32(cu_q, "cu_q", B + 1, dev),
             _i32(kv_len, "kv_len", B, dev), _i32(accepted, "accepted", B, dev),
             _i32(block_table, "block_table", B * W, dev), W, _i32(free_pages, "free_pages", 0, dev),
