@@ -15,8 +15,15 @@
 // TFLOP/s (the 16-bit cache's: 100).  Tried: codes in registers instead of LDS 133
 // to 146, stages of 32 keys 145, three workgroups a CU of 168 registers 213 (they
 // spill), codes taken to fp16 between the products 126; the same without any scales
-// (which is no attention, but a bound) 119.
-#include "ifx_attn_q8.h"
+// (which is no attention, but a bound) 119; two stages of codes on their way 129.
+//
+// Requests of up to 32 rows of a key/value head, single tokens next to chunks or
+// trees, would leave three of the four waves idle: their chunks go through
+// rows32_q8, where the waves share the keys.  24 trees of 1 to 38 nodes behind 110
+// to 7302 tokens, 40 / 8 heads: 63 us with it and 78 without; 32 of 2 to 23 nodes
+// 58 and 85; 16 single tokens and 8 chunks of 17 to 304 tokens 70 and 92, of 16 / 2
+// heads 37 and 39.
+#include "ifx_attn_rows_q8.h"
 #include "ifx_attn_tile.h"
 
 namespace ifx {
@@ -41,6 +48,23 @@ __device__ __forceinline__ void group_barrier() {
 
 constexpr int kScales = 2 * TK + 4;  // of a stage: K's, V's, the largest of V's
 
+// LDS: fp16 K and V of a stage, its codes and scales; or the tiles of few rows and
+// their waves' sums, of which a request's chunks' weights take the place.
+template <int D>
+constexpr int tile_bytes() {
+  constexpr int sums = kRowWaves * D * 4 * kRowsMax;
+  constexpr int rows = rows32_bytes<D>() > sums ? rows32_bytes<D>() : sums;
+  constexpr int stages = 2 * TK * D * 3 + 256 + kScales * 4;
+  return stages > rows ? stages : rows;
+}
+// Whether a request's rows go through rows32_q8: a wave's tile has them all, and
+// the weights of its chunks, of kMinChunk units at least, have their place.
+template <int D>
+__device__ __forceinline__ bool few_rows(const AttnArgs &a, const Request &r) {
+  constexpr int most = tile_bytes<D>() / (kRowsMax * 8) * kMinChunk * kRowKeys;
+  return r.nq * a.G <= kRowsMax && rows_keys(a, r) <= most;
+}
+
 }  // namespace
 
 template <int D>
@@ -50,6 +74,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void k_attn_tile_q8(con
   constexpr int kRaw = TK * D / 16;             // of codes
   constexpr int NL = (kRaw + kThreads - 1) / kThreads;
   extern __shared__ u32x4 lds[];                // fp16 [K, V][kPieces], codes and scales as copied, kScales
+  __shared__ RowSums sums;                      // of few rows
   u32x4 *raw = lds + 2 * kPieces;               // [K, V][kRaw], 64 dwords
   float *scales = reinterpret_cast<float *>(raw + 2 * kRaw + 16);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -60,11 +85,18 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void k_attn_tile_q8(con
 
   const Split split = find_item<kMinChunk>(
       a, reinterpret_cast<int2 *>(lds), blockIdx.x / a.Hkv, [&](const Request &r) {
+        if (few_rows<D>(a, r)) return make_int2(1, max(1, (rows_keys(a, r) + kRowKeys - 1) / kRowKeys));
         int keys = r.kv;  // that a tile sees
         if (a.window > 0) keys = min<int64_t>(keys, static_cast<int64_t>(a.window) + kQueryRows + TK);
         return make_int2((r.nq * a.G + kQueryRows - 1) / kQueryRows, max(1, (keys + TK - 1) / TK));
       });
   if (split.chunk == 0) return;
+  if (few_rows<D>(a, split.req)) {
+    RowsWork w;
+    if (rows_work(a, split, kRowsMax, w))
+      rows32_q8<D>(a, w, reinterpret_cast<float *>(lds), sums, tile_slot_bytes<D>(), kvh);
+    return;
+  }
   // the same in all lanes, and kept in scalar registers
   const int b = __builtin_amdgcn_readfirstlane(split.b);
   const int z = __builtin_amdgcn_readfirstlane(split.item / split.tiles);
@@ -311,9 +343,9 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void k_attn_tile_q8(con
 namespace {
 template <int D>
 hipError_t launch_tile(const AttnArgs &a, int items, hipStream_t s) {
-  constexpr int stages = 2 * TK * D * 3 + 256 + kScales * 4, requests = IFX_ATTN_MAX_BATCH * 8;
-  constexpr int bytes = stages > requests ? stages : requests;
-  if constexpr (bytes > 65536 - 256) {
+  constexpr int requests = IFX_ATTN_MAX_BATCH * 8;
+  constexpr int bytes = tile_bytes<D>() > requests ? tile_bytes<D>() : requests;
+  if constexpr (bytes > 65536 - 2048) {  // what a launch may ask for without more ado
     static std::atomic<uint64_t> done{0};
     if (!dry_run()) {
       const hipError_t e = allow_lds(reinterpret_cast<const void *>(&k_attn_tile_q8<D>), bytes, done);

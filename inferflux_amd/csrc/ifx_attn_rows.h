@@ -17,14 +17,14 @@ struct RowSums {
 // Of a wave the lanes with the same n hold row n, one of them (lead) besides the
 // others its maximum m and sum l; exponents are (s - m) c.  put(scale): the
 // lane writes its part of the row's sums, times scale, to red[wave][D / 4][R][4].
-// red later holds [chunk][row].  The R rows are those from row0 on of the
+// red later holds [chunk][row].  slot_bytes: of a chunk's place in the workspace.  The R rows are those from row0 on of the
 // request, its row block number `block`, whose keys are cut into ns chunks, this
 // one z.  none(t): whether the rows of new token t see nothing.  kAtOnce: chunks
 // whose sums a thread reads at a time, 4 registers each.
 template <int D, int kAtOnce = 24, class Put, class None>
 __device__ __forceinline__ void rows_finish(const AttnArgs &a, const Split &split, float *red,
                                             RowSums &sums, int n, bool lead, float m, float l,
-                                            float c, int lds_rows, int R, int block, int z, int ns,
+                                            float c, uint32_t slot_bytes, int R, int block, int z, int ns,
                                             int kvh, Put put, None none) {
   constexpr uint32_t kOut = 1u << 30;  // an offset past the workspace's end: reads zeros
   const int tid = threadIdx.x;
@@ -76,7 +76,6 @@ __device__ __forceinline__ void rows_finish(const AttnArgs &a, const Split &spli
 
   // split: this chunk's sums to its slot, (m, l) of its rows behind them
   const rsrc_t part = make_rsrc(a.part, a.part_bytes);
-  const uint32_t slot_bytes = lds_rows * (D + 4) * 4;
   const uint32_t first = split.slot * a.Hkv + (block * a.Hkv + kvh) * split.ns;  // the block's slots
   const uint32_t slot0 = first * slot_bytes;
   const uint32_t slot = slot0 + z * slot_bytes;

@@ -9,6 +9,15 @@ namespace ifx {
 
 constexpr int kTileWaves = 4;                // of a workgroup
 constexpr int kQueryRows = 32 * kTileWaves;   // its query rows
+// Bytes of the workspace that a wave's sums of a chunk take, and the workgroup's.
+template <int D>
+constexpr uint32_t tile_wave_bytes() {
+  return 32 * D * 4 + 64 * 4 * 2;
+}
+template <int D>
+constexpr uint32_t tile_slot_bytes() {
+  return kTileWaves * tile_wave_bytes<D>();
+}
 
 // Lane n of each half of a wave holds row 128 tile + 32 wave + n of the
 // request's R: maximum m and sum l, and in acc the dims
@@ -54,7 +63,7 @@ __device__ __forceinline__ void tile_finish(const AttnArgs &a, const Split &spli
   // Lanes without a row have their places behind the buffer's end: they write
   // nothing and read zeros.
   const rsrc_t part = make_rsrc(a.part, a.part_bytes);
-  constexpr uint32_t kWaveBytes = 32 * D * 4 + 64 * 4 * 2, kSlotBytes = kTileWaves * kWaveBytes;
+  constexpr uint32_t kWaveBytes = tile_wave_bytes<D>(), kSlotBytes = tile_slot_bytes<D>();
   const uint32_t first = split.slot * a.Hkv + (tile * a.Hkv + kvh) * split.ns;  // the tile's slots
   constexpr uint32_t kOut = 1u << 30;
   const uint32_t out = row0 + 32 * wave + n < R ? 0 : kOut;

@@ -6,8 +6,9 @@ import random
 import pytest
 
 from tests import drafts_ref as ref
+from tests.attn_ref import check
 from tests.test_gpu_attention import counters_clear, gen, i32
-from tests.test_gpu_attention_q8 import dev, make_cache as cache8, run_append  # noqa: F401
+from tests.test_gpu_attention_q8 import dev, make_cache as cache8, run_append, run_paged  # noqa: F401
 from tests.test_gpu_drafts import cu_of, make_cache as cache16, signed, tree_masks
 from tests.test_gpu_parity import note
 
@@ -258,3 +259,53 @@ def test_refusals_on_device(dev):  # noqa: F811
         with pytest.raises((ValueError, TypeError, RuntimeError)):
             call(**change)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("qdt,Hq,Hkv,D,P", [("f16", 16, 2, 128, 64), ("bf16", 40, 8, 128, 16), ("f16", 6, 6, 64, 32),
+                                            ("f16", 9, 3, 96, 16), ("bf16", 8, 2, 256, 128)])
+@pytest.mark.parametrize("window", [0, 100, 2000])
+def test_few_rows_beside_many(dev, qdt, Hq, Hkv, D, P, window):  # noqa: F811
+    """Requests of up to 32 rows of a key/value head in a batch with larger ones:
+    split and whole, at their bound, in windows; the same bits again."""
+    import torch
+    from inferflux_amd import attention as at
+    note(f"q8 few beside many {Hq}/{Hkv} D={D} window={window}")
+    G = Hq // Hkv
+    ctx = [9000, 3000, 40, 0, 700, 129, 0, 2500, 5]
+    new = [1, 60, 33, 2, 32 // G, 200, 0, 32 // G + 1, 1]
+    ws = at.workspace(dev)
+    a, b = (run_paged(dev, qdt, ctx, new, Hq, Hkv, D, P, window=window, workspace=ws) for _ in range(2))
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("B", [3, 70])
+def test_few_rows_beside_trees(dev, B):  # noqa: F811
+    note(f"q8 trees, few beside many B={B}")
+    rng = random.Random(B)
+    new = [64] + [rng.choice([0, 1, 1, 2, 6, 7, 40]) for _ in range(B - 1)]
+    ctx = [rng.choice([0, 50, rng.randint(0, 700)]) for _ in new]
+    ctx[-1], new[-1] = 4000, 1
+    run_paged(dev, "f16", ctx, new, 40, 8, 128, 16, masks=tree_masks(rng, new))
+
+
+def test_few_rows_past_their_bound(dev):  # noqa: F811
+    """A request of few rows and more keys than its chunks' weights have room for
+    goes the way of the others."""
+    import torch
+    from inferflux_amd import attention as at, attention_q8 as q8
+    note("q8 few rows, many keys")
+    D, P, kv = 64, 256, 150000
+    c = q8.kv_cache(kv // P + 1, 1, D, P, device=dev)
+    g = gen(dev, 1)
+    slots = torch.arange(kv, device=dev).int()
+    k = torch.randn(kv, 1, D, generator=g, device=dev)
+    q8.rope_append(torch.zeros(kv, 1, D, device=dev), k, k, slots, slots, c)
+    table = torch.arange(kv // P + 1, device=dev).int().expand(2, -1).contiguous()
+    for few in (130000, 150000):
+        q = torch.randn(41, 1, D, generator=g, device=dev).half()
+        o = q8.paged_attention(q, c, table, i32([0, 1, 41], dev), i32([few, 300], dev), 40, kv, scale=0.3,
+                               workspace=at.workspace(dev))
+        kk, vv = q8.read_rows(c, slots[:few], dtype=torch.float32)
+        want, bound = ref.attend_seen(q[:1], kk.double(), vv.double(), torch.ones(1, few, dtype=torch.bool), 0.3,
+                                      weigh=2.0 ** -11)
+        check(o[:1], want, bound + few * 2.0 ** -30 * 127 * 0.05, "few")
