@@ -50,31 +50,31 @@ constexpr int kScales = 2 * TK + 4;  // of a stage: K's, V's, the largest of V's
 
 // LDS: fp16 K and V of a stage, its codes and scales; or the tiles of few rows and
 // their waves' sums, of which a request's chunks' weights take the place.
-template <int D>
+template <int D, bool MIXED>
 constexpr int tile_bytes() {
   constexpr int sums = kRowWaves * D * 4 * kRowsMax;
   constexpr int rows = rows32_bytes<D>() > sums ? rows32_bytes<D>() : sums;
   constexpr int stages = 2 * TK * D * 3 + 256 + kScales * 4;
-  return stages > rows ? stages : rows;
+  return MIXED && rows > stages ? rows : stages;
 }
 // Whether a request's rows go through rows32_q8: a wave's tile has them all, and
 // the weights of its chunks, of kMinChunk units at least, have their place.
 template <int D>
 __device__ __forceinline__ bool few_rows(const AttnArgs &a, const Request &r) {
-  constexpr int most = tile_bytes<D>() / (kRowsMax * 8) * kMinChunk * kRowKeys;
+  constexpr int most = tile_bytes<D, true>() / (kRowsMax * 8) * kMinChunk * kRowKeys;
   return r.nq * a.G <= kRowsMax && rows_keys(a, r) <= most;
 }
 
 }  // namespace
 
-template <int D>
+// MIXED: of several requests, of which some may have few rows.
+template <int D, bool MIXED = false>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void k_attn_tile_q8(const AttnArgs a) {
   constexpr int ND = D / 32, NS = D / 16;
   constexpr int kPieces = TK * D / 8;           // 16-byte pieces of fp16, of K and of V
   constexpr int kRaw = TK * D / 16;             // of codes
   constexpr int NL = (kRaw + kThreads - 1) / kThreads;
   extern __shared__ u32x4 lds[];                // fp16 [K, V][kPieces], codes and scales as copied, kScales
-  __shared__ RowSums sums;                      // of few rows
   u32x4 *raw = lds + 2 * kPieces;               // [K, V][kRaw], 64 dwords
   float *scales = reinterpret_cast<float *>(raw + 2 * kRaw + 16);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -85,17 +85,20 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void k_attn_tile_q8(con
 
   const Split split = find_item<kMinChunk>(
       a, reinterpret_cast<int2 *>(lds), blockIdx.x / a.Hkv, [&](const Request &r) {
-        if (few_rows<D>(a, r)) return make_int2(1, max(1, (rows_keys(a, r) + kRowKeys - 1) / kRowKeys));
+        if (MIXED && few_rows<D>(a, r)) return make_int2(1, max(1, (rows_keys(a, r) + kRowKeys - 1) / kRowKeys));
         int keys = r.kv;  // that a tile sees
         if (a.window > 0) keys = min<int64_t>(keys, static_cast<int64_t>(a.window) + kQueryRows + TK);
         return make_int2((r.nq * a.G + kQueryRows - 1) / kQueryRows, max(1, (keys + TK - 1) / TK));
       });
   if (split.chunk == 0) return;
-  if (few_rows<D>(a, split.req)) {
-    RowsWork w;
-    if (rows_work(a, split, kRowsMax, w))
-      rows32_q8<D>(a, w, reinterpret_cast<float *>(lds), sums, tile_slot_bytes<D>(), kvh);
-    return;
+  if constexpr (MIXED) {
+    if (few_rows<D>(a, split.req)) {
+      __shared__ RowSums sums;
+      RowsWork w;
+      if (rows_work(a, split, kRowsMax, w))
+        rows32_q8<D>(a, w, reinterpret_cast<float *>(lds), sums, tile_slot_bytes<D>(), kvh);
+      return;
+    }
   }
   // the same in all lanes, and kept in scalar registers
   const int b = __builtin_amdgcn_readfirstlane(split.b);
@@ -341,19 +344,26 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void k_attn_tile_q8(con
 }
 
 namespace {
-template <int D>
+template <int D, bool MIXED>
 hipError_t launch_tile(const AttnArgs &a, int items, hipStream_t s) {
-  constexpr int requests = IFX_ATTN_MAX_BATCH * 8;
-  constexpr int bytes = tile_bytes<D>() > requests ? tile_bytes<D>() : requests;
+  constexpr int requests = MIXED ? IFX_ATTN_MAX_BATCH * 8 : 0;
+  constexpr int bytes = tile_bytes<D, MIXED>() > requests ? tile_bytes<D, MIXED>() : requests;
   if constexpr (bytes > 65536 - 2048) {  // what a launch may ask for without more ado
     static std::atomic<uint64_t> done{0};
     if (!dry_run()) {
-      const hipError_t e = allow_lds(reinterpret_cast<const void *>(&k_attn_tile_q8<D>), bytes, done);
+      const hipError_t e = allow_lds(reinterpret_cast<const void *>(&k_attn_tile_q8<D, MIXED>), bytes, done);
       if (e != hipSuccess) return e;
     }
   }
-  IFX_LAUNCH(k_attn_tile_q8, (D), dim3(a.Hkv * items), dim3(kThreads), bytes, s, a);
+  if constexpr (MIXED)
+    IFX_LAUNCH(k_attn_tile_q8, (D, true), dim3(a.Hkv * items), dim3(kThreads), bytes, s, a);
+  else
+    IFX_LAUNCH(k_attn_tile_q8, (D), dim3(a.Hkv * items), dim3(kThreads), bytes, s, a);
   return last_error();
+}
+template <int D>
+hipError_t launch_tile(const AttnArgs &a, int items, hipStream_t s) {
+  return a.B > 1 ? launch_tile<D, true>(a, items, s) : launch_tile<D, false>(a, items, s);
 }
 }  // namespace
 
