@@ -342,9 +342,9 @@ def test_every_kernel_is_reached(dev):
     lib = _lib.load()
     lib.ifx_launch_log_begin(0)
     for Hq, Hkv, D, P in SHAPES[:5]:
-        for B, n in ((1, 1), (1, 64), (34, 40)):
+        for B, n in ((1, 1), (1, 64), (1, 700), (34, 40)):
             cache = q8.kv_cache(4, Hkv, D, P, device=dev)
-            table = torch.zeros(B, 4, dtype=torch.int32, device=dev)
+            table = torch.zeros(B, 700 // P + 1, dtype=torch.int32, device=dev)
             q = torch.zeros(B * n, Hq, D, dtype=torch.float16, device=dev)
             cu, kv = i32([i * n for i in range(B + 1)], dev), i32([n] * B, dev)
             q8.paged_attention(q, cache, table, cu, kv, n, 60, workspace=at.workspace(dev))
@@ -353,6 +353,7 @@ def test_every_kernel_is_reached(dev):
     for D in (64, 96, 128, 256):
         for k in ("rows16_q8", "rows_q8", "tile_q8"):
             assert f"k_attn_{k}<{D}>" in log, (k, D)
+        assert f"k_attn_tile_q8<{D},1>" in log, D  # of several requests
 
 
 def test_bounds_below_the_lengths(dev):

@@ -540,3 +540,27 @@ def test_step_of_drafts(dev, graph):
     assert accepted > 3
     pages = sorted(free.tolist()[:int(count)] + [x for b in range(B) for x in table[b, :-(-int(ctx[b]) // P)].tolist()])
     assert pages == list(range(40))
+
+
+def test_verify_offsets_past_32_bits(dev):
+    """Rows of probabilities further than 2^32 bytes from the first."""
+    import torch
+    from inferflux_amd import attention as at, drafts
+    note("verify large")
+    V, n, B = 151936, 64, 129
+    T = n * B
+    p = torch.zeros(T, V, device=dev)
+    assert p.nbytes > 1 << 32
+    rng = random.Random(1)
+    p[-n:] = torch.softmax(4 * torch.randn(n, V, generator=gen(dev, 1), device=dev), 1)
+    parents, tokens = ref.tree(rng, n), [5]
+    best = p[-n:].topk(4, 1).indices.tolist()
+    for j in range(1, n):
+        tokens.append(best[parents[j]][rng.randrange(4)])
+    au, su = torch.full((T,), 0.2, device=dev), torch.full((B,), 0.6, device=dev)
+    r = drafts.verify(i32([1] * (T - n) + tokens, dev), i32([n * b for b in range(B + 1)], dev), p, au, su, n,
+                      parents=i32(parents * B, dev), workspace=at.workspace(dev))
+    want = ref.verify(parents, tokens, [0, n], p[-n:].cpu().tolist(), [float(au[0])] * n, [float(su[0])])
+    assert r.accepted.tolist() == [0] * (B - 1) + want[0]
+    assert r.path[-n:].tolist() == want[1] and r.emitted[-n:].tolist() == want[2]
+    assert r.emitted[:-n].eq(-1).all() and r.path[:-n].view(-1, n)[:, 0].eq(0).all()
