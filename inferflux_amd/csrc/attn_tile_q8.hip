@@ -20,8 +20,8 @@
 // Requests of up to 32 rows of a key/value head, single tokens next to chunks or
 // trees, would leave three of the four waves idle: their chunks go through
 // rows32_q8, where the waves share the keys.  24 trees of 1 to 38 nodes behind 110
-// to 7302 tokens, 40 / 8 heads: 63 us with it and 78 without; 32 of 2 to 23 nodes
-// 58 and 85; 16 single tokens and 8 chunks of 17 to 304 tokens 70 and 92, of 16 / 2
+// to 7302 tokens, 40 / 8 heads: 62 us with it and 78 without; 32 of 2 to 23 nodes
+// 56 and 85; 16 single tokens and 8 chunks of 17 to 304 tokens 62 and 92, of 16 / 2
 // heads 37 and 39.
 #include "ifx_attn_rows_q8.h"
 #include "ifx_attn_tile.h"
@@ -48,6 +48,11 @@ __device__ __forceinline__ void group_barrier() {
 
 constexpr int kScales = 2 * TK + 4;  // of a stage: K's, V's, the largest of V's
 
+// Keys of few rows that count as a stage of a row tile, as they take about as long:
+// with 128 / 160 / 192 / 224 / 256 the batches above take 63/62/62/62/66 us (24
+// trees), 58/59/61/56/56 (32 trees) and 70/63/62/62/58 (40 / 8 heads' mixed step).
+constexpr int kFewKeys = 224;
+
 // LDS: fp16 K and V of a stage, its codes and scales; or the tiles of few rows and
 // their waves' sums, of which a request's chunks' weights take the place.
 template <int D, bool MIXED>
@@ -61,7 +66,7 @@ constexpr int tile_bytes() {
 // the weights of its chunks, of kMinChunk units at least, have their place.
 template <int D>
 __device__ __forceinline__ bool few_rows(const AttnArgs &a, const Request &r) {
-  constexpr int most = tile_bytes<D, true>() / (kRowsMax * 8) * kMinChunk * kRowKeys;
+  constexpr int most = tile_bytes<D, true>() / (kRowsMax * 8) * kMinChunk * kFewKeys;
   return r.nq * a.G <= kRowsMax && rows_keys(a, r) <= most;
 }
 
@@ -85,7 +90,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void k_attn_tile_q8(con
 
   const Split split = find_item<kMinChunk>(
       a, reinterpret_cast<int2 *>(lds), blockIdx.x / a.Hkv, [&](const Request &r) {
-        if (MIXED && few_rows<D>(a, r)) return make_int2(1, max(1, (rows_keys(a, r) + kRowKeys - 1) / kRowKeys));
+        if (MIXED && few_rows<D>(a, r)) return make_int2(1, max(1, (rows_keys(a, r) + kFewKeys - 1) / kFewKeys));
         int keys = r.kv;  // that a tile sees
         if (a.window > 0) keys = min<int64_t>(keys, static_cast<int64_t>(a.window) + kQueryRows + TK);
         return make_int2((r.nq * a.G + kQueryRows - 1) / kQueryRows, max(1, (keys + TK - 1) / TK));
@@ -95,7 +100,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void k_attn_tile_q8(con
     if (few_rows<D>(a, split.req)) {
       __shared__ RowSums sums;
       RowsWork w;
-      if (rows_work(a, split, kRowsMax, w))
+      if (rows_work(a, split, kFewKeys, kRowsMax, w))
         rows32_q8<D>(a, w, reinterpret_cast<float *>(lds), sums, tile_slot_bytes<D>(), kvh);
       return;
     }

@@ -38,8 +38,9 @@ struct RowsWork {
 __device__ __forceinline__ int rows_keys(const AttnArgs &a, const Request &r) {
   return a.window > 0 ? min<int64_t>(r.kv, static_cast<int64_t>(a.window) + r.nq + kRowKeys) : r.kv;
 }
-// Chunks are of kRowKeys keys.  False: no such chunk.
-__device__ __forceinline__ bool rows_work(const AttnArgs &a, const Split &split, int lds_rows, RowsWork &w) {
+// Chunks are of `unit` keys, a multiple of 32.  False: no such chunk.
+__device__ __forceinline__ bool rows_work(const AttnArgs &a, const Split &split, int unit, int lds_rows,
+                                          RowsWork &w) {
   w.split = split;
   if (w.split.chunk == 0) return false;
   w.b = w.split.b, w.q0 = w.split.req.q0, w.nq = w.split.req.nq, w.kv = w.split.req.kv;
@@ -48,7 +49,7 @@ __device__ __forceinline__ bool rows_work(const AttnArgs &a, const Split &split,
   w.ctx = w.kv - w.nq;  // position of the first row; below 0 it sees nothing
   w.tree = a.masks != nullptr;
   w.lo0 = a.window > 0 ? max(0, w.ctx - a.window + 1) : 0;
-  const int kbeg = w.lo0 & ~(kRowKeys - 1), kend = w.kv, chunk = w.split.chunk * kRowKeys;
+  const int kbeg = w.lo0 & ~(kRowKeys - 1), kend = w.kv, chunk = w.split.chunk * unit;
   w.ns = kend > kbeg ? (kend - kbeg + chunk - 1) / chunk : 1;
   if (w.z >= w.ns) return false;
   w.zbeg = kbeg + w.z * chunk, w.zend = min(w.zbeg + chunk, kend);
@@ -61,7 +62,7 @@ __device__ __forceinline__ bool rows_work(const AttnArgs &a, float *reqs, int ld
                                      return make_int2((r.nq * a.G + 31) / 32,
                                                       max(1, (rows_keys(a, r) + kRowKeys - 1) / kRowKeys));
                                    }),
-                   lds_rows, w);
+                   kRowKeys, lds_rows, w);
 }
 
 // What a lane's row sees.

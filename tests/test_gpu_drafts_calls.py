@@ -294,14 +294,14 @@ def test_few_rows_past_their_bound(dev):  # noqa: F811
     import torch
     from inferflux_amd import attention as at, attention_q8 as q8
     note("q8 few rows, many keys")
-    D, P, kv = 64, 256, 150000
+    D, P, kv = 64, 256, 300000
     c = q8.kv_cache(kv // P + 1, 1, D, P, device=dev)
     g = gen(dev, 1)
     slots = torch.arange(kv, device=dev).int()
     k = torch.randn(kv, 1, D, generator=g, device=dev)
     q8.rope_append(torch.zeros(kv, 1, D, device=dev), k, k, slots, slots, c)
     table = torch.arange(kv // P + 1, device=dev).int().expand(2, -1).contiguous()
-    for few in (130000, 150000):
+    for few in (130000, 150000, 300000):
         q = torch.randn(41, 1, D, generator=g, device=dev).half()
         o = q8.paged_attention(q, c, table, i32([0, 1, 41], dev), i32([few, 300], dev), 40, kv, scale=0.3,
                                workspace=at.workspace(dev))
