@@ -166,8 +166,8 @@ int attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cache,
                const void *v_cache, const void *scales, int64_t num_pages, int page_size,
                const int32_t *block_table, int table_width, const int32_t *cu_q,
                const int32_t *kv_len, const uint64_t *masks, int B, int T, int Hq, int Hkv, int D,
-               int max_q, int max_kv, float scale, int window, void *out, int64_t out_stride, int out_dtype, void *workspace,
-               int64_t workspace_bytes, void *stream) {
+               int max_q, int max_kv, float scale, int window, void *out, int64_t out_stride,
+               int out_dtype, void *workspace, int64_t workspace_bytes, void *stream) {
   if (!is_elem(dtype) || !is_out(out_dtype)) return IFX_UNSUPPORTED_TYPE;
   const int sh = page_shift_of(page_size);
   if (sh < 0 || num_pages < 1 || num_pages > (INT_MAX >> sh) || table_width < 1 ||

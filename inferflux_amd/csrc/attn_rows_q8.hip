@@ -17,7 +17,7 @@
 // of 404.5 MB (40 / 8 heads of 128, 531 to 22591 keys) against 99, and 85 with the
 // 16x16 products below: 4.8 TB/s, where a kernel that only copied the tiles took
 // 82 and the 16-bit cache's takes 148.  One request of 3000 keys, 16 / 2 heads:
-// 10.3 us.  768 to 3072 work items instead of 1024: the same.
+// 10.3 us.  768 to 2048 work items instead of 1024: the same.
 #include "ifx_attn_rows_q8.h"
 
 namespace ifx {

@@ -17,10 +17,11 @@ struct RowSums {
 // Of a wave the lanes with the same n hold row n, one of them (lead) besides the
 // others its maximum m and sum l; exponents are (s - m) c.  put(scale): the
 // lane writes its part of the row's sums, times scale, to red[wave][D / 4][R][4].
-// red later holds [chunk][row].  slot_bytes: of a chunk's place in the workspace.  The R rows are those from row0 on of the
-// request, its row block number `block`, whose keys are cut into ns chunks, this
-// one z.  none(t): whether the rows of new token t see nothing.  kAtOnce: chunks
-// whose sums a thread reads at a time, 4 registers each.
+// red later holds [chunk][row].  slot_bytes: of a chunk's place in the workspace.
+// The R rows are those from row0 on of the request, its row block number `block`,
+// whose keys are cut into ns chunks, this one z.  none(t): whether the rows of new
+// token t see nothing.  kAtOnce: chunks whose sums a thread reads at a time, 4
+// registers each.
 template <int D, int kAtOnce = 24, class Put, class None>
 __device__ __forceinline__ void rows_finish(const AttnArgs &a, const Split &split, float *red,
                                             RowSums &sums, int n, bool lead, float m, float l,

@@ -94,8 +94,8 @@ constexpr float kLeast = 0x1p-100f;
 
 // A workgroup takes NTOK consecutive tokens, and of them a part: some of K's
 // heads (blockIdx.y below kv_parts), of V's (the next kv_parts) or of Q's units,
-// pieces of 8 values (and their partners' where pairs lie half a rotation apart).  A row of K or V is shared by LANES lanes, a
-// piece of 8 values each.
+// pieces of 8 values (and their partners' where pairs lie half a rotation apart).
+// A row of K or V is shared by LANES lanes, a piece of 8 values each.
 template <int DT, int SRC, int LANES, int NTOK>
 __global__ __launch_bounds__(256) void k_rope_append_q8(const AppendQ8Args args) {
   using T = Elem<DT>;
