@@ -371,6 +371,8 @@ namespace {
 // angles anew: with a turn / two / four of the workgroup's lanes over them
 //   40 /  8 heads  512 tokens 11.1/13.3/19.2, 2048 24.1/22.5/24.6, 4096 44.5/41.7/40.2
 //   32 / 32        512 19.7/20.3/24.1, 1024 31.2/29.8/31.7, 2048 58.7/52.8/50.0
+// and of Q with 512 / 1024 / 1536 / 2560 units of them
+//   40 /  8 heads  2048 tokens 22.6/22.2/21.6/23.2, 4096 40.5/39.6/39.0/38.1, 5299 52.5/52.5/51.2/51.9
 template <int DT, int SRC, int LANES>
 void launch(AppendQ8Args a, hipStream_t s) {
   const AppendArgs &p = a.a;
@@ -379,9 +381,10 @@ void launch(AppendQ8Args a, hipStream_t s) {
     const int64_t groups = static_cast<int64_t>(p.T + 7) / 8 * turns;
     const int each = groups < 1024 ? 1 : groups < 2048 ? 2 : 4;
     const int units = 8 * p.Hq * ((p.D >> 3) - (p.interleaved ? 0 : p.rot_dim >> 4));
+    const int share = each == 1 ? 512 : 1536;  // of Q's units
     a.kv_parts = (turns + each - 1) / each;
     IFX_LAUNCH(k_rope_append_q8, (DT, SRC, LANES, 8),
-               dim3((p.T + 7) / 8, 2 * a.kv_parts + (units + 511) / 512), dim3(256), 0, s, a);
+               dim3((p.T + 7) / 8, 2 * a.kv_parts + (units + share - 1) / share), dim3(256), 0, s, a);
   } else {
     a.kv_parts = 1;
     IFX_LAUNCH(k_rope_append_q8, (DT, SRC, LANES, 1), dim3(p.T, 3), dim3(256), 0, s, a);
