@@ -71,7 +71,7 @@ def _new(shape, dtype, like, stream):
     pending that `stream` does not wait for.  The caller goes on with it on the
     current stream, so the allocator is told of that one."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        return like.new_empty(shape, dtype=dtype)
     user = torch.cuda.current_stream(like.device)
     with torch.cuda.stream(stream):
         t = torch.empty(shape, dtype=dtype, device=like.device)
@@ -106,7 +106,7 @@ def _i32(t, name, n, device):
 def _rows(t, name, T, H, D):
     """Pointer and row stride of rows [T, H, D]: heads of D values one after
     the other, rows any distance apart."""
-    if tuple(t.shape) != (T, H, D):
+    if t.shape != (T, H, D):
         raise ValueError(f"{name} must be [{T}, {H}, {D}], got {list(t.shape)}")
     row, head, one = t.stride()
     if T <= 1:
