@@ -71,7 +71,7 @@ def _new(shape, dtype, like, stream):
     pending that `stream` does not wait for.  The caller goes on with it on the
     current stream, so the allocator is told of that one."""
     if stream is None:
-        return like.new_empty(shape, dtype=dtype)
+        return torch.empty(shape, dtype=dtype, device=like.device)
     user = torch.cuda.current_stream(like.device)
     with torch.cuda.stream(stream):
         t = torch.empty(shape, dtype=dtype, device=like.device)

@@ -21,27 +21,10 @@ from collections import namedtuple
 import torch
 
 from . import _lib
-from .attention import (_DTYPES, _ELEMS, PAGE_SIZES, _count, _device, _i32, _launch, _new, _on, _out,
-                        _rows)
-from .drafts import _all_on, _masks, _table, _workspace
+from .attention import _DTYPES, _ELEMS, PAGE_SIZES, _count, _device, _i32, _launch, _on, _out, _rows
+from .drafts import _all_on, _made, _masks, _q8_caches, _table, _workspace
 
 Q8Cache = namedtuple("Q8Cache", "k v scales")
-
-
-def _q8_caches(c):
-    """(pages, kv heads, page size, head size) of a layer's cache."""
-    k, v, s = c
-    if k.dtype is not torch.int8 or v.dtype is not torch.int8 or s.dtype is not torch.bfloat16:
-        raise TypeError("an 8-bit cache has int8 codes and bfloat16 scales")
-    shape = k.shape
-    if len(shape) == 5:
-        n, h, d16, p, e = shape
-        if e == 16 and v.shape == (n, h, p // 16, d16 * 16, 16) and s.shape == (n, h, p, 2):
-            if not (k.is_contiguous() and v.is_contiguous() and s.is_contiguous()):
-                raise ValueError("the cache must be contiguous")
-            return n, h, p, d16 * 16
-    raise ValueError("the cache must be as kv_cache makes it: [pages, heads, D / 16, page, 16], "
-                     "[pages, heads, page / 16, D, 16] and [pages, heads, page, 2]")
 
 
 def kv_cache(num_pages, kv_heads, head_dim, page_size=64, device="cuda"):
@@ -79,7 +62,7 @@ def rope_append(q, k, v, positions, slots, cache, inv_freq=None, interleaved=Fal
             raise TypeError("inv_freq must be contiguous float64")
         rot, freq = 2 * inv_freq.numel(), _on(inv_freq, "inv_freq", dev).data_ptr()
     if q_out is None:
-        q_out = _new((T, Hq, D), want, cache.k, stream)
+        q_out = _made((T, Hq, D), want, cache.k, stream)
     _all_on(dev, q, k, v, cache.v, cache.scales, q_out)
     qp, qs = _rows(q, "q", T, Hq, D)
     kp, ks = _rows(k, "k", T, Hkv, D)
@@ -98,8 +81,8 @@ def read_rows(cache, slots, dtype=torch.float16, k_out=None, v_out=None, stream=
     they are given), 0 for a slot outside the cache."""
     n, Hkv, P, D = _q8_caches(cache)
     dev, N = _device(cache.k, "cache.k"), slots.numel()
-    k_out = _new((N, Hkv, D), dtype, cache.k, stream) if k_out is None else k_out
-    v_out = _new((N, Hkv, D), k_out.dtype, cache.k, stream) if v_out is None else v_out
+    k_out = _made((N, Hkv, D), dtype, cache.k, stream) if k_out is None else k_out
+    v_out = _made((N, Hkv, D), k_out.dtype, cache.k, stream) if v_out is None else v_out
     if k_out.dtype not in _DTYPES or v_out.dtype is not k_out.dtype:
         raise TypeError("k_out and v_out must be float32, float16 or bfloat16, both the same")
     _all_on(dev, cache.v, cache.scales, k_out, v_out)

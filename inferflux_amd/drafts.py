@@ -37,6 +37,11 @@ Verified = namedtuple("Verified", "accepted path emitted")
 KeptPlan = namedtuple("KeptPlan", "ctx_len free_left status")
 
 
+def _made(shape, dtype, like, stream):
+    """attention's _new, sooner where the output is the current stream's."""
+    return like.new_empty(shape, dtype=dtype) if stream is None else _new(shape, dtype, like, stream)
+
+
 def _masks(t, n, device):
     if t.dtype is not torch.int64:
         raise TypeError("masks must be int64")
@@ -49,6 +54,22 @@ def _all_on(device, *tensors):
     for t in tensors:
         if t.get_device() != device:
             raise ValueError(f"all tensors of a call must be on cuda:{device}")
+
+
+def _q8_caches(c):
+    """(pages, kv heads, page size, head size) of an attention_q8.Q8Cache."""
+    k, v, s = c
+    if k.dtype is not torch.int8 or v.dtype is not torch.int8 or s.dtype is not torch.bfloat16:
+        raise TypeError("an 8-bit cache has int8 codes and bfloat16 scales")
+    shape = k.shape
+    if len(shape) == 5:
+        n, h, d16, p, e = shape
+        if e == 16 and v.shape == (n, h, p // 16, d16 * 16, 16) and s.shape == (n, h, p, 2):
+            if not (k.is_contiguous() and v.is_contiguous() and s.is_contiguous()):
+                raise ValueError("the cache must be contiguous")
+            return n, h, p, d16 * 16
+    raise ValueError("the cache must be as kv_cache makes it: [pages, heads, D / 16, page, 16], "
+                     "[pages, heads, page / 16, D, 16] and [pages, heads, page, 2]")
 
 
 def _f32(t, name, n, device):
@@ -74,7 +95,7 @@ def plan_tree(parents, cu_q, kv_len, out=None, stream=None):
     root.  Rows past a request's first MAX_NODES and behind cu_q[B]: 0."""
     dev, T, B = _device(parents, "parents"), parents.numel(), kv_len.numel()
     if out is None:
-        out = TreePlan(_new((T,), torch.int32, parents, stream), _new((T,), torch.int64, parents, stream))
+        out = TreePlan(_made((T,), torch.int32, parents, stream), _made((T,), torch.int64, parents, stream))
     _launch(_lib.load().ifx_plan_tree, "ifx_plan_tree", dev, stream, _i32(parents, "parents", T, dev),
             _i32(cu_q, "cu_q", B + 1, dev), _i32(kv_len, "kv_len", B, dev), B, T,
             _i32(out.positions, "positions", T, dev), _masks(out.masks, T, dev))
@@ -177,7 +198,7 @@ def verify(tokens, cu_q, target_probs, accept_u, sample_u, max_q, parents=None, 
         raise ValueError("verify needs a workspace")
     wp, wn = _workspace(workspace, dev)
     if out is None:
-        out = Verified(*_new(B + 2 * T, torch.int32, tokens, stream).split_with_sizes((B, T, T)))
+        out = Verified(*_made(B + 2 * T, torch.int32, tokens, stream).split_with_sizes((B, T, T)))
     _launch(_lib.load().ifx_verify, "ifx_verify", dev, stream, _i32(tokens, "tokens", T, dev),
             None if parents is None else _i32(parents, "parents", T, dev),
             _i32(cu_q, "cu_q", B + 1, dev), B, T, _count(max_q, "max_q"), tp, ts, dp, ds,
@@ -193,7 +214,6 @@ def keep_path(cache, block_table, cu_q, kv_len, path, accepted, max_q, stream=No
     v_cache) of attention.kv_cache or an attention_q8.Q8Cache; path [T] and
     accepted [B] as verify returns them."""
     if len(cache) == 3:
-        from .attention_q8 import _q8_caches
         n, Hkv, P, D = _q8_caches(cache)
     else:
         n, Hkv, P, D = _caches(*cache)
@@ -218,7 +238,7 @@ def plan_kept(cu_q, kv_len, accepted, block_table, free_pages, free_count, page_
     dev, B = _device(kv_len, "kv_len"), kv_len.numel()
     W = _table(block_table, B)
     if out is None:
-        out = KeptPlan(*_new(B + 2, torch.int32, kv_len, stream).split_with_sizes((B, 1, 1)))
+        out = KeptPlan(*_made(B + 2, torch.int32, kv_len, stream).split_with_sizes((B, 1, 1)))
     _launch(_lib.load().ifx_plan_kept, "ifx_plan_kept", dev, stream, _i32(cu_q, "cu_q", B + 1, dev),
             _i32(kv_len, "kv_len", B, dev), _i32(accepted, "accepted", B, dev),
             _i32(block_table, "block_table", B * W, dev), W, _i32(free_pages, "free_pages", 0, dev),
