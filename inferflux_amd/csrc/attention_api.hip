@@ -102,6 +102,10 @@ struct PagedPlan {
 // keys, 40 / 8 heads of 128: 162 us with 512, 150 with 768, 148 with 1024, 150
 // with 1536, 153 with 2048.
 //
+// Blocks of rows: as many workgroups as CUs.  us with 256 / 512 / 1024, 3000 keys:
+// 16 / 2 heads, 160 rows 22/22/22, 512 rows 25/26/26, 8-bit 24/26/26; 40 / 8 heads, 150
+// rows, 8-bit 24/26/30; 12000 keys, 160 rows 28/36/36, 512 rows 38/35/35.
+//
 // Fewer where the split sums would not fit the largest workspace.
 //
 // Trees over the 16-bit cache go to attn_tile from 17 rows on, but for a few
@@ -144,7 +148,7 @@ PagedPlan plan_paged(PagedKind kind, int B, int T, int Hq, int Hkv, int D, int m
   const int unit = p.rows ? kRowKeys : attn_tile_min_keys();
   p.row_slots = static_cast<int>(rows < kRowsMax ? rows : kRowsMax);
   const int64_t slot = p.rows ? p.row_slots * (D + 4) * 4 : attn_tile_slot_bytes(D);
-  const int all = p.rows ? 1024 : D == 256 ? 256 : D == 64 ? 768 : 512;
+  const int all = blocks ? 256 : p.rows ? 1024 : D == 256 ? 256 : D == 64 ? 768 : 512;
   int64_t goal = all / Hkv;
   const int64_t use = tiles * ((static_cast<int64_t>(max_kv) + unit - 1) / unit);
   const int64_t fit = (IFX_ATTN_WORKSPACE_BYTES - kCntBytes) / slot / Hkv;

@@ -57,7 +57,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(const AttnA
   const int sh = a.page_shift, P = 1 << sh;
 
   // the workgroup's request and chunk of its keys
-  const Split split = find_item<1>(
+  const Split split = find_item<1, TREE ? kRowsRoot : 0>(
       a, reinterpret_cast<int2 *>(red), blockIdx.x / a.Hkv, [&](const Request &r) {
         int keys = r.kv;
         if (a.window > 0) keys = min<int64_t>(keys, static_cast<int64_t>(a.window) + r.nq + kRowKeys);

@@ -98,7 +98,7 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
   int b, tile, z = 0;  // request, its row tile, its chunk of the keys
   Split split = {};
   if constexpr (PAGED) {
-    split = find_item<kMinChunk>(
+    split = find_item<kMinChunk, 0>(
         a, reinterpret_cast<int2 *>(lds), blockIdx.x / a.Hkv, [&](const Request &r) {
           int keys = r.kv;  // that a tile sees
           if (a.window > 0) keys = min<int64_t>(keys, static_cast<int64_t>(a.window) + kRows + TK);

@@ -88,7 +88,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void k_attn_tile_q8(con
   const int n = lane & 31, h = lane >> 5;
   const int kvh = blockIdx.x % a.Hkv;
 
-  const Split split = find_item<kMinChunk>(
+  const Split split = find_item<kMinChunk, 0>(
       a, reinterpret_cast<int2 *>(lds), blockIdx.x / a.Hkv, [&](const Request &r) {
         if (MIXED && few_rows<D>(a, r)) return make_int2(1, max(1, (rows_keys(a, r) + kFewKeys - 1) / kFewKeys));
         int keys = r.kv;  // that a tile sees

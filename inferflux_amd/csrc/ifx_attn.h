@@ -275,10 +275,21 @@ __device__ __forceinline__ int ceil_div(int x, int d, float r) {
   return q + (rest > 0) + (rest > d) - (rest <= -d);
 }
 
-// Chunks of a request of x stages: of `chunk` (r = 1 / chunk), or of least at least.
-template <int LEAST>
+// Of the 8-bit cache's rows and of trees.  us with a cap of 2 / 3 / 4 sqrt(stages)
+// and with none, one token over 12000 and 50000 keys, then 3 tokens over 12000:
+//   16 / 2 heads of 128  14.9/13.9/13.1/16.1, 23.4/20.4/20.2/39.9, 20.1/19.1/22.5/29.5
+//   40 / 8               15.7/14.8/14.2/18.5, 35.0/32.1/34.1/36.7, 18.5/17.7/17.4/24.6
+// 3000 keys: 11.6/10.6/10.5/10.8; 32 requests of 531 to 22591 the same with each.
+constexpr int kRowsRoot = 24;
+
+// Chunks of a request of x stages: of `chunk` (r = 1 / chunk), or of LEAST at least;
+// with ROOT no more than ROOT / 8 sqrt(x) of them: a chunk less to read for each
+// workgroup is one more to be added by the last, so the two are kept in balance.
+template <int LEAST, int ROOT>
 __device__ __forceinline__ int chunks_of(int x, int chunk, float r) {
-  return min(ceil_div(x, chunk, r), max(x / LEAST, 1));
+  const int n = min(ceil_div(x, chunk, r), max(x / LEAST, 1));
+  if constexpr (ROOT == 0) return n;
+  return min(n, max(1, static_cast<int>(ROOT * 0.125f * __builtin_amdgcn_sqrtf(static_cast<float>(x)))));
 }
 
 // A piece of paged work: item `item` (chunk major) of request b's `tiles` row
@@ -298,7 +309,7 @@ struct Split {
 // s / c + 1 < 2 s / c of them, leaves no more.  Lane l has requests l, l + 64,
 // ...: their places in LDS are neighbours' (with consecutive ones a lane, 1024
 // prompts of 30 to 60 tokens of 16 / 2 heads took 283 us; 177 now).
-template <int MIN_CHUNK, class Work>
+template <int MIN_CHUNK, int ROOT, class Work>
 __device__ __forceinline__ Split find_item(const AttnArgs &a, int2 *reqs, int i, Work work) {
   const int lane = threadIdx.x & 63, B = a.B, goal = a.goal;
   Request req = {0, 0, 0};
@@ -311,7 +322,7 @@ __device__ __forceinline__ Split find_item(const AttnArgs &a, int2 *reqs, int i,
     if (goal >= r.x && r.x > 0) {
       const int share = r.x == 1 ? goal : goal / r.x;  // chunks of a tile
       f.chunk = max(MIN_CHUNK, ceil_div(r.y, share, __builtin_amdgcn_rcpf(static_cast<float>(share))));
-      f.ns = chunks_of<MIN_CHUNK>(r.y, f.chunk, __builtin_amdgcn_rcpf(static_cast<float>(f.chunk)));
+      f.ns = chunks_of<MIN_CHUNK, ROOT>(r.y, f.chunk, __builtin_amdgcn_rcpf(static_cast<float>(f.chunk)));
       f.chunk = (r.y + f.ns - 1) / f.ns;  // of equal length
     }
     f.chunk = i < r.x * f.ns ? __builtin_amdgcn_readfirstlane(f.chunk) : 0;
@@ -348,7 +359,7 @@ __device__ __forceinline__ Split find_item(const AttnArgs &a, int2 *reqs, int i,
       for (int tries = 0; tries < 3 && !fits; ++tries) {
         float items = 0.0f;
         inv = __builtin_amdgcn_rcpf(static_cast<float>(chunk));
-        each([&](int2 r) { items += static_cast<float>(r.x * chunks_of<MIN_CHUNK>(r.y, chunk, inv)); });
+        each([&](int2 r) { items += static_cast<float>(r.x * chunks_of<MIN_CHUNK, ROOT>(r.y, chunk, inv)); });
         items = wave_sum(items);
         fits = items <= goal;
         if (!fits) chunk = max(chunk + 1, static_cast<int>(chunk * (items / goal)));
@@ -360,7 +371,7 @@ __device__ __forceinline__ Split find_item(const AttnArgs &a, int2 *reqs, int i,
   }
   int items = 0, slots = 0;
   each([&](int2 r) {
-    const int ns = chunks_of<MIN_CHUNK>(r.y, chunk, inv);
+    const int ns = chunks_of<MIN_CHUNK, ROOT>(r.y, chunk, inv);
     items += r.x * ns;
     slots += ns > 1 ? r.x * ns : 0;
   });
@@ -373,7 +384,7 @@ __device__ __forceinline__ Split find_item(const AttnArgs &a, int2 *reqs, int i,
   if (B > 64) {  // which of lane who's: a lane for each
     const int b = who + 64 * lane;
     mine = b < B ? reqs[b] : make_int2(0, 1);
-    const int ns = chunks_of<MIN_CHUNK>(mine.y, chunk, inv);
+    const int ns = chunks_of<MIN_CHUNK, ROOT>(mine.y, chunk, inv);
     items = mine.x * ns, slots = ns > 1 ? items : 0;
     const int to = at + wave_scan(items), slot_to = slot + wave_scan(slots);
     row = __builtin_ctzll(__ballot(i < to));
@@ -384,7 +395,7 @@ __device__ __forceinline__ Split find_item(const AttnArgs &a, int2 *reqs, int i,
   f.b = who + 64 * row;
   f.tiles = __builtin_amdgcn_readlane(mine.x, which);
   const int stages = __builtin_amdgcn_readlane(mine.y, which);
-  f.ns = __builtin_amdgcn_readfirstlane(chunks_of<MIN_CHUNK>(stages, chunk, inv));
+  f.ns = __builtin_amdgcn_readfirstlane(chunks_of<MIN_CHUNK, ROOT>(stages, chunk, inv));
   f.chunk = (stages + f.ns - 1) / f.ns;  // of equal length
   f.slot = slot;
   f.item = i - at;

@@ -57,7 +57,7 @@ __device__ __forceinline__ bool rows_work(const AttnArgs &a, const Split &split,
 }
 
 __device__ __forceinline__ bool rows_work(const AttnArgs &a, float *reqs, int lds_rows, RowsWork &w) {
-  return rows_work(a, find_item<1>(a, reinterpret_cast<int2 *>(reqs), blockIdx.x / a.Hkv,
+  return rows_work(a, find_item<1, kRowsRoot>(a, reinterpret_cast<int2 *>(reqs), blockIdx.x / a.Hkv,
                                    [&](const Request &r) {
                                      return make_int2((r.nq * a.G + 31) / 32,
                                                       max(1, (rows_keys(a, r) + kRowKeys - 1) / kRowKeys));
