@@ -215,8 +215,9 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void k_attn_rows16_q8(const 
       __builtin_memcpy(red + ((wave * (D / 4) + 4 * d + g) * w.R + m) * 4, &v, 16);
     }
   };
-  rows_finish<D, 16>(a, w.split, red, sums, m, g == 0, level.of_sums(), l, 1.0f, lds_rows * (D + 4) * 4, w.R, w.block,
-                     w.z, w.ns, kvh, put, [&](int t) { return row_sees_nothing(a, w, t); });
+  rows_finish<D, 16, D == 256>(a, w.split, red, sums, m, g == 0, level.of_sums(), l, 1.0f,
+                               lds_rows * (D + 4) * 4, w.R, w.block, w.z, w.ns, kvh, put,
+                               [&](int t) { return row_sees_nothing(a, w, t); });
 }
 
 namespace {
