@@ -108,38 +108,37 @@ struct PagedPlan {
 //
 // Fewer where the split sums would not fit the largest workspace.
 //
-// Trees over the 16-bit cache go to attn_tile from 17 rows on, but for a few
-// units (requests times key/value heads) of up to 24.  us with attn_rows /
-// attn_tile, with the plan's launch:
-//   16 / 2 heads of 128, 24 rows of 3000 keys  1 request 19.9/21.8, 4 21.3/22.8,
-//     8 25.4/23.1; 32 of 1000 to 9000 51/42.6
-//   40 / 8 heads, 20 rows  1 20.1/22.1, 2 24.4/23.0, 8 42.6/37.4, 32 114/112
-//     30 rows              1 23.1/22.3, 2 28.5/23.0, 8 48.1/36.9, 32 122/113
+// Trees over the 16-bit cache go to attn_rows with up to 32 rows for a few units
+// (requests times key/value heads), 24 for some, else 16.  us with attn_tile /
+// attn_rows, 3000 keys, heads of 128:
+//   40 / 8 heads, 20 rows  2 requests 25.7/20.2, 4 26.6/24.3, 8 42.9/40.4, 16 55/61
+//                 30 rows  1 24.4/21.1, 2 25.4/22.8, 4 26.6/27.5, 8 42.4/45.4, 16 55/67
+//   16 / 2 heads, 24 rows  8 26.0/21.2, 32 42.2/34.2
 // The 8-bit cache's attn_rows is faster up to its 32 rows (30 rows of 40 / 8
-// heads: 1 request 23.4/33.4, 8 38.6/39.5, 32 83/128).
+// heads: 32 requests 83 against 128).
 //
-// More rows as blocks of 32 of attn_rows, where there are so few units that
-// attn_tile's workgroups would leave most of the chip idle (both read the keys
-// once for each block or tile).  us in blocks / with attn_tile, 3000 keys:
-//   16-bit  16 / 1 heads, 640 rows  1 request 24/33, 2 27.5/34, 4 33.5/35
-//                        1024 rows  1 26/33.4, 2 33/34.6, 4 48/36
-//           16 / 2 heads, 160 rows  1 23.5/33, 2 29.7/34.2, 4 31.7/34.8
-//                         512 rows  1 26/33.3, 2 31.5/34.7, 4 38.9/36
-//           16 / 4 heads,  80 rows  1 25/30.5, 2 32.5/31.8, 4 35.7/32.5
-//           40 / 8 heads, 100 rows  1 30.4/32.2, 2 35.4/33.7, 4 47.5/35.1
-//                         200 rows  1 34.7/33.3, 2 39.7/35.2
-//   8-bit   16 / 2 heads, 160 rows  1 23.5/35.8, 4 28.6/36.9, 16 41.5/51
-//           40 / 8 heads,  60 rows  1 25/34, 2 32/35, 4 37/35.4, 16 65/55
-//                         300 rows  1 34.8/37, 2 50/49, 4 64/55
+// More rows as blocks of 32 of attn_rows, where attn_tile's workgroups would leave
+// much of the chip idle (both read the keys once for each block or tile): up to 112
+// blocks, over the 8-bit cache 256 if a unit has no more than 8.  us with attn_tile /
+// in blocks, 3000 keys, by blocks of all units:
+//   16-bit  1 head of K    640 rows   20 32.6/21.9,  80 34.9/28.9;  1024 128 36.1/47.9
+//           16 / 2 heads   160 rows   10 31.9/21.7,  40 34.0/23.5;  512 128 35.7/35.0
+//           40 / 8 heads   100 rows   32 32.4/22.7,  64 33.7/25.1, 128 35.0/34.1
+//                          200 rows   56 33.2/24.0, 112 35.4/33.5, 224 47.0/47.2
+//   8-bit   1 head of K   1024 rows   32 35.6/19.4, 128 38.6/39.5;  640 320 55.1/57.6
+//           16 / 2 heads   160 rows   10 34.8/19.7,  40 37.3/22.2, 160 49.9/40.2
+//           40 / 8 heads   100 rows   32 34.4/21.4, 128 37.8/30.1, 512 65.6/65.4
+//                          200 rows   56 36.3/22.6, 224 49.9/40.8, 896 96.5/109
+//                          640 rows  160 50.2/70.7 (7000 keys)
 enum PagedKind { kPaged16, kTree16, kPaged8 };
 PagedPlan plan_paged(PagedKind kind, int B, int T, int Hq, int Hkv, int D, int max_q, int max_kv) {
   PagedPlan p{};
   const int G = Hq / Hkv;
   const int64_t rows = static_cast<int64_t>(max_q) * G, units = static_cast<int64_t>(B) * Hkv;
-  p.rows = rows <= (kind != kTree16 ? kRowsMax : units <= 8 ? 24 : 16);
-  const int most = kind == kPaged8 ? 60 : units <= 4 ? 80 : 32;
+  p.rows = rows <= (kind != kTree16 ? kRowsMax : units <= 16 ? kRowsMax : units <= 64 ? 24 : 16);
+  const int64_t each = (rows + kRowsMax - 1) / kRowsMax;  // blocks of a unit
   const bool blocks = !p.rows && kind != kPaged16 && rows > kRowsMax &&
-                      units * ((rows + kRowsMax - 1) / kRowsMax) <= most;
+                      (units * each <= 112 || (kind == kPaged8 && each <= 8 && units * each <= 256));
   p.rows |= blocks;
   // row tiles, stages of the longest request that a split must have, bytes of a slot
   const int64_t tiles = p.rows && !blocks

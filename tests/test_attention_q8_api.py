@@ -78,13 +78,14 @@ ATTN = dict(q=F, qs=2048, dt=1, kc=F, vc=F, s=F, pages=100, page=64, table=F, wi
 
 @pytest.mark.parametrize("change,want", [
     ({}, "k_attn_rows_q8<128>"), (dict(max_q=2), "k_attn_rows16_q8<128>"), (dict(dt=2), "k_attn_rows_q8<128>"),
-    # blocks of rows: 4 requests x 2 heads x 7 blocks, and row tiles from 8 on
-    (dict(max_q=28), "k_attn_rows_q8<128>"), (dict(max_q=29), "k_attn_tile_q8<128,1>"),
-    (dict(max_q=5, B=15), "k_attn_rows_q8<128>"), (dict(max_q=5, B=16), "k_attn_tile_q8<128,1>"),
+    # blocks of 32 rows: 112 of all units, 256 where each has 8 at most
+    (dict(max_q=56), "k_attn_rows_q8<128>"), (dict(max_q=57), "k_attn_tile_q8<128,1>"),
+    (dict(max_q=32, B=16), "k_attn_rows_q8<128>"), (dict(max_q=33, B=16), "k_attn_tile_q8<128,1>"),
+    (dict(max_q=5, B=64), "k_attn_rows_q8<128>"), (dict(max_q=5, B=65), "k_attn_tile_q8<128,1>"),
     (dict(D=64, qs=1024, os=1024), "k_attn_rows_q8<64>"), (dict(D=96), "k_attn_rows_q8<96>"),
     (dict(D=256, qs=4096, os=4096, max_q=90), "k_attn_tile_q8<256,1>"), (dict(masks=F), "k_attn_rows_q8<128>"),
     (dict(masks=F, max_q=64), "k_attn_tile_q8<128,1>"), (dict(masks=F, max_q=65), GEOM),
-    (dict(max_q=200, B=1, T=200), "k_attn_tile_q8<128>"),
+    (dict(max_q=256, B=1, T=256), "k_attn_tile_q8<128>"),
     (dict(masks=F, window=9), GEOM), (dict(window=9), "k_attn_rows_q8<128>"), (dict(window=-1), GEOM),
     (dict(T=0, s=None), OK), (dict(s=None), NULL), (dict(s=ODD), GEOM), (dict(kc=ODD), GEOM), (dict(dt=0), TYPE),
     (dict(odt=3), TYPE), (dict(page=24), GEOM), (dict(D=160), GEOM), (dict(Hq=15), GEOM), (dict(scale=0.0), GEOM),

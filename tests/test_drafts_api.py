@@ -58,10 +58,11 @@ ATTN = dict(q=F, qs=2048, dt=1, kc=F, vc=F, pages=100, page=64, table=F, width=5
 
 
 @pytest.mark.parametrize("change,want", [
-    ({}, "k_attn_tile<1,128,1,1>"), (dict(max_q=12, B=3), "k_attn_rows<1,128,1>"), (dict(max_q=20, B=3), "k_attn_rows<1,128,1>"),
-    (dict(max_q=21, B=3), "k_attn_tile<1,128,1,1>"), (dict(max_q=2), "k_attn_rows<1,128,1>"), (dict(max_q=3), "k_attn_rows<1,128,1>"),
-    (dict(max_q=3, B=5), "k_attn_tile<1,128,1,1>"), (dict(max_q=2, B=5), "k_attn_rows<1,128,1>"),
-    (dict(dt=2, max_q=1), "k_attn_rows<2,128,1>"), (dict(dt=2), "k_attn_tile<2,128,1,1>"),
+    # up to 32 rows of 16 units, 24 of 64, 16 of more; blocks of 32 rows: 112 of all units
+    ({}, "k_attn_rows<1,128,1>"), (dict(dt=2), "k_attn_rows<2,128,1>"), (dict(max_q=3, B=32), "k_attn_rows<1,128,1>"),
+    (dict(max_q=4, B=9), "k_attn_tile<1,128,1,1>"), (dict(max_q=2, B=33), "k_attn_rows<1,128,1>"),
+    (dict(max_q=3, B=33), "k_attn_tile<1,128,1,1>"), (dict(max_q=56, B=4), "k_attn_rows<1,128,1>"),
+    (dict(max_q=57, B=4), "k_attn_tile<1,128,1,1>"), (dict(dt=2, max_q=57, B=4), "k_attn_tile<2,128,1,1>"),
     (dict(max_q=64), "k_attn_tile<1,128,1,1>"), (dict(max_q=65), GEOM), (dict(max_q=0), GEOM),
     (dict(masks=None), NULL), (dict(T=0, masks=None), OK), (dict(dt=0), TYPE), (dict(odt=3), TYPE),
     (dict(page=24), GEOM), (dict(D=80), GEOM), (dict(Hq=15), GEOM), (dict(scale=0.0), GEOM),
