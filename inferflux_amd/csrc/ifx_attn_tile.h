@@ -107,7 +107,7 @@ __device__ __forceinline__ void tile_finish(const AttnArgs &a, const Split &spli
     for (int y = 0; y < 8; ++y) {
       const float my = y0 + y < ns ? ml[y].x : -__builtin_inff();
       const float mn = fmaxf(top, my);
-      total = total * weight(top, mn, c) + ml[y].y * weight(my, mn, c);
+      total = __builtin_fmaf(total, weight(top, mn, c), ml[y].y * weight(my, mn, c));
       top = mn;
     }
   }
