@@ -82,7 +82,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void k_attn_rows16_q8(const 
   RowsWork w;
   if (!rows_work(a, red, lds_rows, w)) return;
 
-  const int row = 32 * w.block + min(m, w.R - 1), tok = row / a.G, head = kvh * a.G + row % a.G;
+  const int row = row_of_lane(w, m), tok = row / a.G, head = kvh * a.G + row % a.G;
   const RowSight sight(a, w, tok);
   u32x4 qf[ND];
   {  // steps 2 i and 2 i + 1: the dims 64 i + 16 g + 0 .. 7 and + 8 .. 15, a piece of

@@ -62,12 +62,11 @@ constexpr int tile_bytes() {
   constexpr int stages = 2 * TK * D * 3 + 256 + kScales * 4;
   return MIXED && rows > stages ? rows : stages;
 }
-// Whether a request's rows go through rows32_q8: a wave's tile has them all, and
-// the weights of its chunks, of kMinChunk units at least, have their place.
-template <int D>
-__device__ __forceinline__ bool few_rows(const AttnArgs &a, const Request &r) {
-  constexpr int most = tile_bytes<D, true>() / (kRowsMax * 8) * kMinChunk * kFewKeys;
-  return r.nq * a.G <= kRowsMax && rows_keys(a, r) <= most;
+// Keys of a request that goes through rows32_q8: the weights of its chunks, of
+// kMinChunk units at least, have their place.
+template <int D, bool MIXED>
+constexpr int few_most() {
+  return MIXED ? tile_bytes<D, true>() / (kRowsMax * 8) * kMinChunk * kFewKeys : -1;
 }
 
 }  // namespace
@@ -90,14 +89,11 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void k_attn_tile_q8(con
 
   const Split split = find_item<kMinChunk, 0>(
       a, reinterpret_cast<int2 *>(lds), blockIdx.x / a.Hkv, [&](const Request &r) {
-        if (MIXED && few_rows<D>(a, r)) return make_int2(1, max(1, (rows_keys(a, r) + kFewKeys - 1) / kFewKeys));
-        int keys = r.kv;  // that a tile sees
-        if (a.window > 0) keys = min<int64_t>(keys, static_cast<int64_t>(a.window) + kQueryRows + TK);
-        return make_int2((r.nq * a.G + kQueryRows - 1) / kQueryRows, max(1, (keys + TK - 1) / TK));
+        return tile_units_q8(a, r, kQueryRows, kFewKeys, few_most<D, MIXED>());
       });
   if (split.chunk == 0) return;
   if constexpr (MIXED) {
-    if (few_rows<D>(a, split.req)) {
+    if (few_rows(a, split.req, few_most<D, true>())) {
       __shared__ RowSums sums;
       RowsWork w;
       if (rows_work(a, split, kFewKeys, kRowsMax, w))

@@ -5,6 +5,7 @@
 
 #include "ifx_attn_q8.h"
 #include "ifx_attn_rows.h"
+#include "ifx_attn_work.h"
 
 namespace ifx {
 
@@ -28,40 +29,9 @@ constexpr int rows32_bytes() {
   return kRowWaves * kDepth * tile_pieces<D>() * 16;
 }
 
-// The workgroup's request, block of 32 of its rows and chunk of its keys.
-struct RowsWork {
-  Split split;
-  int b, q0, nq, kv, R, ctx, lo0, block, z, ns, zbeg, zend;  // R: rows of the block
-  bool tree;
-};
-// Keys of a request that a block has to go through at most.
-__device__ __forceinline__ int rows_keys(const AttnArgs &a, const Request &r) {
-  return a.window > 0 ? min<int64_t>(r.kv, static_cast<int64_t>(a.window) + r.nq + kRowKeys) : r.kv;
-}
-// Chunks are of `unit` keys, a multiple of 32.  False: no such chunk.
-__device__ __forceinline__ bool rows_work(const AttnArgs &a, const Split &split, int unit, int lds_rows,
-                                          RowsWork &w) {
-  w.split = split;
-  if (w.split.chunk == 0) return false;
-  w.b = w.split.b, w.q0 = w.split.req.q0, w.nq = w.split.req.nq, w.kv = w.split.req.kv;
-  w.z = w.split.item / w.split.tiles, w.block = w.split.item - w.z * w.split.tiles;
-  w.R = min(w.nq * a.G - 32 * w.block, lds_rows);
-  w.ctx = w.kv - w.nq;  // position of the first row; below 0 it sees nothing
-  w.tree = a.masks != nullptr;
-  w.lo0 = a.window > 0 ? max(0, w.ctx - a.window + 1) : 0;
-  const int kbeg = w.lo0 & ~(kRowKeys - 1), kend = w.kv, chunk = w.split.chunk * unit;
-  w.ns = kend > kbeg ? (kend - kbeg + chunk - 1) / chunk : 1;
-  if (w.z >= w.ns) return false;
-  w.zbeg = kbeg + w.z * chunk, w.zend = min(w.zbeg + chunk, kend);
-  return true;
-}
-
 __device__ __forceinline__ bool rows_work(const AttnArgs &a, float *reqs, int lds_rows, RowsWork &w) {
   return rows_work(a, find_item<1, kRowsRoot>(a, reinterpret_cast<int2 *>(reqs), blockIdx.x / a.Hkv,
-                                   [&](const Request &r) {
-                                     return make_int2((r.nq * a.G + 31) / 32,
-                                                      max(1, (rows_keys(a, r) + kRowKeys - 1) / kRowKeys));
-                                   }),
+                                   [&](const Request &r) { return rows_units(a, r); }),
                    kRowKeys, lds_rows, w);
 }
 
@@ -118,8 +88,7 @@ __device__ __forceinline__ void rows32_q8(const AttnArgs &a, const RowsWork &w, 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int sh = a.page_shift, P = 1 << sh;
 
-  // this lane's row; rows behind the last repeat it
-  const int row = 32 * w.block + min(n, w.R - 1), tok = row / a.G, head = kvh * a.G + row % a.G;
+  const int row = row_of_lane(w, n), tok = row / a.G, head = kvh * a.G + row % a.G;
   const RowSight sight(a, w, tok);
   u32x4 qf[NS];
   {  // of step s the dims 32 (s / 2) + 16 h + 8 (s % 2), as K's pieces hold them
