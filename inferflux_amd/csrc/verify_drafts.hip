@@ -139,7 +139,8 @@ __device__ __forceinline__ Place find_place(double mine, double share, double ta
 template <int DT>
 __global__ __launch_bounds__(kThreads, 4) void k_verify(const VerifyArgs a) {
   __shared__ double sums[kThreads / 64 + 1], whole[kThreads / 64];
-  __shared__ int found[2];
+  __shared__ int found[2];  // find_place's, which clears it without waiting for who still reads it
+  __shared__ int place_token;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = blockIdx.x / a.chunks, z = blockIdx.x - b * a.chunks;
   const int r0 = min(max(a.cu[b], 0), a.T), rows = max(min(max(a.cu[b + 1], 0), a.T) - r0, 0);
@@ -326,11 +327,11 @@ __global__ __launch_bounds__(kThreads, 4) void k_verify(const VerifyArgs a) {
             }
           }
         }
-        found[0] = token;
+        place_token = token;
       }
       __syncthreads();
       // rounding apart the sum passes `rest` in one of them; else the last weight's
-      if (place.thread >= 0) drawn = found[0];
+      if (place.thread >= 0) drawn = place_token;
       passed = place.passed;
       run += place.total;
     }
