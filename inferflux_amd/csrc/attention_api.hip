@@ -86,6 +86,7 @@ constexpr int64_t kCntBytes = kSplitCntBytes;
 struct PagedPlan {
   bool rows;         // attn_rows, else attn_tile
   int row_slots;     // attn_rows: rows of a workgroup
+  int blocks;        // attn_rows: of max_q rows
   int goal, items;   // AttnArgs; workgroups of a key/value head
   int64_t bytes;     // of workspace
 };
@@ -145,6 +146,7 @@ PagedPlan plan_paged(PagedKind kind, int B, int T, int Hq, int Hkv, int D, int m
                             ? B
                             : static_cast<int64_t>(T) * G / (blocks ? kRowsMax : attn_tile_rows(D)) + B;
   const int unit = p.rows ? kRowKeys : attn_tile_min_keys();
+  p.blocks = static_cast<int>(each);
   p.row_slots = static_cast<int>(rows < kRowsMax ? rows : kRowsMax);
   const int64_t slot = p.rows ? p.row_slots * (D + 4) * 4 : attn_tile_slot_bytes(D);
   const int all = blocks ? 256 : p.rows ? 1024 : D == 256 ? 256 : D == 64 ? 768 : 512;
@@ -210,9 +212,9 @@ int attn_paged(const void *q, int64_t q_stride, int dtype, const void *k_cache,
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (scales)
-    return status_of(p.rows ? launch_attn_rows_q8(a, D, p.row_slots, p.items, s)
+    return status_of(p.rows ? launch_attn_rows_q8(a, D, p.row_slots, p.blocks, p.items, s)
                             : launch_attn_tile_q8(a, D, p.items, s));
-  if (p.rows) return status_of(launch_attn_rows(a, dtype, D, p.row_slots, p.items, s));
+  if (p.rows) return status_of(launch_attn_rows(a, dtype, D, p.row_slots, p.blocks, p.items, s));
   return status_of(launch_attn_tile(a, dtype, D, true, p.items, s));
 }
 

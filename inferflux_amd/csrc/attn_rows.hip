@@ -44,9 +44,10 @@ __device__ __forceinline__ PieceMask piece_mask(int key, int lo, int hi) {
 }  // namespace
 
 // TREE: rows see the cached tokens and the nodes of their masks; more than 32
-// are blocks of 32, the keys of each split by themselves.
+// are blocks of 32, the keys of each split by themselves, `most` blocks of a request
+// at most.
 template <int DT, int D, bool TREE = false>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(const AttnArgs a, int lds_rows) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(const AttnArgs a, int lds_rows, int most) {
   using T = Elem<DT>;
   constexpr int ND = D / 32, NS = D / 16;
   extern __shared__ float red[];  // [wave][D / 4][row][4]; at first the requests
@@ -61,7 +62,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(const AttnA
       a, reinterpret_cast<int2 *>(red), blockIdx.x / a.Hkv, [&](const Request &r) {
         int keys = r.kv;
         if (a.window > 0) keys = min<int64_t>(keys, static_cast<int64_t>(a.window) + r.nq + kRowKeys);
-        const int blocks = TREE ? (r.nq * a.G + 31) / 32 : r.nq > 0 ? 1 : 0;
+        const int blocks = TREE ? min((r.nq * a.G + 31) / 32, most) : r.nq > 0 ? 1 : 0;
         return make_int2(blocks, max(1, (keys + kRowKeys - 1) / kRowKeys));
       });
   if (split.chunk == 0) return;
@@ -240,7 +241,7 @@ namespace {
 constexpr int kMaxLds = 65536 - 2048;  // what a launch may ask for without more ado
 
 template <int DT, int D, bool TREE>
-hipError_t launch_rows(const AttnArgs &a, int max_rows, int items, hipStream_t s) {
+hipError_t launch_rows(const AttnArgs &a, int max_rows, int blocks, int items, hipStream_t s) {
   constexpr int row_bytes = kWaves * D * 4;  // LDS of a row: the waves' sums
   if constexpr (row_bytes * kRowsMax > kMaxLds) {
     static std::atomic<uint64_t> done{0};
@@ -255,33 +256,33 @@ hipError_t launch_rows(const AttnArgs &a, int max_rows, int items, hipStream_t s
   if (bytes < a.B * 8) bytes = a.B * 8;
   if (bytes < a.goal * max_rows * 8) bytes = a.goal * max_rows * 8;
   if constexpr (TREE)
-    IFX_LAUNCH(k_attn_rows, (DT, D, true), dim3(a.Hkv * items), dim3(64 * kWaves), bytes, s, a, max_rows);
+    IFX_LAUNCH(k_attn_rows, (DT, D, true), dim3(a.Hkv * items), dim3(64 * kWaves), bytes, s, a, max_rows, blocks);
   else
-    IFX_LAUNCH(k_attn_rows, (DT, D), dim3(a.Hkv * items), dim3(64 * kWaves), bytes, s, a, max_rows);
+    IFX_LAUNCH(k_attn_rows, (DT, D), dim3(a.Hkv * items), dim3(64 * kWaves), bytes, s, a, max_rows, blocks);
   return last_error();
 }
 template <int DT, bool TREE>
-hipError_t launch_rows(const AttnArgs &a, int D, int max_rows, int items, hipStream_t s) {
+hipError_t launch_rows(const AttnArgs &a, int D, int max_rows, int blocks, int items, hipStream_t s) {
   switch (D) {
-    case 64: return launch_rows<DT, 64, TREE>(a, max_rows, items, s);
-    case 96: return launch_rows<DT, 96, TREE>(a, max_rows, items, s);
-    case 128: return launch_rows<DT, 128, TREE>(a, max_rows, items, s);
-    default: return launch_rows<DT, 256, TREE>(a, max_rows, items, s);
+    case 64: return launch_rows<DT, 64, TREE>(a, max_rows, blocks, items, s);
+    case 96: return launch_rows<DT, 96, TREE>(a, max_rows, blocks, items, s);
+    case 128: return launch_rows<DT, 128, TREE>(a, max_rows, blocks, items, s);
+    default: return launch_rows<DT, 256, TREE>(a, max_rows, blocks, items, s);
   }
 }
 template <int DT>
-hipError_t launch_rows(const AttnArgs &a, int D, int max_rows, int items, hipStream_t s) {
-  return a.masks ? launch_rows<DT, true>(a, D, max_rows, items, s)
-                 : launch_rows<DT, false>(a, D, max_rows, items, s);
+hipError_t launch_rows(const AttnArgs &a, int D, int max_rows, int blocks, int items, hipStream_t s) {
+  return a.masks ? launch_rows<DT, true>(a, D, max_rows, blocks, items, s)
+                 : launch_rows<DT, false>(a, D, max_rows, blocks, items, s);
 }
 }  // namespace
 
 int attn_rows_max_goal(int max_rows) { return kMaxLds / 8 / max_rows; }
 
-hipError_t launch_attn_rows(const AttnArgs &a, int dtype, int D, int max_rows, int items,
+hipError_t launch_attn_rows(const AttnArgs &a, int dtype, int D, int max_rows, int blocks, int items,
                             hipStream_t s) {
-  return dtype == IFX_ATTN_F16 ? launch_rows<IFX_ATTN_F16>(a, D, max_rows, items, s)
-                               : launch_rows<IFX_ATTN_BF16>(a, D, max_rows, items, s);
+  return dtype == IFX_ATTN_F16 ? launch_rows<IFX_ATTN_F16>(a, D, max_rows, blocks, items, s)
+                               : launch_rows<IFX_ATTN_BF16>(a, D, max_rows, blocks, items, s);
 }
 
 }  // namespace ifx

@@ -54,13 +54,13 @@ __device__ __forceinline__ float quarters_sum(float v) {
 }  // namespace
 
 template <int D>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows_q8(const AttnArgs a, int lds_rows) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows_q8(const AttnArgs a, int lds_rows, int blocks) {
   // Aligned, as copies of 16 bytes a lane to LDS need it: behind 1028 bytes of
   // other data they left parts of pieces wrong where many workgroups ran.
   extern __shared__ __attribute__((aligned(16))) float red[];
   __shared__ RowSums sums;
   RowsWork w;
-  if (rows_work(a, red, lds_rows, w))
+  if (rows_work(a, red, lds_rows, blocks, w))
     rows32_q8<D>(a, w, red, sums, lds_rows * (D + 4) * 4, blockIdx.x % a.Hkv);
 }
 
@@ -70,7 +70,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows_q8(const At
 // (register r of product i), which are the B operand of O^T = V^T P^T as they
 // stand; of O^T the dims 16 d + 4 g + r.
 template <int D>
-__global__ __launch_bounds__(256, D == 256 ? 2 : 4) void k_attn_rows16_q8(const AttnArgs a, int lds_rows) {
+__global__ __launch_bounds__(256, D == 256 ? 2 : 4) void k_attn_rows16_q8(const AttnArgs a, int lds_rows,
+                                                                             int blocks) {
   constexpr int ND = D / 32, NB = D / 16;
   // at first the requests, then [wave][piece], then [wave][D / 4][row][4]
   extern __shared__ __attribute__((aligned(16))) float red[];
@@ -80,7 +81,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void k_attn_rows16_q8(const 
   const int kvh = blockIdx.x % a.Hkv;
   const int sh = a.page_shift, P = 1 << sh;
   RowsWork w;
-  if (!rows_work(a, red, lds_rows, w)) return;
+  if (!rows_work(a, red, lds_rows, blocks, w)) return;
 
   const int row = row_of_lane(w, m), tok = row / a.G, head = kvh * a.G + row % a.G;
   const RowSight sight(a, w, tok);
@@ -222,7 +223,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void k_attn_rows16_q8(const 
 
 namespace {
 template <int D, bool FEW>
-hipError_t launch_rows(const AttnArgs &a, int max_rows, int items, hipStream_t s) {
+hipError_t launch_rows(const AttnArgs &a, int max_rows, int blocks, int items, hipStream_t s) {
   constexpr int row_bytes = kRowWaves * D * 4;  // LDS of a row: the waves' sums
   constexpr int rows = FEW ? kFewRows : kRowsMax;
   constexpr int ring_bytes = FEW ? kRowWaves * tile_pieces<D>() * 16 : rows32_bytes<D>();
@@ -243,24 +244,25 @@ hipError_t launch_rows(const AttnArgs &a, int max_rows, int items, hipStream_t s
     if (bytes < need) bytes = need;
   const dim3 grid(a.Hkv * items), block(64 * kRowWaves);
   if constexpr (FEW)
-    IFX_LAUNCH(k_attn_rows16_q8, (D), grid, block, bytes, s, a, max_rows);
+    IFX_LAUNCH(k_attn_rows16_q8, (D), grid, block, bytes, s, a, max_rows, blocks);
   else
-    IFX_LAUNCH(k_attn_rows_q8, (D), grid, block, bytes, s, a, max_rows);
+    IFX_LAUNCH(k_attn_rows_q8, (D), grid, block, bytes, s, a, max_rows, blocks);
   return last_error();
 }
 template <int D>
-hipError_t launch_rows(const AttnArgs &a, int max_rows, int items, hipStream_t s) {
-  return max_rows <= kFewRows ? launch_rows<D, true>(a, max_rows, items, s)
-                              : launch_rows<D, false>(a, max_rows, items, s);
+hipError_t launch_rows(const AttnArgs &a, int max_rows, int blocks, int items, hipStream_t s) {
+  return max_rows <= kFewRows ? launch_rows<D, true>(a, max_rows, blocks, items, s)
+                              : launch_rows<D, false>(a, max_rows, blocks, items, s);
 }
 }  // namespace
 
-hipError_t launch_attn_rows_q8(const AttnArgs &a, int D, int max_rows, int items, hipStream_t s) {
+hipError_t launch_attn_rows_q8(const AttnArgs &a, int D, int max_rows, int blocks, int items,
+                               hipStream_t s) {
   switch (D) {
-    case 64: return launch_rows<64>(a, max_rows, items, s);
-    case 96: return launch_rows<96>(a, max_rows, items, s);
-    case 128: return launch_rows<128>(a, max_rows, items, s);
-    default: return launch_rows<256>(a, max_rows, items, s);
+    case 64: return launch_rows<64>(a, max_rows, blocks, items, s);
+    case 96: return launch_rows<96>(a, max_rows, blocks, items, s);
+    case 128: return launch_rows<128>(a, max_rows, blocks, items, s);
+    default: return launch_rows<256>(a, max_rows, blocks, items, s);
   }
 }
 

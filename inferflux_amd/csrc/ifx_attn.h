@@ -175,7 +175,7 @@ struct AttnArgs {
   const uint64_t *masks;   // trees: per row, its request's nodes that it sees
   const uint32_t *scales;  // 8-bit cache: K's and V's of a token and head
 };
-// With the argument behind it within three of the scalar cache's lines: a fourth
+// With the arguments behind it within three of the scalar cache's lines: a fourth
 // costs a kernel a miss: 0.2 us of 10.4 for one request of 3000 tokens.
 static_assert(sizeof(AttnArgs) <= 3 * 64 - 8, "a kernel's arguments");
 constexpr int kAttnThreads = 256;  // of a workgroup of every attention kernel
@@ -482,7 +482,8 @@ __device__ __forceinline__ Tile find_tile(const AttnArgs &a, int *reqs, int i, T
   return f;
 }
 
-hipError_t launch_attn_rows(const AttnArgs &a, int dtype, int D, int max_rows, int items,
+// max_rows: of a block; blocks: of a request at most, as the items are counted.
+hipError_t launch_attn_rows(const AttnArgs &a, int dtype, int D, int max_rows, int blocks, int items,
                             hipStream_t s);
 int attn_rows_max_goal(int max_rows);
 hipError_t launch_attn_tile(const AttnArgs &a, int dtype, int D, bool paged, int items,

@@ -24,7 +24,8 @@ struct ReadArgs {
 };
 hipError_t launch_read_rows_q8(const ReadArgs &a, int out_dtype, hipStream_t s);
 
-hipError_t launch_attn_rows_q8(const AttnArgs &a, int D, int max_rows, int items, hipStream_t s);
+hipError_t launch_attn_rows_q8(const AttnArgs &a, int D, int max_rows, int blocks, int items,
+                               hipStream_t s);
 hipError_t launch_attn_tile_q8(const AttnArgs &a, int D, int items, hipStream_t s);
 
 // 16 or 4 bytes a lane from memory to 64 consecutive places in LDS.

@@ -29,9 +29,9 @@ constexpr int rows32_bytes() {
   return kRowWaves * kDepth * tile_pieces<D>() * 16;
 }
 
-__device__ __forceinline__ bool rows_work(const AttnArgs &a, float *reqs, int lds_rows, RowsWork &w) {
+__device__ __forceinline__ bool rows_work(const AttnArgs &a, float *reqs, int lds_rows, int blocks, RowsWork &w) {
   return rows_work(a, find_item<1, kRowsRoot>(a, reinterpret_cast<int2 *>(reqs), blockIdx.x / a.Hkv,
-                                   [&](const Request &r) { return rows_units(a, r); }),
+                                   [&](const Request &r) { return rows_units(a, r, blocks); }),
                    kRowKeys, lds_rows, w);
 }
 

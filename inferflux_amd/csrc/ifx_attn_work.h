@@ -26,9 +26,12 @@ IFX_HOST_TOO int rows_keys(const AttnArgs &a, const Request &r) {
   return window_keys(a, r, static_cast<int64_t>(r.nq) + kRowKeys);
 }
 
-// {blocks of 32 rows, stages} in the kernels of few rows.
-IFX_HOST_TOO int2 rows_units(const AttnArgs &a, const Request &r) {
-  return make_int2((r.nq * a.G + kRowsMax - 1) / kRowsMax, stages_of(rows_keys(a, r), kRowKeys));
+// {blocks of 32 rows, stages} in the kernels of few rows.  A request has no more
+// than `most` blocks, those of max_q rows: the launch has workgroups for as many, and
+// a request of more rows must not take the others'.
+IFX_HOST_TOO int2 rows_units(const AttnArgs &a, const Request &r, int most) {
+  const int blocks = (r.nq * a.G + kRowsMax - 1) / kRowsMax;
+  return make_int2(blocks < most ? blocks : most, stages_of(rows_keys(a, r), kRowKeys));
 }
 
 // Whether a request goes as one block of rows among row tiles: it has no more rows

@@ -71,8 +71,12 @@ int main() {
           for (size_t b = 0; b < t.kv.size(); ++b) {
             const Request r{q0, t.nq[b], t.kv[b]};
             q0 += t.nq[b];
-            items(t, a, r, rows_units(a, r), kRowKeys, kRowsMax, "few rows");
-            if (r.nq * G <= 16) items(t, a, r, rows_units(a, r), kRowKeys, std::max(r.nq * G, 1), "16 rows");
+            for (int most : {1, 2, 1 << 20}) {
+              const int2 units = rows_units(a, r, most);
+              CHECK(units.x <= most, "%s: %d blocks where there are %d", t.name, units.x, most);
+              items(t, a, r, units, kRowKeys, kRowsMax, "few rows");
+              if (r.nq * G <= 16) items(t, a, r, units, kRowKeys, std::max(r.nq * G, 1), "16 rows");
+            }
             const int2 mixed = tile_units_q8(a, r, kQueryRows, kFew, kMost);
             const int2 tiles = tile_units_q8(a, r, kQueryRows, kFew, -1);
             if (few_rows(a, r, kMost)) {
