@@ -227,9 +227,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(const AttnA
   }
 
   l = halves_sum(l);
-  const auto put = [&](float scale) { put_rows32<D>(red, acc, scale, R); };
+  const float top = rows_top(sums, wave, n, h == 0, m, l);
+  if (n < R) put_rows32<D>(red, acc, weight(m, top, a.c), R, n, h, wave);
   const uint32_t slot_bytes = lds_rows * (D + 4) * 4;
-  rows_finish<D, 24, TREE>(a, split, red, sums, n, h == 0, m, l, a.c, slot_bytes, R, block, z, ns, kvh, put, [&](int t) {
+  rows_finish<D, 24, TREE>(a, split, red, sums, n, h == 0, top, a.c, slot_bytes, R, block, z, ns, kvh, [&](int t) {
     if constexpr (TREE)
       return Sight<true>{0, 0, ctx, node_bits(a, q0 + t, nq)}.nothing();
     else

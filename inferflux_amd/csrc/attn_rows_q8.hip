@@ -209,16 +209,17 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void k_attn_rows16_q8(const 
   }
 
   l = quarters_sum(l);
-  const auto put = [&](float scale) {
+  const float level_of = level.of_sums(), top = rows_top(sums, wave, m, g == 0, level_of, l);
+  if (m < w.R) {
+    const float scale = weight(level_of, top, 1.0f);
 #pragma unroll
     for (int d = 0; d < NB; ++d) {
       const f32x4 v = acc[d] * scale;
       __builtin_memcpy(red + ((wave * (D / 4) + 4 * d + g) * w.R + m) * 4, &v, 16);
     }
-  };
-  rows_finish<D, 16, D == 256>(a, w.split, red, sums, m, g == 0, level.of_sums(), l, 1.0f,
-                               lds_rows * (D + 4) * 4, w.R, w.block, w.z, w.ns, kvh, put,
-                               [&](int t) { return row_sees_nothing(a, w, t); });
+  }
+  rows_finish<D, 16, D == 256>(a, w.split, red, sums, m, g == 0, top, 1.0f, lds_rows * (D + 4) * 4, w.R,
+                               w.block, w.z, w.ns, kvh, [&](int t) { return row_sees_nothing(a, w, t); });
 }
 
 namespace {

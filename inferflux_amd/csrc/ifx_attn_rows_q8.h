@@ -207,9 +207,10 @@ __device__ __forceinline__ void rows32_q8(const AttnArgs &a, const RowsWork &w, 
   }
 
   l = halves_sum(l);
-  const auto put = [&](float scale) { put_rows32<D>(red, acc, scale, w.R); };
-  rows_finish<D>(a, w.split, red, sums, n, h == 0, level.of_sums(), l, 1.0f, slot_bytes, w.R, w.block,
-                 w.z, w.ns, kvh, put, [&](int t) { return row_sees_nothing(a, w, t); });
+  const float level_of = level.of_sums(), top = rows_top(sums, wave, n, h == 0, level_of, l);
+  if (n < w.R) put_rows32<D>(red, acc, weight(level_of, top, 1.0f), w.R, n, h, wave);
+  rows_finish<D>(a, w.split, red, sums, n, h == 0, top, 1.0f, slot_bytes, w.R, w.block, w.z, w.ns, kvh,
+                 [&](int t) { return row_sees_nothing(a, w, t); });
 }
 
 }  // namespace ifx
