@@ -27,8 +27,7 @@
 //
 // Registers: 256 a wave, two workgroups a CU.  D = 64 does with 168, three a
 // CU: 8111 tokens of 40 / 8 heads took 370 us, with two 387, with four 1330
-// (spills).  D = 256 needs 512: 4111 tokens of 16 / 2 heads in 241 us (fp16) or
-// 276 (bf16).
+// (spills).  D = 256 needs 512: 4111 tokens of 16 / 2 heads in 215 us.
 #include "ifx_attn_tile.h"
 
 namespace ifx {
@@ -306,7 +305,11 @@ __global__ __launch_bounds__(64 * kNW, D == 256 ? 1 : D == 64 ? 3 : 2) void k_at
   // first products: a wave waits at its next copy until the last is under way.
   const f32x16 none_yet = {};
   auto step = [&](const char *sk, const char *sv, auto next) IFX_INLINE {
-    constexpr int kAhead = 4;
+    // D = 256: with 3 or 4 parts of Q are in scratch memory, and what is read of them
+    // waits for the copies on their way.  us with 1 / 2 / 3 / 4, fp16: 4111 tokens of
+    // 16 / 2 heads 240/215/250/258, all 4111 seen 590/521/656/674; 16 / 4 heads, 512
+    // behind 7000 cached 120/116/117/125, 16 decode steps and 8 chunks 172/168/175/191.
+    constexpr int kAhead = D == 256 ? 2 : 4;
     f32x16 s[2];
     u32x4 f[4 * NS];  // K of both halves, V: at most kAhead + 1 are alive
     int swap = k_swap;
