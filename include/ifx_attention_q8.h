@@ -55,10 +55,11 @@ int ifx_read_rows_q8(const void *k_cache, const void *v_cache, const void *scale
  *
  * Codes are exact in the products, which are summed in fp32.  Q of bf16 is
  * taken to fp16 with a power of two for each row, which loses nothing of what is
- * at least 2^-28 of the row's largest value.  Probabilities times V's scales are
- * rounded to fp16, relative to the largest scale among the keys that the row has
- * met: what weighs 2^-20 of that and less loses bits.  Scales of V count as
- * 2^-80 at least in this. */
+ * at least 2^-28 of the row's largest value, if that is 2^-63 or more.
+ * Probabilities times V's scales are rounded to fp16, relative to the largest
+ * scale among the keys that the row has met: what weighs 2^-20 of that and less
+ * loses bits.  Scales of V count as 2^-80 at least in this; where they pass 2^108,
+ * keys whose weight is less than 2^-132 of them count as nothing. */
 int64_t ifx_attn_paged_q8_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int max_q,
                                           int max_kv);
 int ifx_attn_paged_q8(const void *q, int64_t q_stride, int q_dtype, const void *k_cache,

@@ -104,33 +104,35 @@ struct PagedPlan {
 // with 1536, 153 with 2048.
 //
 // Blocks of rows: as many workgroups as CUs.  us with 256 / 512 / 1024, 3000 keys:
-// 16 / 2 heads, 160 rows 22/22/22, 512 rows 25/26/26, 8-bit 24/26/26; 40 / 8 heads, 150
-// rows, 8-bit 24/26/30; 12000 keys, 160 rows 28/36/36, 512 rows 38/35/35.
+// 16 / 2 heads, 160 rows 16.7 with each, 512 rows 17.7/18.7/18.8, 8-bit 16.9/18.7/18.6;
+// 40 / 8 heads, 150 rows, 8-bit 16.0/18.4/18.6; 12000 keys, 16 / 2 heads, 160 rows 26.2
+// with each, 512 rows 34.7/33.9/34.0.
 //
 // Fewer where the split sums would not fit the largest workspace.
 //
 // Trees over the 16-bit cache go to attn_rows with up to 32 rows for a few units
 // (requests times key/value heads), 24 for some, else 16.  us with attn_tile /
-// attn_rows, 3000 keys, heads of 128:
-//   40 / 8 heads, 20 rows  2 requests 25.7/20.2, 4 26.6/24.3, 8 42.9/40.4, 16 55/61
-//                 30 rows  1 24.4/21.1, 2 25.4/22.8, 4 26.6/27.5, 8 42.4/45.4, 16 55/67
-//   16 / 2 heads, 24 rows  8 26.0/21.2, 32 42.2/34.2
-// The 8-bit cache's attn_rows is faster up to its 32 rows (30 rows of 40 / 8
-// heads: 32 requests 83 against 128).
+// attn_rows, 3000 keys, heads of 128, the caches from memory:
+//   40 / 8 heads, 20 rows  2 requests 23.4/17.5, 4 25.2/22.6, 8 38.7/36.4, 16 50.7/54.6
+//                 30 rows  1 22.2/17.3, 2 23.3/19.0, 4 25.1/24.9, 8 39.3/39.9, 16 51.9/58.4
+//   16 / 2 heads, 24 rows  8 23.5/18.2, 32 39.3/31.2
+// Over the 8-bit cache all of up to 32 rows go to attn_rows; from 17 on many of them
+// would be sooner done in attn_tile's way for few rows (32 requests of 30 rows, 40 / 8
+// heads, 43 against 59).
 //
 // More rows as blocks of 32 of attn_rows, where attn_tile's workgroups would leave
 // much of the chip idle (both read the keys once for each block or tile): up to 112
 // blocks, over the 8-bit cache 256 if a unit has no more than 8.  us with attn_tile /
 // in blocks, 3000 keys, by blocks of all units:
-//   16-bit  1 head of K    640 rows   20 32.6/21.9,  80 34.9/28.9;  1024 128 36.1/47.9
-//           16 / 2 heads   160 rows   10 31.9/21.7,  40 34.0/23.5;  512 128 35.7/35.0
-//           40 / 8 heads   100 rows   32 32.4/22.7,  64 33.7/25.1, 128 35.0/34.1
-//                          200 rows   56 33.2/24.0, 112 35.4/33.5, 224 47.0/47.2
-//   8-bit   1 head of K   1024 rows   32 35.6/19.4, 128 38.6/39.5;  640 320 55.1/57.6
-//           16 / 2 heads   160 rows   10 34.8/19.7,  40 37.3/22.2, 160 49.9/40.2
-//           40 / 8 heads   100 rows   32 34.4/21.4, 128 37.8/30.1, 512 65.6/65.4
-//                          200 rows   56 36.3/22.6, 224 49.9/40.8, 896 96.5/109
-//                          640 rows  160 50.2/70.7 (7000 keys)
+//   16-bit  1 head of K    640 rows   20 29.5/17.0,  80 31.1/24.1;  1024 128 31.9/42.7
+//           16 / 2 heads   160 rows   10 29.2/16.7,  40 30.8/20.8;  512 128 32.6/34.0
+//           40 / 8 heads   100 rows   32 29.7/18.9,  64 31.5/23.9, 128 33.2/35.2
+//                          200 rows   56 30.1/22.5, 112 31.9/34.4, 224 45.4/53.8
+//   8-bit   1 head of K   1024 rows   32 32.6/16.4, 128 34.5/36.8;  640 320 48.5/51.7
+//           16 / 2 heads   160 rows   10 32.1/16.0,  40 33.3/17.9, 160 45.5/37.8
+//           40 / 8 heads   100 rows   32 31.6/17.2, 128 33.8/26.6, 512 56.1/57.2
+//                          200 rows   56 32.6/18.7, 224 45.6/37.2, 896 82.6/100.9
+//                          640 rows  160 50.8/71.3 (7000 keys)
 enum PagedKind { kPaged16, kTree16, kPaged8 };
 PagedPlan plan_paged(PagedKind kind, int B, int T, int Hq, int Hkv, int D, int max_q, int max_kv) {
   PagedPlan p{};

@@ -1,5 +1,6 @@
 // attn_rows.hip -- paged attention of requests with few query rows (at most
-// 32 = new tokens x query heads of a group: decode steps).
+// 32 = new tokens x query heads of a group: decode steps), and of trees of drafts
+// with more, in blocks of 32.
 //
 //   s_j = c q . k_j (c = scale log2 e), p_j = 2^(s_j - m), l = sum p_j,
 //   o = sum p_j v_j / l

@@ -11,8 +11,11 @@
 //
 // Bound by the vector units and LDS beside the matrix cores: 375 vector
 // instructions and 32 products of 32x32x16 for a wave's stage, LDS read and written
-// for about as long.  512 tokens behind 7430, 40 / 8 heads of 128: 124 us, 650
-// TFLOP/s (the 16-bit cache's: 100).  Tried: codes in registers instead of LDS 133
+// for about as long.  512 tokens behind 7430, 40 / 8 heads of 128: 126 us, 640
+// TFLOP/s (the 16-bit cache's: 94), and 146 where the same launches in a row have
+// lowered the card's clock.  36 registers (one request) or 17 (several) of D = 128, 105
+// of D = 256, are kept in scratch memory over the stages; none of them is used in one
+// that its rows see whole.  Tried: codes in registers instead of LDS 133
 // to 146, stages of 32 keys 145, three workgroups a CU of 168 registers 213 (they
 // spill), codes taken to fp16 between the products 126; the same without any scales
 // (which is no attention, but a bound) 119; two stages of codes on their way 129.
@@ -20,9 +23,11 @@
 // Requests of up to 32 rows of a key/value head, single tokens next to chunks or
 // trees, would leave three of the four waves idle: their chunks go through
 // rows32_q8, where the waves share the keys.  24 trees of 1 to 38 nodes behind 110
-// to 7302 tokens, 40 / 8 heads: 62 us with it and 78 without; 32 of 2 to 23 nodes
-// 56 and 85; 16 single tokens and 8 chunks of 17 to 304 tokens 62 and 92, of 16 / 2
-// heads 37 and 39.
+// to 7302 tokens, 40 / 8 heads, with their plan: 58 us with it and 75 without; 32 of 2
+// to 23 nodes behind 107 to 7471 71 and 73; 16 single tokens and 8 chunks of 17 to 182
+// tokens 50 and 68, of 16 / 2 heads 36 and 38.  A request without new tokens is no
+// work: as many idle ones of 20000 keys beside such batches change their times by
+// less than 3 %.
 #include "ifx_attn_rows_q8.h"
 #include "ifx_attn_tile.h"
 
@@ -49,8 +54,8 @@ __device__ __forceinline__ void group_barrier() {
 constexpr int kScales = 2 * TK + 4;  // of a stage: K's, V's, the largest of V's
 
 // Keys of few rows that count as a stage of a row tile, as they take about as long:
-// with 128 / 160 / 192 / 224 / 256 the batches above take 63/62/62/62/66 us (24
-// trees), 58/59/61/56/56 (32 trees) and 70/63/62/62/58 (40 / 8 heads' mixed step).
+// with 128 / 160 / 192 / 224 / 256 the batches above take 59/59/60/58/63 us (24
+// trees), 73/71/71/71/71 (32 trees) and 53/56/51/50/50 (40 / 8 heads' mixed step).
 constexpr int kFewKeys = 224;
 
 // LDS: fp16 K and V of a stage, its codes and scales; or the tiles of few rows and

@@ -1,6 +1,7 @@
 // ifx_attn.h -- what the attention kernels (kv_plan.hip, rope_append.hip,
-// attn_rows.hip, attn_tile.hip) and their entry points (attention_api.hip)
-// share.
+// attn_rows.hip, attn_tile.hip, those of the 8-bit cache by way of ifx_attn_q8.h and
+// those of drafted tokens by way of ifx_drafts_impl.h) and their entry points
+// (attention_api.hip, drafts_api.hip) share.
 #pragma once
 
 #include <atomic>
@@ -277,9 +278,9 @@ __device__ __forceinline__ int ceil_div(int x, int d, float r) {
 
 // Of the 8-bit cache's rows and of trees.  us with a cap of 2 / 3 / 4 sqrt(stages)
 // and with none, one token over 12000 and 50000 keys, then 3 tokens over 12000:
-//   16 / 2 heads of 128  14.9/13.9/13.1/16.1, 23.4/20.4/20.2/39.9, 20.1/19.1/22.5/29.5
-//   40 / 8               15.7/14.8/14.2/18.5, 35.0/32.1/34.1/36.7, 18.5/17.7/17.4/24.6
-// 3000 keys: 11.6/10.6/10.5/10.8; 32 requests of 531 to 22591 the same with each.
+//   16 / 2 heads of 128  15.1/13.9/13.2/15.6, 23.4/20.2/19.9/38.1, 19.9/18.8/21.4/28.2
+//   40 / 8               15.5/14.5/14.1/18.4, 31.8/29.3/32.1/34.3, 18.3/17.5/17.1/23.9
+// 3000 keys: 11.6/10.4/10.5/10.7; 32 requests of 531 to 22591 the same with each.
 constexpr int kRowsRoot = 24;
 
 // Chunks of a request of x stages: of `chunk` (r = 1 / chunk), or of LEAST at least;

@@ -140,10 +140,9 @@ __device__ __forceinline__ void add_chunks(const AttnArgs &a, ChunkSums k, float
 // request, its row block number `block`, whose keys are cut into ns chunks, this one
 // z.  none(t): whether the rows of new token t see nothing.  kAtOnce: chunks whose
 // sums a thread reads at a time, 4 registers each.  GROUPED: for many rows, of several
-// places at a time.  A tree of 64 nodes, 3000 keys, 16 / 2 heads of 128: 23.1 us with
-// it and 24.9 without, over the 8-bit cache 22.2 and 24.8; 49 rows of 450 keys, 28 / 4
-// heads of 256, 22.4 and 31.0.  Single tokens, which have no such places, lost 0.3 by
-// the longer code.
+// places at a time.  A tree of 64 nodes, 3000 keys, 16 / 2 heads of 128: 17.7 us with
+// it and 21.0 without, over the 8-bit cache 17.0 and 20.5; 49 rows of 450 keys, 28 / 4
+// heads of 256, 22.3 and 31.0.  Single tokens have no such places and gain nothing.
 //
 // In functions with values as arguments, not closures: accumulators that a closure
 // held by reference took 12 vector registers more, which with heads of 64 left two
