@@ -194,6 +194,8 @@ def verify(tokens, cu_q, target_probs, accept_u, sample_u, max_q, parents=None, 
         if draft_probs.shape != target_probs.shape:
             raise ValueError("draft_probs must have the shape of target_probs")
         dp, ds = _probs(draft_probs, "draft_probs", T, target_probs.dtype, dev)
+    if B < 1:
+        raise ValueError("cu_q must have a value for each request and one more")
     if workspace is None:
         raise ValueError("verify needs a workspace")
     wp, wn = _workspace(workspace, dev)

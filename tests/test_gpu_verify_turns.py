@@ -26,3 +26,16 @@ def test_turns_that_hold_nothing(dev, B, dtype, turns):  # noqa: F811
     su = [rng.choice([1.0, 1 - 2.0 ** -24, 0.0, rng.randrange(len(at)) / len(at) + rng.choice([0, 2.0 ** -20])])
           for _ in range(B)]
     run_verify(dev, [1] * B, [-1] * B, [rng.choice(at) for _ in range(B)], p, [0.5] * B, su, dtype=dtype)
+
+
+def test_no_requests(dev):  # noqa: F811
+    """cu_q of one value or none is refused as other bad arguments are."""
+    import torch
+    from inferflux_amd import attention as at, drafts
+    ws = at.workspace(dev)
+    for T in (0, 3):
+        for n in (0, 1):
+            with pytest.raises(ValueError):
+                drafts.verify(torch.zeros(T, dtype=torch.int32, device=dev), torch.zeros(n, dtype=torch.int32, device=dev),
+                              torch.ones(T, 5, device=dev), torch.zeros(T, device=dev), torch.zeros(0, device=dev), 4,
+                              workspace=ws)
