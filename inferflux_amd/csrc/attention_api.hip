@@ -27,15 +27,6 @@ namespace {
 
 using namespace ifx;
 
-int status_of(hipError_t e) { return e == hipSuccess ? IFX_OK : -static_cast<int>(e); }
-
-// log2 of a page size the cache can have, else -1.
-int page_shift_of(int page_size) {
-  for (int sh = 4; sh <= 8; ++sh)
-    if (page_size == 1 << sh) return sh;
-  return -1;
-}
-
 bool is_elem(int dtype) { return dtype == IFX_ATTN_F16 || dtype == IFX_ATTN_BF16; }
 bool is_out(int dtype) { return dtype == IFX_ATTN_F32 || is_elem(dtype); }
 

@@ -9,17 +9,8 @@ namespace {
 
 using namespace ifx;
 
-int status_of(hipError_t e) { return e == hipSuccess ? IFX_OK : -static_cast<int>(e); }
-
 bool batch_ok(int B, int T) { return B >= 1 && B <= IFX_ATTN_MAX_BATCH && T >= 0 && T < (1 << 30); }
 bool nodes_ok(int max_q) { return max_q >= 1 && max_q <= IFX_TREE_MAX_NODES; }
-
-// log2 of a page size the cache can have, else -1.
-int page_shift_of(int page_size) {
-  for (int sh = 4; sh <= 8; ++sh)
-    if (page_size == 1 << sh) return sh;
-  return -1;
-}
 
 // Whether an output is in the place of an input or another output.
 bool overlap(std::initializer_list<const void *> out, std::initializer_list<const void *> in) {

@@ -5,6 +5,7 @@
 
 #include "ifx_attn.h"
 #include "ifx_drafts.h"
+#include "ifx_qgemm.h"
 
 namespace ifx {
 
@@ -51,5 +52,14 @@ struct KeepArgs {
   int page_shift, Hkv, D, table_width, B, T, max_q;
 };
 hipError_t launch_keep_path(const KeepArgs &a, int elem_bytes, hipStream_t s);
+
+// Of the entry points: what a launch's result is to the caller, and log2 of a page
+// size that the cache can have, else -1.
+inline int status_of(hipError_t e) { return e == hipSuccess ? IFX_OK : -static_cast<int>(e); }
+inline int page_shift_of(int page_size) {
+  for (int sh = 4; sh <= 8; ++sh)
+    if (page_size == 1 << sh) return sh;
+  return -1;
+}
 
 }  // namespace ifx
